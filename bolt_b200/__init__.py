@@ -125,6 +125,37 @@ class GemmCall(C.Structure):
                 ("offsetC", C.c_void_p), ("C", C.c_void_p), ("epilogue", GemmEpilogue)]
 
 
+class KvCache(C.Structure):
+    """bolt_b200_kv_cache"""
+    _fields_ = [("dt", C.c_uint32), ("pages", C.c_uint32), ("page_size", C.c_uint32), ("kv_heads", C.c_uint32), ("dim", C.c_uint32),
+                ("page_stride", C.c_uint64), ("token_stride", C.c_uint64), ("head_stride", C.c_uint64), ("k", C.c_void_p),
+                ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p)]
+
+
+class KvAppend(C.Structure):
+    """bolt_b200_kv_append_call"""
+    _fields_ = [("tokens", C.c_uint32), ("heads", C.c_uint32), ("dt", C.c_uint32), ("q_out_dt", C.c_uint32), ("q", C.c_void_p),
+                ("k", C.c_void_p), ("v", C.c_void_p), ("q_out", C.c_void_p), ("q_stride", C.c_uint64), ("k_stride", C.c_uint64),
+                ("v_stride", C.c_uint64), ("q_out_stride", C.c_uint64), ("sequence", C.c_void_p), ("position", C.c_void_p),
+                ("table", C.c_void_p), ("sequences", C.c_uint32), ("table_pages", C.c_uint32), ("rotary_dim", C.c_uint32),
+                ("interleaved", C.c_uint32), ("rotary_positions", C.c_uint32), ("cos", C.c_void_p), ("sin", C.c_void_p)]
+
+
+class PagedAttention(C.Structure):
+    """bolt_b200_paged_attention_call"""
+    _fields_ = [("sequences", C.c_uint32), ("heads", C.c_uint32), ("q_dt", C.c_uint32), ("out_dt", C.c_uint32), ("q", C.c_void_p),
+                ("out", C.c_void_p), ("lse", C.c_void_p), ("q_stride", C.c_uint64), ("out_stride", C.c_uint64), ("table", C.c_void_p),
+                ("length", C.c_void_p), ("table_pages", C.c_uint32), ("window", C.c_uint32), ("scale", C.c_float), ("out_scale", C.c_float)]
+
+
+class Lora(C.Structure):
+    """bolt_b200_lora_call"""
+    _fields_ = [("rows", C.c_uint32), ("N", C.c_uint32), ("K", C.c_uint32), ("rank", C.c_uint32), ("adapters", C.c_uint32),
+                ("segments", C.c_uint32), ("x_dt", C.c_uint32), ("x", C.c_void_p), ("y", C.c_void_p), ("x_stride", C.c_uint64),
+                ("y_stride", C.c_uint64), ("a", C.c_void_p), ("b", C.c_void_p), ("a_stride", C.c_uint64), ("scale", C.c_void_p),
+                ("first_row", C.c_void_p), ("adapter", C.c_void_p), ("sA", C.c_float), ("d_sA", C.c_void_p), ("row_scale", C.c_void_p)]
+
+
 _vp, _u32, _u32p, _f32p = C.c_void_p, C.c_uint32, C.POINTER(C.c_uint32), C.POINTER(C.c_float)
 _TDp = C.POINTER(TensorDesc)
 
@@ -171,6 +202,11 @@ SIGNATURES = {
     "dequantize_cuda_b200": (C.c_int, [_TDp, _vp, _f32p, _TDp, _vp, _TDp, _vp]),
     "bolt_b200_absmax_scale_f32": (C.c_int, [_vp, C.c_uint64, _vp]),
     "bolt_b200_quantize_f32_u8_noalloc": (C.c_int, [_vp, C.c_uint64, _vp, _vp]),
+    "bolt_b200_kv_append": (C.c_int, [C.POINTER(KvCache), C.POINTER(KvAppend)]),
+    "bolt_b200_paged_attention_tmp_bytes": (C.c_int, [C.POINTER(KvCache), C.POINTER(PagedAttention), _u32p]),
+    "bolt_b200_paged_attention": (C.c_int, [C.POINTER(KvCache), C.POINTER(PagedAttention), _u32, _vp]),
+    "bolt_b200_lora_tmp_bytes": (C.c_int, [C.POINTER(Lora), _u32p]),
+    "bolt_b200_lora": (C.c_int, [C.POINTER(Lora), _u32, _vp]),
     "convolution_infer_output_size_cuda_b200": (
         C.c_int, [_TDp, _TDp, C.POINTER(ConvolutionParamSpec), _TDp, _u32]),
     "convolution_infer_forward_algorithm_cuda_b200": (
@@ -303,6 +339,34 @@ def dequantize(qDesc, qData, scale, dDesc, dData):
     b = tensor1d(DT_F32, 0)
     CHECK_STATUS(lib().dequantize_cuda_b200(C.byref(qDesc), qData, C.cast(arr, _f32p), C.byref(b), None,
                                             C.byref(dDesc), dData), "dequantize")
+
+
+# ---- a decoding step: paged key-value cache, attention of one new token, adapters (include/bolt_b200.h) ---------
+def kv_append(cache, call):
+    """cache: KvCache, call: KvAppend"""
+    CHECK_STATUS(lib().bolt_b200_kv_append(cache, call), "kv_append")
+
+
+def paged_attention_tmp_bytes(cache, call):
+    n = C.c_uint32(0)
+    CHECK_STATUS(lib().bolt_b200_paged_attention_tmp_bytes(cache, call, C.byref(n)), "paged_attention_tmp_bytes")
+    return n.value
+
+
+def paged_attention(cache, call, tmp_bytes, tmp):
+    """cache: KvCache, call: PagedAttention"""
+    CHECK_STATUS(lib().bolt_b200_paged_attention(cache, call, tmp_bytes, tmp), "paged_attention")
+
+
+def lora_tmp_bytes(call):
+    n = C.c_uint32(0)
+    CHECK_STATUS(lib().bolt_b200_lora_tmp_bytes(call, C.byref(n)), "lora_tmp_bytes")
+    return n.value
+
+
+def lora(call, tmp_bytes, tmp):
+    """call: Lora"""
+    CHECK_STATUS(lib().bolt_b200_lora(call, tmp_bytes, tmp), "lora")
 
 
 # ---- pooling (u8, NCHWc16) ------------------------------------------------------------------------------

@@ -1,0 +1,352 @@
+// kv_append.cu -- rows of new keys and values into a paged cache, rotated by position on the way; queries are rotated in
+// the same launch.
+//
+// A pair (a, b) of a head turns by the angle of its position: a' = a cos - b sin, b' = b cos + a sin, each step one binary32
+// operation, so that the rows are the same bits wherever they are computed.  HBM bound: every row is read once and
+// written once, and the angles of a position are shared through L1 by the heads of a token.  16 or 32 lanes hold a row in
+// registers, four neighbouring elements each: its largest magnitude (signed bytes) is a few shuffles away, and nobody
+// reads a row twice except for the partner half of a pair, which comes from L1.
+#include "decode.cuh"
+
+namespace b200 {
+
+bool on_this_device(const void *p)
+{
+    if (p == nullptr) {
+        return false;
+    }
+    if (tls().device_only) {
+        return true;
+    }
+    cudaPointerAttributes a;
+    if (cudaPointerGetAttributes(&a, p) != cudaSuccess) {
+        cudaGetLastError();
+        return false;
+    }
+    if (a.type == cudaMemoryTypeManaged) {
+        return true;
+    }
+    int dev = tls().device;
+    if (a.type != cudaMemoryTypeDevice || (dev < 0 && cudaGetDevice(&dev) != cudaSuccess)) {
+        return false;
+    }
+    return a.device == dev;
+}
+
+EE check_cache(const bolt_b200_kv_cache *c)
+{
+    if (c->k == nullptr || c->v == nullptr) {
+        return NULL_POINTER;
+    }
+    if (c->dt != DT_F16 && c->dt != DT_I8) {
+        return NOT_SUPPORTED;
+    }
+    const uint64_t size = c->dt == DT_F16 ? 2 : 1;
+    if (c->pages == 0 || c->page_size == 0 || c->kv_heads == 0 || c->dim == 0) {
+        return NOT_MATCH;
+    }
+    if (c->dim > 256 || c->dim * size % 16 != 0 || !aligned(c->k, 16) || !aligned(c->v, 16)) {
+        return NOT_SUPPORTED;
+    }
+    const uint64_t strides[3] = {c->page_stride, c->token_stride, c->head_stride};
+    const uint32_t counts[3] = {c->pages, c->page_size, c->kv_heads};
+    for (int i = 0; i < 3; ++i) {
+        if (counts[i] > 1 && strides[i] < c->dim) {
+            return NOT_MATCH;
+        }
+        if (strides[i] > MAX_STRIDE * 64 || strides[i] * size % 16 != 0) {
+            return NOT_SUPPORTED;
+        }
+    }
+    // 2^62 bytes and 2^31 rows of one number: more is no cache, and offsets stay within 64 bits
+    if (c->pages > 0x7FFFFFFFu || c->page_size > 0x7FFFFFFFu || c->kv_heads > 65535u) {
+        return NOT_SUPPORTED;
+    }
+    if (c->dt == DT_I8) {
+        if (c->k_scale == nullptr || c->v_scale == nullptr) {
+            return NULL_POINTER;
+        }
+        if (!aligned(c->k_scale, 4) || !aligned(c->v_scale, 4)) {
+            return NOT_SUPPORTED;
+        }
+        if (!on_this_device(c->k_scale) || !on_this_device(c->v_scale)) {
+            return NOT_MATCH;
+        }
+    }
+    return on_this_device(c->k) && on_this_device(c->v) ? SUCCESS : NOT_MATCH;
+}
+
+namespace {
+
+struct AppendParams {
+    CacheView cache;
+    void *k_cache, *v_cache;
+    float *k_scale, *v_scale;   // signed bytes
+    const void *src[3];         // q, k, v
+    uint64_t stride[3], q_out_stride;
+    void *q_out;
+    const int32_t *sequence, *position, *table;
+    uint32_t tokens, heads, sequences, table_pages;
+    uint32_t rotary, interleaved, rotary_positions;
+    const float *cos, *sin;
+    int i8, q_out_f16;
+    int *status;
+};
+
+// one row of TIN by LANES lanes, VW neighbouring elements at a time, PER times
+template <typename TIN, int VW, int LANES, int PER>
+__global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ AppendParams p)
+{
+    const uint32_t rows_per_token = p.heads + 2 * p.cache.kv_heads;
+    const uint64_t row = ((uint64_t)blockIdx.x * 256 + threadIdx.x) / LANES;
+    const uint32_t lane = threadIdx.x % LANES;
+    bool live = row < (uint64_t)p.tokens * rows_per_token;
+    const uint32_t token = live ? (uint32_t)row / rows_per_token : 0, h = live ? (uint32_t)row - token * rows_per_token : 0;
+    const int kind = h < p.heads ? 0 : (h < p.heads + p.cache.kv_heads ? 1 : 2);
+    const uint32_t head = kind == 0 ? h : (kind == 1 ? h - p.heads : h - p.heads - p.cache.kv_heads);
+    const uint32_t dim = p.cache.dim, rotary = kind == 2 ? 0 : p.rotary, half = rotary / 2;
+    const int32_t position = live ? p.position[token] : -1;
+    live = live && position >= 0;
+    uint32_t page = 0, at = 0;
+    if (live) {
+        const int64_t seq = p.sequence != nullptr ? p.sequence[token] : (int64_t)token;
+        const bool good = seq >= 0 && seq < (int64_t)p.sequences && (p.rotary == 0 || (uint32_t)position < p.rotary_positions) &&
+            page_of(p.table, (uint64_t)seq, p.table_pages, p.cache.pages, p.cache.page_size, (uint32_t)position, &page, &at);
+        if (!good) {
+            if (lane == 0) {
+                atomicExch(p.status, BAD_APPEND);
+            }
+            live = false;
+        }
+    }
+    const TIN *src = reinterpret_cast<const TIN *>(p.src[kind]) + token * p.stride[kind] + (uint64_t)head * dim;
+    const float *cos = p.cos + (uint64_t)(uint32_t)position * (p.rotary / 2), *sin = p.sin + (uint64_t)(uint32_t)position * (p.rotary / 2);
+    float x[PER][VW];
+    int top = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const uint32_t i = (lane + j * LANES) * VW;
+#pragma unroll
+        for (int e = 0; e < VW; ++e) {
+            x[j][e] = 0.f;
+        }
+        if (!live || i >= dim) {
+            continue;
+        }
+        if constexpr (VW == 4) {
+            load4(src + i, x[j]);
+            if (i < rotary) {
+                if (p.interleaved) {
+#pragma unroll
+                    for (int e = 0; e < 4; e += 2) {
+                        const float c = cos[(i + e) / 2], s = sin[(i + e) / 2], a = x[j][e], b = x[j][e + 1];
+                        x[j][e] = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s));
+                        x[j][e + 1] = __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s));
+                    }
+                } else {
+                    float y[4], c[4], s[4];
+                    const bool first = i < half;
+                    const uint32_t k = first ? i : i - half;
+                    load4(src + (first ? i + half : k), y);
+                    load4(cos + k, c);
+                    load4(sin + k, s);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float own = __fmul_rn(x[j][e], c[e]), other = __fmul_rn(y[e], s[e]);
+                        x[j][e] = first ? __fsub_rn(own, other) : __fadd_rn(own, other);
+                    }
+                }
+            }
+        } else {
+            x[j][0] = load1(src + i);
+            if (i < rotary) {
+                const bool first = p.interleaved ? (i & 1) == 0 : i < half;
+                const uint32_t k = p.interleaved ? i / 2 : (first ? i : i - half);
+                const uint32_t o = p.interleaved ? i ^ 1 : (first ? i + half : k);
+                const float own = __fmul_rn(x[j][0], cos[k]), other = __fmul_rn(load1(src + o), sin[k]);
+                x[j][0] = first ? __fsub_rn(own, other) : __fadd_rn(own, other);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < VW; ++e) {
+            top = max(top, magnitude(x[j][e]));
+        }
+    }
+    __syncwarp();   // q_out may be q: every lane has read its row
+    if (kind == 0) {
+        if (!live) {
+            return;
+        }
+        const uint64_t o = token * p.q_out_stride + (uint64_t)head * dim;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const uint32_t i = (lane + j * LANES) * VW;
+            if (i < dim) {
+                if constexpr (VW == 4) {
+                    if (p.q_out_f16) {
+                        *reinterpret_cast<uint2 *>(reinterpret_cast<__half *>(p.q_out) + o + i) =
+                            make_uint2(half2_bits(x[j][0], x[j][1]), half2_bits(x[j][2], x[j][3]));
+                    } else {
+                        *reinterpret_cast<float4 *>(reinterpret_cast<float *>(p.q_out) + o + i) = make_float4(x[j][0], x[j][1], x[j][2], x[j][3]);
+                    }
+                } else if (p.q_out_f16) {
+                    reinterpret_cast<__half *>(p.q_out)[o + i] = __float2half_rn(x[j][0]);
+                } else {
+                    reinterpret_cast<float *>(p.q_out)[o + i] = x[j][0];
+                }
+            }
+        }
+        return;
+    }
+    const uint64_t o = row_element(p.cache, page, at, head);
+    void *cache = kind == 1 ? p.k_cache : p.v_cache;
+    if (!p.i8) {
+        if (!live) {
+            return;
+        }
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const uint32_t i = (lane + j * LANES) * VW;
+            if (i < dim) {
+                __half *d = reinterpret_cast<__half *>(cache) + o + i;
+                if constexpr (VW == 4) {
+                    *reinterpret_cast<uint2 *>(d) = make_uint2(half2_bits(x[j][0], x[j][1]), half2_bits(x[j][2], x[j][3]));
+                } else {
+                    *d = __float2half_rn(x[j][0]);
+                }
+            }
+        }
+        return;
+    }
+    const unsigned mask = LANES == 32 ? 0xFFFFFFFFu : 0xFFFFu << (threadIdx.x & 16);
+#pragma unroll
+    for (int s = LANES / 2; s > 0; s >>= 1) {
+        top = max(top, __shfl_xor_sync(mask, top, s, LANES));
+    }
+    if (!live) {
+        return;
+    }
+    const float scale = top == 0 ? 1.0f : __fdiv_rn(127.0f, __int_as_float(top));
+    auto byte = [scale](float v) { return (uint32_t)(min(127, max(-127, cvt_rne_x86(__fmul_rn(v, scale)))) & 0xFF); };
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const uint32_t i = (lane + j * LANES) * VW;
+        if (i < dim) {
+            uint8_t *d = reinterpret_cast<uint8_t *>(cache) + o + i;
+            if constexpr (VW == 4) {
+                *reinterpret_cast<uint32_t *>(d) = byte(x[j][0]) | byte(x[j][1]) << 8 | byte(x[j][2]) << 16 | byte(x[j][3]) << 24;
+            } else {
+                *d = (uint8_t)byte(x[j][0]);
+            }
+        }
+    }
+    if (lane == 0) {
+        (kind == 1 ? p.k_scale : p.v_scale)[scale_element(p.cache, page, at, head)] = scale;
+    }
+}
+
+template <typename TIN>
+EE launch(const AppendParams &p, bool vectors, cudaStream_t st)
+{
+    const uint64_t rows = (uint64_t)p.tokens * (p.heads + 2 * p.cache.kv_heads);
+    const uint32_t lanes = vectors && p.cache.dim <= 64 ? 16 : 32;
+    const uint32_t grid = (uint32_t)((rows * lanes + 255) / 256);
+    if (!vectors) {
+        return launch_kernel(grid, 256, 0, st, kv_append_kernel<TIN, 1, 32, 8>, p);
+    }
+    if (p.cache.dim <= 64) {
+        return launch_kernel(grid, 256, 0, st, kv_append_kernel<TIN, 4, 16, 1>, p);
+    }
+    if (p.cache.dim <= 128) {
+        return launch_kernel(grid, 256, 0, st, kv_append_kernel<TIN, 4, 32, 1>, p);
+    }
+    return launch_kernel(grid, 256, 0, st, kv_append_kernel<TIN, 4, 32, 2>, p);
+}
+
+}  // namespace
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" EE bolt_b200_kv_append(const bolt_b200_kv_cache *cache, const bolt_b200_kv_append_call *a)
+{
+    if (cache == nullptr || a == nullptr) {
+        return NULL_POINTER;
+    }
+    DeviceCtx *c = ctx();
+    if (c == nullptr) {
+        return UNKNOWN;
+    }
+    B200_EE(check_cache(cache));
+    if (a->tokens == 0) {
+        return SUCCESS;
+    }
+    if (a->k == nullptr || a->v == nullptr || a->position == nullptr || a->table == nullptr || (a->heads != 0 && (a->q == nullptr || a->q_out == nullptr)) ||
+        (a->rotary_dim != 0 && (a->cos == nullptr || a->sin == nullptr))) {
+        return NULL_POINTER;
+    }
+    if ((a->dt != DT_F32 && a->dt != DT_F16) || (a->heads != 0 && a->q_out_dt != DT_F32 && a->q_out_dt != DT_F16)) {
+        return NOT_SUPPORTED;
+    }
+    if (a->sequences == 0 || a->table_pages == 0 || (a->sequence == nullptr && a->tokens > a->sequences) || a->rotary_dim > cache->dim ||
+        a->rotary_dim % 2 != 0) {
+        return NOT_MATCH;
+    }
+    const uint64_t rows = (uint64_t)a->tokens * ((uint64_t)a->heads + 2ull * cache->kv_heads);
+    if (a->heads > 65535u || rows > 0xFFFFFFFFull / 32 * 8) {
+        return NOT_SUPPORTED;
+    }
+    const uint32_t size = a->dt == DT_F32 ? 4 : 2, q_size = a->q_out_dt == DT_F32 ? 4 : 2;
+    const uint64_t q_row = (uint64_t)a->heads * cache->dim, kv_row = (uint64_t)cache->kv_heads * cache->dim;
+    if (a->tokens > 1 && (a->k_stride < kv_row || a->v_stride < kv_row || (a->heads != 0 && (a->q_stride < q_row || a->q_out_stride < q_row)))) {
+        return NOT_MATCH;
+    }
+    if (a->k_stride > MAX_STRIDE || a->v_stride > MAX_STRIDE || a->q_stride > MAX_STRIDE || a->q_out_stride > MAX_STRIDE) {
+        return NOT_SUPPORTED;
+    }
+    if (!aligned(a->k, size) || !aligned(a->v, size) || !aligned(a->position, 4) || !aligned(a->table, 4) || !aligned(a->sequence, 4) ||
+        (a->heads != 0 && (!aligned(a->q, size) || !aligned(a->q_out, q_size))) || (a->rotary_dim != 0 && (!aligned(a->cos, 4) || !aligned(a->sin, 4)))) {
+        return NOT_SUPPORTED;
+    }
+    if (!on_this_device(a->k) || !on_this_device(a->v) || !on_this_device(a->position) || !on_this_device(a->table) ||
+        (a->sequence != nullptr && !on_this_device(a->sequence)) || (a->heads != 0 && (!on_this_device(a->q) || !on_this_device(a->q_out))) ||
+        (a->rotary_dim != 0 && (!on_this_device(a->cos) || !on_this_device(a->sin)))) {
+        return NOT_MATCH;
+    }
+    AppendParams p;
+    p.cache = view_of(*cache);
+    p.k_cache = cache->k;
+    p.v_cache = cache->v;
+    p.k_scale = cache->k_scale;
+    p.v_scale = cache->v_scale;
+    p.src[0] = a->heads != 0 ? a->q : a->k;
+    p.src[1] = a->k;
+    p.src[2] = a->v;
+    p.stride[0] = a->q_stride;
+    p.stride[1] = a->k_stride;
+    p.stride[2] = a->v_stride;
+    p.q_out = a->q_out;
+    p.q_out_stride = a->q_out_stride;
+    p.sequence = a->sequence;
+    p.position = a->position;
+    p.table = a->table;
+    p.tokens = a->tokens;
+    p.heads = a->heads;
+    p.sequences = a->sequences;
+    p.table_pages = a->table_pages;
+    p.rotary = a->rotary_dim;
+    p.interleaved = a->interleaved != 0;
+    p.rotary_positions = a->rotary_positions;
+    p.cos = a->cos;
+    p.sin = a->sin;
+    p.i8 = cache->dt == DT_I8;
+    p.q_out_f16 = a->q_out_dt == DT_F16;
+    p.status = c->d_status;
+    // Four elements at a time where rows and angles lie on their grid and no group of four holds rotated and other
+    // elements, or both halves of its pairs; dim is a multiple of 8 (16-byte rows of the cache).
+    const uint32_t q4 = size * 4;
+    const bool vectors = aligned(a->k, q4) && aligned(a->v, q4) && a->k_stride % 4 == 0 && a->v_stride % 4 == 0 &&
+        (a->heads == 0 || (aligned(a->q, q4) && a->q_stride % 4 == 0 && aligned(a->q_out, q_size * 4) && a->q_out_stride % 4 == 0)) &&
+        (a->rotary_dim == 0 || (a->interleaved ? a->rotary_dim % 4 == 0 : a->rotary_dim % 8 == 0 && aligned(a->cos, 16) && aligned(a->sin, 16)));
+    return a->dt == DT_F32 ? launch<float>(p, vectors, tls().stream) : launch<__half>(p, vectors, tls().stream);
+}

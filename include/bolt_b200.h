@@ -474,6 +474,115 @@ EE matmul_cuda_b200(const TensorDesc *matrixADesc, int transposeA, const void *m
     const TensorDesc *biasDesc, const void *bias, U32 tmpBytes, void *tmp,
     const TensorDesc *matrixCDesc, void *matrixC, F32 *cScale);
 
+/* ---- a decoding step: paged key-value cache, attention of one new token, adapters -----------------------
+ * Bolt serves a language model through its engine's graphs and has no operator of these kinds (no counterpart).
+ * All pointers are device pointers of the GPU the call runs on (anything else: NOT_MATCH); the work is enqueued on
+ * the thread's stream and the call returns without waiting.  Lengths, positions, page numbers and segments are
+ * read on the device, so one captured graph serves every step.  What they say is checked there: a number that
+ * would lead outside the arrays described by the call is not followed, and the device status word is set (51 by
+ * bolt_b200_kv_append, 52 by bolt_b200_paged_attention, 53 by bolt_b200_lora), so that the next
+ * bolt_b200_synchronize returns UNKNOWN.  Calls that run at the same time need a tmp each, two captured graphs
+ * that may do so as well; tmp need not be initialised. */
+
+/* A cache of pages, each `page_size` tokens of `kv_heads` heads.  The row of (page, token of the page, head) is `dim`
+ * contiguous elements at element page * page_stride + token * token_stride + head * head_stride of k and of v
+ * ([page][head][token][dim], [page][token][head][dim] or a slice of a larger array).
+ *   DT_F16: binary16.
+ *   DT_I8:  signed bytes; row (page, token, head) stands for byte / scale[(page * kv_heads + head) * page_size + token],
+ *           scale = 127 / absmax of the row as everywhere in this library.
+ * A row has at most 256 elements; its size in bytes, the strides in bytes and k and v are multiples of 16 (else
+ * NOT_SUPPORTED).  Rows must not overlap. */
+typedef struct {
+    DataType dt;
+    U32 pages, page_size, kv_heads, dim;
+    uint64_t page_stride, token_stride, head_stride; /* in elements */
+    void *k, *v;
+    F32 *k_scale, *v_scale; /* DT_I8 only, [pages][kv_heads][page_size] */
+} bolt_b200_kv_cache;
+
+/* Rows of `tokens` new tokens into the cache, of any number of sequences at once: token i is number position[i] of
+ * sequence sequence[i] (NULL: of sequence i, the decoding step) and goes to page
+ * table[sequence * table_pages + position / page_size], place position % page_size.  position[i] < 0 marks padding:
+ * nothing is written for it.  No two tokens of a call may have the same place (one of the rows, or parts of
+ * both, would stay).
+ * q, k and v: row i starts at element i * stride, its heads follow one another (slices of one projection's result).
+ * Keys and queries are rotated by position; queries (heads > 0) go to q_out, which may be q if strides and types agree.
+ * The first rotary_dim elements (even, 0: no rotation) of a head turn in pairs, (i, i + rotary_dim / 2), or
+ * (2i, 2i + 1) if interleaved, by the angle whose cosine and sine are cos / sin[position * rotary_dim / 2 + i]
+ * (positions below rotary_positions):
+ *   a' = a * cos - b * sin, b' = b * cos + a * sin, every product, difference and sum one binary32 operation.
+ * DT_F16 results are rounded once.  A DT_I8 row is quantized as by quantize_cuda_b200 (F32 -> I8) with a dynamic
+ * scale of its own: scale = 127 / absmax (1 for a row of zeros), byte = clamp(rne(x * scale), -127, 127).
+ * A token that is refused on the device (see above) leaves cache and q_out as they were. */
+typedef struct {
+    U32 tokens, heads; /* heads: of the queries */
+    DataType dt;       /* of q, k and v: DT_F32 or DT_F16 */
+    DataType q_out_dt; /* DT_F32 or DT_F16 */
+    const void *q, *k, *v;
+    void *q_out;
+    uint64_t q_stride, k_stride, v_stride, q_out_stride; /* elements from token to token */
+    const I32 *sequence, *position; /* [tokens] */
+    const I32 *table;               /* [sequences][table_pages] */
+    U32 sequences, table_pages;
+    U32 rotary_dim, interleaved, rotary_positions;
+    const F32 *cos, *sin; /* [rotary_positions][rotary_dim / 2] */
+} bolt_b200_kv_append_call;
+EE bolt_b200_kv_append(const bolt_b200_kv_cache *cache, const bolt_b200_kv_append_call *call);
+
+/* Attention of one token per sequence over the first length[i] tokens of the cache's sequence i (its own among them,
+ * appended before; the last `window` of them if window > 0): with query head h on key head h / (heads / kv_heads),
+ *   s_t = scale * q . k_t,  lse = log sum exp(s_t),  out = sum exp(s_t - lse) v_t.
+ * A sequence without tokens gets zeros and lse = -infinity.  What pages hold behind a sequence's end is never used,
+ * whatever it is.  out_dt: DT_F32, DT_F16, or, for a projection that follows, DT_U8_Q as by quantize_cuda_b200 with the
+ * scale out_scale: clamp(rne(x * out_scale + 128), 1, 255).
+ * Statistics and sums are binary32; queries and probabilities enter the products with 22 bits at least.
+ * tmp: the bytes asked for by _tmp_bytes, 16-byte aligned. */
+typedef struct {
+    U32 sequences, heads;
+    DataType q_dt;   /* DT_F32 or DT_F16 */
+    DataType out_dt; /* DT_F32, DT_F16 or DT_U8_Q */
+    const void *q;   /* row i at element i * q_stride, heads follow one another */
+    void *out;
+    F32 *lse;        /* [sequences][heads] or NULL */
+    uint64_t q_stride, out_stride;
+    const I32 *table;  /* [sequences][table_pages]; entries behind a sequence's last page are not read */
+    const I32 *length; /* [sequences] */
+    U32 table_pages, window;
+    F32 scale, out_scale;
+} bolt_b200_paged_attention_call;
+EE bolt_b200_paged_attention_tmp_bytes(
+    const bolt_b200_kv_cache *cache, const bolt_b200_paged_attention_call *call, U32 *bytes);
+EE bolt_b200_paged_attention(
+    const bolt_b200_kv_cache *cache, const bolt_b200_paged_attention_call *call, U32 tmpBytes, void *tmp);
+
+/* Low-rank adapters of many requests beside a shared projection (bolt_b200_gemm_u8s8_ex, mmm_cuda_b200), in place on its
+ * fp32 result: rows first_row[s] .. first_row[s + 1] - 1 belong to request s, whose adapter is adapter[s] (< 0: none):
+ *   y[m][n] += scale[adapter] * sum_r (sum_k x[m][k] * a[adapter][r][k]) * b[adapter][n][r]
+ * Rows in front of first_row[0] and behind the last segment stay as they are.  first_row must not fall and stay within
+ * [0, rows]: a segment that begins before an earlier bound or before 0, or ends before it begins or behind the rows, or
+ * whose adapter does not exist, is left out (and reported, see above).  rank: a multiple of 8 up to 128 (adapters of
+ * lower rank are filled up with zeros).  a, b: binary16, 16-byte aligned, a_stride (elements from row to row of a,
+ * >= K) a multiple of 8.  x: DT_F32, or DT_U8_Q = the product's own input, which stands for
+ * (byte - 128) / (row_scale[m], or *d_sA, or sA).  x and y rows may start anywhere.  Sums are binary32 (22 bits at least
+ * of x and of the inner sums enter the products).  x must not overlap y.  tmp: as for attention. */
+typedef struct {
+    U32 rows, N, K, rank, adapters, segments;
+    DataType x_dt; /* DT_F32 or DT_U8_Q */
+    const void *x;
+    F32 *y;
+    uint64_t x_stride, y_stride; /* elements from row to row */
+    const void *a;               /* [adapters][rank][a_stride] */
+    const void *b;               /* [adapters][N][rank] */
+    uint64_t a_stride;
+    const F32 *scale;     /* [adapters] or NULL: 1 */
+    const I32 *first_row; /* [segments + 1] */
+    const I32 *adapter;   /* [segments] */
+    F32 sA;
+    const F32 *d_sA, *row_scale;
+} bolt_b200_lora_call;
+EE bolt_b200_lora_tmp_bytes(const bolt_b200_lora_call *call, U32 *bytes);
+EE bolt_b200_lora(const bolt_b200_lora_call *call, U32 tmpBytes, void *tmp);
+
 /* ============================== 3. operators ================================================= */
 /* Bolt's public signatures (compute/blas_enhance/include/blas_enhance.h:21-88); arch must be
  * CUDA_B200, anything else returns NOT_SUPPORTED.  Argument checks follow mmm.cpp:161-197 and

@@ -1,0 +1,524 @@
+"""Cache append, paged attention and adapters against plain 64-bit computations, at the sizes and masks where they can go wrong.
+
+Tolerances (u = 2^-23, twice the unit roundoff of binary32, which also covers sums that truncate):
+  append     every step is one binary32 operation of defined order: equal bits.
+  attention  a score of dim products is off by at most (dim + 16) u sum |q_i k_i| scale (products, sums, 22-bit operands, the
+             multiplication with the scale); its exponential by that much relative, plus 8 u; the sum over n tokens adds
+             16 at a time: (n / 16 + 64) u sum p |v|.  Numerator and denominator together: twice that.  Exponentials below
+             2^-126, the smallest normal number, may count as nothing: n 2^-126 max |v|.
+  lora       inner sums: (K / 16 + 40) u sum |x a|; outer: (rank / 16 + 40) u sum |t b|; y itself: 2 u |y|.
+A result in binary16 is rounded once more (half of torch.finfo.eps, 2^-25 below the normal numbers), one in bytes by 1/2.
+"""
+import ctypes as C
+import math
+import os
+import sys
+
+import numpy as np
+import pytest
+import torch
+
+sys.path.insert(0, os.path.dirname(__file__))
+import bolt_b200 as B  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -23
+DT = {torch.float32: B.DT_F32, torch.float16: B.DT_F16, torch.int8: B.DT_I8, torch.uint8: B.DT_U8_Q}
+
+
+def rand(seed, *shape, dtype=torch.float32, scale=1.0):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return (scale * torch.randn(shape, device="cuda", generator=g)).to(dtype)
+
+
+def perm(seed, n):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return torch.randperm(n, device="cuda", generator=g)
+
+
+def ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def status():
+    torch.cuda.synchronize()
+    return B.lib().bolt_b200_device_status()
+
+
+class Cache:
+    """pages of finite noise; `poison`: what lies between rows and (later) behind the sequences"""
+
+    def __init__(self, seed, pages, page, heads, dim, i8, order="hnd", gap=0):
+        dt = torch.int8 if i8 else torch.float16
+        shape = (pages, heads, page, dim + gap) if order == "hnd" else (pages, page, heads, dim + gap)
+        make = (lambda s: torch.randint(-127, 128, shape, device="cuda", dtype=torch.int8)) if i8 else (lambda s: rand(s, *shape, dtype=dt))
+        torch.manual_seed(seed)
+        self.k_all, self.v_all = make(seed), make(seed + 1)
+        if gap and not i8:
+            self.k_all[..., dim:] = self.v_all[..., dim:] = math.nan
+        self.k, self.v = self.k_all[..., :dim], self.v_all[..., :dim]
+        self.i8, self.order, self.page, self.heads, self.dim, self.pages = i8, order, page, heads, dim, pages
+        self.ks = self.vs = None
+        if i8:
+            self.ks, self.vs = (20 + 100 * torch.rand((pages, heads, page), device="cuda") for _ in range(2))
+
+    def desc(self):
+        s = self.k.stride()
+        token, head = (s[2], s[1]) if self.order == "hnd" else (s[1], s[2])
+        return B.KvCache(B.DT_I8 if self.i8 else B.DT_F16, self.pages, self.page, self.heads, self.dim, s[0], token, head,
+                         ptr(self.k), ptr(self.v), ptr(self.ks), ptr(self.vs))
+
+    def rows(self, which, table_row, begin, end):
+        """[heads, tokens, dim] in 64 bits"""
+        t = torch.arange(begin, end, device="cuda")
+        page, at = table_row[t // self.page].long(), t % self.page
+        x, s = (self.k, self.ks) if which == "k" else (self.v, self.vs)
+        r = (x[page, :, at] if self.order == "hnd" else x[page, at]).double()
+        if self.i8:
+            r = r / s[page, :, at].double()[..., None]
+        return r.transpose(0, 1)
+
+
+# ---- append --------------------------------------------------------------------------------------------------------
+def turned(x, pos, cos, sin, rotary, interleaved):
+    """x [rows, heads, dim], numpy binary32 operations one by one"""
+    x = x.astype(np.float32)
+    if rotary == 0:
+        return x
+    c, s = cos[pos][:, None, :], sin[pos][:, None, :]
+    y = x.copy()
+    ia, ib = (np.arange(0, rotary, 2), np.arange(1, rotary, 2)) if interleaved else (np.arange(rotary // 2), np.arange(rotary // 2, rotary))
+    a, b = x[..., ia], x[..., ib]
+    y[..., ia], y[..., ib] = a * c - b * s, b * c + a * s
+    return y
+
+
+def quantized(rows):
+    top = np.abs(rows).max(-1)
+    with np.errstate(divide="ignore"):
+        s = np.where(top == 0, np.float32(1), np.float32(127) / top).astype(np.float32)
+    return np.clip(np.rint(rows * s[..., None]), -127, 127).astype(np.int8), s
+
+
+def append_case(tokens, heads, kv, dim, i8, page, order, dt, rotary, interleaved, gap=0, offset=0, in_place=False, with_seq=True, pad=True, q_out=None):
+    seqs, tp = 3, 6
+    cap = tp * page
+    tokens = min(tokens, seqs * cap)
+    cache = Cache(7, seqs * tp + 1, page, kv, dim, i8, order, gap)
+    table = perm(3, seqs * tp + 1)[: seqs * tp].int().view(seqs, tp).contiguous()
+    place = perm(5, seqs * cap)[:tokens]
+    if not with_seq:
+        tokens = min(tokens, seqs)
+        place = torch.arange(tokens, device="cuda") * cap + perm(6, cap)[:1]
+    seq, pos = (place // cap).int(), (place % cap).int()
+    if pad and tokens > 2:
+        pos[1] = -1
+    width = (heads + 2 * kv) * dim + offset
+    qkv = rand(11, tokens, width, dtype=dt)[:, offset:]
+    qkv[0, heads * dim: (heads + 1) * dim] = 0                      # a row of zeros has scale 1
+    width = qkv.stride(0)
+    cos, sin = (rand(s, cap, max(rotary // 2, 1)).contiguous() for s in (21, 22))
+    before_k, before_v = cache.k_all.clone(), cache.v_all.clone()
+    before_s = [x.clone() for x in (cache.ks, cache.vs)] if i8 else []
+    src = qkv.clone()
+    qo = qkv if in_place else torch.full((tokens, heads * dim), 9.0, dtype=q_out or dt, device="cuda")
+    p, e = qkv.data_ptr(), qkv.element_size()
+    call = B.KvAppend(tokens, heads, DT[dt], DT[qo.dtype], p, p + heads * dim * e, p + (heads + kv) * dim * e, qo.data_ptr(), width, width, width,
+                      qo.stride(0), seq.data_ptr() if with_seq else None, pos.data_ptr(), table.data_ptr(), seqs, tp, rotary, interleaved,
+                      cap if rotary else 0, ptr(cos) if rotary else None, ptr(sin) if rotary else None)
+    B.kv_append(cache.desc(), call)
+    assert status() == 0
+    # what it has to be
+    live = (pos >= 0).cpu().numpy()
+    ps, sq = pos.cpu().numpy(), seq.cpu().numpy()
+    x = src.cpu().numpy().reshape(tokens, heads + 2 * kv, dim)
+    y = turned(x, np.maximum(ps, 0), cos.cpu().numpy(), sin.cpu().numpy(), rotary, interleaved)
+    want_q = src.cpu().numpy()[:, : heads * dim].copy() if in_place else np.full((tokens, heads * dim), 9.0, np.float32)
+    want_q[live] = y[live, :heads].reshape(int(live.sum()), heads * dim)
+    got_q = qo.cpu()[:, : heads * dim]
+    assert torch.equal(got_q, torch.from_numpy(want_q).to(got_q.dtype))
+    if in_place:
+        assert torch.equal(qo.cpu()[:, heads * dim:], src.cpu()[:, heads * dim:])
+    tab = table.cpu().numpy()
+    page_i, at = tab[sq[live], ps[live] // page], ps[live] % page
+    for got, before, rows, scales, sb in ((cache.k_all, before_k, y[live, heads: heads + kv], cache.ks, before_s[:1]),
+                                          (cache.v_all, before_v, x[live, heads + kv:].astype(np.float32), cache.vs, before_s[1:])):
+        want, got = before.cpu().numpy().copy(), got.cpu().numpy()
+        if i8:
+            rows, s = quantized(rows)
+            ws = sb[0].cpu().numpy().copy()
+            ws[page_i, :, at] = s
+            assert ws.tobytes() == scales.cpu().numpy().tobytes()
+        if order == "hnd":
+            want[page_i, :, at, :dim] = rows
+        else:
+            want[page_i, at, :, :dim] = rows
+        assert want.tobytes() == got.tobytes()
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(1, 1, 16), (12, 12, 64), (8, 2, 128), (5, 1, 256), (4, 4, 80), (3, 3, 48), (0, 2, 192), (6, 2, 96)])
+@pytest.mark.parametrize("i8", [0, 1])
+@pytest.mark.parametrize("dt", [torch.float32, torch.float16])
+@pytest.mark.parametrize("order,page,tokens", [("hnd", 16, 40), ("nhd", 7, 100), ("hnd", 1, 5), ("nhd", 33, 1)])
+def test_append(heads, kv, dim, i8, dt, order, page, tokens):
+    for rotary, interleaved in ((dim, 0), (dim, 1), (0, 0), (dim // 2, 0)):
+        append_case(tokens, heads, kv, dim, i8, page, order, dt, rotary, interleaved)
+
+
+@pytest.mark.parametrize("i8", [0, 1])
+@pytest.mark.parametrize("interleaved", [0, 1])
+def test_append_off_the_grid(i8, interleaved):
+    """halves that are no multiple of four, rows at odd addresses, gaps between the cache's rows, queries in place and in another type"""
+    for rotary in (2, 6, 10, 36):
+        append_case(9, 4, 2, 48, i8, 5, "hnd", torch.float32, rotary, interleaved)
+    for offset in (1, 2, 3):
+        append_case(9, 4, 2, 64, i8, 5, "nhd", torch.float16, 64, interleaved, offset=offset)
+        append_case(9, 4, 2, 256, i8, 5, "hnd", torch.float32, 256, interleaved, offset=offset)
+    append_case(9, 4, 2, 64, i8, 5, "nhd", torch.float32, 32, interleaved, gap=16)
+    append_case(9, 4, 2, 128, i8, 5, "hnd", torch.float32, 128, interleaved, in_place=True)
+    append_case(9, 4, 2, 128, i8, 5, "hnd", torch.float16, 64, interleaved, in_place=True, offset=1)
+    append_case(9, 4, 2, 128, i8, 5, "hnd", torch.float32, 64, interleaved, q_out=torch.float16)
+    append_case(9, 4, 2, 128, i8, 5, "hnd", torch.float16, 64, interleaved, q_out=torch.float32)
+    append_case(3, 4, 2, 128, i8, 5, "hnd", torch.float16, 64, interleaved, with_seq=False, pad=False)
+
+
+def test_append_refuses_on_the_device_what_leads_outside():
+    """sequence, position, page and angle out of range: nothing is written for these tokens, the others are done"""
+    cache = Cache(1, 4, 8, 2, 64, 0)
+    table = torch.tensor([[0, 1], [2, 99], [-5, 3]], dtype=torch.int32, device="cuda")
+    #      good  sequence sequence position page -5   page 99  angle   good
+    seq = torch.tensor([0, 3, -1, 0, 2, 1, 0, 2], dtype=torch.int32, device="cuda")
+    pos = torch.tensor([3, 0, 0, 16, 1, 9, 15, 8], dtype=torch.int32, device="cuda")
+    kv = rand(1, 8, 4 * 64, dtype=torch.float16)
+    cos, sin = rand(2, 15, 32), rand(3, 15, 32)
+    before = cache.k.clone(), cache.v.clone()
+    q = torch.full((8, 64), 5.0, device="cuda", dtype=torch.float16)
+    call = B.KvAppend(8, 1, B.DT_F16, B.DT_F16, kv.data_ptr(), kv.data_ptr(), kv.data_ptr() + 256, q.data_ptr(), 256, 256, 256, 64, seq.data_ptr(),
+                      pos.data_ptr(), table.data_ptr(), 3, 2, 64, 0, 15, cos.data_ptr(), sin.data_ptr())
+    B.kv_append(cache.desc(), call)
+    assert B.lib().bolt_b200_synchronize() == B.UNKNOWN
+    changed = [(cache.k != before[0]).any(-1).any(1), (cache.v != before[1]).any(-1).any(1)]     # [page, token]
+    want = torch.zeros((4, 8), dtype=torch.bool, device="cuda")
+    want[0, 3] = want[3, 0] = True
+    assert torch.equal(changed[0], want) and torch.equal(changed[1], want)
+    assert ((q != 5).any(1)).tolist() == [True] + [False] * 6 + [True]
+    assert status() == 0
+
+
+# ---- attention ---------------------------------------------------------------------------------------------------
+def attend(cache, q, table, length, window=0, scale=None, out=torch.float32, out_scale=1.0, lse=True, q_stride=None, out_gap=0):
+    """one call; (out [sequences, heads, dim], lse)"""
+    b, h, d = q.shape
+    o_all = torch.full((b, h * d + out_gap), 77, dtype=out, device="cuda")
+    l = torch.full((b, h), 5.0, device="cuda") if lse else None
+    call = B.PagedAttention(b, h, DT[q.dtype], DT[out], q.data_ptr(), o_all.data_ptr(), ptr(l), q.stride(0), o_all.stride(0), table.data_ptr(),
+                            length.data_ptr(), table.shape[1], window, scale if scale is not None else d ** -0.5, out_scale)
+    n = B.paged_attention_tmp_bytes(cache.desc(), call)
+    tmp = torch.full((n + 64,), 0xA5, dtype=torch.uint8, device="cuda")
+    B.paged_attention(cache.desc(), call, n, tmp.data_ptr())
+    if out_gap:
+        assert bool((o_all[:, h * d:] == 77).all())
+    assert bool((tmp[n:] == 0xA5).all())
+    return o_all[:, : h * d].view(b, h, d) if not out_gap else o_all[:, : h * d].reshape(b, h, d), l
+
+
+def check_attention(cache, q, table, length, got, lse, window=0, scale=None, out_scale=None):
+    b, h, d = q.shape
+    scale = np.float32(scale if scale is not None else d ** -0.5).item()
+    group = h // cache.heads
+    for i, end in enumerate(length.tolist()):
+        begin = max(0, end - window) if window else 0
+        if end == 0:
+            want, tol = torch.zeros((h, d), device="cuda", dtype=torch.float64), torch.zeros((h, d), device="cuda", dtype=torch.float64)
+            if lse is not None:
+                assert bool((lse[i] == -math.inf).all())
+        else:
+            k, v = (cache.rows(x, table[i], begin, end).repeat_interleave(group, 0) for x in "kv")
+            qq = q[i].double()
+            s = torch.einsum("hd,htd->ht", qq, k) * scale
+            off = ((d + 16) * U * abs(scale) * torch.einsum("hd,htd->ht", qq.abs(), k.abs())).amax(-1)     # of a score
+            top = torch.logsumexp(s, -1)
+            p = torch.exp(s - top[:, None])
+            want = torch.einsum("ht,htd->hd", p, v)
+            n = end - begin
+            tol = 2 * (off[:, None] + (n / 16 + 72) * U) * torch.einsum("ht,htd->hd", p, v.abs()) + n * 2.0 ** -126 * v.abs().amax(1)
+            if lse is not None:
+                assert bool(((lse[i].double() - top).abs() <= off + (n / 16 + 72) * U + 2 * U * top.abs()).all()), (i, end)
+        g = got[i].double()
+        if got.dtype == torch.float16:
+            tol = tol + want.abs() * 2.0 ** -11 + 2.0 ** -25
+        if got.dtype == torch.uint8:
+            want, tol = (want * out_scale).clamp(-127, 127) + 128, tol * out_scale + 0.5
+        bad = ~((g - want).abs() <= tol * (1 + 1e-9))
+        n_bad = int(bad.sum())
+        assert n_bad == 0, (i, end, n_bad, float((g - want).abs()[bad].max()), float(tol[bad].min()))
+
+
+def batch(seed, lens, cache_args, heads, q_dt=torch.float32, q_scale=1.0, poison=True):
+    """cache, queries, table and lengths of a batch; what the pages hold behind a sequence is poison"""
+    page, kv, dim, i8, order, gap = cache_args
+    tp = max(1, max(-(-n // page) for n in lens))
+    need = [-(-n // page) for n in lens]
+    cache = Cache(seed, sum(need) + 1, page, kv, dim, i8, order, gap)
+    order_ = perm(seed, sum(need) + 1)
+    table = torch.full((len(lens), tp), -1, dtype=torch.int32, device="cuda")
+    at = 0
+    for i, n in enumerate(need):
+        table[i, :n] = order_[at: at + n].int()
+        at += n
+        if poison and lens[i] % page:
+            last, tail = int(table[i, n - 1]), lens[i] % page
+            for x in (cache.k, cache.v):
+                dst = x[last, :, tail:] if order == "hnd" else x[last, tail:]
+                dst.fill_(127 if i8 else math.nan)
+            if i8:
+                cache.ks[last, :, tail:] = 0.0
+                cache.vs[last, :, tail:] = math.nan
+    q = rand(seed + 9, len(lens), heads, dim, dtype=q_dt, scale=q_scale)
+    return cache, q, table, torch.tensor(lens, dtype=torch.int32, device="cuda")
+
+
+LENS = [0, 1, 2, 15, 16, 17, 31, 33, 64, 127, 128, 129, 255, 257, 300, 0, 513, 1025]
+
+
+@pytest.mark.parametrize("dim", [8, 16, 32, 48, 64, 80, 96, 112, 128, 144, 192, 256])
+@pytest.mark.parametrize("kv,group", [(1, 1), (2, 2), (1, 5), (3, 8), (2, 9), (1, 16), (1, 20), (1, 40)])
+@pytest.mark.parametrize("i8", [0, 1])
+def test_attention_heads(dim, kv, group, i8):
+    if i8 and dim % 16:
+        pytest.skip("rows of a cache of bytes are multiples of 16")
+    page, order = ((16, "hnd"), (5, "nhd"), (100, "hnd"))[(dim // 8 + group) % 3]
+    lens = LENS[(dim + group) % 5::2] + [700]
+    cache, q, table, length = batch(dim + group, lens, (page, kv, dim, i8, order, 0), kv * group, (torch.float32, torch.float16)[group % 2])
+    got, lse = attend(cache, q, table, length)
+    assert status() == 0
+    check_attention(cache, q, table, length, got, lse)
+
+
+@pytest.mark.parametrize("page", [1, 3, 16, 24, 64, 1000])
+@pytest.mark.parametrize("order,gap", [("hnd", 0), ("nhd", 0), ("nhd", 16)])
+@pytest.mark.parametrize("i8", [0, 1])
+@pytest.mark.parametrize("out", [torch.float32, torch.float16, torch.uint8])
+def test_attention_pages_and_outputs(page, order, gap, i8, out):
+    cache, q, table, length = batch(page, LENS + [2000], (page, 2, 64, i8, order, gap), 8)
+    for window in (0, 1, 20, 300, 5000):
+        got, lse = attend(cache, q, table, length, window=window, out=out, out_scale=100.0, lse=window != 20, out_gap=window % 3)
+        assert status() == 0
+        check_attention(cache, q, table, length, got, lse, window, out_scale=100.0)
+
+
+@pytest.mark.parametrize("i8", [0, 1])
+@pytest.mark.parametrize("lens", [[40000], [30000, 5, 1, 0, 17000], [257] * 70, [3] * 700, [0, 0, 0], [0], [1], [1025] * 149])
+def test_attention_splits(i8, lens):
+    """few long sequences, many short ones, none with a token"""
+    cache, q, table, length = batch(4, lens, (16, 2, 128, i8, "hnd", 0), 16)
+    got, lse = attend(cache, q, table, length)
+    again, _ = attend(cache, q, table, length)
+    assert status() == 0
+    check_attention(cache, q, table, length, got, lse)
+    assert torch.equal(got, again)          # no order of arrival in the result
+
+
+@pytest.mark.parametrize("i8", [0, 1])
+def test_attention_values(i8):
+    """peaked softmax, large and small queries, one value far above the rest, negative scales, equal scores"""
+    for q_scale, scale in ((1e-6, None), (30.0, None), (1e5, 1e-6), (1e-30, 1e29), (1.0, -0.5), (1.0, 0.0)):
+        cache, q, table, length = batch(8, [900, 1, 77], (16, 2, 64, i8, "hnd", 0), 8, q_scale=q_scale)
+        got, lse = attend(cache, q, table, length, scale=scale)
+        check_attention(cache, q, table, length, got, lse, scale=scale)
+    cache, q, table, length = batch(9, [900, 1, 77], (16, 2, 64, i8, "hnd", 0), 8)
+    if i8:
+        cache.vs *= torch.pow(10.0, -6 + 9 * torch.rand_like(cache.vs))       # rows of very different magnitude
+        cache.vs[int(table[0, 3]), :, 5] = 1e-3
+    else:
+        cache.v *= 1e-3
+        cache.v[int(table[0, 3]), :, 5] = 60000.0
+        cache.k[int(table[0, 0]), :, 0] = 200.0 * q[0, 0].sign().half()
+    got, lse = attend(cache, q, table, length)
+    check_attention(cache, q, table, length, got, lse)
+
+
+def test_attention_infinite_scores_only_lose_their_tokens():
+    """keys whose scores are -infinity weigh nothing, in a tile of their own and among others"""
+    cache, q, table, length = batch(3, [700], (16, 1, 64, 0, "hnd", 0), 4)
+    q = q.abs() + 0.1
+    for t in list(range(0, 300)) + [310, 699]:
+        cache.k[int(table[0, t // 16]), :, t % 16] = -math.inf
+    got, lse = attend(cache, q, table, length)
+    keep = torch.tensor([t for t in range(300, 699) if t != 310], device="cuda")
+    k, v = (cache.rows(x, table[0], 0, 700)[0][keep] for x in "kv")
+    s = q[0].double() @ k.T / 8
+    want = torch.softmax(s, -1) @ v
+    assert float((got[0].double() - want).abs().max()) < 1e-4 and bool(((lse[0] - torch.logsumexp(s, -1)).abs() < 1e-4).all())
+
+
+def test_attention_refuses_on_the_device_what_leads_outside():
+    """a page outside the cache is left out, a length beyond the table is cut, a negative one is none"""
+    cache, q, table, length = batch(2, [100, 100, 100, 64], (16, 2, 64, 0, "hnd", 0), 4)
+    good = table.clone()
+    table[0, 2], table[1, 0] = cache.pages, -7
+    length[2], length[3] = 1 << 30, -1
+    table[2] = table[0, 3]
+    got, _ = attend(cache, q, table, length)
+    assert B.lib().bolt_b200_synchronize() == B.UNKNOWN
+    for i, lost in ((0, range(32, 48)), (1, range(16))):
+        keep = torch.tensor([t for t in range(100) if t not in lost], device="cuda")
+        k, v = (cache.rows(x, good[i], 0, 100)[:, keep].repeat_interleave(2, 0) for x in "kv")
+        want = torch.softmax(torch.einsum("hd,htd->ht", q[i].double(), k) / 8, -1)
+        assert float((got[i].double() - torch.einsum("ht,htd->hd", want, v)).abs().max()) < 1e-4
+    assert bool((got[3] == 0).all())
+    attend(cache, q, good, torch.tensor([100, 100, 100, 64], dtype=torch.int32, device="cuda"))
+    length.fill_(10)
+    attend(cache, q, good, length)
+    assert status() == 0
+
+
+def test_attention_far_into_a_large_cache():
+    """rows behind 2^32 bytes and 2^31 elements"""
+    pages, page, kv, dim = 70000, 64, 4, 128                       # 2.3 G elements, 4.6 GB per cache
+    cache = Cache.__new__(Cache)
+    cache.k_all = cache.k = torch.empty((pages, kv, page, dim), dtype=torch.float16, device="cuda")
+    cache.v_all = cache.v = torch.empty((pages, kv, page, dim), dtype=torch.float16, device="cuda")
+    cache.i8, cache.order, cache.page, cache.heads, cache.dim, cache.pages, cache.ks, cache.vs = 0, "hnd", page, kv, dim, pages, None, None
+    table = torch.tensor([[pages - 1, 0, pages - 2, 65536]], dtype=torch.int32, device="cuda")
+    for x, s in ((cache.k, 1), (cache.v, 2)):
+        x[table[0].long()] = rand(s, 4, kv, page, dim, dtype=torch.float16)
+    row = rand(5, 1, 3 * kv * dim)
+    pos, zero = torch.tensor([63], dtype=torch.int32, device="cuda"), None
+    call = B.KvAppend(1, kv, B.DT_F32, B.DT_F32, row.data_ptr(), row.data_ptr() + 4 * kv * dim, row.data_ptr() + 8 * kv * dim, row.data_ptr(),
+                      3 * kv * dim, 3 * kv * dim, 3 * kv * dim, 3 * kv * dim, zero, pos.data_ptr(), table.data_ptr(), 1, 4, 0, 0, 0, None, None)
+    B.kv_append(cache.desc(), call)
+    assert torch.equal(cache.k[pages - 1, :, 63].reshape(-1), row[0, kv * dim: 2 * kv * dim].half())
+    q, length = rand(6, 1, 8, dim), torch.tensor([250], dtype=torch.int32, device="cuda")
+    got, lse = attend(cache, q, table, length)
+    check_attention(cache, q, table, length, got, lse)
+    assert status() == 0
+
+
+def test_attention_in_a_graph_follows_lengths_and_tables():
+    """captured once, replayed for other lengths; two graphs with a workspace each on two streams"""
+    works = []
+    for s in (1, 2):
+        cache, q, table, length = batch(s, [600, 900, 3], (16, 2, 128, s - 1, "hnd", 0), 8, poison=False)
+        out, lse = torch.empty_like(q), torch.empty(q.shape[:2], device="cuda")
+        call = B.PagedAttention(3, 8, B.DT_F32, B.DT_F32, q.data_ptr(), out.data_ptr(), lse.data_ptr(), q.stride(0), out.stride(0), table.data_ptr(),
+                                length.data_ptr(), table.shape[1], 0, 128 ** -0.5, 0.0)
+        n = B.paged_attention_tmp_bytes(cache.desc(), call)
+        tmp = torch.empty(n + 16, dtype=torch.uint8, device="cuda")
+        B.paged_attention(cache.desc(), call, n, tmp.data_ptr())
+        torch.cuda.synchronize()
+        stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            B.lib().bolt_b200_set_stream(C.c_void_p(torch.cuda.current_stream().cuda_stream))
+            B.paged_attention(cache.desc(), call, n, tmp.data_ptr())
+            B.lib().bolt_b200_set_stream(None)
+        works.append((cache, q, table, length, out, lse, stream, graph, tmp))
+    for lens in ([600, 900, 3], [1, 0, 3], [256, 17, 2], [0, 0, 0], [599, 900, 1]):
+        for w in works:
+            w[3].copy_(torch.tensor(lens, dtype=torch.int32))
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for w in works:
+                with torch.cuda.stream(w[6]):
+                    w[7].replay()
+        torch.cuda.synchronize()
+        for cache, q, table, length, out, lse, *_ in works:
+            check_attention(cache, q, table, length, out, lse)
+    assert status() == 0
+
+
+# ---- adapters ------------------------------------------------------------------------------------------------------
+def lora_case(rows, n, k, rank, bounds, adapters, x_dt, seed=1, which=None, scale=True, unit="row", x_gap=0, y_gap=0, x_off=0, y_off=0, a_gap=0, values=1.0):
+    seg = len(bounds) - 1
+    which = which or [i % adapters for i in range(seg)]
+    first, adapter = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in (bounds, which))
+    if x_dt == torch.uint8:
+        x_all = torch.randint(0, 256, (rows, k + x_gap + x_off), device="cuda", dtype=torch.uint8)
+    else:
+        x_all = rand(seed, rows, k + x_gap + x_off, scale=values)
+        x_all[:, :x_off] = x_all[:, x_off + k:] = math.nan
+    x = x_all[:, x_off: x_off + k]
+    y_all = rand(seed + 1, rows, n + y_gap + y_off)
+    y = y_all[:, y_off: y_off + n]
+    a_all = rand(seed + 2, adapters, rank, (k + 7) // 8 * 8 + a_gap, dtype=torch.float16, scale=k ** -0.5)
+    a_all[:, :, k:] = math.nan
+    b = rand(seed + 3, adapters, n, rank, dtype=torch.float16, scale=rank ** -0.5)
+    s = 0.5 + torch.rand(adapters, device="cuda") if scale else None
+    row_scale = 10 + 50 * torch.rand(rows, device="cuda") if unit == "row" else None
+    d_sA = torch.full((1,), 33.0, device="cuda") if unit == "device" else None
+    before = y_all.clone()
+    call = B.Lora(rows, n, k, rank, adapters, seg, DT[x_dt], x.data_ptr(), y.data_ptr(), x.stride(0), y.stride(0), a_all.data_ptr(), b.data_ptr(),
+                  a_all.shape[2], ptr(s), first.data_ptr(), adapter.data_ptr(), 21.0, ptr(d_sA), ptr(row_scale))
+    nb = B.lora_tmp_bytes(call)
+    tmp = torch.full((nb + 64,), 0xA5, dtype=torch.uint8, device="cuda")
+    B.lora(call, nb, tmp.data_ptr())
+    torch.cuda.synchronize()
+    assert bool((tmp[nb:] == 0xA5).all())
+    want, tol = before.double(), torch.zeros_like(before, dtype=torch.float64)
+    wy, ty = want[:, y_off: y_off + n], tol[:, y_off: y_off + n]
+    for i, ad in enumerate(which):
+        if ad < 0 or ad >= adapters or not max(0, *bounds[:i + 1]) <= bounds[i] <= bounds[i + 1] <= rows:
+            continue
+        r = slice(bounds[i], bounds[i + 1])
+        xx = x[r].double()
+        if x_dt == torch.uint8:
+            xx = (xx - 128) / (row_scale[r].double()[:, None] if unit == "row" else (33.0 if unit == "device" else 21.0))
+        aa, bb, ss = a_all[ad, :, :k].double(), b[ad].double(), float(s[ad]) if scale else 1.0
+        t, dt = xx @ aa.T, (k / 16 + 40) * U * (xx.abs() @ aa.abs().T)
+        add = ss * (t @ bb.T)
+        ty[r] = ss * (dt @ bb.abs().T + (rank / 16 + 40) * U * (t.abs() @ bb.abs().T)) + 2 * U * (wy[r].abs() + add.abs())
+        wy[r] += add
+    bad = ~((y_all.double() - want).abs() <= tol)
+    n_bad = int(bad.sum())
+    assert n_bad == 0, (rows, n, k, rank, n_bad, float((y_all.double() - want).abs()[bad].max()), float(tol[bad].min()))
+    return before, y_all
+
+
+@pytest.mark.parametrize("rank", [8, 16, 24, 32, 40, 64, 72, 128])
+@pytest.mark.parametrize("x_dt", [torch.float32, torch.uint8])
+@pytest.mark.parametrize("n,k", [(1, 8), (7, 33), (64, 64), (100, 515), (1001, 40), (768, 768), (130, 4100)])
+def test_lora_sizes(rank, x_dt, n, k):
+    lora_case(1, n, k, rank, [0, 1], 1, x_dt)
+    lora_case(70, n, k, rank, [0, 1, 1, 18, 34, 65], 3, x_dt)
+
+
+@pytest.mark.parametrize("x_dt", [torch.float32, torch.uint8])
+def test_lora_segments(x_dt):
+    """no rows, rows in front and behind, requests without an adapter, one adapter twice, many requests"""
+    for bounds, which in (([7, 7, 7], None), ([0, 10, 20], [-1, -1])):
+        before, after = lora_case(20, 48, 64, 16, bounds, 2, x_dt, which=which)
+        same = torch.equal(before, after)
+        assert same
+    lora_case(100, 200, 128, 16, [5, 40, 41, 60, 90], 3, x_dt, which=[2, -1, 0, 2])
+    lora_case(300, 96, 128, 8, list(range(301)), 7, x_dt)
+    lora_case(333, 200, 264, 32, [0] + sorted(int(i) for i in perm(4, 333)[:40]), 5, x_dt)
+    lora_case(1500, 300, 300, 16, [0, 1400], 1, x_dt)
+    assert status() == 0
+
+
+@pytest.mark.parametrize("x_dt", [torch.float32, torch.uint8])
+def test_lora_strides_and_units(x_dt):
+    for x_off in (0, 1, 2, 3, 4):
+        lora_case(37, 65, 120, 16, [0, 20, 37], 2, x_dt, x_off=x_off, x_gap=3, y_off=x_off % 3, y_gap=x_off, a_gap=8)
+    for unit in ("row", "device", "host"):
+        lora_case(37, 64, 128, 16, [0, 20, 37], 2, x_dt, unit=unit, scale=unit != "device")
+    for values in (1e-20, 1e-6, 1e6, 1e20):
+        lora_case(37, 64, 128, 16, [0, 20, 37], 2, torch.float32, values=values)
+
+
+def test_lora_refuses_on_the_device_what_leads_outside():
+    """segments that fall or leave the rows, adapters that do not exist: left out, the others are done"""
+    for bounds, which in (([0, 10, 41], [0, 1]), ([-1, 5, 20], [0, 1]), ([0, 10, 20], [0, 2]), ([0, 30, 20, 40], [0, 1, 1]), ([0, 10, 1 << 30], [1, 0])):
+        lora_case(40, 64, 64, 16, bounds, 2, torch.float32, which=which)
+        assert status() == 53
+    lora_case(40, 64, 64, 16, [0, 40], 2, torch.float32)
+    assert B.lib().bolt_b200_synchronize() == B.SUCCESS
+
+
+def test_lora_gives_the_same_bits_again():
+    for args in ((64, 1000, 2048, 16, list(range(65)), 64), (600, 700, 4096, 32, [0, 100, 590], 2)):
+        a, b = (lora_case(*args, torch.uint8 if args[3] == 16 else torch.float32, seed=3, scale=False, unit="host") for _ in range(2))
+        if args[3] == 32:                       # (bytes of x come from the generator's state)
+            assert torch.equal(a[1], b[1])
