@@ -100,7 +100,8 @@ struct WeightTwin {
 
 // kernel families whose dynamic shared-memory limit has to be raised above 48 KiB; the attribute
 // belongs to the device that is current when it is set, so it is remembered per device context
-enum KernelFamily { KF_GEMM = 0, KF_CONV, KF_CONV_HALF, KF_GEMV, KF_GEMV_ROW, KF_BNN, KF_GATHER, KF_MATMUL, KF_MATMUL_ROW, KF_PROBE, KF_COUNT };
+enum KernelFamily { KF_GEMM = 0, KF_CONV, KF_CONV_HALF, KF_GEMV, KF_GEMV_ROW, KF_BNN, KF_GATHER, KF_MATMUL, KF_MATMUL_ROW, KF_PROBE,
+    KF_ATTENTION, KF_COUNT = KF_ATTENTION + 12 };
 
 // A maximum that a kernel finds and the host waits for.  Device words {running maximum, finished blocks}, both zero
 // between uses (the last block rewinds them); it then stores sequence number and maximum, as one 8-byte word, into

@@ -37,6 +37,30 @@ __host__ __device__ inline uint64_t scale_element(const CacheView &c, uint32_t p
     return ((uint64_t)page * c.kv_heads + head) * c.page_size + at;
 }
 
+// [begin, end) of a sequence's tokens: the last `window` (if any) of those that its table has room for.  False: the length is none.
+__host__ __device__ inline bool live_tokens(int32_t length, uint32_t table_pages, uint32_t page_size, uint32_t window, uint32_t *begin, uint32_t *end)
+{
+    const uint64_t room = (uint64_t)table_pages * page_size;
+    const bool good = length >= 0 && (uint64_t)length <= room;
+    *end = good ? (uint32_t)length : (length < 0 ? 0u : (uint32_t)room);
+    *begin = window != 0 && *end > window ? *end - window : 0;
+    return good;
+}
+// Work that stands in a row, cut into `parts` contiguous parts of equal length.
+__host__ __device__ inline uint64_t part_begin(uint64_t i, uint64_t total, uint32_t parts)
+{
+    return i * total / parts;
+}
+// the part that holds a place
+__host__ __device__ inline uint32_t part_of(uint64_t place, uint64_t total, uint32_t parts)
+{
+    return (uint32_t)(((place + 1) * parts + total - 1) / total) - 1;
+}
+__host__ __device__ inline uint32_t tiles_of(uint32_t begin, uint32_t end, uint32_t tile_tokens)
+{
+    return end <= begin ? 0 : (end - 1) / tile_tokens - begin / tile_tokens + 1;
+}
+
 inline bool aligned(const void *p, size_t n)
 {
     return reinterpret_cast<uintptr_t>(p) % n == 0;

@@ -533,8 +533,9 @@ EE bolt_b200_kv_append(const bolt_b200_kv_cache *cache, const bolt_b200_kv_appen
  * appended before; the last `window` of them if window > 0): with query head h on key head h / (heads / kv_heads),
  *   s_t = scale * q . k_t,  lse = log sum exp(s_t),  out = sum exp(s_t - lse) v_t.
  * A sequence without tokens gets zeros and lse = -infinity.  What pages hold behind a sequence's end is never used,
- * whatever it is.  out_dt: DT_F32, DT_F16, or, for a projection that follows, DT_U8_Q as by quantize_cuda_b200 with the
- * scale out_scale: clamp(rne(x * out_scale + 128), 1, 255).
+ * whatever it is; rows of live tokens have to be finite (one that is not spoils its own sequence and key head only).
+ * out_dt: DT_F32, DT_F16, or, for a projection that follows, DT_U8_Q as by quantize_cuda_b200 with the scale out_scale:
+ * clamp(rne(x * out_scale + 128), 1, 255).
  * Statistics and sums are binary32; queries and probabilities enter the products with 22 bits at least.
  * tmp: the bytes asked for by _tmp_bytes, 16-byte aligned. */
 typedef struct {

@@ -22,4 +22,21 @@ long long harness_scale(uint32_t pages, uint32_t page_size, uint32_t kv_heads, u
     return (long long)scale_element(c, page, at, head);
 }
 
+int harness_tokens(int32_t length, uint32_t table_pages, uint32_t page_size, uint32_t window, uint32_t *range)
+{
+    return live_tokens(length, table_pages, page_size, window, range, range + 1);
+}
+unsigned long long harness_part_begin(unsigned long long i, unsigned long long total, uint32_t parts)
+{
+    return part_begin(i, total, parts);
+}
+uint32_t harness_part_of(unsigned long long place, unsigned long long total, uint32_t parts)
+{
+    return part_of(place, total, parts);
+}
+uint32_t harness_tiles(uint32_t begin, uint32_t end, uint32_t tile)
+{
+    return tiles_of(begin, end, tile);
+}
+
 }  // extern "C"

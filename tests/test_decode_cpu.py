@@ -29,6 +29,10 @@ def harness(tmp_path_factory):
     u, l = C.c_uint32, C.c_uint64
     lib.harness_row.argtypes = [C.c_void_p, l, u, u, u, u, u, l, l, l, u, u, u]
     lib.harness_scale.argtypes = [u] * 6
+    lib.harness_tokens.argtypes = [C.c_int32, u, u, u, C.c_void_p]
+    lib.harness_part_begin.argtypes, lib.harness_part_begin.restype = [l, l, u], l
+    lib.harness_part_of.argtypes, lib.harness_part_of.restype = [l, l, u], u
+    lib.harness_tiles.argtypes, lib.harness_tiles.restype = [u, u, u], u
     return lib
 
 
@@ -54,6 +58,30 @@ def test_rows_of_a_cache(harness):
     assert harness.harness_row(t.ctypes.data, 0, 1, (1 << 31) - 1, 64, 8, 256, 1 << 17, 256, 1 << 14, 0, 0, 2) == -1
     assert harness.harness_row(t.ctypes.data, 0, 1, 1 << 31, 64, 8, 256, 1 << 17, 256, 1 << 14, 63, 7, 2) == 2 * (((1 << 31) - 1) * (1 << 17) + 63 * 256 + (7 << 14))
     assert harness.harness_scale(1 << 31, 64, 8, (1 << 31) - 1, 63, 7) == (((1 << 31) - 1) * 8 + 7) * 64 + 63
+
+
+def test_tokens_of_a_sequence(harness):
+    r = (C.c_uint32 * 2)()
+    for length, pages, page, window, good, begin, end in (
+            (0, 3, 16, 0, 1, 0, 0), (48, 3, 16, 0, 1, 0, 48), (49, 3, 16, 0, 0, 0, 48), (-1, 3, 16, 5, 0, 0, 0), (40, 3, 16, 5, 1, 35, 40), (4, 3, 16, 5, 1, 0, 4),
+            (5, 3, 16, 5, 1, 0, 5), (0x7FFFFFFF, 1 << 20, 1 << 20, 7, 1, 0x7FFFFFF8, 0x7FFFFFFF), (-2147483648, 1, 1, 0, 0, 0, 0), (0x7FFFFFFF, 2, 1, 1, 0, 1, 2)):
+        assert harness.harness_tokens(length, pages, page, window, r) == good and list(r) == [begin, end]
+
+
+def test_parts_cover_the_row_once(harness):
+    """every place of the row is in one part, the parts differ by one place at most, and a part is found from a place"""
+    for total in (1, 2, 3, 147, 148, 149, 1000, 12345, (1 << 40) + 7):
+        for parts in (1, 2, 147, 148):
+            borders = [harness.harness_part_begin(i, total, parts) for i in range(parts + 1)]
+            assert borders[0] == 0 and borders[-1] == total
+            sizes = {b - a for a, b in zip(borders, borders[1:])}
+            assert min(sizes) >= 0 and max(sizes) - min(sizes) <= 1
+            for place in sorted({0, total - 1, total // 2, *[b for b in borders[:-1] if b < total], *[b - 1 for b in borders if b]}):
+                i = harness.harness_part_of(place, total, parts)
+                assert borders[i] <= place < borders[i + 1], (total, parts, place, i)
+    for begin, end, tile, n in ((0, 0, 128, 0), (5, 5, 128, 0), (0, 1, 128, 1), (0, 128, 128, 1), (0, 129, 128, 2), (127, 129, 128, 2), (128, 129, 128, 1),
+                                (130, 700, 128, 5), (0, 0x7FFFFFFF, 256, 1 << 23)):
+        assert harness.harness_tiles(begin, end, tile) == n
 
 
 def cache(**kw):

@@ -340,18 +340,20 @@ def test_attention_values(i8):
     check_attention(cache, q, table, length, got, lse)
 
 
-def test_attention_infinite_scores_only_lose_their_tokens():
-    """keys whose scores are -infinity weigh nothing, in a tile of their own and among others"""
-    cache, q, table, length = batch(3, [700], (16, 1, 64, 0, "hnd", 0), 4)
-    q = q.abs() + 0.1
-    for t in list(range(0, 300)) + [310, 699]:
-        cache.k[int(table[0, t // 16]), :, t % 16] = -math.inf
-    got, lse = attend(cache, q, table, length)
-    keep = torch.tensor([t for t in range(300, 699) if t != 310], device="cuda")
-    k, v = (cache.rows(x, table[0], 0, 700)[0][keep] for x in "kv")
-    s = q[0].double() @ k.T / 8
-    want = torch.softmax(s, -1) @ v
-    assert float((got[0].double() - want).abs().max()) < 1e-4 and bool(((lse[0] - torch.logsumexp(s, -1)).abs() < 1e-4).all())
+@pytest.mark.parametrize("group", [2, 12])
+def test_attention_rows_that_are_not_finite_stay_with_their_sequence(group):
+    """live rows have to be finite; where one is not, the other sequences and key heads are as they would be"""
+    for bad in (math.nan, math.inf, -math.inf):
+        cache, q, table, length = batch(3, [700, 90, 300, 900], (16, 2, 64, 0, "hnd", 0), 2 * group)
+        cache.k[int(table[1, 2]), 0, 5] = bad
+        cache.v[int(table[3, 20]), 1, 7] = bad
+        got, lse = attend(cache, q, table, length)
+        cache.k[int(table[1, 2]), 0, 5] = 0
+        cache.v[int(table[3, 20]), 1, 7] = 0
+        clean, clean_lse = attend(cache, q, table, length)
+        got[1, :group], lse[1, :group], got[3, group:] = clean[1, :group], clean_lse[1, :group], clean[3, group:]
+        same = torch.equal(got, clean), torch.equal(lse, clean_lse)
+        assert same == (True, True)
 
 
 def test_attention_refuses_on_the_device_what_leads_outside():
