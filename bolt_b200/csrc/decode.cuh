@@ -49,7 +49,8 @@ __host__ __device__ inline bool live_tokens(int32_t length, uint32_t table_pages
 // Work that stands in a row, cut into `parts` contiguous parts of equal length.
 __host__ __device__ inline uint64_t part_begin(uint64_t i, uint64_t total, uint32_t parts)
 {
-    return i * total / parts;
+    const uint64_t x = i * total;   // (a 64-bit division takes ten times as long as a 32-bit one)
+    return x >> 32 == 0 ? (uint32_t)x / parts : x / parts;
 }
 // the part that holds a place
 __host__ __device__ inline uint32_t part_of(uint64_t place, uint64_t total, uint32_t parts)

@@ -10,6 +10,8 @@
 // The products run on mma.m16n8k16: eight query heads that share a key head are half a tile's rows, and the other half
 // holds what binary16 has cut off of them, so that one instruction per operand tile multiplies 22-bit queries (and
 // probabilities) with the cache's binary16; bytes become binary16 in registers, two instructions for two of them.
+#include <type_traits>
+
 #include "decode.cuh"
 
 namespace b200 {
@@ -137,6 +139,10 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void *src, uint32_t b
 {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void copy4(uint32_t dst, const void *src, uint32_t bytes)
 {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -161,6 +167,12 @@ __device__ __forceinline__ float exp2_fast(float x)
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float reciprocal(float x)    // within 2^-23
+{
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 // Bytes 0 and 2 (shift 0) or 1 and 3 (shift 8) of a word, as signed numbers, in binary16: 0x6400 is 1024, whose last ten bits
 // count ones, so 0x6400 | (byte ^ 0x80) is 1152 + byte.
 template <int SHIFT>
@@ -179,7 +191,7 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t &hi, uint3
     lo = half2_bits(x - f.x, y - f.y);
 }
 
-constexpr int WARPS = 8;
+constexpr int WARPS = 8, MAX_PARTS = 256;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 // DP: elements of a row, rounded up; HB: blocks of eight query heads
@@ -187,6 +199,7 @@ template <int DP, bool I8, int HB>
 struct Shape {
     static constexpr int SIZE = I8 ? 1 : 2, ROW = DP * SIZE, PITCH = ROW + 16;   // an odd number of 16-byte pieces: ldmatrix meets every bank once
     static constexpr int STEP = ROW <= 128 ? 32 : 16;                            // tokens that a warp takes at a time
+    static constexpr uint32_t ALL = STEP == 32 ? 0xFFFFFFFFu : 0xFFFFu;
     static constexpr int SLOT = STEP * PITCH + (I8 ? STEP * 4 : 0);
     static constexpr int HEADS = 8 * HB, COLS = 64 / HB;
     static constexpr int Q_PITCH = DP * 2 + 16, Q_BYTES = 2 * HEADS * Q_PITCH;
@@ -277,11 +290,13 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_attention_kernel(const __
     ld.mask = 0;
     ld.row = ld.scale_row = 0;
     enter();
-    uint32_t issued = 0;    // items: K, V, K, V ...
-    auto issue = [&]() {
-        const bool values = issued & 1;
-        const uint32_t slot = issued % S::SLOTS;
-        ++issued;
+    uint32_t fill_slot = 0;    // items: K, V, K, V ...
+    const uint32_t copy_row = lane / (S::ROW / 16), copy_piece = lane % (S::ROW / 16);   // of the first piece that the lane copies
+    const uint64_t token_bytes = p.cache.token_stride * S::SIZE, lane_bytes = copy_row * token_bytes + copy_piece * 16;
+    const uint32_t ring_at = smem_at(ring), lane_at = ring_at + copy_row * S::PITCH + copy_piece * 16;
+    auto issue = [&](bool values) {
+        const uint32_t slot = fill_slot;
+        fill_slot = fill_slot + 1 == S::SLOTS ? 0 : fill_slot + 1;
         if (!values) {
             ld.mask = 0;
             if (ld.left != 0) {
@@ -322,38 +337,31 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_attention_kernel(const __
             }
         }
         if (ld.mask != 0) {
-            constexpr uint32_t ACROSS = S::ROW / 16, ROWS = 32 / ACROSS;      // pieces of a row, rows of one instruction
-            const uint32_t r0 = lane / ACROSS, piece = lane % ACROSS;
+            constexpr int ROWS = 32 / (S::ROW / 16);      // rows of one instruction
             const char *base = reinterpret_cast<const char *>(values ? p.v : p.k);
-            uint32_t dst = smem_at(ring + slot * S::SLOT + r0 * S::PITCH + piece * 16);
-            if (one_page) {
-                const uint64_t stride = p.cache.token_stride * S::SIZE;
-                const char *src = base + ld.row * S::SIZE + r0 * stride + piece * 16;
+            uint32_t dst = lane_at + slot * S::SLOT;
+            if (one_page && dim == DP && ld.mask == S::ALL) {
+                const char *src = base + ld.row * S::SIZE + lane_bytes;
 #pragma unroll
-                for (int i = 0; i < S::STEP / (int)ROWS; ++i) {
-                    if (piece < pieces) {
-                        const bool on = ld.mask >> (r0 + i * ROWS) & 1;
-                        copy16(dst, on ? src : base, on ? 16 : 0);
-                    }
-                    src += ROWS * stride;
-                    dst += ROWS * S::PITCH;
+                for (int i = 0; i < S::STEP / ROWS; ++i) {
+                    copy16(dst + i * ROWS * S::PITCH, src);
+                    src += ROWS * token_bytes;
                 }
             } else {
-#pragma unroll
-                for (int i = 0; i < S::STEP / (int)ROWS; ++i) {
-                    const uint32_t r = r0 + i * ROWS;
-                    const uint64_t row = __shfl_sync(0xFFFFFFFFu, ld.row, r);
-                    if (piece < pieces) {
+#pragma unroll 1
+                for (int i = 0; i < S::STEP / ROWS; ++i) {
+                    const uint32_t r = copy_row + i * ROWS;
+                    const uint64_t row = one_page ? ld.row + r * p.cache.token_stride : __shfl_sync(0xFFFFFFFFu, ld.row, r);
+                    if (copy_piece < pieces) {
                         const bool on = ld.mask >> r & 1;
-                        copy16(dst, on ? base + row * S::SIZE + piece * 16 : base, on ? 16 : 0);
+                        copy16(dst + i * ROWS * S::PITCH, on ? base + row * S::SIZE + copy_piece * 16 : base, on ? 16 : 0);
                     }
-                    dst += ROWS * S::PITCH;
                 }
             }
             if (I8 && lane < S::STEP) {
                 const float *s = values ? p.v_scale : p.k_scale;
                 const bool on = ld.mask >> lane & 1;
-                copy4(smem_at(ring + slot * S::SLOT + S::STEP * S::PITCH + lane * 4), on ? s + ld.scale_row : s, on ? 4 : 0);
+                copy4(ring_at + slot * S::SLOT + S::STEP * S::PITCH + lane * 4, on ? s + ld.scale_row : s, on ? 4 : 0);
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -361,16 +369,16 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_attention_kernel(const __
     __syncwarp();
 #pragma unroll 1
     for (int i = 0; i < S::SLOTS - 1; ++i) {
-        issue();
+        issue(i & 1);
     }
-    uint32_t taken = 0;
+    uint32_t take_slot = 0;
     // the next item is there; the slot of the one before it is filled again
-    auto next = [&]() {
+    auto next = [&](bool values) {
         asm volatile("cp.async.wait_group %0;" ::"n"(S::SLOTS - 2) : "memory");
         __syncwarp();
-        issue();
-        const uint32_t slot = taken % S::SLOTS;
-        ++taken;
+        issue(values != (S::SLOTS % 2 == 0));    // item n + SLOTS - 1
+        const uint32_t slot = take_slot;
+        take_slot = take_slot + 1 == S::SLOTS ? 0 : take_slot + 1;
         return slot;
     };
 
@@ -439,7 +447,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_attention_kernel(const __
 #pragma unroll 1
         for (uint32_t i = 0; i < count; ++i) {
             // scores: [heads] x [tokens]
-            const uint32_t ks = next();
+            const uint32_t ks = next(false);
             const char *const kt = ring + ks * S::SLOT;
             const uint32_t mask = masks[warp * S::SLOTS + ks];
             float sc[NT][4];
@@ -492,21 +500,22 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_attention_kernel(const __
             }
             // weights: exp(s - m) times 2^14, which the division by their sum takes back
             float keep[HB], w[HB][NT][2];
+            auto weights = [&](auto all) {
 #pragma unroll
-            for (int b = 0; b < HB; ++b) {
+              for (int b = 0; b < HB; ++b) {
                 float top = m[b];
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
                     float unit_k[2] = {1.f, 1.f};
                     if constexpr (I8) {
                         const float2 u = *reinterpret_cast<const float2 *>(kt + S::STEP * S::PITCH + (8 * j + 2 * c4) * 4);
-                        unit_k[0] = __frcp_rn(u.x);
-                        unit_k[1] = __frcp_rn(u.y);
+                        unit_k[0] = reciprocal(u.x);
+                        unit_k[1] = reciprocal(u.y);
                     }
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const float s = HB == 1 ? sc[j][e] + sc[j][e + 2] : sc[j][e + 2 * b];
-                        const bool on = mask >> (8 * j + 2 * c4 + e) & 1;
+                        const bool on = all.value || (mask >> (8 * j + 2 * c4 + e) & 1);
                         w[b][j][e] = on ? s * (fac[b] * unit_k[e]) : -INFINITY;
                         top = fmaxf(top, w[b][j][e]);
                     }
@@ -525,8 +534,14 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_attention_kernel(const __
                         l[b] += w[b][j][e];
                     }
                 }
+              }
+            };
+            if (mask == S::ALL) {
+                weights(std::true_type());
+            } else {
+                weights(std::false_type());
             }
-            const uint32_t vs = next();
+            const uint32_t vs = next(true);
             if (mask == 0) {
                 continue;
             }
@@ -538,13 +553,13 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_attention_kernel(const __
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
                     const float2 u = *reinterpret_cast<const float2 *>(vt + S::STEP * S::PITCH + (8 * j + 2 * c4) * 4);
-                    unit_v[j][0] = mask >> (8 * j + 2 * c4) & 1 ? __frcp_rn(u.x) : 0.f;
-                    unit_v[j][1] = mask >> (8 * j + 2 * c4 + 1) & 1 ? __frcp_rn(u.y) : 0.f;
+                    unit_v[j][0] = mask >> (8 * j + 2 * c4) & 1 ? reciprocal(u.x) : 0.f;
+                    unit_v[j][1] = mask >> (8 * j + 2 * c4 + 1) & 1 ? reciprocal(u.y) : 0.f;
                     top = fmaxf(top, fmaxf(unit_v[j][0], unit_v[j][1]));
                 }
                 top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-                const float inv = top > 0.f ? __frcp_rn(top) : 0.f, change = top_unit * inv;
+                const float inv = top > 0.f ? reciprocal(top) : 0.f, change = top_unit * inv;
                 top_unit = top;
 #pragma unroll
                 for (int b = 0; b < HB; ++b) {
@@ -707,6 +722,7 @@ __global__ void __launch_bounds__(128) paged_attention_join_kernel(const __grid_
     constexpr int HEADS = 8 * HB, PART = HEADS * (DP + 2);
     __shared__ uint64_t sums[32];
     __shared__ Found found[1];
+    __shared__ float weight[MAX_PARTS], share[MAX_PARTS], warp_top[4];
     const uint32_t i = blockIdx.x, units = p.cache.kv_heads * p.head_blocks, h = blockIdx.y;
     // sequences without a token, which no part holds: every parts-th is this block column's
     for (uint32_t s0 = 0; s0 < p.sequences; s0 += 32 * parts) {
@@ -750,29 +766,42 @@ __global__ void __launch_bounds__(128) paged_attention_join_kernel(const __grid_
     if (a < from || a + tiles <= stop || block * HEADS + h >= p.group) {
         return;    // cut before, or not here
     }
-    const uint32_t last = part_of(a + tiles - 1, total, parts);
+    const uint32_t n = part_of(a + tiles - 1, total, parts) - i + 1;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    auto part = [&](uint32_t c) { return p.parts + ((uint64_t)c * 2 + (c == i ? 1 : 0)) * PART; };
-    auto empty = [&](uint32_t c) { return part_begin(c, total, parts) == part_begin(c + 1, total, parts); };
-    float top = -INFINITY, all = 0.f;
-    for (uint32_t c = i; c <= last; ++c) {
-        top = empty(c) ? top : fmaxf(top, part(c)[HEADS * DP + h]);
+    // part c of the unit is a share of CTA i + c: what it began (slot 1) in the first, what it went on with in the others
+    auto part = [&](uint32_t c) { return p.parts + ((uint64_t)(i + c) * 2 + (c == 0 ? 1 : 0)) * PART; };
+    float top = -INFINITY;
+    for (uint32_t c = threadIdx.x; c < n; c += 128) {
+        // (with fewer tiles than CTAs, some have none)
+        const bool empty = total < parts && part_begin(i + c, total, parts) == part_begin(i + c + 1, total, parts);
+        weight[c] = empty ? -INFINITY : part(c)[HEADS * DP + h];
+        share[c] = empty ? 0.f : part(c)[HEADS * (DP + 1) + h];
+        top = fmaxf(top, weight[c]);
     }
-    const float base = top == -INFINITY ? 0.f : top;
-    float sum[(DP + 127) / 128] = {};
-    for (uint32_t c = i; c <= last; ++c) {
-        if (empty(c)) {
-            continue;
-        }
-        const float *q = part(c);
-        const float w = exp2_fast(q[HEADS * DP + h] - base);
-        all = fmaf(q[HEADS * (DP + 1) + h], w, all);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    }
+    if (threadIdx.x % 32 == 0) {
+        warp_top[threadIdx.x / 32] = top;
+    }
+    __syncthreads();
+    top = fmaxf(fmaxf(warp_top[0], warp_top[1]), fmaxf(warp_top[2], warp_top[3]));
+    for (uint32_t c = threadIdx.x; c < n; c += 128) {
+        weight[c] = exp2_fast(weight[c] - (top == -INFINITY ? 0.f : top));
+    }
+    __syncthreads();
+    float all = 0.f, sum[(DP + 127) / 128] = {};
+#pragma unroll 8
+    for (uint32_t c = 0; c < n; ++c) {
+        const float *q = part(c) + h * DP;
+        const float w = weight[c];
+        all = fmaf(share[c], w, all);
 #pragma unroll
         for (int k = 0; k < (DP + 127) / 128; ++k) {
             const uint32_t d = threadIdx.x + 128 * k;
-            if (d < DP) {
-                sum[k] = fmaf(q[h * DP + d], w, sum[k]);
-            }
+            const float x = d < DP && w != 0.f ? q[d] : 0.f;
+            sum[k] = fmaf(x, w, sum[k]);
         }
     }
     const uint32_t hq = head * p.group + block * HEADS + h;
@@ -788,13 +817,17 @@ __global__ void __launch_bounds__(128) paged_attention_join_kernel(const __grid_
     }
 }
 
+uint32_t parts_of(const DeviceCtx *c)
+{
+    return c->sm_count < MAX_PARTS ? (uint32_t)c->sm_count : MAX_PARTS;
+}
 template <int DP, bool I8, int HB>
 EE launch(DeviceCtx *c, AttentionParams &p, cudaStream_t st)
 {
     using S = Shape<DP, I8, HB>;
     const void *kernel = reinterpret_cast<const void *>(paged_attention_kernel<DP, I8, HB>);
     B200_EE(raise_smem_limit(c, (KernelFamily)(KF_ATTENTION + (DP == 64 ? 0 : (DP == 128 ? 1 : 2)) + 3 * I8 + 6 * (HB - 1)), &kernel, 1, S::SMEM));
-    const uint32_t parts = (uint32_t)c->sm_count;
+    const uint32_t parts = parts_of(c);
     B200_EE(launch_kernel(parts, 32 * WARPS, S::SMEM, st, paged_attention_kernel<DP, I8, HB>, p));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(parts, S::HEADS < (int)p.group ? S::HEADS : p.group);
@@ -868,7 +901,7 @@ EE check(const bolt_b200_kv_cache *cache, const bolt_b200_paged_attention_call *
 U32 workspace_bytes(const AttentionParams &p, const DeviceCtx *c)
 {
     const U32 dp = p.cache.dim <= 64 ? 64 : (p.cache.dim <= 128 ? 128 : 256);
-    return (U32)c->sm_count * 2 * (p.group <= 8 ? 8 : 16) * (dp + 2) * 4;
+    return parts_of(c) * 2 * (p.group <= 8 ? 8 : 16) * (dp + 2) * 4;
 }
 
 }  // namespace
