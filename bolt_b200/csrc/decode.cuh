@@ -46,17 +46,29 @@ __host__ __device__ inline bool live_tokens(int32_t length, uint32_t table_pages
     *begin = window != 0 && *end > window ? *end - window : 0;
     return good;
 }
-// Work that stands in a row, cut into `parts` contiguous parts of equal length.
-__host__ __device__ inline uint64_t part_begin(uint64_t i, uint64_t total, uint32_t parts)
-{
-    const uint64_t x = i * total;   // (a 64-bit division takes ten times as long as a 32-bit one)
-    return x >> 32 == 0 ? (uint32_t)x / parts : x / parts;
-}
-// the part that holds a place
-__host__ __device__ inline uint32_t part_of(uint64_t place, uint64_t total, uint32_t parts)
-{
-    return (uint32_t)(((place + 1) * parts + total - 1) / total) - 1;
-}
+// Work that stands in a row, cut into n contiguous parts, none empty, of equal length but for one.
+struct Parts {
+    uint64_t each;
+    uint32_t longer, n;   // the first `longer` parts have each + 1
+    __host__ __device__ Parts(uint64_t total, uint32_t most)
+    {
+        n = total < most ? (uint32_t)total : most;
+        // (a 64-bit division takes ten times as long as a 32-bit one)
+        each = n == 0 ? 0 : (total >> 32 == 0 ? (uint32_t)total / n : total / n);
+        longer = (uint32_t)(total - each * n);
+    }
+    __host__ __device__ uint64_t begin(uint32_t i) const
+    {
+        return i * each + (i < longer ? i : longer);
+    }
+    // the part that holds a place
+    __host__ __device__ uint32_t of(uint64_t place) const
+    {
+        const uint64_t border = (each + 1) * longer, d = place < border ? each + 1 : each, x = place < border ? place : place - border;
+        const uint64_t i = (x | d) >> 32 == 0 ? (uint32_t)x / (uint32_t)d : x / d;
+        return (uint32_t)i + (place < border ? 0 : longer);
+    }
+};
 __host__ __device__ inline uint32_t tiles_of(uint32_t begin, uint32_t end, uint32_t tile_tokens)
 {
     return end <= begin ? 0 : (end - 1) / tile_tokens - begin / tile_tokens + 1;
@@ -108,6 +120,18 @@ __device__ __forceinline__ void load4(const __half *p, float (&x)[4])
     x[1] = a.y;
     x[2] = b.x;
     x[3] = b.y;
+}
+__device__ __forceinline__ void load2(const float *p, float &x, float &y)
+{
+    const float2 v = *reinterpret_cast<const float2 *>(p);
+    x = v.x;
+    y = v.y;
+}
+__device__ __forceinline__ void load2(const __half *p, float &x, float &y)
+{
+    const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(p));
+    x = v.x;
+    y = v.y;
 }
 __device__ __forceinline__ float load1(const float *p)
 {

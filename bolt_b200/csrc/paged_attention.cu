@@ -17,6 +17,11 @@
 namespace b200 {
 namespace {
 
+// a unit that a part has begun and others have gone on with
+struct Cut {
+    uint32_t parts;            // how many, 0: none
+    uint32_t sequence, head0, heads;   // query heads
+};
 struct AttentionParams {
     CacheView cache;
     const void *k, *v;
@@ -29,7 +34,9 @@ struct AttentionParams {
     uint32_t sequences, heads, group, head_blocks, table_pages, window;
     float scale, out_scale;
     int i8, q_f16, out_kind;   // 0 binary32, 1 binary16, 2 u8
-    float *parts;   // workspace: two partial results for every CTA
+    uint32_t team, part_count, q_vectors, out_pairs;   // warps that share a unit; parts of the row
+    float *parts;   // workspace: two partial results for every part,
+    struct Cut *cuts;   // and what is to be joined
     int *status;
 };
 
@@ -38,6 +45,11 @@ __device__ __forceinline__ bool live_tokens(const AttentionParams &p, uint32_t s
     return b200::live_tokens(p.length[sequence], p.table_pages, p.cache.page_size, p.window, begin, end);
 }
 
+// as quantize_cuda_b200, F32 -> U8_Q
+__device__ __forceinline__ uint32_t to_u8(float x, float scale)
+{
+    return (uint32_t)min(255, max(1, cvt_rne_x86(__fadd_rn(__fmul_rn(x, scale), 128.0f))));
+}
 __device__ __forceinline__ void store_out(const AttentionParams &p, uint64_t at, float x)
 {
     if (p.out_kind == 0) {
@@ -45,70 +57,110 @@ __device__ __forceinline__ void store_out(const AttentionParams &p, uint64_t at,
     } else if (p.out_kind == 1) {
         reinterpret_cast<__half *>(p.out)[at] = __float2half_rn(x);
     } else {
-        // as quantize_cuda_b200, F32 -> U8_Q
-        reinterpret_cast<uint8_t *>(p.out)[at] = (uint8_t)min(255, max(1, cvt_rne_x86(__fadd_rn(__fmul_rn(x, p.out_scale), 128.0f))));
+        reinterpret_cast<uint8_t *>(p.out)[at] = (uint8_t)to_u8(x, p.out_scale);
+    }
+}
+__device__ __forceinline__ void store_pair(const AttentionParams &p, uint64_t at, float x, float y)
+{
+    if (!p.out_pairs) {
+        store_out(p, at, x);
+        store_out(p, at + 1, y);
+    } else if (p.out_kind == 0) {
+        *reinterpret_cast<float2 *>(reinterpret_cast<float *>(p.out) + at) = make_float2(x, y);
+    } else if (p.out_kind == 1) {
+        *reinterpret_cast<uint32_t *>(reinterpret_cast<__half *>(p.out) + at) = half2_bits(x, y);
+    } else {
+        *reinterpret_cast<uint16_t *>(reinterpret_cast<uint8_t *>(p.out) + at) = (uint16_t)(to_u8(x, p.out_scale) | to_u8(y, p.out_scale) << 8);
     }
 }
 
 // ---- how the work is divided -----------------------------------------------------------------------------------
-// A unit is one sequence, key head and block of query heads; it has tiles of WARPS x STEP tokens on a grid that starts at
-// token 0.  All units' tiles stand in one row, in which every CTA takes an equal, contiguous part.
-// By all THREADS threads of a CTA: the row's length, and the sequence that holds a place of it (place_of(length), if that is
-// within the row) with that sequence's own first place.  sums[32] and *found are shared memory.
+// A unit is one sequence, key head and block of query heads; it has tiles of team x STEP tokens on a grid that starts at
+// token 0.  All units' tiles stand in one row, in which every team of warps takes an equal, contiguous part.
+constexpr int WARPS = 8;
+constexpr uint32_t MAX_SEQUENCES = 65535;
+constexpr uint32_t BY_WARP = 1024;    // up to so many sequences every warp counts for itself; beyond, the CTA's share the counting
 struct Found {
-    uint32_t sequence;
     uint64_t first;
+    uint32_t sequence;
 };
-template <int THREADS, typename F>
-__device__ __forceinline__ uint64_t locate(const AttentionParams &p, uint32_t units, uint32_t tile_tokens, bool report, uint64_t *sums, Found *found, F place_of)
+struct Counting {     // shared memory
+    uint64_t sums[WARPS];
+    Found found[WARPS];
+};
+__device__ __forceinline__ uint32_t count_tiles(const AttentionParams &p, uint32_t s, uint32_t tile_tokens)
 {
-    const uint32_t per = (p.sequences + THREADS - 1) / THREADS;
-    const uint32_t s0 = min(threadIdx.x * per, p.sequences), s1 = min(s0 + per, p.sequences);
+    uint32_t begin, end;
+    live_tokens(p, s, &begin, &end);
+    return tiles_of(begin, end, tile_tokens);
+}
+// By all warps of a CTA, for each its team's part: the row's length, and the sequence that holds the part's first tile with
+// that sequence's own first place.
+__device__ __forceinline__ uint64_t locate(const AttentionParams &p, uint32_t units, uint32_t tile_tokens, uint32_t team, Counting *c, Found *mine)
+{
+    const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, teams = WARPS / team;
+    const bool shared = p.sequences > BY_WARP;
+    const uint32_t segment = shared ? (p.sequences + WARPS - 1) / WARPS : p.sequences;
+    const uint32_t a = shared ? min(warp * segment, p.sequences) : 0, b = min(a + segment, p.sequences), per = (b - a + 31) / 32;
+    const uint32_t s0 = min(a + lane * per, b), s1 = min(s0 + per, b);
     uint64_t own = 0;
     for (uint32_t s = s0; s < s1; ++s) {
-        uint32_t begin, end;
-        if (!live_tokens(p, s, &begin, &end) && report) {
-            atomicExch(p.status, BAD_ATTENTION);
-        }
-        own += tiles_of(begin, end, tile_tokens);
+        own += count_tiles(p, s, tile_tokens);
     }
     own *= units;
     uint64_t upto = own;
-    const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const uint64_t v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
         upto += lane >= o ? v : 0;
     }
-    if (lane == 31) {
-        sums[warp] = upto;
-    }
-    if (threadIdx.x == 0) {   // (always something inside the arrays, even if lengths change under the call)
-        found->sequence = 0;
-        found->first = 0;
-    }
-    __syncthreads();
-    uint64_t total = 0;
-    for (uint32_t w = 0; w < THREADS / 32; ++w) {
-        upto += w < warp ? sums[w] : 0;
-        total += sums[w];
-    }
-    const uint64_t place = total != 0 ? place_of(total) : 0;
-    uint64_t first = upto - own;
-    if (place >= first && place < upto) {
-        for (uint32_t s = s0; s < s1; ++s) {
-            uint32_t begin, end;
-            live_tokens(p, s, &begin, &end);
-            const uint64_t n = (uint64_t)tiles_of(begin, end, tile_tokens) * units;
-            if (place < first + n) {
-                found->sequence = s;
-                found->first = first;
-                break;
-            }
-            first += n;
+    uint64_t total = __shfl_sync(0xFFFFFFFFu, upto, 31);
+    if (shared) {
+        if (lane == 0) {
+            c->sums[warp] = total;
+        }
+        __syncthreads();
+        total = 0;
+        for (uint32_t w = 0; w < WARPS; ++w) {
+            upto += w < warp ? c->sums[w] : 0;
+            total += c->sums[w];
         }
     }
-    __syncthreads();
+    const Parts parts(total, p.part_count);
+    mine->first = 0;
+    mine->sequence = 0;     // (always something inside the arrays, even if lengths change under the call)
+    for (uint32_t t = shared ? 0 : warp / team; t < (shared ? teams : warp / team + 1); ++t) {
+        const uint32_t part = blockIdx.x * teams + t;
+        const uint64_t place = parts.begin(part), first = upto - own;
+        const uint32_t holder = __ballot_sync(0xFFFFFFFFu, part < parts.n && place >= first && place < upto);
+        if (holder == 0) {
+            continue;
+        }
+        Found f = {first, s0};
+        if (holder >> lane & 1) {
+            while (f.sequence < s1) {
+                const uint64_t next = f.first + (uint64_t)count_tiles(p, f.sequence, tile_tokens) * units;
+                if (place < next) {
+                    break;
+                }
+                f.first = next;
+                ++f.sequence;
+            }
+        }
+        f.first = __shfl_sync(0xFFFFFFFFu, f.first, __ffs(holder) - 1);
+        f.sequence = min(__shfl_sync(0xFFFFFFFFu, f.sequence, __ffs(holder) - 1), p.sequences - 1);
+        if (shared) {
+            c->found[t] = f;
+        } else {
+            *mine = f;
+        }
+    }
+    if (shared) {
+        __syncthreads();
+        if (blockIdx.x * teams + warp / team < parts.n) {
+            *mine = c->found[warp / team];
+        }
+    }
     return total;
 }
 // By a warp: the first sequence behind `sequence` that has a token (there is one).
@@ -191,7 +243,6 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t &hi, uint3
     lo = half2_bits(x - f.x, y - f.y);
 }
 
-constexpr int WARPS = 8, MAX_PARTS = 256;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 // DP: elements of a row, rounded up; HB: blocks of eight query heads
@@ -201,28 +252,25 @@ struct Shape {
     static constexpr int STEP = ROW <= 128 ? 32 : 16;                            // tokens that a warp takes at a time
     static constexpr uint32_t ALL = STEP == 32 ? 0xFFFFFFFFu : 0xFFFFu;
     static constexpr int SLOT = STEP * PITCH + (I8 ? STEP * 4 : 0);
-    static constexpr int HEADS = 8 * HB, COLS = 64 / HB;
-    static constexpr int Q_PITCH = DP * 2 + 16, Q_BYTES = 2 * HEADS * Q_PITCH;
-    static constexpr int MERGE = WARPS * HEADS * (COLS + 4) * 4;
-    static constexpr int FIXED = Q_BYTES + MERGE + 4096;
+    static constexpr int HEADS = 8 * HB;
+    static constexpr bool Q_IN_REGISTERS = HB == 1 && DP <= 128;
+    static constexpr int Q_PITCH = DP * 2 + 16, Q_BYTES = Q_IN_REGISTERS ? 0 : 2 * HEADS * Q_PITCH;
+    static constexpr int MERGE = WARPS / 2 * 32 * 32 * 4;                        // 32 numbers of every lane of half the warps
+    static constexpr int FIXED = Q_BYTES + MERGE + 2048;
     static constexpr int FIT = (232448 - FIXED) / (WARPS * SLOT);
     static constexpr int SLOTS = FIT > 6 ? 6 : FIT;                              // ring of a warp: K, V, K, V ...
     static constexpr int SMEM = FIXED + WARPS * SLOTS * SLOT;
     static constexpr int PART = HEADS * (DP + 2);                                // floats of a partial result: sums, then maxima, then totals
-    static constexpr bool Q_IN_REGISTERS = HB == 1 && DP <= 128;
     static_assert(SLOTS >= 2, "a ring needs two slots");
 };
 
-// What a warp loads next.  It runs ahead of what the warp computes, across the borders of units.
-template <typename S>
-struct Loader {
-    uint64_t left;                         // tiles of the CTA's part, this one included
-    uint32_t sequence, unit, tile, tile_end, begin, end;
-    uint32_t page_index, at;               // of the lane's token
-    uint32_t page;                         // table entry, asked for one tile ahead
-    uint64_t row;                          // element of the lane's row in the tile at hand
-    uint64_t scale_row;
-    uint32_t mask;                         // its tokens that count
+// What a warp loads next: a run of tiles of one unit whose pages are at most 32 neighbours of the table, one in each lane.
+struct Run {
+    uint32_t unit, begin, end;
+    uint32_t left;                         // tiles
+    uint32_t token;                        // first one of the warp's step
+    uint32_t first_page;                   // of the table's row
+    uint32_t pages;
 };
 
 template <int DP, bool I8, int HB>
@@ -233,63 +281,99 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_attention_kernel(const __
     char *const q_smem = smem;
     float *const merge = reinterpret_cast<float *>(smem + S::Q_BYTES);
     char *const small = smem + S::Q_BYTES + S::MERGE;
-    uint64_t *const sums = reinterpret_cast<uint64_t *>(small);                 // 32
-    Found *const found = reinterpret_cast<Found *>(small + 256);
-    float *const factor = reinterpret_cast<float *>(small + 512);               // [16]
+    Counting *const counting = reinterpret_cast<Counting *>(small);             // 192 bytes
+    float *const factor = reinterpret_cast<float *>(small + 256);               // [16]
     float *const warp_m = factor + 16, *const warp_l = warp_m + WARPS * 16;     // [WARPS][16]
-    uint32_t *const masks = reinterpret_cast<uint32_t *>(warp_l + WARPS * 16);  // [WARPS][SLOTS]
+    uint32_t *const masks = reinterpret_cast<uint32_t *>(warp_l + WARPS * 16);  // [WARPS][8]
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, c4 = lane % 4;
     char *const ring = smem + S::FIXED + warp * S::SLOTS * S::SLOT;
     const uint32_t dim = p.cache.dim, pieces = dim * S::SIZE / 16, units = p.cache.kv_heads * p.head_blocks;
-    constexpr uint32_t TILE = WARPS * S::STEP;
+    const uint32_t team = S::Q_IN_REGISTERS ? p.team : WARPS, member = warp % team, teams = WARPS / team;
+    const uint32_t tile_tokens = team * S::STEP, tile_shift = __ffs(tile_tokens) - 1;
+    const uint32_t part = blockIdx.x * teams + warp / team;
 
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (dim < DP) {   // what no copy fills counts as zeros
         for (uint32_t i = lane; i < S::SLOTS * S::SLOT / 16; i += 32) {
             reinterpret_cast<uint4 *>(ring)[i] = make_uint4(0, 0, 0, 0);
         }
     }
-    const uint64_t total = locate<32 * WARPS>(p, units, TILE, blockIdx.x == 0, sums, found,
-        [&](uint64_t n) { return part_begin(blockIdx.x, n, gridDim.x); });
-    if (total == 0) {
-        return;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");    // nothing in front of this touches global memory
+    Found found;
+    const uint64_t total = locate(p, units, tile_tokens, team, counting, &found);
+    const Parts parts(total, p.part_count);
+    uint64_t place = part < parts.n ? parts.begin(part) : 0;
+    const uint64_t stop = part < parts.n ? parts.begin(part + 1) : 0;
+    if (lane == 0 && member == 0) {
+        p.cuts[part].parts = 0;
     }
-    uint64_t place = part_begin(blockIdx.x, total, gridDim.x);
-    const uint64_t stop = part_begin(blockIdx.x + 1, total, gridDim.x);
-    if (place == stop) {
-        return;
-    }
-    uint32_t sequence = found->sequence, begin, end;
+    auto team_sync = [&]() {
+        if (team == WARPS) {
+            __syncthreads();
+        } else if (team == 1) {
+            __syncwarp();
+        } else {
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / team), "r"(32 * team) : "memory");
+        }
+    };
+
+  if (place < stop) {
+    uint32_t sequence = found.sequence, begin, end;
     live_tokens(p, sequence, &begin, &end);
-    uint32_t tiles = max(tiles_of(begin, end, TILE), 1u);
-    uint32_t unit = min((uint32_t)((place - found->first) / tiles), units - 1), tile = (uint32_t)((place - found->first) % tiles);
+    uint32_t tiles = max(tiles_of(begin, end, tile_tokens), 1u), unit, tile;
+    {
+        const uint64_t within = place - found.first;   // of the sequence's tiles x units
+        const uint64_t u = within >> 32 == 0 ? (uint32_t)within / tiles : within / tiles;
+        unit = (uint32_t)min(u, (uint64_t)units - 1);
+        tile = (uint32_t)(within - u * tiles);
+    }
 
     // ---- the copies ----
     const uint32_t page_size = p.cache.page_size;
     const bool one_page = page_size % S::STEP == 0;    // a step's tokens are neighbours in one page
-    const uint32_t lane_token = lane % S::STEP, step_pages = TILE / page_size, step_at = TILE % page_size;
-    Loader<S> ld;
-    auto token0 = [&]() { return (ld.begin / TILE + ld.tile) * TILE + warp * S::STEP; };
-    auto look_up = [&]() {
-        const uint32_t t = token0() + (one_page ? 0 : lane_token);
-        ld.page = t < ld.end && ld.page_index < p.table_pages ? (uint32_t)__ldg(p.table + (uint64_t)ld.sequence * p.table_pages + ld.page_index) : 0xFFFFFFFFu;
+    const uint32_t lane_token = lane % S::STEP, step_pages = tile_tokens / page_size, step_at = tile_tokens % page_size;
+    // tiles whose steps lie in 32 pages: (n - 1) tile_tokens + STEP tokens, beginning anywhere in a page
+    const uint32_t run_tiles = 1 + (uint32_t)min((31ull * page_size - min(31ull * page_size, (unsigned long long)S::STEP + page_size - 2)) / tile_tokens, 1ull << 20);
+    Run run, ahead;
+    // the cursor behind `ahead`
+    uint64_t left = stop - place;
+    uint32_t a_sequence = sequence, a_unit = unit, a_tile = tile, a_tiles = tiles, a_begin = begin, a_end = end;
+    auto look_ahead = [&]() {
+        ahead.left = (uint32_t)min((uint64_t)min(run_tiles, a_tiles - a_tile), left);
+        if (ahead.left == 0) {
+            return;
+        }
+        ahead.unit = a_unit;
+        ahead.begin = a_begin;
+        ahead.end = a_end;
+        ahead.token = (((a_begin >> tile_shift) + a_tile) << tile_shift) + member * S::STEP;
+        ahead.first_page = ahead.token / page_size;
+        const uint64_t entry = (uint64_t)ahead.first_page + lane;
+        ahead.pages = entry < p.table_pages && entry * page_size < a_end ? (uint32_t)__ldg(p.table + (uint64_t)a_sequence * p.table_pages + entry) : 0xFFFFFFFFu;
+        left -= ahead.left;
+        a_tile += ahead.left;
+        if (a_tile == a_tiles && left != 0) {
+            a_tile = 0;
+            if (++a_unit == units) {
+                a_unit = 0;
+                a_sequence = next_sequence(p, a_sequence);
+                live_tokens(p, a_sequence, &a_begin, &a_end);
+                a_tiles = max(tiles_of(a_begin, a_end, tile_tokens), 1u);
+            }
+        }
     };
+    uint32_t page_index = 0, at = 0;    // of the lane's token
     auto enter = [&]() {
-        const uint32_t t = token0() + (one_page ? 0 : lane_token);
-        ld.page_index = t / page_size;
-        ld.at = t - ld.page_index * page_size;
-        look_up();
+        run = ahead;
+        const uint32_t t = run.token + (one_page ? 0 : lane_token);
+        page_index = t / page_size;
+        at = t - page_index * page_size;
+        look_ahead();
     };
-    ld.left = stop - place;
-    ld.sequence = sequence;
-    ld.unit = unit;
-    ld.tile = tile;
-    ld.tile_end = tiles;
-    ld.begin = begin;
-    ld.end = end;
-    ld.mask = 0;
-    ld.row = ld.scale_row = 0;
+    look_ahead();
     enter();
+    uint64_t row = 0, scale_row = 0;    // elements of the lane's row in the tile at hand
+    uint32_t live = 0;                  // its tokens that count
     uint32_t fill_slot = 0;    // items: K, V, K, V ...
     const uint32_t copy_row = lane / (S::ROW / 16), copy_piece = lane % (S::ROW / 16);   // of the first piece that the lane copies
     const uint64_t token_bytes = p.cache.token_stride * S::SIZE, lane_bytes = copy_row * token_bytes + copy_piece * 16;
@@ -298,70 +382,58 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_attention_kernel(const __
         const uint32_t slot = fill_slot;
         fill_slot = fill_slot + 1 == S::SLOTS ? 0 : fill_slot + 1;
         if (!values) {
-            ld.mask = 0;
-            if (ld.left != 0) {
-                const uint32_t head = ld.unit / p.head_blocks, t = token0() + lane_token;
-                const bool inside = t >= ld.begin && t < ld.end, good = ld.page < p.cache.pages;
+            live = 0;
+            if (run.left != 0) {
+                const uint32_t head = run.unit / p.head_blocks, t = run.token + lane_token;
+                const uint32_t page = __shfl_sync(0xFFFFFFFFu, run.pages, page_index - run.first_page);
+                const bool inside = t >= run.begin && t < run.end, good = page < p.cache.pages;
                 if (inside && !good) {
                     atomicExch(p.status, BAD_ATTENTION);
                 }
-                ld.mask = __ballot_sync(0xFFFFFFFFu, inside && good);
-                if (S::STEP == 16) {
-                    ld.mask &= 0xFFFFu;
+                live = __ballot_sync(0xFFFFFFFFu, inside && good) & S::ALL;
+                row = good ? row_element(p.cache, page, at, head) : 0;
+                scale_row = I8 && good ? scale_element(p.cache, page, at, head) + (one_page ? lane_token : 0) : 0;
+                run.token += tile_tokens;
+                page_index += step_pages;
+                at += step_at;
+                if (at >= page_size) {
+                    at -= page_size;
+                    ++page_index;
                 }
-                ld.row = good ? row_element(p.cache, ld.page, ld.at, head) : 0;
-                ld.scale_row = I8 && good ? scale_element(p.cache, ld.page, ld.at, head) + (one_page ? lane_token : 0) : 0;
-                // on to the next tile
-                --ld.left;
-                if (++ld.tile < ld.tile_end) {
-                    ld.page_index += step_pages;
-                    ld.at += step_at;
-                    if (ld.at >= page_size) {
-                        ld.at -= page_size;
-                        ++ld.page_index;
-                    }
-                    look_up();
-                } else if (ld.left != 0) {
-                    ld.tile = 0;
-                    if (++ld.unit == units) {
-                        ld.unit = 0;
-                        ld.sequence = next_sequence(p, ld.sequence);
-                        live_tokens(p, ld.sequence, &ld.begin, &ld.end);
-                        ld.tile_end = tiles_of(ld.begin, ld.end, TILE);
-                    }
+                if (--run.left == 0) {
                     enter();
                 }
             }
             if (lane == 0) {
-                masks[warp * S::SLOTS + slot] = ld.mask;
+                masks[warp * 8 + slot] = live;
             }
         }
-        if (ld.mask != 0) {
+        if (live != 0) {
             constexpr int ROWS = 32 / (S::ROW / 16);      // rows of one instruction
             const char *base = reinterpret_cast<const char *>(values ? p.v : p.k);
             uint32_t dst = lane_at + slot * S::SLOT;
-            if (one_page && dim == DP && ld.mask == S::ALL) {
-                const char *src = base + ld.row * S::SIZE + lane_bytes;
+            if (one_page && dim == DP && live == S::ALL) {
+                const char *src = base + row * S::SIZE + lane_bytes;
 #pragma unroll
                 for (int i = 0; i < S::STEP / ROWS; ++i) {
                     copy16(dst + i * ROWS * S::PITCH, src);
                     src += ROWS * token_bytes;
                 }
             } else {
-#pragma unroll 1
+#pragma unroll 4
                 for (int i = 0; i < S::STEP / ROWS; ++i) {
                     const uint32_t r = copy_row + i * ROWS;
-                    const uint64_t row = one_page ? ld.row + r * p.cache.token_stride : __shfl_sync(0xFFFFFFFFu, ld.row, r);
+                    const uint64_t from = one_page ? row + r * p.cache.token_stride : __shfl_sync(0xFFFFFFFFu, row, r);
                     if (copy_piece < pieces) {
-                        const bool on = ld.mask >> r & 1;
-                        copy16(dst + i * ROWS * S::PITCH, on ? base + row * S::SIZE + copy_piece * 16 : base, on ? 16 : 0);
+                        const bool on = live >> r & 1;
+                        copy16(dst + i * ROWS * S::PITCH, on ? base + from * S::SIZE + copy_piece * 16 : base, on ? 16 : 0);
                     }
                 }
             }
             if (I8 && lane < S::STEP) {
                 const float *s = values ? p.v_scale : p.k_scale;
-                const bool on = ld.mask >> lane & 1;
-                copy4(ring_at + slot * S::SLOT + S::STEP * S::PITCH + lane * 4, on ? s + ld.scale_row : s, on ? 4 : 0);
+                const bool on = live >> lane & 1;
+                copy4(ring_at + slot * S::SLOT + S::STEP * S::PITCH + lane * 4, on ? s + scale_row : s, on ? 4 : 0);
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -389,51 +461,108 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_attention_kernel(const __
         const uint32_t heads_here = min((uint32_t)S::HEADS, p.group - block * S::HEADS), head0 = head * p.group + block * S::HEADS;
         const uint32_t count = (uint32_t)min((uint64_t)(tiles - tile), stop - place);
         // Queries: brought to 2^13 .. 2^14 by a power of two (which the factor of the scores takes back), then two binary16
-        // numbers each, in rows (hi of every head, lo of every head) of the matrix instruction's left operand.  Bytes come
+        // numbers each, in the rows (hi of every head, lo of every head) of the matrix instruction's left operand.  Bytes come
         // out of their words in the order 0, 2, 1, 3; the queries' elements stand in the same order.
-        for (uint32_t h = warp; h < S::HEADS; h += WARPS) {
-            float x[DP / 32];
-            int top = 0;
-#pragma unroll
-            for (int i = 0; i < DP / 32; ++i) {
-                const uint32_t d = lane + 32 * i;
-                x[i] = 0.f;
-                if (h < heads_here && d < dim) {
-                    const uint64_t e = sequence * p.q_stride + (uint64_t)(head0 + h) * dim + d;
-                    x[i] = p.q_f16 ? load1(reinterpret_cast<const __half *>(p.q) + e) : load1(reinterpret_cast<const float *>(p.q) + e);
-                }
-                top = max(top, magnitude(x[i]));
+        const uint64_t q_row = sequence * p.q_stride + (uint64_t)head0 * dim;
+        auto query = [&](uint32_t h, uint32_t d) {
+            if (h >= heads_here || d >= dim) {
+                return 0.f;
             }
-            top = __reduce_max_sync(0xFFFFFFFFu, top);
+            const uint64_t e = q_row + h * dim + d;
+            return p.q_f16 ? load1(reinterpret_cast<const __half *>(p.q) + e) : load1(reinterpret_cast<const float *>(p.q) + e);
+        };
+        auto powers = [&](int top, float &up, float &fac) {
             const int e = max(top >> 23, 20);
-            const float up = __int_as_float((127 + 13 + 127 - e) << 23);
-            if (lane == 0) {
-                factor[h] = __int_as_float((e - 13) << 23) * (p.scale * LOG2E);
-            }
-            const uint32_t hi_row = h, lo_row = S::HEADS + h;
-#pragma unroll
-            for (int i = 0; i < DP / 32; ++i) {
-                const uint32_t d = lane + 32 * i, r = d % 4;
-                const uint32_t k = I8 ? d / 16 * 16 + d % 16 / 4 * 2 + r / 2 + r % 2 * 8 : d;
-                const float v = x[i] * up;
-                const __half hi = __float2half_rn(v);
-                *reinterpret_cast<__half *>(q_smem + hi_row * S::Q_PITCH + k * 2) = hi;
-                *reinterpret_cast<__half *>(q_smem + lo_row * S::Q_PITCH + k * 2) = __float2half_rn(v - __half2float(hi));
-            }
-        }
-        __syncthreads();
+            up = __int_as_float((127 + 13 + 127 - e) << 23);
+            fac = __int_as_float((e - 13) << 23) * (p.scale * LOG2E);
+        };
+        float fac[HB];
         uint32_t qa[S::Q_IN_REGISTERS ? KS : 1][4];
         const uint32_t q_at = smem_at(q_smem + (lane % 16) * S::Q_PITCH + lane / 16 * 16);
         if constexpr (S::Q_IN_REGISTERS) {
+            // columns 2c, 2c + 1, 2c + 8, 2c + 9 of every step (rows of heads that do not exist repeat the first: nobody reads
+            // their results)
+            float x[KS][4], up;
+            int top = 0;
+            const uint64_t mine = q_row + (g < heads_here ? g : 0) * dim + (I8 ? 4 : 2) * c4;
+            if (p.q_vectors && dim == DP) {
+                auto fetch = [&](auto *q) {
+#pragma unroll
+                    for (int s = 0; s < KS; ++s) {
+                        if constexpr (I8) {
+                            float v[4];
+                            load4(q + 16 * s, v);
+                            x[s][0] = v[0];
+                            x[s][1] = v[2];
+                            x[s][2] = v[1];
+                            x[s][3] = v[3];
+                        } else {
+                            load2(q + 16 * s, x[s][0], x[s][1]);
+                            load2(q + 16 * s + 8, x[s][2], x[s][3]);
+                        }
+                    }
+                };
+                if (p.q_f16) {
+                    fetch(reinterpret_cast<const __half *>(p.q) + mine);
+                } else {
+                    fetch(reinterpret_cast<const float *>(p.q) + mine);
+                }
+            } else {
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        x[s][e] = query(g, 16 * s + (I8 ? 4 * c4 + e % 2 * 2 + e / 2 : 2 * c4 + e % 2 + e / 2 * 8));
+                    }
+                }
+            }
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
-                matrices(qa[s], q_at + s * 32);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    top = max(top, magnitude(x[s][e]));
+                }
+            }
+            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+            powers(top, up, fac[0]);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                split_pair(x[s][0] * up, x[s][1] * up, qa[s][0], qa[s][1]);
+                split_pair(x[s][2] * up, x[s][3] * up, qa[s][2], qa[s][3]);
+            }
+        } else {
+            for (uint32_t h = warp; h < S::HEADS; h += WARPS) {
+                float x[DP / 32], up, f;
+                int top = 0;
+#pragma unroll
+                for (int i = 0; i < DP / 32; ++i) {
+                    x[i] = query(h, lane + 32 * i);
+                    top = max(top, magnitude(x[i]));
+                }
+                powers(__reduce_max_sync(0xFFFFFFFFu, top), up, f);
+                if (lane == 0) {
+                    factor[h] = f;
+                }
+#pragma unroll
+                for (int i = 0; i < DP / 32; ++i) {
+                    const uint32_t d = lane + 32 * i, r = d % 4;
+                    const uint32_t k = I8 ? d / 16 * 16 + d % 16 / 4 * 2 + r / 2 + r % 2 * 8 : d;
+                    const float v = x[i] * up;
+                    const __half hi = __float2half_rn(v);
+                    *reinterpret_cast<__half *>(q_smem + h * S::Q_PITCH + k * 2) = hi;
+                    *reinterpret_cast<__half *>(q_smem + (S::HEADS + h) * S::Q_PITCH + k * 2) = __float2half_rn(v - __half2float(hi));
+                }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int b = 0; b < HB; ++b) {
+                fac[b] = factor[g + 8 * b];
             }
         }
-        float fac[HB], m[HB], l[HB], acc[TILES_D][2 * HB], top_unit = 0.f;
+        float m[HB], l[HB], acc[TILES_D][2 * HB], top_unit = 0.f;
 #pragma unroll
         for (int b = 0; b < HB; ++b) {
-            fac[b] = factor[g + 8 * b];
             m[b] = -INFINITY;
             l[b] = 0.f;
         }
@@ -449,7 +578,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_attention_kernel(const __
             // scores: [heads] x [tokens]
             const uint32_t ks = next(false);
             const char *const kt = ring + ks * S::SLOT;
-            const uint32_t mask = masks[warp * S::SLOTS + ks];
+            const uint32_t mask = masks[warp * 8 + ks];
             float sc[NT][4];
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
@@ -638,6 +767,10 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_attention_kernel(const __
             }
         }
         // ---- the warps' shares, and out ----
+        const bool whole = count == tiles;
+        float *const share = p.parts + ((uint64_t)part * 2 + (tile != 0 ? 0 : 1)) * S::PART;
+        float own[HB];
+        const uint32_t warp0 = warp - member;
 #pragma unroll
         for (int b = 0; b < HB; ++b) {
             l[b] += __shfl_xor_sync(0xFFFFFFFFu, l[b], 1);
@@ -647,60 +780,81 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_attention_kernel(const __
                 warp_l[warp * 16 + g + 8 * b] = l[b];
             }
         }
-        __syncthreads();
-        const bool whole = count == tiles;
-        float *const part = p.parts + ((uint64_t)blockIdx.x * 2 + (tile != 0 ? 0 : 1)) * S::PART;
-        float own[HB];
+        team_sync();
 #pragma unroll
         for (int b = 0; b < HB; ++b) {
-            float top = -INFINITY;
-            for (int w = 0; w < WARPS; ++w) {
-                top = fmaxf(top, warp_m[w * 16 + g + 8 * b]);
+            const uint32_t h = g + 8 * b;
+            float top = -INFINITY, all = 0.f;
+            for (uint32_t w = 0; w < team; ++w) {
+                top = fmaxf(top, warp_m[(warp0 + w) * 16 + h]);
             }
-            own[b] = exp2_fast(m[b] - (top == -INFINITY ? 0.f : top)) * (I8 ? top_unit : 1.f);
+            const float base = top == -INFINITY ? 0.f : top;
+            for (uint32_t w = 0; w < team; ++w) {
+                all = fmaf(warp_l[(warp0 + w) * 16 + h], exp2_fast(warp_m[(warp0 + w) * 16 + h] - base), all);
+            }
+            own[b] = exp2_fast(m[b] - base) * (I8 ? top_unit : 1.f);
+            if (whole) {
+                own[b] *= all == 0.f ? 0.f : __frcp_rn(all);
+            }
+            if (member == 0 && c4 == 0) {
+                if (!whole) {
+                    share[S::HEADS * DP + h] = top;
+                    share[S::HEADS * (DP + 1) + h] = all;
+                } else if (p.lse != nullptr && h < heads_here) {
+                    p.lse[(uint64_t)sequence * p.heads + head0 + h] = (top + log2f(all) - 14.f) * LN2;
+                }
+            }
         }
-        for (int col = 0; col < DP; col += S::COLS) {
+        if (!whole && tile == 0 && member == 0 && lane == 0) {
+            p.cuts[part] = Cut{parts.of(place + tiles - 1) - part + 1, sequence, head0, heads_here};
+        }
+        // Sums of the team's upper half are added to the lower half's, and so on; 32 numbers of a lane at a time.
+        constexpr int NUMBERS = TILES_D * 2 * HB, GO = NUMBERS < 32 ? NUMBERS : 32;
 #pragma unroll
-            for (int n = 0; n < TILES_D; ++n) {
+        for (int x = 0; x < NUMBERS; ++x) {
+            acc[x / (2 * HB)][x % (2 * HB)] *= own[x % (2 * HB) / 2];
+        }
 #pragma unroll
-                for (int e = 0; e < 2 * HB; ++e) {
-                    // element of the row: pairs of neighbours, or (bytes) every second one
-                    const uint32_t d = I8 ? n / 2 * 16 + 4 * c4 + e % 2 * 2 + n % 2 : 8 * n + 2 * c4 + e % 2;
-                    const bool here = I8 ? n / 2 * 16 >= col && n / 2 * 16 < col + S::COLS : 8 * n >= col && 8 * n < col + S::COLS;
-                    if (here) {
-                        merge[(warp * S::HEADS + g + e / 2 * 8) * (S::COLS + 4) + d - col] = acc[n][e] * own[e / 2];
+        for (int x0 = 0; x0 < NUMBERS; x0 += GO) {
+#pragma unroll 1
+            for (uint32_t half = team / 2; half != 0; half /= 2) {
+                float *const to = merge + (warp0 / 2 + member % half) * 1024 + lane;
+                if (member >= half && member < 2 * half) {
+#pragma unroll
+                    for (int x = 0; x < GO; ++x) {
+                        to[x * 32] = acc[(x0 + x) / (2 * HB)][(x0 + x) % (2 * HB)];
+                    }
+                }
+                team_sync();
+                if (member < half) {
+#pragma unroll
+                    for (int x = 0; x < GO; ++x) {
+                        acc[(x0 + x) / (2 * HB)][(x0 + x) % (2 * HB)] += to[x * 32];
+                    }
+                }
+                team_sync();
+            }
+        }
+        if (member == 0) {
+#pragma unroll
+            for (int b = 0; b < HB; ++b) {
+                const uint32_t h = g + 8 * b;
+                const uint64_t to = sequence * p.out_stride + (uint64_t)(head0 + h) * dim;
+#pragma unroll
+                for (int n = 0; n < TILES_D; n += 2) {
+                    // neighbours of the row: pairs in two tiles, or (bytes) all four numbers of two tiles
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const uint32_t d = I8 ? 8 * n + 4 * c4 + 2 * k : 8 * (n + k) + 2 * c4;
+                        const float x = I8 ? acc[n][2 * b + k] : acc[n + k][2 * b], y = I8 ? acc[n + 1][2 * b + k] : acc[n + k][2 * b + 1];
+                        if (!whole) {
+                            *reinterpret_cast<float2 *>(share + h * DP + d) = make_float2(x, y);
+                        } else if (h < heads_here && d < dim) {
+                            store_pair(p, to + d, x, y);
+                        }
                     }
                 }
             }
-            __syncthreads();
-            for (uint32_t i = threadIdx.x; i < S::HEADS * S::COLS; i += 32 * WARPS) {
-                const uint32_t h = i / S::COLS, d = i % S::COLS;
-                float top = -INFINITY, sum = 0.f, all = 0.f;
-                for (int w = 0; w < WARPS; ++w) {
-                    top = fmaxf(top, warp_m[w * 16 + h]);
-                }
-                const float base = top == -INFINITY ? 0.f : top;
-#pragma unroll
-                for (int w = 0; w < WARPS; ++w) {
-                    sum += merge[(w * S::HEADS + h) * (S::COLS + 4) + d];
-                    all += warp_l[w * 16 + h] * exp2_fast(warp_m[w * 16 + h] - base);
-                }
-                if (whole) {
-                    if (h < heads_here && col + d < dim) {
-                        store_out(p, sequence * p.out_stride + (uint64_t)(head0 + h) * dim + col + d, all == 0.f ? 0.f : __fdiv_rn(sum, all));
-                    }
-                    if (p.lse != nullptr && h < heads_here && col + d == 0) {
-                        p.lse[(uint64_t)sequence * p.heads + head0 + h] = (top + log2f(all) - 14.f) * LN2;
-                    }
-                } else {
-                    part[h * DP + col + d] = sum;
-                    if (col + d == 0) {
-                        part[S::HEADS * DP + h] = top;
-                        part[S::HEADS * (DP + 1) + h] = all;
-                    }
-                }
-            }
-            __syncthreads();
         }
         // ---- the next unit ----
         place += count;
@@ -709,136 +863,120 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_attention_kernel(const __
             unit = 0;
             sequence = next_sequence(p, sequence);
             live_tokens(p, sequence, &begin, &end);
-            tiles = max(tiles_of(begin, end, TILE), 1u);
+            tiles = max(tiles_of(begin, end, tile_tokens), 1u);
         }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-}
-
-// Units that several CTAs have worked on: one block for the border at which such a unit is cut first, and each head.
-template <int DP, int HB>
-__global__ void __launch_bounds__(128) paged_attention_join_kernel(const __grid_constant__ AttentionParams p, uint32_t tile_tokens, uint32_t parts)
-{
-    constexpr int HEADS = 8 * HB, PART = HEADS * (DP + 2);
-    __shared__ uint64_t sums[32];
-    __shared__ Found found[1];
-    __shared__ float weight[MAX_PARTS], share[MAX_PARTS], warp_top[4];
-    const uint32_t i = blockIdx.x, units = p.cache.kv_heads * p.head_blocks, h = blockIdx.y;
-    // sequences without a token, which no part holds: every parts-th is this block column's
-    for (uint32_t s0 = 0; s0 < p.sequences; s0 += 32 * parts) {
-        const uint64_t mine = s0 + (uint64_t)(threadIdx.x % 32) * parts + i;
-        uint32_t begin, end = 1;
-        if (mine < p.sequences) {
-            live_tokens(p, (uint32_t)mine, &begin, &end);
+  }
+    // sequences without a token, a warp each, and lengths that are none
+    for (uint32_t s = blockIdx.x * WARPS + warp; s < p.sequences; s += gridDim.x * WARPS) {
+        uint32_t begin, end;
+        if (!live_tokens(p, s, &begin, &end) && lane == 0) {
+            atomicExch(p.status, BAD_ATTENTION);
         }
-        for (uint32_t none = __ballot_sync(0xFFFFFFFFu, end == 0); none != 0; none &= none - 1) {
-            const uint32_t s = s0 + (__ffs(none) - 1) * parts + i;
-            for (uint32_t hq = h; hq < p.heads; hq += gridDim.y) {
-                for (uint32_t d = threadIdx.x; d < p.cache.dim; d += 128) {
-                    store_out(p, s * p.out_stride + (uint64_t)hq * p.cache.dim + d, 0.f);
-                }
-                if (p.lse != nullptr && threadIdx.x == 0) {
-                    p.lse[(uint64_t)s * p.heads + hq] = -INFINITY;
-                }
+        if (end == 0) {
+            for (uint32_t i = lane; i < p.heads * dim; i += 32) {
+                store_out(p, s * p.out_stride + i, 0.f);
+            }
+            for (uint32_t i = lane; p.lse != nullptr && i < p.heads; i += 32) {
+                p.lse[(uint64_t)s * p.heads + i] = -INFINITY;
             }
         }
     }
-    const uint64_t total = locate<128>(p, units, tile_tokens, false, sums, found, [&](uint64_t n) {
-        const uint64_t stop = part_begin(i + 1, n, parts);
-        return stop != 0 ? stop - 1 : 0;
-    });
-    if (total == 0) {
-        return;
-    }
-    const uint64_t from = part_begin(i, total, parts), stop = part_begin(i + 1, total, parts);
-    if (from == stop || stop == total) {
-        return;
-    }
-    // the unit that holds the part's last tile
-    const uint32_t sequence = found->sequence;
-    const uint64_t first = found->first;
-    uint32_t begin, end;
-    live_tokens(p, sequence, &begin, &end);
-    const uint32_t tiles = max(tiles_of(begin, end, tile_tokens), 1u);
-    const uint32_t unit = min((uint32_t)((stop - 1 - first) / tiles), units - 1);
-    const uint64_t a = first + (uint64_t)unit * tiles;
-    const uint32_t head = unit / p.head_blocks, block = unit % p.head_blocks;
-    if (a < from || a + tiles <= stop || block * HEADS + h >= p.group) {
-        return;    // cut before, or not here
-    }
-    const uint32_t n = part_of(a + tiles - 1, total, parts) - i + 1;
+}
+
+// Units that several parts have worked on: one query head of one of them for each `team` warps, which divide the shares
+// among themselves (as many as the teams that made them: fewer, larger parts mean more shares of a unit).
+template <int DP, int HB>
+__global__ void __launch_bounds__(32 * WARPS) paged_attention_join_kernel(const __grid_constant__ AttentionParams p, uint32_t team)
+{
+    constexpr int HEADS = 8 * HB, PART = HEADS * (DP + 2), PER = DP / 32;
+    __shared__ float totals[WARPS], tops[WARPS], sums[WARPS][DP];
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, member = warp % team, warp0 = warp - member, h = blockIdx.y;
+    const uint32_t part = blockIdx.x * (WARPS / team) + warp / team;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    // part c of the unit is a share of CTA i + c: what it began (slot 1) in the first, what it went on with in the others
-    auto part = [&](uint32_t c) { return p.parts + ((uint64_t)(i + c) * 2 + (c == 0 ? 1 : 0)) * PART; };
-    float top = -INFINITY;
-    for (uint32_t c = threadIdx.x; c < n; c += 128) {
-        // (with fewer tiles than CTAs, some have none)
-        const bool empty = total < parts && part_begin(i + c, total, parts) == part_begin(i + c + 1, total, parts);
-        weight[c] = empty ? -INFINITY : part(c)[HEADS * DP + h];
-        share[c] = empty ? 0.f : part(c)[HEADS * (DP + 1) + h];
-        top = fmaxf(top, weight[c]);
+    const Cut cut = p.cuts[part];
+    const uint32_t n = h < cut.heads ? cut.parts : 0;
+    // share c: what the part began (slot 1), or the following ones went on with (slot 0)
+    auto share = [&](uint32_t c) { return p.parts + ((uint64_t)(part + c) * 2 + (c == 0 ? 1 : 0)) * PART; };
+    const uint32_t c0 = n * member / team, c1 = n * (member + 1) / team;
+    float top = -INFINITY, all = 0.f, sum[PER] = {};
+    for (uint32_t c = c0 + lane; c < c1; c += 32) {
+        top = fmaxf(top, share(c)[HEADS * DP + h]);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
     }
-    if (threadIdx.x % 32 == 0) {
-        warp_top[threadIdx.x / 32] = top;
-    }
-    __syncthreads();
-    top = fmaxf(fmaxf(warp_top[0], warp_top[1]), fmaxf(warp_top[2], warp_top[3]));
-    for (uint32_t c = threadIdx.x; c < n; c += 128) {
-        weight[c] = exp2_fast(weight[c] - (top == -INFINITY ? 0.f : top));
-    }
-    __syncthreads();
-    float all = 0.f, sum[(DP + 127) / 128] = {};
+    const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll 8
-    for (uint32_t c = 0; c < n; ++c) {
-        const float *q = part(c) + h * DP;
-        const float w = weight[c];
-        all = fmaf(share[c], w, all);
+    for (uint32_t c = c0; c < c1; ++c) {
+        const float *q = share(c);
+        const float w = exp2_fast(q[HEADS * DP + h] - base);
+        all = fmaf(q[HEADS * (DP + 1) + h], w, all);
 #pragma unroll
-        for (int k = 0; k < (DP + 127) / 128; ++k) {
-            const uint32_t d = threadIdx.x + 128 * k;
-            const float x = d < DP && w != 0.f ? q[d] : 0.f;
-            sum[k] = fmaf(x, w, sum[k]);
+        for (int k = 0; k < PER; ++k) {
+            sum[k] = fmaf(q[h * DP + lane + 32 * k], w, sum[k]);
         }
     }
-    const uint32_t hq = head * p.group + block * HEADS + h;
-#pragma unroll
-    for (int k = 0; k < (DP + 127) / 128; ++k) {
-        const uint32_t d = threadIdx.x + 128 * k;
-        if (d < p.cache.dim) {
-            store_out(p, sequence * p.out_stride + (uint64_t)hq * p.cache.dim + d, all == 0.f ? 0.f : __fdiv_rn(sum[k], all));
-        }
+    if (lane == 0) {
+        tops[warp] = top;
+        totals[warp] = all;
     }
-    if (p.lse != nullptr && threadIdx.x == 0) {
-        p.lse[(uint64_t)sequence * p.heads + hq] = (top + log2f(all) - 14.f) * LN2;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        sums[warp][lane + 32 * k] = sum[k];
+    }
+    __syncthreads();
+    if (n == 0) {
+        return;
+    }
+    top = -INFINITY;
+    for (uint32_t w = 0; w < team; ++w) {
+        top = fmaxf(top, tops[warp0 + w]);
+    }
+    const float floor = top == -INFINITY ? 0.f : top;
+    all = 0.f;
+    for (uint32_t w = 0; w < team; ++w) {
+        all = fmaf(totals[warp0 + w], exp2_fast(tops[warp0 + w] - floor), all);
+    }
+    const uint32_t hq = cut.head0 + h;
+    const float inv = all == 0.f ? 0.f : __frcp_rn(all);
+    for (uint32_t d = member * 32 + lane; d < p.cache.dim; d += 32 * team) {
+        float x = 0.f;
+        for (uint32_t w = 0; w < team; ++w) {
+            x = fmaf(sums[warp0 + w][d], exp2_fast(tops[warp0 + w] - floor), x);
+        }
+        store_out(p, cut.sequence * p.out_stride + (uint64_t)hq * p.cache.dim + d, x * inv);
+    }
+    if (p.lse != nullptr && member == 0 && lane == 0) {
+        p.lse[(uint64_t)cut.sequence * p.heads + hq] = (top + log2f(all) - 14.f) * LN2;
     }
 }
 
-uint32_t parts_of(const DeviceCtx *c)
-{
-    return c->sm_count < MAX_PARTS ? (uint32_t)c->sm_count : MAX_PARTS;
-}
 template <int DP, bool I8, int HB>
-EE launch(DeviceCtx *c, AttentionParams &p, cudaStream_t st)
+EE launch(DeviceCtx *c, const AttentionParams &p, cudaStream_t st)
 {
     using S = Shape<DP, I8, HB>;
     const void *kernel = reinterpret_cast<const void *>(paged_attention_kernel<DP, I8, HB>);
     B200_EE(raise_smem_limit(c, (KernelFamily)(KF_ATTENTION + (DP == 64 ? 0 : (DP == 128 ? 1 : 2)) + 3 * I8 + 6 * (HB - 1)), &kernel, 1, S::SMEM));
-    const uint32_t parts = parts_of(c);
-    B200_EE(launch_kernel(parts, 32 * WARPS, S::SMEM, st, paged_attention_kernel<DP, I8, HB>, p));
+    const uint32_t ctas = p.part_count * p.team / WARPS;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(parts, S::HEADS < (int)p.group ? S::HEADS : p.group);
-    cfg.blockDim = dim3(128);
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(32 * WARPS);
+    cfg.dynamicSmemBytes = S::SMEM;
     cfg.stream = st;
-    B200_CUDA(launch_programmatic(cfg, paged_attention_join_kernel<DP, HB>, p, (uint32_t)(WARPS * S::STEP), parts));
+    B200_CUDA(launch_programmatic(cfg, paged_attention_kernel<DP, I8, HB>, p));
+    count_launch();
+    cfg.gridDim = dim3(ctas, S::HEADS < (int)p.group ? S::HEADS : p.group);
+    cfg.dynamicSmemBytes = 0;
+    B200_CUDA(launch_programmatic(cfg, paged_attention_join_kernel<DP, HB>, p, p.team));
     count_launch();
     return SUCCESS;
 }
 template <bool I8>
-EE launch(DeviceCtx *c, AttentionParams &p, cudaStream_t st)
+EE launch(DeviceCtx *c, const AttentionParams &p, cudaStream_t st)
 {
     const uint32_t dim = p.cache.dim;
     if (p.group <= 8) {
@@ -862,7 +1000,7 @@ EE check(const bolt_b200_kv_cache *cache, const bolt_b200_paged_attention_call *
         return NOT_MATCH;
     }
     if ((a->q_dt != DT_F32 && a->q_dt != DT_F16) || (a->out_dt != DT_F32 && a->out_dt != DT_F16 && a->out_dt != DT_U8_Q) || a->heads > 65535u ||
-        a->sequences > 65535u) {
+        a->sequences > MAX_SEQUENCES) {
         return NOT_SUPPORTED;
     }
     const uint64_t row = (uint64_t)a->heads * cache->dim;
@@ -887,6 +1025,11 @@ EE check(const bolt_b200_kv_cache *cache, const bolt_b200_paged_attention_call *
     p->sequences = a->sequences;
     p->heads = a->heads;
     p->group = a->heads / cache->kv_heads;
+    const uint32_t ctas = (uint32_t)(*c)->sm_count;
+    // rows that can be read four at a time and written two at a time (dim is a multiple of 8)
+    const uint32_t q_size = a->q_dt == DT_F16 ? 2 : 4, out_size = a->out_dt == DT_F32 ? 4 : (a->out_dt == DT_F16 ? 2 : 1);
+    p->q_vectors = aligned(a->q, 4 * q_size) && a->q_stride % 4 == 0;
+    p->out_pairs = aligned(a->out, 2 * out_size) && a->out_stride % 2 == 0;
     p->head_blocks = p->group <= 8 ? 1 : (p->group + 15) / 16;
     p->table_pages = a->table_pages;
     p->window = a->window;
@@ -896,12 +1039,24 @@ EE check(const bolt_b200_kv_cache *cache, const bolt_b200_paged_attention_call *
     p->q_f16 = a->q_dt == DT_F16;
     p->out_kind = a->out_dt == DT_F32 ? 0 : (a->out_dt == DT_F16 ? 1 : 2);
     p->status = (*c)->d_status;
+    // As many warps to a team as leave a part for every unit: eight for few units (fewer shares to join), one for very
+    // many (no warp waits for others at a unit's end).  Queries in shared memory belong to the whole CTA.
+    const uint64_t units = (uint64_t)a->sequences * cache->kv_heads * p->head_blocks;
+    p->team = WARPS;
+    while (p->group <= 8 && cache->dim <= 128 && p->team > 1 && ctas * WARPS / p->team < units) {
+        p->team /= 2;
+    }
+    p->part_count = ctas * WARPS / p->team;
     return SUCCESS;
 }
-U32 workspace_bytes(const AttentionParams &p, const DeviceCtx *c)
+U32 share_bytes(const AttentionParams &p)
 {
     const U32 dp = p.cache.dim <= 64 ? 64 : (p.cache.dim <= 128 ? 128 : 256);
-    return parts_of(c) * 2 * (p.group <= 8 ? 8 : 16) * (dp + 2) * 4;
+    return p.part_count * 2 * (p.group <= 8 ? 8 : 16) * (dp + 2) * 4;
+}
+U32 workspace_bytes(const AttentionParams &p)
+{
+    return share_bytes(p) + p.part_count * (U32)sizeof(Cut);
 }
 
 }  // namespace
@@ -919,7 +1074,7 @@ EE bolt_b200_paged_attention_tmp_bytes(const bolt_b200_kv_cache *cache, const bo
     AttentionParams p;
     DeviceCtx *c = nullptr;
     B200_EE(check(cache, call, &p, &c));
-    *bytes = workspace_bytes(p, c);
+    *bytes = workspace_bytes(p);
     return SUCCESS;
 }
 
@@ -934,7 +1089,7 @@ EE bolt_b200_paged_attention(const bolt_b200_kv_cache *cache, const bolt_b200_pa
     if (p.q == nullptr || p.out == nullptr || p.table == nullptr || p.length == nullptr) {
         return NULL_POINTER;
     }
-    const U32 need = workspace_bytes(p, c);
+    const U32 need = workspace_bytes(p);
     if (tmpBytes < need) {
         return NOT_MATCH;
     }
@@ -951,6 +1106,7 @@ EE bolt_b200_paged_attention(const bolt_b200_kv_cache *cache, const bolt_b200_pa
         return NOT_MATCH;
     }
     p.parts = reinterpret_cast<float *>(tmp);
+    p.cuts = reinterpret_cast<Cut *>(reinterpret_cast<char *>(tmp) + share_bytes(p));
     return p.i8 ? launch<true>(c, p, tls().stream) : launch<false>(c, p, tls().stream);
 }
 

@@ -30,7 +30,8 @@ def harness(tmp_path_factory):
     lib.harness_row.argtypes = [C.c_void_p, l, u, u, u, u, u, l, l, l, u, u, u]
     lib.harness_scale.argtypes = [u] * 6
     lib.harness_tokens.argtypes = [C.c_int32, u, u, u, C.c_void_p]
-    lib.harness_part_begin.argtypes, lib.harness_part_begin.restype = [l, l, u], l
+    lib.harness_parts.argtypes, lib.harness_parts.restype = [l, u], u
+    lib.harness_part_begin.argtypes, lib.harness_part_begin.restype = [u, l, u], l
     lib.harness_part_of.argtypes, lib.harness_part_of.restype = [l, l, u], u
     lib.harness_tiles.argtypes, lib.harness_tiles.restype = [u, u, u], u
     return lib
@@ -69,16 +70,19 @@ def test_tokens_of_a_sequence(harness):
 
 
 def test_parts_cover_the_row_once(harness):
-    """every place of the row is in one part, the parts differ by one place at most, and a part is found from a place"""
-    for total in (1, 2, 3, 147, 148, 149, 1000, 12345, (1 << 40) + 7):
-        for parts in (1, 2, 147, 148):
-            borders = [harness.harness_part_begin(i, total, parts) for i in range(parts + 1)]
+    """every place of the row is in one part, no part is empty, they differ by one place at most, and a part is found from a place"""
+    assert harness.harness_parts(0, 148) == 0
+    for total in (1, 2, 3, 147, 148, 149, 1000, 12345, (1 << 32) - 1, (1 << 32) + 5, (1 << 40) + 7, (1 << 55) + 3):
+        for most in (1, 2, 147, 148, 1184):
+            parts = harness.harness_parts(total, most)
+            assert parts == min(total, most)
+            borders = [harness.harness_part_begin(i, total, most) for i in range(parts + 1)]
             assert borders[0] == 0 and borders[-1] == total
             sizes = {b - a for a, b in zip(borders, borders[1:])}
-            assert min(sizes) >= 0 and max(sizes) - min(sizes) <= 1
-            for place in sorted({0, total - 1, total // 2, *[b for b in borders[:-1] if b < total], *[b - 1 for b in borders if b]}):
-                i = harness.harness_part_of(place, total, parts)
-                assert borders[i] <= place < borders[i + 1], (total, parts, place, i)
+            assert min(sizes) >= 1 and max(sizes) - min(sizes) <= 1
+            for place in sorted({0, total - 1, total // 2, *borders[:-1], *[b - 1 for b in borders[1:]]}):
+                i = harness.harness_part_of(place, total, most)
+                assert borders[i] <= place < borders[i + 1], (total, most, place, i)
     for begin, end, tile, n in ((0, 0, 128, 0), (5, 5, 128, 0), (0, 1, 128, 1), (0, 128, 128, 1), (0, 129, 128, 2), (127, 129, 128, 2), (128, 129, 128, 1),
                                 (130, 700, 128, 5), (0, 0x7FFFFFFF, 256, 1 << 23)):
         assert harness.harness_tiles(begin, end, tile) == n
