@@ -46,32 +46,31 @@ __host__ __device__ inline bool live_tokens(int32_t length, uint32_t table_pages
     *begin = window != 0 && *end > window ? *end - window : 0;
     return good;
 }
-// Work that stands in a row, cut into n contiguous parts, none empty, of equal length but for one.
+// Work that stands in a row, cut into n contiguous parts, none empty, of equal length but for one.  (32 bits: a 64-bit
+// division takes ten times as long.)
 struct Parts {
-    uint64_t each;
-    uint32_t longer, n;   // the first `longer` parts have each + 1
-    __host__ __device__ Parts(uint64_t total, uint32_t most)
+    uint32_t each, longer, n;   // the first `longer` parts have each + 1
+    __host__ __device__ Parts(uint32_t total, uint32_t most)
     {
-        n = total < most ? (uint32_t)total : most;
-        // (a 64-bit division takes ten times as long as a 32-bit one)
-        each = n == 0 ? 0 : (total >> 32 == 0 ? (uint32_t)total / n : total / n);
-        longer = (uint32_t)(total - each * n);
+        n = total < most ? total : most;
+        each = n == 0 ? 0 : total / n;
+        longer = total - each * n;
     }
-    __host__ __device__ uint64_t begin(uint32_t i) const
+    __host__ __device__ uint32_t begin(uint32_t i) const
     {
         return i * each + (i < longer ? i : longer);
     }
     // the part that holds a place
-    __host__ __device__ uint32_t of(uint64_t place) const
+    __host__ __device__ uint32_t of(uint32_t place) const
     {
-        const uint64_t border = (each + 1) * longer, d = place < border ? each + 1 : each, x = place < border ? place : place - border;
-        const uint64_t i = (x | d) >> 32 == 0 ? (uint32_t)x / (uint32_t)d : x / d;
-        return (uint32_t)i + (place < border ? 0 : longer);
+        const uint32_t border = (each + 1) * longer;
+        return place < border ? place / (each + 1) : (place - border) / each + longer;
     }
 };
-__host__ __device__ inline uint32_t tiles_of(uint32_t begin, uint32_t end, uint32_t tile_tokens)
+// tiles of 2^shift tokens, on a grid that starts at token 0
+__host__ __device__ inline uint32_t tiles_of(uint32_t begin, uint32_t end, uint32_t shift)
 {
-    return end <= begin ? 0 : (end - 1) / tile_tokens - begin / tile_tokens + 1;
+    return end <= begin ? 0 : ((end - 1) >> shift) - (begin >> shift) + 1;
 }
 
 inline bool aligned(const void *p, size_t n)

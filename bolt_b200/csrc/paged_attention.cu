@@ -34,7 +34,8 @@ struct AttentionParams {
     uint32_t sequences, heads, group, head_blocks, table_pages, window;
     float scale, out_scale;
     int i8, q_f16, out_kind;   // 0 binary32, 1 binary16, 2 u8
-    uint32_t team, part_count, q_vectors, out_pairs;   // warps that share a unit; parts of the row
+    uint32_t team, part_count, share_bytes, out_pairs;
+    uint32_t even_bytes, to_1152;   // 0x00FF00FF, 0x64806480   // warps that share a unit; parts of the row
     float *parts;   // workspace: two partial results for every part,
     struct Cut *cuts;   // and what is to be joined
     int *status;
@@ -77,44 +78,45 @@ __device__ __forceinline__ void store_pair(const AttentionParams &p, uint64_t at
 // ---- how the work is divided -----------------------------------------------------------------------------------
 // A unit is one sequence, key head and block of query heads; it has tiles of team x STEP tokens on a grid that starts at
 // token 0.  All units' tiles stand in one row, in which every team of warps takes an equal, contiguous part.
-constexpr int WARPS = 8;
+constexpr int MAX_WARPS = 16;
 constexpr uint32_t MAX_SEQUENCES = 65535;
 constexpr uint32_t BY_WARP = 1024;    // up to so many sequences every warp counts for itself; beyond, the CTA's share the counting
 struct Found {
-    uint64_t first;
-    uint32_t sequence;
+    uint32_t sequence, first;
 };
 struct Counting {     // shared memory
-    uint64_t sums[WARPS];
-    Found found[WARPS];
+    uint32_t sums[MAX_WARPS];
+    Found found[MAX_WARPS];
 };
-__device__ __forceinline__ uint32_t count_tiles(const AttentionParams &p, uint32_t s, uint32_t tile_tokens)
+__device__ __forceinline__ uint32_t count_tiles(const AttentionParams &p, uint32_t s, uint32_t tile_shift)
 {
     uint32_t begin, end;
     live_tokens(p, s, &begin, &end);
-    return tiles_of(begin, end, tile_tokens);
+    return tiles_of(begin, end, tile_shift);
 }
 // By all warps of a CTA, for each its team's part: the row's length, and the sequence that holds the part's first tile with
 // that sequence's own first place.
-__device__ __forceinline__ uint64_t locate(const AttentionParams &p, uint32_t units, uint32_t tile_tokens, uint32_t team, Counting *c, Found *mine)
+template <int WARPS>
+__device__ __forceinline__ uint32_t locate(const AttentionParams &p, uint32_t units, uint32_t tile_shift, uint32_t team, Counting *c, Found *mine)
 {
     const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, teams = WARPS / team;
     const bool shared = p.sequences > BY_WARP;
     const uint32_t segment = shared ? (p.sequences + WARPS - 1) / WARPS : p.sequences;
     const uint32_t a = shared ? min(warp * segment, p.sequences) : 0, b = min(a + segment, p.sequences), per = (b - a + 31) / 32;
     const uint32_t s0 = min(a + lane * per, b), s1 = min(s0 + per, b);
-    uint64_t own = 0;
+    uint32_t own = 0;
+#pragma unroll 1
     for (uint32_t s = s0; s < s1; ++s) {
-        own += count_tiles(p, s, tile_tokens);
+        own += count_tiles(p, s, tile_shift);
     }
     own *= units;
-    uint64_t upto = own;
+    uint32_t upto = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const uint64_t v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+        const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
         upto += lane >= o ? v : 0;
     }
-    uint64_t total = __shfl_sync(0xFFFFFFFFu, upto, 31);
+    uint32_t total = __shfl_sync(0xFFFFFFFFu, upto, 31);
     if (shared) {
         if (lane == 0) {
             c->sums[warp] = total;
@@ -127,19 +129,20 @@ __device__ __forceinline__ uint64_t locate(const AttentionParams &p, uint32_t un
         }
     }
     const Parts parts(total, p.part_count);
-    mine->first = 0;
-    mine->sequence = 0;     // (always something inside the arrays, even if lengths change under the call)
+    *mine = Found{0, 0};     // (always something inside the arrays, even if lengths change under the call)
+#pragma unroll 1
     for (uint32_t t = shared ? 0 : warp / team; t < (shared ? teams : warp / team + 1); ++t) {
         const uint32_t part = blockIdx.x * teams + t;
-        const uint64_t place = parts.begin(part), first = upto - own;
-        const uint32_t holder = __ballot_sync(0xFFFFFFFFu, part < parts.n && place >= first && place < upto);
+        const uint32_t place = parts.begin(part);
+        const uint32_t holder = __ballot_sync(0xFFFFFFFFu, part < parts.n && place >= upto - own && place < upto);
         if (holder == 0) {
             continue;
         }
-        Found f = {first, s0};
+        Found f = {s0, upto - own};
         if (holder >> lane & 1) {
+#pragma unroll 1
             while (f.sequence < s1) {
-                const uint64_t next = f.first + (uint64_t)count_tiles(p, f.sequence, tile_tokens) * units;
+                const uint32_t next = f.first + count_tiles(p, f.sequence, tile_shift) * units;
                 if (place < next) {
                     break;
                 }
@@ -213,6 +216,18 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)   // c = a b
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f), "f"(0.f), "f"(0.f), "f"(0.f));
+}
+__device__ __forceinline__ float2 shared_pair(uint32_t at)
+{
+    float2 v;
+    asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+    return v;
+}
 __device__ __forceinline__ float exp2_fast(float x)
 {
     float y;
@@ -227,10 +242,12 @@ __device__ __forceinline__ float reciprocal(float x)    // within 2^-23
 }
 // Bytes 0 and 2 (shift 0) or 1 and 3 (shift 8) of a word, as signed numbers, in binary16: 0x6400 is 1024, whose last ten bits
 // count ones, so 0x6400 | (byte ^ 0x80) is 1152 + byte.
+// (The two constants come from the parameters: as immediates they take an instruction and a half more, since a three-way
+// logic instruction has room for one.)
 template <int SHIFT>
-__device__ __forceinline__ uint32_t bytes_to_half2(uint32_t x)
+__device__ __forceinline__ uint32_t bytes_to_half2(const AttentionParams &p, uint32_t x)
 {
-    const uint32_t y = ((x >> SHIFT) & 0x00FF00FFu) ^ 0x64806480u, k = 0x64806480u;
+    const uint32_t y = ((x >> SHIFT) & p.even_bytes) ^ p.to_1152, k = 0x64806480u;
     const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&y), *reinterpret_cast<const __half2 *>(&k));
     return *reinterpret_cast<const uint32_t *>(&h);
 }
@@ -253,10 +270,14 @@ struct Shape {
     static constexpr uint32_t ALL = STEP == 32 ? 0xFFFFFFFFu : 0xFFFFu;
     static constexpr int SLOT = STEP * PITCH + (I8 ? STEP * 4 : 0);
     static constexpr int HEADS = 8 * HB;
-    static constexpr bool Q_IN_REGISTERS = HB == 1 && DP <= 128;
-    static constexpr int Q_PITCH = DP * 2 + 16, Q_BYTES = Q_IN_REGISTERS ? 0 : 2 * HEADS * Q_PITCH;
-    static constexpr int MERGE = WARPS / 2 * 32 * 32 * 4;                        // 32 numbers of every lane of half the warps
-    static constexpr int FIXED = Q_BYTES + MERGE + 2048;
+    static constexpr int NUMBERS = DP / 8 * 2 * HB;                              // running sums of a lane
+    // Steps are chains of dependent instructions: sixteen warps (128 registers a lane) hide them where the running sums fit.
+    static constexpr int WARPS = NUMBERS <= 32 && HB == 1 ? 16 : 8;
+    static constexpr int Q_PITCH = DP * 2 + 16, Q_BYTES = 2 * HEADS * Q_PITCH;   // queries of a team
+    static constexpr int TEAMS = 4 * Q_BYTES <= 20480 ? 4 : (2 * Q_BYTES <= 20480 ? 2 : 1);
+    static constexpr int GO = 16, MERGE = WARPS / 2 * GO * 32 * 4;               // numbers of a lane of half the warps
+    static constexpr int SMALL = 1024 + WARPS * 128;
+    static constexpr int FIXED = TEAMS * Q_BYTES + MERGE + SMALL;
     static constexpr int FIT = (232448 - FIXED) / (WARPS * SLOT);
     static constexpr int SLOTS = FIT > 6 ? 6 : FIT;                              // ring of a warp: K, V, K, V ...
     static constexpr int SMEM = FIXED + WARPS * SLOTS * SLOT;
@@ -266,7 +287,7 @@ struct Shape {
 
 // What a warp loads next: a run of tiles of one unit whose pages are at most 32 neighbours of the table, one in each lane.
 struct Run {
-    uint32_t unit, begin, end;
+    uint32_t head, begin, end;
     uint32_t left;                         // tiles
     uint32_t token;                        // first one of the warp's step
     uint32_t first_page;                   // of the table's row
@@ -274,23 +295,27 @@ struct Run {
 };
 
 template <int DP, bool I8, int HB>
-__global__ void __launch_bounds__(32 * WARPS, 1) paged_attention_kernel(const __grid_constant__ AttentionParams p)
+__global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attention_kernel(const __grid_constant__ AttentionParams p)
 {
     using S = Shape<DP, I8, HB>;
+    constexpr int WARPS = S::WARPS;
     extern __shared__ __align__(16) char smem[];
-    char *const q_smem = smem;
-    float *const merge = reinterpret_cast<float *>(smem + S::Q_BYTES);
-    char *const small = smem + S::Q_BYTES + S::MERGE;
+    float *const merge = reinterpret_cast<float *>(smem + S::TEAMS * S::Q_BYTES);
+    char *const small = smem + S::TEAMS * S::Q_BYTES + S::MERGE;
     Counting *const counting = reinterpret_cast<Counting *>(small);             // 192 bytes
-    float *const factor = reinterpret_cast<float *>(small + 256);               // [16]
-    float *const warp_m = factor + 16, *const warp_l = warp_m + WARPS * 16;     // [WARPS][16]
-    uint32_t *const masks = reinterpret_cast<uint32_t *>(warp_l + WARPS * 16);  // [WARPS][8]
-    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, c4 = lane % 4;
+    float *const factors = reinterpret_cast<float *>(small + 512);              // [TEAMS][16]
+    float *const warp_m = reinterpret_cast<float *>(small + 1024), *const warp_l = warp_m + WARPS * 16;     // [WARPS][16]
+    uint32_t lane, warp = threadIdx.x / 32;
+    asm volatile("mov.u32 %0, %%laneid;" : "=r"(lane));     // (kept in a register, not asked for again and again)
+    asm volatile("mov.u32 %0, %0;" : "+r"(warp));
+    const uint32_t g = lane / 4, c4 = lane % 4;
     char *const ring = smem + S::FIXED + warp * S::SLOTS * S::SLOT;
     const uint32_t dim = p.cache.dim, pieces = dim * S::SIZE / 16, units = p.cache.kv_heads * p.head_blocks;
-    const uint32_t team = S::Q_IN_REGISTERS ? p.team : WARPS, member = warp % team, teams = WARPS / team;
+    const uint32_t team = p.team, member = warp % team, teams = WARPS / team;
     const uint32_t tile_tokens = team * S::STEP, tile_shift = __ffs(tile_tokens) - 1;
     const uint32_t part = blockIdx.x * teams + warp / team;
+    char *const q_smem = smem + warp / team * S::Q_BYTES;
+    float *const factor = factors + warp / team * 16;
 
     if (dim < DP) {   // what no copy fills counts as zeros
         for (uint32_t i = lane; i < S::SLOTS * S::SLOT / 16; i += 32) {
@@ -300,10 +325,10 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_attention_kernel(const __
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");    // nothing in front of this touches global memory
     Found found;
-    const uint64_t total = locate(p, units, tile_tokens, team, counting, &found);
+    const uint32_t total = locate<WARPS>(p, units, tile_shift, team, counting, &found);
     const Parts parts(total, p.part_count);
-    uint64_t place = part < parts.n ? parts.begin(part) : 0;
-    const uint64_t stop = part < parts.n ? parts.begin(part + 1) : 0;
+    uint32_t place = part < parts.n ? parts.begin(part) : 0;
+    const uint32_t stop = part < parts.n ? parts.begin(part + 1) : 0;
     if (lane == 0 && member == 0) {
         p.cuts[part].parts = 0;
     }
@@ -320,13 +345,8 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_attention_kernel(const __
   if (place < stop) {
     uint32_t sequence = found.sequence, begin, end;
     live_tokens(p, sequence, &begin, &end);
-    uint32_t tiles = max(tiles_of(begin, end, tile_tokens), 1u), unit, tile;
-    {
-        const uint64_t within = place - found.first;   // of the sequence's tiles x units
-        const uint64_t u = within >> 32 == 0 ? (uint32_t)within / tiles : within / tiles;
-        unit = (uint32_t)min(u, (uint64_t)units - 1);
-        tile = (uint32_t)(within - u * tiles);
-    }
+    uint32_t tiles = max(tiles_of(begin, end, tile_shift), 1u);
+    uint32_t unit = min((place - found.first) / tiles, units - 1), tile = (place - found.first) % tiles;
 
     // ---- the copies ----
     const uint32_t page_size = p.cache.page_size;
@@ -336,14 +356,13 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_attention_kernel(const __
     const uint32_t run_tiles = 1 + (uint32_t)min((31ull * page_size - min(31ull * page_size, (unsigned long long)S::STEP + page_size - 2)) / tile_tokens, 1ull << 20);
     Run run, ahead;
     // the cursor behind `ahead`
-    uint64_t left = stop - place;
-    uint32_t a_sequence = sequence, a_unit = unit, a_tile = tile, a_tiles = tiles, a_begin = begin, a_end = end;
+    uint32_t left = stop - place, a_sequence = sequence, a_unit = unit, a_tile = tile, a_tiles = tiles, a_begin = begin, a_end = end;
     auto look_ahead = [&]() {
-        ahead.left = (uint32_t)min((uint64_t)min(run_tiles, a_tiles - a_tile), left);
+        ahead.left = min(min(run_tiles, a_tiles - a_tile), left);
         if (ahead.left == 0) {
             return;
         }
-        ahead.unit = a_unit;
+        ahead.head = a_unit / p.head_blocks;
         ahead.begin = a_begin;
         ahead.end = a_end;
         ahead.token = (((a_begin >> tile_shift) + a_tile) << tile_shift) + member * S::STEP;
@@ -358,7 +377,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_attention_kernel(const __
                 a_unit = 0;
                 a_sequence = next_sequence(p, a_sequence);
                 live_tokens(p, a_sequence, &a_begin, &a_end);
-                a_tiles = max(tiles_of(a_begin, a_end, tile_tokens), 1u);
+                a_tiles = max(tiles_of(a_begin, a_end, tile_shift), 1u);
             }
         }
     };
@@ -374,193 +393,154 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_attention_kernel(const __
     enter();
     uint64_t row = 0, scale_row = 0;    // elements of the lane's row in the tile at hand
     uint32_t live = 0;                  // its tokens that count
-    uint32_t fill_slot = 0;    // items: K, V, K, V ...
     const uint32_t copy_row = lane / (S::ROW / 16), copy_piece = lane % (S::ROW / 16);   // of the first piece that the lane copies
-    const uint64_t token_bytes = p.cache.token_stride * S::SIZE, lane_bytes = copy_row * token_bytes + copy_piece * 16;
-    const uint32_t ring_at = smem_at(ring), lane_at = ring_at + copy_row * S::PITCH + copy_piece * 16;
-    auto issue = [&](bool values) {
-        const uint32_t slot = fill_slot;
-        fill_slot = fill_slot + 1 == S::SLOTS ? 0 : fill_slot + 1;
-        if (!values) {
-            live = 0;
-            if (run.left != 0) {
-                const uint32_t head = run.unit / p.head_blocks, t = run.token + lane_token;
-                const uint32_t page = __shfl_sync(0xFFFFFFFFu, run.pages, page_index - run.first_page);
-                const bool inside = t >= run.begin && t < run.end, good = page < p.cache.pages;
-                if (inside && !good) {
-                    atomicExch(p.status, BAD_ATTENTION);
-                }
-                live = __ballot_sync(0xFFFFFFFFu, inside && good) & S::ALL;
-                row = good ? row_element(p.cache, page, at, head) : 0;
-                scale_row = I8 && good ? scale_element(p.cache, page, at, head) + (one_page ? lane_token : 0) : 0;
-                run.token += tile_tokens;
-                page_index += step_pages;
-                at += step_at;
-                if (at >= page_size) {
-                    at -= page_size;
-                    ++page_index;
-                }
-                if (--run.left == 0) {
-                    enter();
-                }
+    const uint64_t token_bytes = p.cache.token_stride * S::SIZE;
+    const uint32_t ring_at = smem_at(ring), lane_at = copy_row * S::PITCH + copy_piece * 16;
+    const bool plain = one_page && dim == DP;
+    uint32_t coming[S::SLOTS / 2];      // `live` of the steps that have been asked for and not been used
+    auto issue = [&](auto kind, uint32_t slot) {    // asks for K (and V) of the next step
+        constexpr bool values = decltype(kind)::value;
+        if constexpr (!values) {
+            // (a run that has come to its end has no tokens inside)
+            const uint32_t page = __shfl_sync(0xFFFFFFFFu, run.pages, page_index - run.first_page), t = run.token + lane_token;
+            const bool inside = t >= run.begin && t < run.end, good = page < p.cache.pages;
+            live = __ballot_sync(0xFFFFFFFFu, inside && good) & S::ALL;
+            if (live != S::ALL && inside && !good) {
+                atomicExch(p.status, BAD_ATTENTION);
             }
-            if (lane == 0) {
-                masks[warp * 8 + slot] = live;
+            row = good ? row_element(p.cache, page, at, run.head) : 0;
+            if (I8) {
+                scale_row = good ? scale_element(p.cache, page, at, run.head) + (one_page ? lane_token : 0) : 0;
+            }
+#pragma unroll
+            for (int k = 0; k + 1 < S::SLOTS / 2; ++k) {
+                coming[k] = coming[k + 1];
+            }
+            coming[S::SLOTS / 2 - 1] = live;
+            run.token += tile_tokens;
+            page_index += step_pages;
+            at += step_at;
+            if (at >= page_size) {
+                at -= page_size;
+                ++page_index;
+            }
+            --run.left;
+        }
+        constexpr int ROWS = 32 / (S::ROW / 16);      // rows of one instruction
+        const char *base = reinterpret_cast<const char *>(values ? p.v : p.k);
+        const uint32_t dst = slot + lane_at;
+        if (plain && live == S::ALL) {
+            const char *src = base + row * S::SIZE + copy_row * token_bytes + copy_piece * 16;
+#pragma unroll
+            for (int i = 0; i < S::STEP / ROWS; ++i) {
+                copy16(dst + i * ROWS * S::PITCH, src);
+                src += ROWS * token_bytes;
+            }
+        } else if (live != 0) {
+#pragma unroll 4
+            for (int i = 0; i < S::STEP / ROWS; ++i) {
+                const uint32_t r = copy_row + i * ROWS;
+                const uint64_t from = one_page ? row + r * p.cache.token_stride : __shfl_sync(0xFFFFFFFFu, row, r);
+                if (copy_piece < pieces) {
+                    const bool on = live >> r & 1;
+                    copy16(dst + i * ROWS * S::PITCH, on ? base + from * S::SIZE + copy_piece * 16 : base, on ? 16 : 0);
+                }
             }
         }
-        if (live != 0) {
-            constexpr int ROWS = 32 / (S::ROW / 16);      // rows of one instruction
-            const char *base = reinterpret_cast<const char *>(values ? p.v : p.k);
-            uint32_t dst = lane_at + slot * S::SLOT;
-            if (one_page && dim == DP && live == S::ALL) {
-                const char *src = base + row * S::SIZE + lane_bytes;
-#pragma unroll
-                for (int i = 0; i < S::STEP / ROWS; ++i) {
-                    copy16(dst + i * ROWS * S::PITCH, src);
-                    src += ROWS * token_bytes;
-                }
-            } else {
-#pragma unroll 4
-                for (int i = 0; i < S::STEP / ROWS; ++i) {
-                    const uint32_t r = copy_row + i * ROWS;
-                    const uint64_t from = one_page ? row + r * p.cache.token_stride : __shfl_sync(0xFFFFFFFFu, row, r);
-                    if (copy_piece < pieces) {
-                        const bool on = live >> r & 1;
-                        copy16(dst + i * ROWS * S::PITCH, on ? base + from * S::SIZE + copy_piece * 16 : base, on ? 16 : 0);
-                    }
-                }
-            }
-            if (I8 && lane < S::STEP) {
-                const float *s = values ? p.v_scale : p.k_scale;
-                const bool on = live >> lane & 1;
-                copy4(ring_at + slot * S::SLOT + S::STEP * S::PITCH + lane * 4, on ? s + scale_row : s, on ? 4 : 0);
+        if constexpr (I8) {
+            const bool on = live >> (lane % S::STEP) & 1;
+            if (S::STEP == 32 || lane < S::STEP) {
+                const float *scales = values ? p.v_scale : p.k_scale;
+                copy4(slot + S::STEP * S::PITCH + lane * 4, on ? scales + scale_row : scales, on ? 4 : 0);
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
+        if (!values && run.left == 0) {
+            if (ahead.left != 0) {
+                enter();
+            } else {
+                run.end = 0;
+                run.left = 0xFFFFFFFFu;
+            }
+        }
     };
     __syncwarp();
-#pragma unroll 1
-    for (int i = 0; i < S::SLOTS - 1; ++i) {
-        issue(i & 1);
-    }
-    uint32_t take_slot = 0;
-    // the next item is there; the slot of the one before it is filled again
-    auto next = [&](bool values) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(S::SLOTS - 2) : "memory");
-        __syncwarp();
-        issue(values != (S::SLOTS % 2 == 0));    // item n + SLOTS - 1
-        const uint32_t slot = take_slot;
-        take_slot = take_slot + 1 == S::SLOTS ? 0 : take_slot + 1;
-        return slot;
-    };
 
-    // ---- unit by unit ----
+    // ---- item by item (K, V, K, V ...) ----
+    // In turn n the warp uses item n and asks for item n + SLOTS - 1, into the slot of item n - 1.  The first turns only
+    // ask, so that the code, which a short call has to fetch before it can run, is there once.
     constexpr int NT = S::STEP / 8, KS = DP / 16, TILES_D = DP / 8;
-    while (place < stop) {
+    constexpr bool EVEN = S::SLOTS % 2 == 0;        // then a K turn asks for V, and a V turn for K
+    uint32_t item = ring_at + S::SLOT, count = 0, done = 0;    // tiles of the unit, and how many of them are through
+    uint32_t head0 = 0, heads_here = 0, mask = 0;
+    float fac[HB], m[HB], l[HB], keep[HB], w[HB][NT][2], acc[TILES_D][2 * HB], top_unit = 0.f;
+    const uint32_t q_at = smem_at(q_smem + (lane % 16) * S::Q_PITCH + lane / 16 * 16);
+    int n = 1 - S::SLOTS;
+    auto turn = [&](auto asks_for_values) {
+        if (n >= 0) {
+            // the item is there, and everybody is through with the one before it
+            asm volatile("cp.async.wait_group %0;" ::"n"(S::SLOTS - 2) : "memory");
+            __syncwarp();
+        }
+        issue(asks_for_values, item == ring_at ? ring_at + (S::SLOTS - 1) * S::SLOT : item - S::SLOT);
+        return n >= 0;
+    };
+    auto turned = [&]() {
+        ++n;
+        item = item == ring_at + (S::SLOTS - 1) * S::SLOT ? ring_at : item + S::SLOT;
+    };
+#pragma unroll 1
+    for (;;) {
+     if (!EVEN || n != 1 - S::SLOTS) {
+      mask = coming[0];
+      if (turn(std::bool_constant<EVEN>())) {
+       if (done == count) {
+        // ---- a unit begins ----
         const uint32_t head = unit / p.head_blocks, block = unit % p.head_blocks;
-        const uint32_t heads_here = min((uint32_t)S::HEADS, p.group - block * S::HEADS), head0 = head * p.group + block * S::HEADS;
-        const uint32_t count = (uint32_t)min((uint64_t)(tiles - tile), stop - place);
+        heads_here = min((uint32_t)S::HEADS, p.group - block * S::HEADS);
+        head0 = head * p.group + block * S::HEADS;
+        count = min(tiles - tile, stop - place);
+        done = 0;
         // Queries: brought to 2^13 .. 2^14 by a power of two (which the factor of the scores takes back), then two binary16
         // numbers each, in the rows (hi of every head, lo of every head) of the matrix instruction's left operand.  Bytes come
         // out of their words in the order 0, 2, 1, 3; the queries' elements stand in the same order.
         const uint64_t q_row = sequence * p.q_stride + (uint64_t)head0 * dim;
-        auto query = [&](uint32_t h, uint32_t d) {
-            if (h >= heads_here || d >= dim) {
-                return 0.f;
-            }
-            const uint64_t e = q_row + h * dim + d;
-            return p.q_f16 ? load1(reinterpret_cast<const __half *>(p.q) + e) : load1(reinterpret_cast<const float *>(p.q) + e);
-        };
-        auto powers = [&](int top, float &up, float &fac) {
-            const int e = max(top >> 23, 20);
-            up = __int_as_float((127 + 13 + 127 - e) << 23);
-            fac = __int_as_float((e - 13) << 23) * (p.scale * LOG2E);
-        };
-        float fac[HB];
-        uint32_t qa[S::Q_IN_REGISTERS ? KS : 1][4];
-        const uint32_t q_at = smem_at(q_smem + (lane % 16) * S::Q_PITCH + lane / 16 * 16);
-        if constexpr (S::Q_IN_REGISTERS) {
-            // columns 2c, 2c + 1, 2c + 8, 2c + 9 of every step (rows of heads that do not exist repeat the first: nobody reads
-            // their results)
-            float x[KS][4], up;
+#pragma unroll 1
+        for (uint32_t h = member; h < S::HEADS; h += team) {
+            // (rows of heads that do not exist repeat the first: nobody reads their results)
+            const uint64_t from = q_row + (h < heads_here ? h : 0) * dim;
+            float x[DP / 32];
             int top = 0;
-            const uint64_t mine = q_row + (g < heads_here ? g : 0) * dim + (I8 ? 4 : 2) * c4;
-            if (p.q_vectors && dim == DP) {
-                auto fetch = [&](auto *q) {
 #pragma unroll
-                    for (int s = 0; s < KS; ++s) {
-                        if constexpr (I8) {
-                            float v[4];
-                            load4(q + 16 * s, v);
-                            x[s][0] = v[0];
-                            x[s][1] = v[2];
-                            x[s][2] = v[1];
-                            x[s][3] = v[3];
-                        } else {
-                            load2(q + 16 * s, x[s][0], x[s][1]);
-                            load2(q + 16 * s + 8, x[s][2], x[s][3]);
-                        }
-                    }
-                };
-                if (p.q_f16) {
-                    fetch(reinterpret_cast<const __half *>(p.q) + mine);
-                } else {
-                    fetch(reinterpret_cast<const float *>(p.q) + mine);
+            for (int i = 0; i < DP / 32; ++i) {
+                const uint32_t d = lane + 32 * i;
+                x[i] = 0.f;
+                if (d < dim) {
+                    x[i] = p.q_f16 ? load1(reinterpret_cast<const __half *>(p.q) + from + d) : load1(reinterpret_cast<const float *>(p.q) + from + d);
                 }
-            } else {
-#pragma unroll
-                for (int s = 0; s < KS; ++s) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        x[s][e] = query(g, 16 * s + (I8 ? 4 * c4 + e % 2 * 2 + e / 2 : 2 * c4 + e % 2 + e / 2 * 8));
-                    }
-                }
+                top = max(top, magnitude(x[i]));
+            }
+            const int e = max(__reduce_max_sync(0xFFFFFFFFu, top) >> 23, 20);
+            const float up = __int_as_float((127 + 13 + 127 - e) << 23);
+            if (lane == 0) {
+                factor[h] = __int_as_float((e - 13) << 23) * (p.scale * LOG2E);
             }
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    top = max(top, magnitude(x[s][e]));
-                }
-            }
-            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-            powers(top, up, fac[0]);
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                split_pair(x[s][0] * up, x[s][1] * up, qa[s][0], qa[s][1]);
-                split_pair(x[s][2] * up, x[s][3] * up, qa[s][2], qa[s][3]);
-            }
-        } else {
-            for (uint32_t h = warp; h < S::HEADS; h += WARPS) {
-                float x[DP / 32], up, f;
-                int top = 0;
-#pragma unroll
-                for (int i = 0; i < DP / 32; ++i) {
-                    x[i] = query(h, lane + 32 * i);
-                    top = max(top, magnitude(x[i]));
-                }
-                powers(__reduce_max_sync(0xFFFFFFFFu, top), up, f);
-                if (lane == 0) {
-                    factor[h] = f;
-                }
-#pragma unroll
-                for (int i = 0; i < DP / 32; ++i) {
-                    const uint32_t d = lane + 32 * i, r = d % 4;
-                    const uint32_t k = I8 ? d / 16 * 16 + d % 16 / 4 * 2 + r / 2 + r % 2 * 8 : d;
-                    const float v = x[i] * up;
-                    const __half hi = __float2half_rn(v);
-                    *reinterpret_cast<__half *>(q_smem + h * S::Q_PITCH + k * 2) = hi;
-                    *reinterpret_cast<__half *>(q_smem + (S::HEADS + h) * S::Q_PITCH + k * 2) = __float2half_rn(v - __half2float(hi));
-                }
-            }
-            __syncthreads();
-#pragma unroll
-            for (int b = 0; b < HB; ++b) {
-                fac[b] = factor[g + 8 * b];
+            for (int i = 0; i < DP / 32; ++i) {
+                const uint32_t d = lane + 32 * i, r = d % 4;
+                const uint32_t k = I8 ? d / 16 * 16 + d % 16 / 4 * 2 + r / 2 + r % 2 * 8 : d;
+                const float v = x[i] * up;
+                const __half hi = __float2half_rn(v);
+                *reinterpret_cast<__half *>(q_smem + h * S::Q_PITCH + k * 2) = hi;
+                *reinterpret_cast<__half *>(q_smem + (S::HEADS + h) * S::Q_PITCH + k * 2) = __float2half_rn(v - __half2float(hi));
             }
         }
-        float m[HB], l[HB], acc[TILES_D][2 * HB], top_unit = 0.f;
+        team_sync();
+#pragma unroll
+        for (int b = 0; b < HB; ++b) {
+            fac[b] = factor[g + 8 * b];
+        }
+        top_unit = 0.f;
 #pragma unroll
         for (int b = 0; b < HB; ++b) {
             m[b] = -INFINITY;
@@ -573,36 +553,24 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_attention_kernel(const __
                 acc[n][e] = 0.f;
             }
         }
-#pragma unroll 1
-        for (uint32_t i = 0; i < count; ++i) {
+       }
             // scores: [heads] x [tokens]
-            const uint32_t ks = next(false);
-            const char *const kt = ring + ks * S::SLOT;
-            const uint32_t mask = masks[warp * 8 + ks];
             float sc[NT][4];
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
-            }
-            if (mask != 0) {
-                uint32_t q_lo[4];
+            {
+                uint32_t qa[4], q_lo[4];
                 auto multiply = [&](int s, int j, uint32_t b0, uint32_t b1) {
-                    if constexpr (HB == 1) {
-                        if constexpr (S::Q_IN_REGISTERS) {
-                            mma(sc[j], qa[s], b0, b1);
-                        } else {
-                            mma(sc[j], qa[0], b0, b1);
-                        }
+                    if (s == 0) {
+                        mma_first(sc[j], qa, b0, b1);
                     } else {
-                        mma(sc[j], qa[0], b0, b1);
+                        mma(sc[j], qa, b0, b1);
+                    }
+                    if constexpr (HB == 2) {
                         mma(sc[j], q_lo, b0, b1);
                     }
                 };
 #pragma unroll
                 for (int s = 0; s < KS; ++s) {
-                    if constexpr (!S::Q_IN_REGISTERS) {
-                        matrices(qa[0], q_at + s * 32);
-                    }
+                    matrices(qa, q_at + s * 32);
                     if constexpr (HB == 2) {
                         matrices(q_lo, q_at + 16 * S::Q_PITCH + s * 32);
                     }
@@ -610,44 +578,59 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_attention_kernel(const __
                     if constexpr (!I8) {
 #pragma unroll
                         for (int j = 0; j < NT; j += 2) {
-                            matrices(r, smem_at(kt + (8 * j + lane % 8 + lane / 16 * 8) * S::PITCH + s * 32 + lane / 8 % 2 * 16));
+                            matrices(r, item + (lane % 8 + lane / 16 * 8) * S::PITCH + lane / 8 % 2 * 16 + 8 * j * S::PITCH + s * 32);
                             multiply(s, j, r[0], r[1]);
                             multiply(s, j + 1, r[2], r[3]);
                         }
                     } else if constexpr (S::STEP == 32) {
-                        matrices(r, smem_at(kt + lane * S::PITCH + s * 16));
+                        matrices(r, item + lane * S::PITCH + s * 16);
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            multiply(s, j, bytes_to_half2<0>(r[j]), bytes_to_half2<8>(r[j]));
+                            multiply(s, j, bytes_to_half2<0>(p, r[j]), bytes_to_half2<8>(p, r[j]));
                         }
                     } else {
-                        matrices(r, smem_at(kt + lane % 16 * S::PITCH + s * 16));
-                        multiply(s, 0, bytes_to_half2<0>(r[0]), bytes_to_half2<8>(r[0]));
-                        multiply(s, 1, bytes_to_half2<0>(r[1]), bytes_to_half2<8>(r[1]));
+                        matrices(r, item + lane % 16 * S::PITCH + s * 16);
+                        multiply(s, 0, bytes_to_half2<0>(p, r[0]), bytes_to_half2<8>(p, r[0]));
+                        multiply(s, 1, bytes_to_half2<0>(p, r[1]), bytes_to_half2<8>(p, r[1]));
                     }
                 }
             }
             // weights: exp(s - m) times 2^14, which the division by their sum takes back
-            float keep[HB], w[HB][NT][2];
-            auto weights = [&](auto all) {
 #pragma unroll
-              for (int b = 0; b < HB; ++b) {
+            for (int j = 0; j < NT; ++j) {
+                float unit_k[2] = {1.f, 1.f};
+                if constexpr (I8) {
+                    const float2 u = shared_pair(item + S::STEP * S::PITCH + (8 * j + 2 * c4) * 4);
+                    unit_k[0] = reciprocal(u.x);
+                    unit_k[1] = reciprocal(u.y);
+                }
+#pragma unroll
+                for (int b = 0; b < HB; ++b) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        w[b][j][e] = (HB == 1 ? sc[j][e] + sc[j][e + 2] : sc[j][e + 2 * b]) * (fac[b] * unit_k[e]);
+                    }
+                }
+            }
+            if (mask != S::ALL) {
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const bool on = mask >> (8 * j + 2 * c4 + e) & 1;
+#pragma unroll
+                        for (int b = 0; b < HB; ++b) {
+                            w[b][j][e] = on ? w[b][j][e] : -INFINITY;
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < HB; ++b) {
                 float top = m[b];
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
-                    float unit_k[2] = {1.f, 1.f};
-                    if constexpr (I8) {
-                        const float2 u = *reinterpret_cast<const float2 *>(kt + S::STEP * S::PITCH + (8 * j + 2 * c4) * 4);
-                        unit_k[0] = reciprocal(u.x);
-                        unit_k[1] = reciprocal(u.y);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float s = HB == 1 ? sc[j][e] + sc[j][e + 2] : sc[j][e + 2 * b];
-                        const bool on = all.value || (mask >> (8 * j + 2 * c4 + e) & 1);
-                        w[b][j][e] = on ? s * (fac[b] * unit_k[e]) : -INFINITY;
-                        top = fmaxf(top, w[b][j][e]);
-                    }
+                    top = fmaxf(top, fmaxf(w[b][j][0], w[b][j][1]));
                 }
                 top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
@@ -663,27 +646,31 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_attention_kernel(const __
                         l[b] += w[b][j][e];
                     }
                 }
-              }
-            };
-            if (mask == S::ALL) {
-                weights(std::true_type());
-            } else {
-                weights(std::false_type());
             }
-            const uint32_t vs = next(true);
-            if (mask == 0) {
-                continue;
-            }
-            const char *const vt = ring + vs * S::SLOT;
+      }
+      turned();
+     }
+     if (turn(std::bool_constant<!EVEN>())) {
+        if (mask != 0) {
             if constexpr (I8) {
                 // Rows of bytes have units of their own.  They go into the weights, relative to the largest unit so far:
                 // weights stay within binary16.
                 float unit_v[NT][2], top = top_unit;
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
-                    const float2 u = *reinterpret_cast<const float2 *>(vt + S::STEP * S::PITCH + (8 * j + 2 * c4) * 4);
-                    unit_v[j][0] = mask >> (8 * j + 2 * c4) & 1 ? reciprocal(u.x) : 0.f;
-                    unit_v[j][1] = mask >> (8 * j + 2 * c4 + 1) & 1 ? reciprocal(u.y) : 0.f;
+                    const float2 u = shared_pair(item + S::STEP * S::PITCH + (8 * j + 2 * c4) * 4);
+                    unit_v[j][0] = reciprocal(u.x);
+                    unit_v[j][1] = reciprocal(u.y);
+                }
+                if (mask != S::ALL) {
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        unit_v[j][0] = mask >> (8 * j + 2 * c4) & 1 ? unit_v[j][0] : 0.f;
+                        unit_v[j][1] = mask >> (8 * j + 2 * c4 + 1) & 1 ? unit_v[j][1] : 0.f;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
                     top = fmaxf(top, fmaxf(unit_v[j][0], unit_v[j][1]));
                 }
                 top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
@@ -727,7 +714,11 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_attention_kernel(const __
                 }
             };
             auto weigh = [&](float (&c)[4], int t, uint32_t b0, uint32_t b1) {
-                mma(c, pa[0][t], b0, b1);
+                if (t == 0) {
+                    mma_first(c, pa[0][t], b0, b1);
+                } else {
+                    mma(c, pa[0][t], b0, b1);
+                }
                 if constexpr (HB == 2) {
                     mma(c, pa[HB - 1][t], b0, b1);
                 }
@@ -735,11 +726,11 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_attention_kernel(const __
             if constexpr (!I8) {
 #pragma unroll
                 for (int n = 0; n < TILES_D; n += 2) {
-                    float c0[4] = {0.f, 0.f, 0.f, 0.f}, c1[4] = {0.f, 0.f, 0.f, 0.f};
+                    float c0[4], c1[4];
 #pragma unroll
                     for (int t = 0; t < NT / 2; ++t) {
                         uint32_t r[4];
-                        matrices_t(r, smem_at(vt + (16 * t + lane % 16) * S::PITCH + n * 16 + lane / 16 * 16));
+                        matrices_t(r, item + lane % 16 * S::PITCH + lane / 16 * 16 + 16 * t * S::PITCH + n * 16);
                         weigh(c0, t, r[0], r[1]);
                         weigh(c1, t, r[2], r[3]);
                     }
@@ -749,15 +740,15 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_attention_kernel(const __
             } else {
 #pragma unroll
                 for (int n = 0; n < TILES_D; n += 4) {     // 32 bytes of a row: even and odd elements of two pieces
-                    float c[4][4] = {};
+                    float c[4][4];
 #pragma unroll
                     for (int t = 0; t < NT / 2; ++t) {
                         uint32_t r[4];
-                        matrices_t(r, smem_at(vt + (16 * t + lane % 16) * S::PITCH + n * 8 + lane / 16 * 16));
-                        weigh(c[0], t, bytes_to_half2<0>(r[0]), bytes_to_half2<0>(r[1]));
-                        weigh(c[1], t, bytes_to_half2<8>(r[0]), bytes_to_half2<8>(r[1]));
-                        weigh(c[2], t, bytes_to_half2<0>(r[2]), bytes_to_half2<0>(r[3]));
-                        weigh(c[3], t, bytes_to_half2<8>(r[2]), bytes_to_half2<8>(r[3]));
+                        matrices_t(r, item + lane % 16 * S::PITCH + lane / 16 * 16 + 16 * t * S::PITCH + n * 8);
+                        weigh(c[0], t, bytes_to_half2<0>(p, r[0]), bytes_to_half2<0>(p, r[1]));
+                        weigh(c[1], t, bytes_to_half2<8>(p, r[0]), bytes_to_half2<8>(p, r[1]));
+                        weigh(c[2], t, bytes_to_half2<0>(p, r[2]), bytes_to_half2<0>(p, r[3]));
+                        weigh(c[3], t, bytes_to_half2<8>(p, r[2]), bytes_to_half2<8>(p, r[3]));
                     }
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
@@ -766,6 +757,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_attention_kernel(const __
                 }
             }
         }
+        if (++done == count) {
         // ---- the warps' shares, and out ----
         const bool whole = count == tiles;
         float *const share = p.parts + ((uint64_t)part * 2 + (tile != 0 ? 0 : 1)) * S::PART;
@@ -808,8 +800,8 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_attention_kernel(const __
         if (!whole && tile == 0 && member == 0 && lane == 0) {
             p.cuts[part] = Cut{parts.of(place + tiles - 1) - part + 1, sequence, head0, heads_here};
         }
-        // Sums of the team's upper half are added to the lower half's, and so on; 32 numbers of a lane at a time.
-        constexpr int NUMBERS = TILES_D * 2 * HB, GO = NUMBERS < 32 ? NUMBERS : 32;
+        // Sums of the team's upper half are added to the lower half's, and so on; GO numbers of a lane at a time.
+        constexpr int NUMBERS = S::NUMBERS, GO = S::GO;
 #pragma unroll
         for (int x = 0; x < NUMBERS; ++x) {
             acc[x / (2 * HB)][x % (2 * HB)] *= own[x % (2 * HB) / 2];
@@ -818,7 +810,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_attention_kernel(const __
         for (int x0 = 0; x0 < NUMBERS; x0 += GO) {
 #pragma unroll 1
             for (uint32_t half = team / 2; half != 0; half /= 2) {
-                float *const to = merge + (warp0 / 2 + member % half) * 1024 + lane;
+                float *const to = merge + (warp0 / 2 + member % half) * GO * 32 + lane;
                 if (member >= half && member < 2 * half) {
 #pragma unroll
                     for (int x = 0; x < GO; ++x) {
@@ -836,35 +828,52 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_attention_kernel(const __
             }
         }
         if (member == 0) {
+            // neighbours of the row: pairs in two tiles, or (bytes) all four numbers of two tiles
+            auto pairs = [&](auto store) {
 #pragma unroll
-            for (int b = 0; b < HB; ++b) {
-                const uint32_t h = g + 8 * b;
-                const uint64_t to = sequence * p.out_stride + (uint64_t)(head0 + h) * dim;
+                for (int b = 0; b < HB; ++b) {
 #pragma unroll
-                for (int n = 0; n < TILES_D; n += 2) {
-                    // neighbours of the row: pairs in two tiles, or (bytes) all four numbers of two tiles
+                    for (int n = 0; n < TILES_D; n += 2) {
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const uint32_t d = I8 ? 8 * n + 4 * c4 + 2 * k : 8 * (n + k) + 2 * c4;
-                        const float x = I8 ? acc[n][2 * b + k] : acc[n + k][2 * b], y = I8 ? acc[n + 1][2 * b + k] : acc[n + k][2 * b + 1];
-                        if (!whole) {
-                            *reinterpret_cast<float2 *>(share + h * DP + d) = make_float2(x, y);
-                        } else if (h < heads_here && d < dim) {
-                            store_pair(p, to + d, x, y);
+                        for (int k = 0; k < 2; ++k) {
+                            const uint32_t d = I8 ? 8 * n + 4 * c4 + 2 * k : 8 * (n + k) + 2 * c4;
+                            store(g + 8 * b, d, I8 ? acc[n][2 * b + k] : acc[n + k][2 * b], I8 ? acc[n + 1][2 * b + k] : acc[n + k][2 * b + 1]);
                         }
                     }
                 }
+            };
+            const uint64_t to = sequence * p.out_stride + (uint64_t)head0 * dim;
+            if (!whole) {
+                pairs([&](uint32_t h, uint32_t d, float x, float y) { *reinterpret_cast<float2 *>(share + h * DP + d) = make_float2(x, y); });
+            } else if (p.out_pairs && p.out_kind == 0) {
+                pairs([&](uint32_t h, uint32_t d, float x, float y) {
+                    if (h < heads_here && d < dim) {
+                        *reinterpret_cast<float2 *>(reinterpret_cast<float *>(p.out) + to + h * dim + d) = make_float2(x, y);
+                    }
+                });
+            } else {
+                pairs([&](uint32_t h, uint32_t d, float x, float y) {
+                    if (h < heads_here && d < dim) {
+                        store_pair(p, to + h * dim + d, x, y);
+                    }
+                });
             }
         }
         // ---- the next unit ----
         place += count;
         tile = 0;
-        if (place < stop && ++unit == units) {
+        if (place >= stop) {
+            break;
+        }
+        if (++unit == units) {
             unit = 0;
             sequence = next_sequence(p, sequence);
             live_tokens(p, sequence, &begin, &end);
-            tiles = max(tiles_of(begin, end, tile_tokens), 1u);
+            tiles = max(tiles_of(begin, end, tile_shift), 1u);
         }
+        }
+      }
+     turned();
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   }
@@ -885,24 +894,36 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_attention_kernel(const __
     }
 }
 
-// Units that several parts have worked on: one query head of one of them for each `team` warps, which divide the shares
-// among themselves (as many as the teams that made them: fewer, larger parts mean more shares of a unit).
-template <int DP, int HB>
-__global__ void __launch_bounds__(32 * WARPS) paged_attention_join_kernel(const __grid_constant__ AttentionParams p, uint32_t team)
+// loads that are issued where they stand, all before the first result is needed
+__device__ __forceinline__ float load_now(const float *p)
 {
-    constexpr int HEADS = 8 * HB, PART = HEADS * (DP + 2), PER = DP / 32;
-    __shared__ float totals[WARPS], tops[WARPS], sums[WARPS][DP];
-    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, member = warp % team, warp0 = warp - member, h = blockIdx.y;
-    const uint32_t part = blockIdx.x * (WARPS / team) + warp / team;
+    float x;
+    asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(x) : "l"(p) : "memory");
+    return x;
+}
+__device__ __forceinline__ void load_now(const float *p, float &x, float &y)
+{
+    asm volatile("ld.global.cg.v2.f32 {%0, %1}, [%2];" : "=f"(x), "=f"(y) : "l"(p) : "memory");
+}
+// Units that several parts have worked on: a block for the part that has begun one, and for each eight query heads.  Shares
+// are read eight at a time, and the warps of a head (two) take every second eight.
+template <int DP, int HB>
+__global__ void __launch_bounds__(512) paged_attention_join_kernel(const __grid_constant__ AttentionParams p)
+{
+    constexpr int HEADS = 8 * HB, PART = HEADS * (DP + 2), PER = DP / 32, AT_ONCE = PER <= 4 ? 8 : 4;
+    __shared__ float other[8][DP + 2];
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, part = blockIdx.x, h = blockIdx.y * 8 + warp % 8, half = warp / 8;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const Cut cut = p.cuts[part];
-    const uint32_t n = h < cut.heads ? cut.parts : 0;
+    if (cut.parts == 0) {
+        return;
+    }
     // share c: what the part began (slot 1), or the following ones went on with (slot 0)
-    auto share = [&](uint32_t c) { return p.parts + ((uint64_t)(part + c) * 2 + (c == 0 ? 1 : 0)) * PART; };
-    const uint32_t c0 = n * member / team, c1 = n * (member + 1) / team;
+    const float *const shares = p.parts + (uint64_t)part * 2 * PART + PART;
+    auto share = [&](uint32_t c) { return shares + (c == 0 ? 0 : c * 2 * PART - PART); };
     float top = -INFINITY, all = 0.f, sum[PER] = {};
-    for (uint32_t c = c0 + lane; c < c1; c += 32) {
+    for (uint32_t c = lane; c < cut.parts; c += 32) {
         top = fmaxf(top, share(c)[HEADS * DP + h]);
     }
 #pragma unroll
@@ -910,79 +931,112 @@ __global__ void __launch_bounds__(32 * WARPS) paged_attention_join_kernel(const 
         top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
     }
     const float base = top == -INFINITY ? 0.f : top;
-#pragma unroll 8
-    for (uint32_t c = c0; c < c1; ++c) {
-        const float *q = share(c);
-        const float w = exp2_fast(q[HEADS * DP + h] - base);
-        all = fmaf(q[HEADS * (DP + 1) + h], w, all);
+    for (uint32_t c0 = half * AT_ONCE; c0 < cut.parts; c0 += 2 * AT_ONCE) {
+        float x[AT_ONCE][PER], w[AT_ONCE], l[AT_ONCE];
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+            const float *q = share(min(c0 + i, cut.parts - 1));
+            w[i] = load_now(q + HEADS * DP + h);
+            l[i] = load_now(q + HEADS * (DP + 1) + h);
+#pragma unroll
+            for (int k = 0; k < PER; k += 2) {
+                load_now(q + h * DP + lane * PER + k, x[i][k], x[i][k + 1]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+            const bool on = c0 + i < cut.parts;
+            const float v = exp2_fast(w[i] - base);
+            all = on ? fmaf(l[i], v, all) : all;
+#pragma unroll
+            for (int k = 0; k < PER; ++k) {
+                sum[k] = on ? fmaf(x[i][k], v, sum[k]) : sum[k];
+            }
+        }
+    }
+    if (half == 1) {
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
-            sum[k] = fmaf(q[h * DP + lane + 32 * k], w, sum[k]);
+            other[warp % 8][lane * PER + k] = sum[k];
         }
-    }
-    if (lane == 0) {
-        tops[warp] = top;
-        totals[warp] = all;
-    }
-#pragma unroll
-    for (int k = 0; k < PER; ++k) {
-        sums[warp][lane + 32 * k] = sum[k];
+        if (lane == 0) {
+            other[warp % 8][DP] = all;
+        }
     }
     __syncthreads();
-    if (n == 0) {
+    if (half == 1 || h >= cut.heads) {
         return;
     }
-    top = -INFINITY;
-    for (uint32_t w = 0; w < team; ++w) {
-        top = fmaxf(top, tops[warp0 + w]);
-    }
-    const float floor = top == -INFINITY ? 0.f : top;
-    all = 0.f;
-    for (uint32_t w = 0; w < team; ++w) {
-        all = fmaf(totals[warp0 + w], exp2_fast(tops[warp0 + w] - floor), all);
-    }
+    all += other[warp][DP];
     const uint32_t hq = cut.head0 + h;
     const float inv = all == 0.f ? 0.f : __frcp_rn(all);
-    for (uint32_t d = member * 32 + lane; d < p.cache.dim; d += 32 * team) {
-        float x = 0.f;
-        for (uint32_t w = 0; w < team; ++w) {
-            x = fmaf(sums[warp0 + w][d], exp2_fast(tops[warp0 + w] - floor), x);
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const uint32_t d = lane * PER + k;
+        if (d < p.cache.dim) {
+            store_out(p, cut.sequence * p.out_stride + (uint64_t)hq * p.cache.dim + d, (sum[k] + other[warp][d]) * inv);
         }
-        store_out(p, cut.sequence * p.out_stride + (uint64_t)hq * p.cache.dim + d, x * inv);
     }
-    if (p.lse != nullptr && member == 0 && lane == 0) {
+    if (p.lse != nullptr && lane == 0) {
         p.lse[(uint64_t)cut.sequence * p.heads + hq] = (top + log2f(all) - 14.f) * LN2;
     }
 }
 
+// The team: as many warps as leave a part for every unit, so that few units mean few shares to join, and with many units no
+// more warps than need be wait for others at a unit's end.
+template <int DP, bool I8, int HB>
+EE plan(const DeviceCtx *c, AttentionParams *p, uint64_t units)
+{
+    using S = Shape<DP, I8, HB>;
+    const uint32_t ctas = (uint32_t)c->sm_count;
+    p->team = S::WARPS;
+    while (p->team > S::WARPS / S::TEAMS && (uint64_t)ctas * S::WARPS / p->team < units) {
+        p->team /= 2;
+    }
+    p->part_count = ctas * S::WARPS / p->team;
+    p->share_bytes = p->part_count * 2 * S::PART * 4;
+    return SUCCESS;
+}
 template <int DP, bool I8, int HB>
 EE launch(DeviceCtx *c, const AttentionParams &p, cudaStream_t st)
 {
     using S = Shape<DP, I8, HB>;
     const void *kernel = reinterpret_cast<const void *>(paged_attention_kernel<DP, I8, HB>);
     B200_EE(raise_smem_limit(c, (KernelFamily)(KF_ATTENTION + (DP == 64 ? 0 : (DP == 128 ? 1 : 2)) + 3 * I8 + 6 * (HB - 1)), &kernel, 1, S::SMEM));
-    const uint32_t ctas = p.part_count * p.team / WARPS;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas);
-    cfg.blockDim = dim3(32 * WARPS);
+    cfg.gridDim = dim3((uint32_t)c->sm_count);
+    cfg.blockDim = dim3(32 * S::WARPS);
     cfg.dynamicSmemBytes = S::SMEM;
     cfg.stream = st;
     B200_CUDA(launch_programmatic(cfg, paged_attention_kernel<DP, I8, HB>, p));
     count_launch();
-    cfg.gridDim = dim3(ctas, S::HEADS < (int)p.group ? S::HEADS : p.group);
+    cfg.gridDim = dim3(p.part_count, HB);
+    cfg.blockDim = dim3(512);
     cfg.dynamicSmemBytes = 0;
-    B200_CUDA(launch_programmatic(cfg, paged_attention_join_kernel<DP, HB>, p, p.team));
+    B200_CUDA(launch_programmatic(cfg, paged_attention_join_kernel<DP, HB>, p));
     count_launch();
     return SUCCESS;
 }
-template <bool I8>
-EE launch(DeviceCtx *c, const AttentionParams &p, cudaStream_t st)
+// f(std::integral_constant<int, DP>, std::bool_constant<I8>, std::integral_constant<int, HB>) for the call's kernel
+template <bool I8, int HB, typename F>
+EE by_dim(uint32_t dim, F f)
 {
-    const uint32_t dim = p.cache.dim;
-    if (p.group <= 8) {
-        return dim <= 64 ? launch<64, I8, 1>(c, p, st) : (dim <= 128 ? launch<128, I8, 1>(c, p, st) : launch<256, I8, 1>(c, p, st));
+    using std::integral_constant;
+    if (dim <= 64) {
+        return f(integral_constant<int, 64>(), std::bool_constant<I8>(), integral_constant<int, HB>());
     }
-    return dim <= 64 ? launch<64, I8, 2>(c, p, st) : (dim <= 128 ? launch<128, I8, 2>(c, p, st) : launch<256, I8, 2>(c, p, st));
+    if (dim <= 128) {
+        return f(integral_constant<int, 128>(), std::bool_constant<I8>(), integral_constant<int, HB>());
+    }
+    return f(integral_constant<int, 256>(), std::bool_constant<I8>(), integral_constant<int, HB>());
+}
+template <typename F>
+EE by_shape(const AttentionParams &p, F f)
+{
+    if (p.i8) {
+        return p.group <= 8 ? by_dim<true, 1>(p.cache.dim, f) : by_dim<true, 2>(p.cache.dim, f);
+    }
+    return p.group <= 8 ? by_dim<false, 1>(p.cache.dim, f) : by_dim<false, 2>(p.cache.dim, f);
 }
 
 // the checks of both entry points; *p is filled in
@@ -1025,10 +1079,8 @@ EE check(const bolt_b200_kv_cache *cache, const bolt_b200_paged_attention_call *
     p->sequences = a->sequences;
     p->heads = a->heads;
     p->group = a->heads / cache->kv_heads;
-    const uint32_t ctas = (uint32_t)(*c)->sm_count;
-    // rows that can be read four at a time and written two at a time (dim is a multiple of 8)
-    const uint32_t q_size = a->q_dt == DT_F16 ? 2 : 4, out_size = a->out_dt == DT_F32 ? 4 : (a->out_dt == DT_F16 ? 2 : 1);
-    p->q_vectors = aligned(a->q, 4 * q_size) && a->q_stride % 4 == 0;
+    // rows that can be written two elements at a time (dim is a multiple of 8)
+    const uint32_t out_size = a->out_dt == DT_F32 ? 4 : (a->out_dt == DT_F16 ? 2 : 1);
     p->out_pairs = aligned(a->out, 2 * out_size) && a->out_stride % 2 == 0;
     p->head_blocks = p->group <= 8 ? 1 : (p->group + 15) / 16;
     p->table_pages = a->table_pages;
@@ -1039,24 +1091,19 @@ EE check(const bolt_b200_kv_cache *cache, const bolt_b200_paged_attention_call *
     p->q_f16 = a->q_dt == DT_F16;
     p->out_kind = a->out_dt == DT_F32 ? 0 : (a->out_dt == DT_F16 ? 1 : 2);
     p->status = (*c)->d_status;
-    // As many warps to a team as leave a part for every unit: eight for few units (fewer shares to join), one for very
-    // many (no warp waits for others at a unit's end).  Queries in shared memory belong to the whole CTA.
+    p->even_bytes = 0x00FF00FFu;
+    p->to_1152 = 0x64806480u;
     const uint64_t units = (uint64_t)a->sequences * cache->kv_heads * p->head_blocks;
-    p->team = WARPS;
-    while (p->group <= 8 && cache->dim <= 128 && p->team > 1 && ctas * WARPS / p->team < units) {
-        p->team /= 2;
+    // tiles are counted in 32 bits (they hold 16 tokens or more)
+    const uint64_t room = (uint64_t)a->table_pages * cache->page_size;
+    if (units != 0 && room / 16 + 1 > 0xFFFFFFFFull / units) {
+        return NOT_SUPPORTED;
     }
-    p->part_count = ctas * WARPS / p->team;
-    return SUCCESS;
-}
-U32 share_bytes(const AttentionParams &p)
-{
-    const U32 dp = p.cache.dim <= 64 ? 64 : (p.cache.dim <= 128 ? 128 : 256);
-    return p.part_count * 2 * (p.group <= 8 ? 8 : 16) * (dp + 2) * 4;
+    return by_shape(*p, [&](auto dp, auto i8, auto hb) { return plan<dp.value, i8.value, hb.value>(*c, p, units); });
 }
 U32 workspace_bytes(const AttentionParams &p)
 {
-    return share_bytes(p) + p.part_count * (U32)sizeof(Cut);
+    return p.share_bytes + p.part_count * (U32)sizeof(Cut);
 }
 
 }  // namespace
@@ -1106,8 +1153,8 @@ EE bolt_b200_paged_attention(const bolt_b200_kv_cache *cache, const bolt_b200_pa
         return NOT_MATCH;
     }
     p.parts = reinterpret_cast<float *>(tmp);
-    p.cuts = reinterpret_cast<Cut *>(reinterpret_cast<char *>(tmp) + share_bytes(p));
-    return p.i8 ? launch<true>(c, p, tls().stream) : launch<false>(c, p, tls().stream);
+    p.cuts = reinterpret_cast<Cut *>(reinterpret_cast<char *>(tmp) + p.share_bytes);
+    return by_shape(p, [&](auto dp, auto i8, auto hb) { return launch<dp.value, i8.value, hb.value>(c, p, tls().stream); });
 }
 
 }  // extern "C"

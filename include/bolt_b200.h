@@ -537,6 +537,7 @@ EE bolt_b200_kv_append(const bolt_b200_kv_cache *cache, const bolt_b200_kv_appen
  * out_dt: DT_F32, DT_F16, or, for a projection that follows, DT_U8_Q as by quantize_cuda_b200 with the scale out_scale:
  * clamp(rne(x * out_scale + 128), 1, 255).
  * Statistics and sums are binary32; queries and probabilities enter the products with 22 bits at least.
+ * At most 65535 sequences, and sequences * kv_heads * table_pages * page_size * ceil(heads / kv_heads / 16) below 2^36.
  * tmp: the bytes asked for by _tmp_bytes, 16-byte aligned. */
 typedef struct {
     U32 sequences, heads;

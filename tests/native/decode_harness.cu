@@ -27,21 +27,21 @@ int harness_tokens(int32_t length, uint32_t table_pages, uint32_t page_size, uin
     return live_tokens(length, table_pages, page_size, window, range, range + 1);
 }
 // parts that are made; their borders; the part that holds a place
-uint32_t harness_parts(unsigned long long total, uint32_t most)
+uint32_t harness_parts(uint32_t total, uint32_t most)
 {
     return Parts(total, most).n;
 }
-unsigned long long harness_part_begin(uint32_t i, unsigned long long total, uint32_t most)
+uint32_t harness_part_begin(uint32_t i, uint32_t total, uint32_t most)
 {
     return Parts(total, most).begin(i);
 }
-uint32_t harness_part_of(unsigned long long place, unsigned long long total, uint32_t most)
+uint32_t harness_part_of(uint32_t place, uint32_t total, uint32_t most)
 {
     return Parts(total, most).of(place);
 }
-uint32_t harness_tiles(uint32_t begin, uint32_t end, uint32_t tile)
+uint32_t harness_tiles(uint32_t begin, uint32_t end, uint32_t shift)
 {
-    return tiles_of(begin, end, tile);
+    return tiles_of(begin, end, shift);
 }
 
 }  // extern "C"
