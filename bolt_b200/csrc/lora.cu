@@ -1,6 +1,14 @@
 // lora.cu -- low-rank adapters of many requests beside a shared projection: y += s (x A^T) B^T for every segment of rows.
 //
-// Two kernels: the inner sums t = x A^T into the workspace, then y.
+// HBM bound: with a few rows the adapters' own bytes, with many the result's (read and written once).  Two kernels: the
+// inner sums t = x A^T (rows x rank) into the workspace, K split over CTAs and warps, then y += t B^T.  Both work on blocks
+// of 16 rows of one segment, which one instruction of the tensor pipe takes at once; with one row to a request 15 of
+// the 16 stand idle, but the weights are streamed all the same.  Operands go from global memory straight into the
+// fragments: the order of K inside an instruction is free, so a lane loads 16 neighbouring bytes of a row of A or B.
+//
+// Bytes of x become binary16 exactly.  Binary32 x enters as two tf32 numbers (22 bits; tf32 has binary32's range), t as two
+// binary16 numbers of rows brought to a common power of two.  The accumulation of the matrix instructions truncates, so
+// sums over K go on in binary32 registers every few instructions.
 #include "decode.cuh"
 
 namespace b200 {
@@ -16,66 +24,511 @@ struct LoraParams {
     const int32_t *first_row, *adapter;
     float sA;
     const float *d_sA, *row_scale;
-    int u8;
-    float *t;   // [rows][rank]
+    int u8, x_vectors, y_pairs;   // whether rows can be read 8 bytes / 4 numbers, written two numbers at a time
+    uint32_t units, splits, columns;   // blocks of 16 rows at most, parts of K, columns of a CTA
+    float *t;   // [splits][rows][rank]
     int *status;
 };
 
-// adapter of a row, or -1
-__device__ __forceinline__ int adapter_of(const LoraParams &p, uint32_t row)
+constexpr uint32_t MAX_SEGMENTS = 65535;
+
+// ---- blocks of rows -----------------------------------------------------------------------------------------------
+struct Unit {
+    uint32_t row, rows;   // 0: there is none
+    int32_t adapter;
+};
+// Segment s, given the largest bound in front of it: false if it is left out.
+__device__ __forceinline__ bool segment(const LoraParams &p, uint32_t s, int32_t top, int32_t *from, int32_t *to, int32_t *adapter)
 {
-    int32_t top = 0;
-    for (uint32_t s = 0; s < p.segments; ++s) {
-        const int32_t f = p.first_row[s], e = p.first_row[s + 1];
-        top = max(top, f);
-        if (f < top || e < f || (uint32_t)e > p.rows || p.adapter[s] >= (int32_t)p.adapters) {
-            atomicExch(p.status, BAD_LORA);
-            continue;
-        }
-        if (row >= (uint32_t)f && row < (uint32_t)e) {
-            return p.adapter[s] < 0 ? -1 : p.adapter[s];
-        }
+    *from = p.first_row[s];
+    *to = p.first_row[s + 1];
+    *adapter = p.adapter[s];
+    return *from >= top && *to >= *from && (uint32_t)*to <= p.rows && *adapter < (int32_t)p.adapters;
+}
+// Unit number `want`, by 256 threads that share the counting.
+__device__ __forceinline__ Unit find_unit(const LoraParams &p, uint32_t want, bool report)
+{
+    __shared__ int32_t tops[8];
+    __shared__ uint32_t counts[8];
+    __shared__ Unit found;
+    const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const uint32_t per = (p.segments + 255) / 256, s0 = min(threadIdx.x * per, p.segments), s1 = min(s0 + per, p.segments);
+    if (threadIdx.x == 0) {
+        found = Unit{0, 0, -1};
     }
-    return -1;
+    // the largest bound in front of the thread's first segment
+    int32_t own = 0;
+    for (uint32_t s = s0; s < s1; ++s) {
+        own = max(own, p.first_row[s]);
+    }
+    int32_t upto = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int32_t v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+        upto = lane >= o ? max(upto, v) : upto;
+    }
+    if (lane == 31) {
+        tops[warp] = upto;
+    }
+    __syncthreads();
+    int32_t top = __shfl_up_sync(0xFFFFFFFFu, upto, 1);
+    top = lane == 0 ? 0 : top;
+    for (uint32_t w = 0; w < warp; ++w) {
+        top = max(top, tops[w]);
+    }
+    // units of the thread's segments
+    auto walk = [&](auto each) {
+        int32_t t = top;
+        for (uint32_t s = s0; s < s1; ++s) {
+            int32_t from, to, adapter;
+            const bool good = segment(p, s, t, &from, &to, &adapter);
+            if (!good && report) {
+                atomicExch(p.status, BAD_LORA);
+            }
+            t = max(t, from);
+            if (good && adapter >= 0) {
+                each((uint32_t)from, (uint32_t)(to - from), adapter);
+            }
+        }
+    };
+    uint32_t mine = 0;
+    walk([&](uint32_t, uint32_t n, int32_t) { mine += (n + 15) / 16; });
+    uint32_t sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, sum, o);
+        sum += lane >= o ? v : 0;
+    }
+    if (lane == 31) {
+        counts[warp] = sum;
+    }
+    __syncthreads();
+    uint32_t first = sum - mine;
+    for (uint32_t w = 0; w < warp; ++w) {
+        first += counts[w];
+    }
+    if (want >= first && want < first + mine) {
+        walk([&](uint32_t row, uint32_t n, int32_t adapter) {
+            const uint32_t blocks = (n + 15) / 16, b = want - first;
+            if (want >= first && b < blocks) {
+                found = Unit{row + 16 * b, min(16u, n - 16 * b), adapter};
+            }
+            first += blocks;
+        });
+    }
+    __syncthreads();
+    return found;
 }
 
-__global__ void __launch_bounds__(128) lora_inner_kernel(const __grid_constant__ LoraParams p)
+// ---- instructions -----------------------------------------------------------------------------------------------
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
 {
-    const uint32_t row = blockIdx.x, r = blockIdx.y * 4 + threadIdx.x / 32, lane = threadIdx.x % 32;
-    const int ad = adapter_of(p, row);
-    if (ad < 0) {
-        return;
-    }
-    const __half *a = p.a + ((uint64_t)ad * p.rank + r) * p.a_stride;
-    float sum = 0.f;
-    for (uint32_t k = lane; k < p.K; k += 32) {
-        const uint64_t at = row * p.x_stride + k;
-        const float x = p.u8 ? (float)((int)reinterpret_cast<const uint8_t *>(p.x)[at] - 128) : reinterpret_cast<const float *>(p.x)[at];
-        sum += x * __half2float(a[k]);
-    }
-    for (int s = 16; s > 0; s >>= 1) {
-        sum += __shfl_xor_sync(0xFFFFFFFFu, sum, s);
-    }
-    if (lane == 0) {
-        const float unit = !p.u8 ? 1.f : (p.row_scale != nullptr ? p.row_scale[row] : (p.d_sA != nullptr ? *p.d_sA : p.sA));
-        p.t[(uint64_t)row * p.rank + r] = sum * (p.scale != nullptr ? p.scale[ad] : 1.f) / unit;
-    }
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__global__ void __launch_bounds__(128) lora_outer_kernel(const __grid_constant__ LoraParams p)
+__device__ __forceinline__ void mma_tf32(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
 {
-    const uint32_t row = blockIdx.x, n = blockIdx.y * 128 + threadIdx.x;
-    const int ad = adapter_of(p, row);
-    if (ad < 0 || n >= p.N) {
-        return;
-    }
-    const __half *b = p.b + ((uint64_t)ad * p.N + n) * p.rank;
-    float sum = 0.f;
-    for (uint32_t r = 0; r < p.rank; ++r) {
-        sum += p.t[(uint64_t)row * p.rank + r] * __half2float(b[r]);
-    }
-    p.y[row * p.y_stride + n] += sum;
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void matrices(uint32_t (&r)[4], const void *at)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"((uint32_t)__cvta_generic_to_shared(at))
+                 : "memory");
+}
+// two neighbouring bytes u (0: the lower two of a word, 1: the upper two) as u - 128 in binary16: 0x6400 | u is 1024 + u
+template <int UPPER>
+__device__ __forceinline__ uint32_t centred(uint32_t x)
+{
+    const uint32_t y = __byte_perm(x, 0x64646464u, UPPER ? 0x4342 : 0x4140), k = 0x64806480u;
+    const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&y), *reinterpret_cast<const __half2 *>(&k));
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+// what the tensor pipe sees of a number, and the rest (which it sees eleven bits of)
+__device__ __forceinline__ uint32_t tf32_of(float x)
+{
+    return __float_as_uint(x) & 0xFFFFE000u;
 }
 
+// ---- inner sums ---------------------------------------------------------------------------------------------------
+// eight neighbours of a row of x from k on, zeros (after centring) behind K or for a row that does not exist
+template <bool U8>
+struct Eight;
+template <>
+struct Eight<true> {
+    uint32_t h[4];   // pairs of binary16
+    __device__ __forceinline__ void load(const LoraParams &p, uint64_t row, uint32_t k, bool on)
+    {
+        uint32_t w[2] = {0x80808080u, 0x80808080u};
+        const uint8_t *x = reinterpret_cast<const uint8_t *>(p.x) + row * p.x_stride + k;
+        if (on && p.x_vectors && k + 8 <= p.K) {
+            const uint2 v = __ldg(reinterpret_cast<const uint2 *>(x));
+            w[0] = v.x;
+            w[1] = v.y;
+        } else if (on) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (k + i < p.K) {
+                    w[i / 4] = (w[i / 4] & ~(0xFFu << (i % 4 * 8))) | (uint32_t)x[i] << (i % 4 * 8);
+                }
+            }
+        }
+        h[0] = w[0];
+        h[1] = w[1];
+    }
+    __device__ __forceinline__ void convert()
+    {
+        const uint32_t a = h[0], b = h[1];
+        h[0] = centred<0>(a);
+        h[1] = centred<1>(a);
+        h[2] = centred<0>(b);
+        h[3] = centred<1>(b);
+    }
+};
+template <>
+struct Eight<false> {
+    float f[8];
+    __device__ __forceinline__ void load(const LoraParams &p, uint64_t row, uint32_t k, bool on)
+    {
+        const float *x = reinterpret_cast<const float *>(p.x) + row * p.x_stride + k;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            f[i] = 0.f;
+        }
+        if (on && p.x_vectors && k + 8 <= p.K) {
+            const float4 u = __ldg(reinterpret_cast<const float4 *>(x)), v = __ldg(reinterpret_cast<const float4 *>(x) + 1);
+            f[0] = u.x;
+            f[1] = u.y;
+            f[2] = u.z;
+            f[3] = u.w;
+            f[4] = v.x;
+            f[5] = v.y;
+            f[6] = v.z;
+            f[7] = v.w;
+        } else if (on) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (k + i < p.K) {
+                    f[i] = __ldg(x + i);
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void convert() {}
+};
+
+// NT: blocks of eight of the rank, rounded up
+template <bool U8, int NT>
+__global__ void __launch_bounds__(256) lora_inner_kernel(const __grid_constant__ LoraParams p)
+{
+    constexpr int AT_ONCE = NT <= 2 ? 4 : (NT <= 4 ? 2 : 1);   // blocks of 32 of K whose loads a warp has in flight
+    __shared__ float merge[4][NT * 4 * 32];
+    const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, c4 = lane % 4;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // (what was in front of this kernel is over)
+    const Unit u = find_unit(p, blockIdx.x, blockIdx.x == 0 && blockIdx.y == 0);
+    if (u.rows == 0) {
+        return;
+    }
+    const uint32_t blocks = (p.K + 31) / 32;
+    const uint32_t from = (uint32_t)((uint64_t)blocks * blockIdx.y / p.splits), to = (uint32_t)((uint64_t)blocks * (blockIdx.y + 1) / p.splits);
+    const __half *a = p.a + (uint64_t)u.adapter * p.rank * p.a_stride + g * p.a_stride + 8 * c4;
+    float sum[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        sum[n][0] = sum[n][1] = sum[n][2] = sum[n][3] = 0.f;
+    }
+#pragma unroll 1
+    for (uint32_t kb = from + warp; kb < to; kb += 8 * AT_ONCE) {
+        uint4 w[AT_ONCE][NT];
+        Eight<U8> x[AT_ONCE][2];
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+            const uint32_t b = kb + 8 * i, k = 32 * b + 8 * c4;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                w[i][n] = make_uint4(0, 0, 0, 0);
+                if (b < to && n * 8 < p.rank && k < p.K) {
+                    w[i][n] = __ldg(reinterpret_cast<const uint4 *>(a + n * 8 * p.a_stride + 32 * b));
+                }
+            }
+            x[i][0].load(p, u.row + g, k, b < to && k < p.K && g < u.rows);
+            x[i][1].load(p, u.row + g + 8, k, b < to && k < p.K && g + 8 < u.rows);
+        }
+        float c[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+            const uint32_t k = 32 * (kb + 8 * i) + 8 * c4;
+            x[i][0].convert();
+            x[i][1].convert();
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                uint32_t h[4] = {w[i][n].x, w[i][n].y, w[i][n].z, w[i][n].w};
+                if (k + 8 > p.K) {   // what lies behind K in a row of A is nobody's
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        if (k + e >= p.K) {
+                            h[e / 2] &= e % 2 ? 0x0000FFFFu : 0xFFFF0000u;
+                        }
+                    }
+                }
+                if constexpr (U8) {
+                    mma_f16(c[n], x[i][0].h[0], x[i][1].h[0], x[i][0].h[1], x[i][1].h[1], h[0], h[1]);
+                    mma_f16(c[n], x[i][0].h[2], x[i][1].h[2], x[i][0].h[3], x[i][1].h[3], h[2], h[3]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&h[e]));
+                        const float r0 = x[i][0].f[2 * e], r1 = x[i][1].f[2 * e], r2 = x[i][0].f[2 * e + 1], r3 = x[i][1].f[2 * e + 1];
+                        const uint32_t b0 = __float_as_uint(b.x), b1 = __float_as_uint(b.y);
+                        mma_tf32(c[n], tf32_of(r0), tf32_of(r1), tf32_of(r2), tf32_of(r3), b0, b1);
+                        mma_tf32(c[n], tf32_of(r0 - __uint_as_float(tf32_of(r0))), tf32_of(r1 - __uint_as_float(tf32_of(r1))),
+                            tf32_of(r2 - __uint_as_float(tf32_of(r2))), tf32_of(r3 - __uint_as_float(tf32_of(r3))), b0, b1);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                sum[n][e] += c[n][e];
+            }
+        }
+    }
+    // the warps' shares, the upper half's added to the lower half's, and so on
+#pragma unroll 1
+    for (uint32_t half = 4; half != 0; half /= 2) {
+        if (warp >= half && warp < 2 * half) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    merge[warp - half][(4 * n + e) * 32 + lane] = sum[n][e];
+                }
+            }
+        }
+        __syncthreads();
+        if (warp < half) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    sum[n][e] += merge[warp][(4 * n + e) * 32 + lane];
+                }
+            }
+        }
+        __syncthreads();
+    }
+    if (warp != 0) {
+        return;
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        const uint32_t row = u.row + g + 8 * r;
+        if (g + 8 * r < u.rows) {
+            float factor = p.scale != nullptr ? p.scale[u.adapter] : 1.f;
+            if (U8) {
+                factor = __fdiv_rn(factor, p.row_scale != nullptr ? p.row_scale[row] : (p.d_sA != nullptr ? *p.d_sA : p.sA));
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                if (n * 8 < p.rank) {
+                    *reinterpret_cast<float2 *>(p.t + ((uint64_t)blockIdx.y * p.rows + row) * p.rank + n * 8 + 2 * c4) =
+                        make_float2(sum[n][2 * r] * factor, sum[n][2 * r + 1] * factor);
+                }
+            }
+        }
+    }
+}
+
+// ---- the result -----------------------------------------------------------------------------------------------------
+// The rank in blocks of 32, then 16, then 8: a lane loads 8, 4 or 2 neighbours of a row of B, and t stands in shared memory in
+// the order in which the instruction then meets them.
+__device__ __forceinline__ uint32_t place_of(uint32_t r, uint32_t rank)
+{
+    const uint32_t b = r & ~31u, left = rank - b, i = r - b;
+    if (left >= 32) {
+        return b + i % 8 / 4 * 16 + i / 8 * 2 + i % 2 + i % 4 / 2 * 8;
+    }
+    if (left >= 16 && i < 16) {
+        return b + i / 4 * 2 + i % 2 + i % 4 / 2 * 8;
+    }
+    return r;
+}
+// KS: blocks of 16 of the rank, rounded up
+template <int KS>
+__global__ void __launch_bounds__(256) lora_outer_kernel(const __grid_constant__ LoraParams p)
+{
+    constexpr int PITCH = KS * 16 + 8, TILES = 4;   // columns of a warp at a time: 4 x 8
+    __shared__ __align__(16) __half hi[16][PITCH], lo[16][PITCH];
+    __shared__ float down[16];
+    const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, c4 = lane % 4;
+    for (uint32_t i = threadIdx.x; i < 16 * PITCH; i += 256) {
+        (&hi[0][0])[i] = (&lo[0][0])[i] = __float2half_rn(0.f);
+    }
+    const Unit u = find_unit(p, blockIdx.x, false);   // (and waits for the zeros)
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (u.rows == 0) {
+        return;
+    }
+    {
+        // sixteen threads to a row
+        const uint32_t row = threadIdx.x / 16, l = threadIdx.x % 16;
+        float x[KS];
+        int top = 0;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            x[i] = 0.f;
+        }
+        if (row < u.rows) {
+            const float *t = p.t + (uint64_t)(u.row + row) * p.rank;
+#pragma unroll 1
+            for (uint32_t s = 0; s < p.splits; ++s, t += (uint64_t)p.rows * p.rank) {
+#pragma unroll
+                for (int i = 0; i < KS; ++i) {
+                    x[i] += l + 16 * i < p.rank ? t[l + 16 * i] : 0.f;
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            top = max(top, magnitude(x[i]));
+        }
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) {
+            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+        }
+        const int e = max(top >> 23, 20);   // to 2^13 .. 2^14
+        const float up = __int_as_float((267 - e) << 23);
+        if (l == 0) {
+            down[row] = __int_as_float((e - 13) << 23);
+        }
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            const uint32_t r = l + 16 * i;
+            if (r < p.rank) {
+                const uint32_t at = place_of(r, p.rank);
+                const float v = x[i] * up;
+                const __half h = __float2half_rn(v);
+                hi[row][at] = h;
+                lo[row][at] = __float2half_rn(v - __half2float(h));
+            }
+        }
+    }
+    __syncthreads();
+    uint32_t th[KS][4], tl[KS][4];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+        matrices(th[s], &hi[lane % 16][16 * s + lane / 16 * 8]);
+        matrices(tl[s], &lo[lane % 16][16 * s + lane / 16 * 8]);
+    }
+    const float down0 = down[g], down1 = down[g + 8];
+    const bool on0 = g < u.rows, on1 = g + 8 < u.rows;
+    float *const y0 = p.y + (uint64_t)(u.row + g) * p.y_stride, *const y1 = y0 + 8 * p.y_stride;
+    const __half *const b = p.b + (uint64_t)u.adapter * p.N * p.rank;
+    const uint32_t end = min(p.N, (blockIdx.y + 1) * p.columns);
+#pragma unroll 1
+    for (uint32_t n0 = blockIdx.y * p.columns + warp * 8 * TILES; n0 < end; n0 += 64 * TILES) {
+        uint32_t w[TILES][KS][2];
+        float2 v0[TILES], v1[TILES];
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+            const uint32_t n = n0 + 8 * t + g, col = n0 + 8 * t + 2 * c4;
+            const __half *row = b + (uint64_t)n * p.rank;
+#pragma unroll
+            for (int s = 0; s < KS; s += 2) {
+                uint32_t q[4] = {0, 0, 0, 0};
+                const uint32_t left = p.rank - 16 * s;
+                if (n < end && 16 * s < p.rank) {
+                    if (KS > 1 && left >= 32) {
+                        const uint4 x = __ldg(reinterpret_cast<const uint4 *>(row + 16 * s + 8 * c4));
+                        q[0] = x.x;
+                        q[1] = x.y;
+                        q[2] = x.z;
+                        q[3] = x.w;
+                    } else {
+                        uint32_t at = 16 * s;
+                        if (left >= 16) {
+                            const uint2 x = __ldg(reinterpret_cast<const uint2 *>(row + at + 4 * c4));
+                            q[0] = x.x;
+                            q[1] = x.y;
+                            at += 16;
+                        }
+                        if (left % 16 == 8) {
+                            const uint32_t x = __ldg(reinterpret_cast<const uint32_t *>(row + at + 2 * c4));
+                            q[left >= 16 ? 2 : 0] = x;
+                        }
+                    }
+                }
+                w[t][s][0] = q[0];
+                w[t][s][1] = q[1];
+                if (s + 1 < KS) {
+                    w[t][s + 1][0] = q[2];
+                    w[t][s + 1][1] = q[3];
+                }
+            }
+            v0[t] = v1[t] = make_float2(0.f, 0.f);
+            auto fetch = [&](const float *y, bool on, float2 &v) {
+                if (on && p.y_pairs && col + 1 < end) {
+                    v = *reinterpret_cast<const float2 *>(y + col);
+                } else if (on && col < end) {
+                    v.x = y[col];
+                    v.y = col + 1 < end ? y[col + 1] : 0.f;
+                }
+            };
+            fetch(y0, on0, v0[t]);
+            fetch(y1, on1, v1[t]);
+        }
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+            const uint32_t col = n0 + 8 * t + 2 * c4;
+            float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                mma_f16(c, tl[s][0], tl[s][1], tl[s][2], tl[s][3], w[t][s][0], w[t][s][1]);
+                mma_f16(c, th[s][0], th[s][1], th[s][2], th[s][3], w[t][s][0], w[t][s][1]);
+            }
+            auto keep = [&](float *y, bool on, float2 v) {
+                if (on && p.y_pairs && col + 1 < end) {
+                    *reinterpret_cast<float2 *>(y + col) = v;
+                } else if (on && col < end) {
+                    y[col] = v.x;
+                    if (col + 1 < end) {
+                        y[col + 1] = v.y;
+                    }
+                }
+            };
+            keep(y0, on0, make_float2(fmaf(c[0], down0, v0[t].x), fmaf(c[1], down0, v0[t].y)));
+            keep(y1, on1, make_float2(fmaf(c[2], down1, v1[t].x), fmaf(c[3], down1, v1[t].y)));
+        }
+    }
+}
+
+// How the work is divided: from what the host knows, the rows and the number of segments.
+void divide(LoraParams *p, const DeviceCtx *c)
+{
+    const uint32_t most = p->rows / 16 + p->segments, sms = (uint32_t)c->sm_count;
+    p->units = most < p->rows ? most : p->rows;
+    // K in as many parts as give every SM two CTAs, each at least 256 long (a warp's 32)
+    const uint32_t want = p->units == 0 ? 1 : 2 * sms / p->units, at_most = (p->K + 255) / 256;
+    p->splits = want < 1 ? 1 : (want < at_most ? want : at_most);
+    // Columns in steps of a CTA's 256: as many CTAs as give every SM four, but no more than eight steps each (the start
+    // of a CTA costs as much as two or three).
+    const uint32_t steps = (p->N + 255) / 256, parts = p->units == 0 ? 1 : (4 * sms + p->units - 1) / p->units;
+    uint32_t each = (steps + parts - 1) / parts;
+    each = each < 1 ? 1 : (each > 8 ? 8 : each);
+    p->columns = 256 * each;
+}
 EE check(const bolt_b200_lora_call *a, LoraParams *p, DeviceCtx **c)
 {
     if (a == nullptr) {
@@ -98,7 +551,7 @@ EE check(const bolt_b200_lora_call *a, LoraParams *p, DeviceCtx **c)
         return NOT_MATCH;
     }
     if (a->x_stride > MAX_STRIDE || a->y_stride > MAX_STRIDE || a->a_stride > MAX_STRIDE || a->rows > (1u << 22) || a->N > (1u << 23) ||
-        a->adapters > 0x7FFFFFFFu || a->segments > (1u << 20)) {
+        a->adapters > 0x7FFFFFFFu || a->segments > MAX_SEGMENTS) {
         return NOT_SUPPORTED;
     }
     p->rows = a->rows;
@@ -121,12 +574,52 @@ EE check(const bolt_b200_lora_call *a, LoraParams *p, DeviceCtx **c)
     p->d_sA = a->d_sA;
     p->row_scale = a->row_scale;
     p->u8 = a->x_dt == DT_U8_Q;
+    p->x_vectors = p->u8 ? aligned(a->x, 8) && a->x_stride % 8 == 0 : aligned(a->x, 16) && a->x_stride % 4 == 0;
+    p->y_pairs = aligned(a->y, 8) && a->y_stride % 2 == 0;
     p->status = (*c)->d_status;
+    divide(p, *c);
+    if ((uint64_t)p->splits * p->rows * p->rank > 0x3FFFFFFFull) {
+        return NOT_SUPPORTED;    // the workspace is counted in 32 bits
+    }
     return SUCCESS;
 }
-U32 workspace_bytes(const LoraParams &p, const DeviceCtx *)
+U32 workspace_bytes(const LoraParams &p)
 {
-    return p.rows * p.rank * 4;
+    return p.splits * p.rows * p.rank * 4;
+}
+template <typename K>
+EE launch(K kernel, dim3 grid, const LoraParams &p, cudaStream_t st)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    B200_CUDA(launch_programmatic(cfg, kernel, p));
+    count_launch();
+    return SUCCESS;
+}
+template <bool U8>
+EE launch_inner(const LoraParams &p, cudaStream_t st)
+{
+    const dim3 grid(p.units, p.splits);
+    if (p.rank <= 16) {
+        return launch(lora_inner_kernel<U8, 2>, grid, p, st);
+    }
+    if (p.rank <= 32) {
+        return launch(lora_inner_kernel<U8, 4>, grid, p, st);
+    }
+    return p.rank <= 64 ? launch(lora_inner_kernel<U8, 8>, grid, p, st) : launch(lora_inner_kernel<U8, 16>, grid, p, st);
+}
+EE launch_outer(const LoraParams &p, cudaStream_t st)
+{
+    const dim3 grid(p.units, (p.N + p.columns - 1) / p.columns);
+    if (p.rank <= 16) {
+        return launch(lora_outer_kernel<1>, grid, p, st);
+    }
+    if (p.rank <= 32) {
+        return launch(lora_outer_kernel<2>, grid, p, st);
+    }
+    return p.rank <= 64 ? launch(lora_outer_kernel<4>, grid, p, st) : launch(lora_outer_kernel<8>, grid, p, st);
 }
 
 }  // namespace
@@ -144,7 +637,7 @@ EE bolt_b200_lora_tmp_bytes(const bolt_b200_lora_call *call, U32 *bytes)
     LoraParams p;
     DeviceCtx *c = nullptr;
     B200_EE(check(call, &p, &c));
-    *bytes = workspace_bytes(p, c);
+    *bytes = workspace_bytes(p);
     return SUCCESS;
 }
 
@@ -159,7 +652,7 @@ EE bolt_b200_lora(const bolt_b200_lora_call *call, U32 tmpBytes, void *tmp)
     if (p.x == nullptr || p.y == nullptr || p.a == nullptr || p.b == nullptr || p.first_row == nullptr || p.adapter == nullptr || tmp == nullptr) {
         return NULL_POINTER;
     }
-    if (tmpBytes < workspace_bytes(p, c)) {
+    if (tmpBytes < workspace_bytes(p)) {
         return NOT_MATCH;
     }
     if (!aligned(p.x, p.u8 ? 1 : 4) || !aligned(p.y, 4) || !aligned(p.a, 16) || !aligned(p.b, 16) || !aligned(p.scale, 4) || !aligned(p.first_row, 4) ||
@@ -173,8 +666,8 @@ EE bolt_b200_lora(const bolt_b200_lora_call *call, U32 tmpBytes, void *tmp)
     }
     p.t = reinterpret_cast<float *>(tmp);
     const cudaStream_t st = tls().stream;
-    B200_EE(launch_kernel(dim3(p.rows, p.rank / 4), 128, 0, st, lora_inner_kernel, p));
-    return launch_kernel(dim3(p.rows, (p.N + 127) / 128), 128, 0, st, lora_outer_kernel, p);
+    B200_EE(p.u8 ? launch_inner<true>(p, st) : launch_inner<false>(p, st));
+    return launch_outer(p, st);
 }
 
 }  // extern "C"
