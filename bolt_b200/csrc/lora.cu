@@ -24,7 +24,7 @@ struct LoraParams {
     const int32_t *first_row, *adapter;
     float sA;
     const float *d_sA, *row_scale;
-    int u8, x_vectors, y_pairs;   // whether rows can be read 8 bytes / 4 numbers, written two numbers at a time
+    int u8, x_vectors, y_vectors;   // whether rows can be read 8 bytes / 4 numbers, written four numbers at a time
     uint32_t units, splits, columns;   // blocks of 16 rows at most, parts of K, columns of a CTA
     float *t;   // [splits][rows][rank]
     int *status;
@@ -366,9 +366,10 @@ __device__ __forceinline__ uint32_t place_of(uint32_t r, uint32_t rank)
 }
 // KS: blocks of 16 of the rank, rounded up
 template <int KS>
-__global__ void __launch_bounds__(256) lora_outer_kernel(const __grid_constant__ LoraParams p)
+__global__ void __launch_bounds__(256, KS <= 2 ? 4 : 1) lora_outer_kernel(const __grid_constant__ LoraParams p)
 {
     constexpr int PITCH = KS * 16 + 8, TILES = 4;   // columns of a warp at a time: 4 x 8
+    constexpr int AT_ONCE = KS <= 2 ? 8 : 4;        // parts of K whose inner sums are asked for at a time
     __shared__ __align__(16) __half hi[16][PITCH], lo[16][PITCH];
     __shared__ float down[16];
     const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, c4 = lane % 4;
@@ -392,11 +393,23 @@ __global__ void __launch_bounds__(256) lora_outer_kernel(const __grid_constant__
         }
         if (row < u.rows) {
             const float *t = p.t + (uint64_t)(u.row + row) * p.rank;
+            const uint64_t split = (uint64_t)p.rows * p.rank;
 #pragma unroll 1
-            for (uint32_t s = 0; s < p.splits; ++s, t += (uint64_t)p.rows * p.rank) {
+            for (uint32_t s = 0; s < p.splits; s += AT_ONCE) {
+                float v[AT_ONCE][KS];
 #pragma unroll
-                for (int i = 0; i < KS; ++i) {
-                    x[i] += l + 16 * i < p.rank ? t[l + 16 * i] : 0.f;
+                for (int j = 0; j < AT_ONCE; ++j) {
+#pragma unroll
+                    for (int i = 0; i < KS; ++i) {
+                        v[j][i] = s + j < p.splits && l + 16 * i < p.rank ? t[(s + j) * split + l + 16 * i] : 0.f;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < AT_ONCE; ++j) {
+#pragma unroll
+                    for (int i = 0; i < KS; ++i) {
+                        x[i] += v[j][i];
+                    }
                 }
             }
         }
@@ -439,11 +452,13 @@ __global__ void __launch_bounds__(256) lora_outer_kernel(const __grid_constant__
     const uint32_t end = min(p.N, (blockIdx.y + 1) * p.columns);
 #pragma unroll 1
     for (uint32_t n0 = blockIdx.y * p.columns + warp * 8 * TILES; n0 < end; n0 += 64 * TILES) {
+        // The order of the columns inside an instruction is free, too: those of two tiles are dealt out so that a lane has
+        // four neighbours of the result.
         uint32_t w[TILES][KS][2];
-        float2 v0[TILES], v1[TILES];
+        float v[2][TILES / 2][4];
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
-            const uint32_t n = n0 + 8 * t + g, col = n0 + 8 * t + 2 * c4;
+            const uint32_t n = n0 + t / 2 * 16 + g / 2 * 4 + t % 2 * 2 + g % 2;
             const __half *row = b + (uint64_t)n * p.rank;
 #pragma unroll
             for (int s = 0; s < KS; s += 2) {
@@ -477,39 +492,61 @@ __global__ void __launch_bounds__(256) lora_outer_kernel(const __grid_constant__
                     w[t][s + 1][1] = q[3];
                 }
             }
-            v0[t] = v1[t] = make_float2(0.f, 0.f);
-            auto fetch = [&](const float *y, bool on, float2 &v) {
-                if (on && p.y_pairs && col + 1 < end) {
-                    v = *reinterpret_cast<const float2 *>(y + col);
-                } else if (on && col < end) {
-                    v.x = y[col];
-                    v.y = col + 1 < end ? y[col + 1] : 0.f;
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+#pragma unroll
+            for (int t = 0; t < TILES / 2; ++t) {
+                const uint32_t col = n0 + 16 * t + 4 * c4;
+                const float *y = (r == 0 ? y0 : y1) + col;
+                const bool on = r == 0 ? on0 : on1;
+                v[r][t][0] = v[r][t][1] = v[r][t][2] = v[r][t][3] = 0.f;
+                if (on && p.y_vectors && col + 3 < end) {
+                    const float4 x = __ldcs(reinterpret_cast<const float4 *>(y));
+                    v[r][t][0] = x.x;
+                    v[r][t][1] = x.y;
+                    v[r][t][2] = x.z;
+                    v[r][t][3] = x.w;
+                } else if (on) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        v[r][t][e] = col + e < end ? y[e] : 0.f;
+                    }
                 }
-            };
-            fetch(y0, on0, v0[t]);
-            fetch(y1, on1, v1[t]);
+            }
         }
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
-            const uint32_t col = n0 + 8 * t + 2 * c4;
             float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
                 mma_f16(c, tl[s][0], tl[s][1], tl[s][2], tl[s][3], w[t][s][0], w[t][s][1]);
                 mma_f16(c, th[s][0], th[s][1], th[s][2], th[s][3], w[t][s][0], w[t][s][1]);
             }
-            auto keep = [&](float *y, bool on, float2 v) {
-                if (on && p.y_pairs && col + 1 < end) {
-                    *reinterpret_cast<float2 *>(y + col) = v;
-                } else if (on && col < end) {
-                    y[col] = v.x;
-                    if (col + 1 < end) {
-                        y[col + 1] = v.y;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                v[0][t / 2][t % 2 * 2 + e] = fmaf(c[e], down0, v[0][t / 2][t % 2 * 2 + e]);
+                v[1][t / 2][t % 2 * 2 + e] = fmaf(c[2 + e], down1, v[1][t / 2][t % 2 * 2 + e]);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+#pragma unroll
+            for (int t = 0; t < TILES / 2; ++t) {
+                const uint32_t col = n0 + 16 * t + 4 * c4;
+                float *y = (r == 0 ? y0 : y1) + col;
+                const bool on = r == 0 ? on0 : on1;
+                if (on && p.y_vectors && col + 3 < end) {
+                    __stcs(reinterpret_cast<float4 *>(y), make_float4(v[r][t][0], v[r][t][1], v[r][t][2], v[r][t][3]));
+                } else if (on) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (col + e < end) {
+                            y[e] = v[r][t][e];
+                        }
                     }
                 }
-            };
-            keep(y0, on0, make_float2(fmaf(c[0], down0, v0[t].x), fmaf(c[1], down0, v0[t].y)));
-            keep(y1, on1, make_float2(fmaf(c[2], down1, v1[t].x), fmaf(c[3], down1, v1[t].y)));
+            }
         }
     }
 }
@@ -575,7 +612,7 @@ EE check(const bolt_b200_lora_call *a, LoraParams *p, DeviceCtx **c)
     p->row_scale = a->row_scale;
     p->u8 = a->x_dt == DT_U8_Q;
     p->x_vectors = p->u8 ? aligned(a->x, 8) && a->x_stride % 8 == 0 : aligned(a->x, 16) && a->x_stride % 4 == 0;
-    p->y_pairs = aligned(a->y, 8) && a->y_stride % 2 == 0;
+    p->y_vectors = aligned(a->y, 16) && a->y_stride % 4 == 0;
     p->status = (*c)->d_status;
     divide(p, *c);
     if ((uint64_t)p->splits * p->rows * p->rank > 0x3FFFFFFFull) {
