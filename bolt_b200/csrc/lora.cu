@@ -25,7 +25,7 @@ struct LoraParams {
     float sA;
     const float *d_sA, *row_scale;
     int u8, x_vectors, y_vectors;   // whether rows can be read 8 bytes / 4 numbers, written four numbers at a time
-    uint32_t units, splits, columns;   // blocks of 16 rows at most, parts of K, columns of a CTA
+    uint32_t units, splits, outer_ctas;   // blocks of 16 rows at most, parts of K, CTAs of the second kernel
     float *t;   // [splits][rows][rank]
     int *status;
 };
@@ -45,39 +45,84 @@ __device__ __forceinline__ bool segment(const LoraParams &p, uint32_t s, int32_t
     *adapter = p.adapter[s];
     return *from >= top && *to >= *from && (uint32_t)*to <= p.rows && *adapter < (int32_t)p.adapters;
 }
-// Unit number `want`, by 256 threads that share the counting.
-__device__ __forceinline__ Unit find_unit(const LoraParams &p, uint32_t want, bool report)
-{
-    __shared__ int32_t tops[8];
-    __shared__ uint32_t counts[8];
-    __shared__ Unit found;
-    const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    const uint32_t per = (p.segments + 255) / 256, s0 = min(threadIdx.x * per, p.segments), s1 = min(s0 + per, p.segments);
-    if (threadIdx.x == 0) {
-        found = Unit{0, 0, -1};
-    }
-    // the largest bound in front of the thread's first segment
-    int32_t own = 0;
-    for (uint32_t s = s0; s < s1; ++s) {
-        own = max(own, p.first_row[s]);
-    }
-    int32_t upto = own;
+// By 256 threads that share the counting: how many units there are, and which is which.
+class Units {
+public:
+    __device__ __forceinline__ Units(const LoraParams &params, bool report) : p(params)
+    {
+        __shared__ int32_t tops[8];
+        __shared__ uint32_t counts[8];
+        const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, per = (p.segments + 255) / 256;
+        s0 = min(threadIdx.x * per, p.segments);
+        s1 = min(s0 + per, p.segments);
+        // the largest bound in front of the thread's first segment
+        int32_t upto = 0;
+        for (uint32_t s = s0; s < s1; ++s) {
+            upto = max(upto, p.first_row[s]);
+        }
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int32_t v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
-        upto = lane >= o ? max(upto, v) : upto;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int32_t v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+            upto = lane >= o ? max(upto, v) : upto;
+        }
+        if (lane == 31) {
+            tops[warp] = upto;
+        }
+        __syncthreads();
+        top = __shfl_up_sync(0xFFFFFFFFu, upto, 1);
+        top = lane == 0 ? 0 : top;
+        for (uint32_t w = 0; w < warp; ++w) {
+            top = max(top, tops[w]);
+        }
+        mine = 0;
+        walk(report, [&](uint32_t, uint32_t n, int32_t) { mine += (n + 15) / 16; });
+        uint32_t sum = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, sum, o);
+            sum += lane >= o ? v : 0;
+        }
+        if (lane == 31) {
+            counts[warp] = sum;
+        }
+        __syncthreads();
+        first = sum - mine;
+        total = 0;
+        for (uint32_t w = 0; w < 8; ++w) {
+            first += w < warp ? counts[w] : 0;
+            total += counts[w];
+        }
     }
-    if (lane == 31) {
-        tops[warp] = upto;
+    __device__ __forceinline__ uint32_t count() const
+    {
+        return total;
     }
-    __syncthreads();
-    int32_t top = __shfl_up_sync(0xFFFFFFFFu, upto, 1);
-    top = lane == 0 ? 0 : top;
-    for (uint32_t w = 0; w < warp; ++w) {
-        top = max(top, tops[w]);
+    __device__ __forceinline__ Unit get(uint32_t want) const
+    {
+        __shared__ Unit found;
+        if (threadIdx.x == 0) {
+            found = Unit{0, 0, 0};
+        }
+        __syncthreads();
+        if (want >= first && want < first + mine) {
+            uint32_t before = first;
+            walk(false, [&](uint32_t row, uint32_t n, int32_t adapter) {
+                const uint32_t blocks = (n + 15) / 16, b = want - before;
+                if (want >= before && b < blocks) {
+                    found = Unit{row + 16 * b, min(16u, n - 16 * b), adapter};
+                }
+                before += blocks;
+            });
+        }
+        __syncthreads();
+        return found;
     }
-    // units of the thread's segments
-    auto walk = [&](auto each) {
+
+private:
+    // the thread's segments
+    template <typename F>
+    __device__ __forceinline__ void walk(bool report, F each) const
+    {
         int32_t t = top;
         for (uint32_t s = s0; s < s1; ++s) {
             int32_t from, to, adapter;
@@ -90,35 +135,11 @@ __device__ __forceinline__ Unit find_unit(const LoraParams &p, uint32_t want, bo
                 each((uint32_t)from, (uint32_t)(to - from), adapter);
             }
         }
-    };
-    uint32_t mine = 0;
-    walk([&](uint32_t, uint32_t n, int32_t) { mine += (n + 15) / 16; });
-    uint32_t sum = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, sum, o);
-        sum += lane >= o ? v : 0;
     }
-    if (lane == 31) {
-        counts[warp] = sum;
-    }
-    __syncthreads();
-    uint32_t first = sum - mine;
-    for (uint32_t w = 0; w < warp; ++w) {
-        first += counts[w];
-    }
-    if (want >= first && want < first + mine) {
-        walk([&](uint32_t row, uint32_t n, int32_t adapter) {
-            const uint32_t blocks = (n + 15) / 16, b = want - first;
-            if (want >= first && b < blocks) {
-                found = Unit{row + 16 * b, min(16u, n - 16 * b), adapter};
-            }
-            first += blocks;
-        });
-    }
-    __syncthreads();
-    return found;
-}
+    const LoraParams &p;
+    uint32_t s0, s1, mine, first, total;
+    int32_t top;
+};
 
 // ---- instructions -----------------------------------------------------------------------------------------------
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
@@ -230,10 +251,11 @@ __global__ void __launch_bounds__(256) lora_inner_kernel(const __grid_constant__
     const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, c4 = lane % 4;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // (what was in front of this kernel is over)
-    const Unit u = find_unit(p, blockIdx.x, blockIdx.x == 0 && blockIdx.y == 0);
-    if (u.rows == 0) {
+    const Units units(p, blockIdx.x == 0 && blockIdx.y == 0);
+    if (blockIdx.x >= units.count()) {
         return;
     }
+    const Unit u = units.get(blockIdx.x);
     const uint32_t blocks = (p.K + 31) / 32;
     const uint32_t from = (uint32_t)((uint64_t)blocks * blockIdx.y / p.splits), to = (uint32_t)((uint64_t)blocks * (blockIdx.y + 1) / p.splits);
     const __half *a = p.a + (uint64_t)u.adapter * p.rank * p.a_stride + g * p.a_stride + 8 * c4;
@@ -364,9 +386,11 @@ __device__ __forceinline__ uint32_t place_of(uint32_t r, uint32_t rank)
     }
     return r;
 }
+// Columns go in steps of 256 (32 to a warp); the steps of all units stand in one row, of which every CTA takes an equal part.
+constexpr uint32_t STEP = 256;
 // KS: blocks of 16 of the rank, rounded up
 template <int KS>
-__global__ void __launch_bounds__(256, KS <= 2 ? 4 : 1) lora_outer_kernel(const __grid_constant__ LoraParams p)
+__global__ void __launch_bounds__(256, KS <= 2 ? 3 : 1) lora_outer_kernel(const __grid_constant__ LoraParams p)
 {
     constexpr int PITCH = KS * 16 + 8, TILES = 4;   // columns of a warp at a time: 4 x 8
     constexpr int AT_ONCE = KS <= 2 ? 8 : 4;        // parts of K whose inner sums are asked for at a time
@@ -376,177 +400,234 @@ __global__ void __launch_bounds__(256, KS <= 2 ? 4 : 1) lora_outer_kernel(const 
     for (uint32_t i = threadIdx.x; i < 16 * PITCH; i += 256) {
         (&hi[0][0])[i] = (&lo[0][0])[i] = __float2half_rn(0.f);
     }
-    const Unit u = find_unit(p, blockIdx.x, false);   // (and waits for the zeros)
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (u.rows == 0) {
-        return;
-    }
-    {
-        // sixteen threads to a row
-        const uint32_t row = threadIdx.x / 16, l = threadIdx.x % 16;
-        float x[KS];
-        int top = 0;
+    // (nothing that the kernel in front of this one writes is read here: it writes the inner sums only, and has seen the end
+    // of what was in front of it)
+    const Units units(p, false);
+    const uint32_t steps = (p.N + STEP - 1) / STEP;
+    const Parts parts(units.count() * steps, gridDim.x);
+    const bool some = blockIdx.x < parts.n;
+    uint32_t at = some ? parts.begin(blockIdx.x) : 0;
+    const uint32_t stop = some ? parts.begin(blockIdx.x + 1) : 0;
+
+    Unit u = {0, 0, 0};
+    uint32_t w[TILES][KS][2];
+    float v[2][TILES / 2][4];
+    // The order of the columns inside an instruction is free, too: those of two tiles are dealt out so that a lane has four
+    // neighbours of the result (and rows g / 2 * 4 + g % 2 of B, and the one two further on, and so on).
+    uint32_t step = 0, n0 = 0;      // of the unit; the warp's first column of the step
+    float *y0 = nullptr, *y1 = nullptr;
+    const __half *b = nullptr;
+    bool on0 = false, on1 = false;
+    auto enter = [&]() {
+        u = units.get(at / steps);
+        step = at % steps;
+        n0 = step * STEP + warp * 8 * TILES;
+        y0 = p.y + (uint64_t)(u.row + g) * p.y_stride + n0 + 4 * c4;
+        y1 = y0 + 8 * p.y_stride;
+        b = p.b + ((uint64_t)u.adapter * p.N + n0 + g / 2 * 4 + g % 2) * p.rank;
+        on0 = g < u.rows;
+        on1 = g + 8 < u.rows;
+    };
+    auto advance = [&]() {
+        ++step;
+        n0 += STEP;
+        y0 += STEP;
+        y1 += STEP;
+        b += (uint64_t)STEP * p.rank;
+    };
+    auto whole = [&]() { return p.y_vectors && n0 + 8 * TILES <= p.N; };    // nothing to look after
+    auto fetch_row = [&](int t, const __half *row, bool on) {
 #pragma unroll
-        for (int i = 0; i < KS; ++i) {
-            x[i] = 0.f;
-        }
-        if (row < u.rows) {
-            const float *t = p.t + (uint64_t)(u.row + row) * p.rank;
-            const uint64_t split = (uint64_t)p.rows * p.rank;
-#pragma unroll 1
-            for (uint32_t s = 0; s < p.splits; s += AT_ONCE) {
-                float v[AT_ONCE][KS];
-#pragma unroll
-                for (int j = 0; j < AT_ONCE; ++j) {
-#pragma unroll
-                    for (int i = 0; i < KS; ++i) {
-                        v[j][i] = s + j < p.splits && l + 16 * i < p.rank ? t[(s + j) * split + l + 16 * i] : 0.f;
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < AT_ONCE; ++j) {
-#pragma unroll
-                    for (int i = 0; i < KS; ++i) {
-                        x[i] += v[j][i];
-                    }
-                }
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < KS; ++i) {
-            top = max(top, magnitude(x[i]));
-        }
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) {
-            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-        }
-        const int e = max(top >> 23, 20);   // to 2^13 .. 2^14
-        const float up = __int_as_float((267 - e) << 23);
-        if (l == 0) {
-            down[row] = __int_as_float((e - 13) << 23);
-        }
-#pragma unroll
-        for (int i = 0; i < KS; ++i) {
-            const uint32_t r = l + 16 * i;
-            if (r < p.rank) {
-                const uint32_t at = place_of(r, p.rank);
-                const float v = x[i] * up;
-                const __half h = __float2half_rn(v);
-                hi[row][at] = h;
-                lo[row][at] = __float2half_rn(v - __half2float(h));
-            }
-        }
-    }
-    __syncthreads();
-    uint32_t th[KS][4], tl[KS][4];
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-        matrices(th[s], &hi[lane % 16][16 * s + lane / 16 * 8]);
-        matrices(tl[s], &lo[lane % 16][16 * s + lane / 16 * 8]);
-    }
-    const float down0 = down[g], down1 = down[g + 8];
-    const bool on0 = g < u.rows, on1 = g + 8 < u.rows;
-    float *const y0 = p.y + (uint64_t)(u.row + g) * p.y_stride, *const y1 = y0 + 8 * p.y_stride;
-    const __half *const b = p.b + (uint64_t)u.adapter * p.N * p.rank;
-    const uint32_t end = min(p.N, (blockIdx.y + 1) * p.columns);
-#pragma unroll 1
-    for (uint32_t n0 = blockIdx.y * p.columns + warp * 8 * TILES; n0 < end; n0 += 64 * TILES) {
-        // The order of the columns inside an instruction is free, too: those of two tiles are dealt out so that a lane has
-        // four neighbours of the result.
-        uint32_t w[TILES][KS][2];
-        float v[2][TILES / 2][4];
-#pragma unroll
-        for (int t = 0; t < TILES; ++t) {
-            const uint32_t n = n0 + t / 2 * 16 + g / 2 * 4 + t % 2 * 2 + g % 2;
-            const __half *row = b + (uint64_t)n * p.rank;
-#pragma unroll
-            for (int s = 0; s < KS; s += 2) {
-                uint32_t q[4] = {0, 0, 0, 0};
-                const uint32_t left = p.rank - 16 * s;
-                if (n < end && 16 * s < p.rank) {
-                    if (KS > 1 && left >= 32) {
-                        const uint4 x = __ldg(reinterpret_cast<const uint4 *>(row + 16 * s + 8 * c4));
+        for (int s = 0; s < KS; s += 2) {
+            uint32_t q[4] = {0, 0, 0, 0};
+            const uint32_t left = p.rank - 16 * s;
+            if (on && 16 * s < p.rank) {
+                if (KS > 1 && left >= 32) {
+                    const uint4 x = __ldg(reinterpret_cast<const uint4 *>(row + 16 * s + 8 * c4));
+                    q[0] = x.x;
+                    q[1] = x.y;
+                    q[2] = x.z;
+                    q[3] = x.w;
+                } else {
+                    uint32_t r = 16 * s;
+                    if (left >= 16) {
+                        const uint2 x = __ldg(reinterpret_cast<const uint2 *>(row + r + 4 * c4));
                         q[0] = x.x;
                         q[1] = x.y;
-                        q[2] = x.z;
-                        q[3] = x.w;
-                    } else {
-                        uint32_t at = 16 * s;
-                        if (left >= 16) {
-                            const uint2 x = __ldg(reinterpret_cast<const uint2 *>(row + at + 4 * c4));
-                            q[0] = x.x;
-                            q[1] = x.y;
-                            at += 16;
-                        }
-                        if (left % 16 == 8) {
-                            const uint32_t x = __ldg(reinterpret_cast<const uint32_t *>(row + at + 2 * c4));
-                            q[left >= 16 ? 2 : 0] = x;
-                        }
+                        r += 16;
+                    }
+                    if (left % 16 == 8) {
+                        const uint32_t x = __ldg(reinterpret_cast<const uint32_t *>(row + r + 2 * c4));
+                        q[left >= 16 ? 2 : 0] = x;
                     }
                 }
-                w[t][s][0] = q[0];
-                w[t][s][1] = q[1];
-                if (s + 1 < KS) {
-                    w[t][s + 1][0] = q[2];
-                    w[t][s + 1][1] = q[3];
-                }
+            }
+            w[t][s][0] = q[0];
+            w[t][s][1] = q[1];
+            if (s + 1 < KS) {
+                w[t][s + 1][0] = q[2];
+                w[t][s + 1][1] = q[3];
             }
         }
+    };
+    auto fetch = [&]() {
+        if (whole()) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
+            for (int t = 0; t < TILES; ++t) {
+                fetch_row(t, b + (t / 2 * 16 + t % 2 * 2) * p.rank, true);
+            }
 #pragma unroll
-            for (int t = 0; t < TILES / 2; ++t) {
-                const uint32_t col = n0 + 16 * t + 4 * c4;
-                const float *y = (r == 0 ? y0 : y1) + col;
-                const bool on = r == 0 ? on0 : on1;
-                v[r][t][0] = v[r][t][1] = v[r][t][2] = v[r][t][3] = 0.f;
-                if (on && p.y_vectors && col + 3 < end) {
-                    const float4 x = __ldcs(reinterpret_cast<const float4 *>(y));
+            for (int r = 0; r < 2; ++r) {
+#pragma unroll
+                for (int t = 0; t < TILES / 2; ++t) {
+                    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (r == 0 ? on0 : on1) {
+                        x = __ldcs(reinterpret_cast<const float4 *>(r == 0 ? y0 : y1) + 4 * t);
+                    }
                     v[r][t][0] = x.x;
                     v[r][t][1] = x.y;
                     v[r][t][2] = x.z;
                     v[r][t][3] = x.w;
-                } else if (on) {
+                }
+            }
+        } else {
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) {
+                const uint32_t further = t / 2 * 16 + t % 2 * 2;
+                fetch_row(t, b + further * p.rank, n0 + g / 2 * 4 + g % 2 + further < p.N);
+            }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+#pragma unroll
+                for (int t = 0; t < TILES / 2; ++t) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        v[r][t][e] = col + e < end ? y[e] : 0.f;
+                        const uint32_t further = 16 * t + e;
+                        v[r][t][e] = (r == 0 ? on0 : on1) && n0 + 4 * c4 + further < p.N ? (r == 0 ? y0 : y1)[further] : 0.f;
                     }
                 }
             }
         }
+    };
+    if (at < stop) {
+        enter();
+        fetch();    // on its way while the inner sums are still being made
+    }
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+#pragma unroll 1
+    while (at < stop) {
+        __syncthreads();    // everybody is through with the unit before (and the zeros are there)
+        {
+            // sixteen threads to a row
+            const uint32_t row = threadIdx.x / 16, l = threadIdx.x % 16;
+            float x[KS];
+            int top = 0;
 #pragma unroll
-        for (int t = 0; t < TILES; ++t) {
-            float c[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                mma_f16(c, tl[s][0], tl[s][1], tl[s][2], tl[s][3], w[t][s][0], w[t][s][1]);
-                mma_f16(c, th[s][0], th[s][1], th[s][2], th[s][3], w[t][s][0], w[t][s][1]);
+            for (int i = 0; i < KS; ++i) {
+                x[i] = 0.f;
             }
+            if (row < u.rows) {
+                const float *t = p.t + (uint64_t)(u.row + row) * p.rank;
+                const uint64_t split = (uint64_t)p.rows * p.rank;
+#pragma unroll 1
+                for (uint32_t s = 0; s < p.splits; s += AT_ONCE) {
+                    float part[AT_ONCE][KS];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                v[0][t / 2][t % 2 * 2 + e] = fmaf(c[e], down0, v[0][t / 2][t % 2 * 2 + e]);
-                v[1][t / 2][t % 2 * 2 + e] = fmaf(c[2 + e], down1, v[1][t / 2][t % 2 * 2 + e]);
-            }
-        }
+                    for (int j = 0; j < AT_ONCE; ++j) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
+                        for (int i = 0; i < KS; ++i) {
+                            part[j][i] = s + j < p.splits && l + 16 * i < p.rank ? __ldcg(t + (s + j) * split + l + 16 * i) : 0.f;
+                        }
+                    }
 #pragma unroll
-            for (int t = 0; t < TILES / 2; ++t) {
-                const uint32_t col = n0 + 16 * t + 4 * c4;
-                float *y = (r == 0 ? y0 : y1) + col;
-                const bool on = r == 0 ? on0 : on1;
-                if (on && p.y_vectors && col + 3 < end) {
-                    __stcs(reinterpret_cast<float4 *>(y), make_float4(v[r][t][0], v[r][t][1], v[r][t][2], v[r][t][3]));
-                } else if (on) {
+                    for (int j = 0; j < AT_ONCE; ++j) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if (col + e < end) {
-                            y[e] = v[r][t][e];
+                        for (int i = 0; i < KS; ++i) {
+                            x[i] += part[j][i];
                         }
                     }
                 }
             }
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                top = max(top, magnitude(x[i]));
+            }
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) {
+                top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+            }
+            const int e = max(top >> 23, 20);   // to 2^13 .. 2^14
+            const float up = __int_as_float((267 - e) << 23);
+            if (l == 0) {
+                down[row] = __int_as_float((e - 13) << 23);
+            }
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                const uint32_t r = l + 16 * i;
+                if (r < p.rank) {
+                    const uint32_t to = place_of(r, p.rank);
+                    const float scaled = x[i] * up;
+                    const __half h = __float2half_rn(scaled);
+                    hi[row][to] = h;
+                    lo[row][to] = __float2half_rn(scaled - __half2float(h));
+                }
+            }
+        }
+        __syncthreads();
+        uint32_t th[KS][4], tl[KS][4];
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            matrices(th[s], &hi[lane % 16][16 * s + lane / 16 * 8]);
+            matrices(tl[s], &lo[lane % 16][16 * s + lane / 16 * 8]);
+        }
+        const float down0 = down[g], down1 = down[g + 8];
+#pragma unroll 1
+        for (;;) {
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) {
+                float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    mma_f16(c, tl[s][0], tl[s][1], tl[s][2], tl[s][3], w[t][s][0], w[t][s][1]);
+                    mma_f16(c, th[s][0], th[s][1], th[s][2], th[s][3], w[t][s][0], w[t][s][1]);
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    v[0][t / 2][t % 2 * 2 + e] = fmaf(c[e], down0, v[0][t / 2][t % 2 * 2 + e]);
+                    v[1][t / 2][t % 2 * 2 + e] = fmaf(c[2 + e], down1, v[1][t / 2][t % 2 * 2 + e]);
+                }
+            }
+            const bool all = whole();
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+#pragma unroll
+                for (int t = 0; t < TILES / 2; ++t) {
+                    if (!(r == 0 ? on0 : on1)) {
+                        continue;
+                    }
+                    float *y = (r == 0 ? y0 : y1) + 16 * t;
+                    if (all) {
+                        __stcs(reinterpret_cast<float4 *>(y), make_float4(v[r][t][0], v[r][t][1], v[r][t][2], v[r][t][3]));
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if (n0 + 4 * c4 + 16 * t + e < p.N) {
+                                y[e] = v[r][t][e];
+                            }
+                        }
+                    }
+                }
+            }
+            advance();
+            if (++at == stop || step == steps) {
+                break;
+            }
+            fetch();
+        }
+        if (at < stop) {
+            enter();
+            fetch();
         }
     }
 }
@@ -556,15 +637,14 @@ void divide(LoraParams *p, const DeviceCtx *c)
 {
     const uint32_t most = p->rows / 16 + p->segments, sms = (uint32_t)c->sm_count;
     p->units = most < p->rows ? most : p->rows;
-    // K in as many parts as give every SM two CTAs, each at least 256 long (a warp's 32)
-    const uint32_t want = p->units == 0 ? 1 : 2 * sms / p->units, at_most = (p->K + 255) / 256;
+    // K in as many parts as give every SM four CTAs, each at least 256 long (a warp's 32), and sixteen at most, which the
+    // second kernel asks for in two goes
+    const uint32_t want = p->units == 0 ? 1 : 4 * sms / p->units, at_most = (p->K + 255) / 256;
     p->splits = want < 1 ? 1 : (want < at_most ? want : at_most);
-    // Columns in steps of a CTA's 256: as many CTAs as give every SM four, but no more than eight steps each (the start
-    // of a CTA costs as much as two or three).
-    const uint32_t steps = (p->N + 255) / 256, parts = p->units == 0 ? 1 : (4 * sms + p->units - 1) / p->units;
-    uint32_t each = (steps + parts - 1) / parts;
-    each = each < 1 ? 1 : (each > 8 ? 8 : each);
-    p->columns = 256 * each;
+    p->splits = p->splits < 16 ? p->splits : 16;
+    // as many CTAs as run at a time, and no more than there are steps
+    const uint64_t steps = (uint64_t)p->units * ((p->N + STEP - 1) / STEP), ctas = (uint64_t)sms * (p->rank <= 32 ? 3 : 1);
+    p->outer_ctas = (uint32_t)(steps < ctas ? steps : ctas);
 }
 EE check(const bolt_b200_lora_call *a, LoraParams *p, DeviceCtx **c)
 {
@@ -615,8 +695,8 @@ EE check(const bolt_b200_lora_call *a, LoraParams *p, DeviceCtx **c)
     p->y_vectors = aligned(a->y, 16) && a->y_stride % 4 == 0;
     p->status = (*c)->d_status;
     divide(p, *c);
-    if ((uint64_t)p->splits * p->rows * p->rank > 0x3FFFFFFFull) {
-        return NOT_SUPPORTED;    // the workspace is counted in 32 bits
+    if ((uint64_t)p->splits * p->rows * p->rank > 0x3FFFFFFFull || (uint64_t)p->units * ((p->N + STEP - 1) / STEP) > 0xFFFFFFFFull) {
+        return NOT_SUPPORTED;    // the workspace and the steps are counted in 32 bits
     }
     return SUCCESS;
 }
@@ -649,7 +729,7 @@ EE launch_inner(const LoraParams &p, cudaStream_t st)
 }
 EE launch_outer(const LoraParams &p, cudaStream_t st)
 {
-    const dim3 grid(p.units, (p.N + p.columns - 1) / p.columns);
+    const dim3 grid(p.outer_ctas);
     if (p.rank <= 16) {
         return launch(lora_outer_kernel<1>, grid, p, st);
     }
