@@ -148,6 +148,12 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)   // c = a b
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f), "f"(0.f), "f"(0.f), "f"(0.f));
+}
 __device__ __forceinline__ void mma_tf32(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
 {
     asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -390,7 +396,7 @@ __device__ __forceinline__ uint32_t place_of(uint32_t r, uint32_t rank)
 constexpr uint32_t STEP = 256;
 // KS: blocks of 16 of the rank, rounded up
 template <int KS>
-__global__ void __launch_bounds__(256, KS <= 2 ? 3 : 1) lora_outer_kernel(const __grid_constant__ LoraParams p)
+__global__ void __launch_bounds__(256, KS <= 1 ? 4 : (KS <= 2 ? 3 : 1)) lora_outer_kernel(const __grid_constant__ LoraParams p)
 {
     constexpr int PITCH = KS * 16 + 8, TILES = 4;   // columns of a warp at a time: 4 x 8
     constexpr int AT_ONCE = KS <= 2 ? 8 : 4;        // parts of K whose inner sums are asked for at a time
@@ -437,6 +443,12 @@ __global__ void __launch_bounds__(256, KS <= 2 ? 3 : 1) lora_outer_kernel(const 
     };
     auto whole = [&]() { return p.y_vectors && n0 + 8 * TILES <= p.N; };    // nothing to look after
     auto fetch_row = [&](int t, const __half *row, bool on) {
+        if (KS == 1 && on && p.rank == 16) {
+            const uint2 x = __ldg(reinterpret_cast<const uint2 *>(row + 4 * c4));
+            w[t][0][0] = x.x;
+            w[t][0][1] = x.y;
+            return;
+        }
 #pragma unroll
         for (int s = 0; s < KS; s += 2) {
             uint32_t q[4] = {0, 0, 0, 0};
@@ -586,10 +598,14 @@ __global__ void __launch_bounds__(256, KS <= 2 ? 3 : 1) lora_outer_kernel(const 
         for (;;) {
 #pragma unroll
             for (int t = 0; t < TILES; ++t) {
-                float c[4] = {0.f, 0.f, 0.f, 0.f};
+                float c[4];
 #pragma unroll
                 for (int s = 0; s < KS; ++s) {
-                    mma_f16(c, tl[s][0], tl[s][1], tl[s][2], tl[s][3], w[t][s][0], w[t][s][1]);
+                    if (s == 0) {
+                        mma_f16_first(c, tl[s][0], tl[s][1], tl[s][2], tl[s][3], w[t][s][0], w[t][s][1]);
+                    } else {
+                        mma_f16(c, tl[s][0], tl[s][1], tl[s][2], tl[s][3], w[t][s][0], w[t][s][1]);
+                    }
                     mma_f16(c, th[s][0], th[s][1], th[s][2], th[s][3], w[t][s][0], w[t][s][1]);
                 }
 #pragma unroll
@@ -643,7 +659,7 @@ void divide(LoraParams *p, const DeviceCtx *c)
     p->splits = want < 1 ? 1 : (want < at_most ? want : at_most);
     p->splits = p->splits < 16 ? p->splits : 16;
     // as many CTAs as run at a time, and no more than there are steps
-    const uint64_t steps = (uint64_t)p->units * ((p->N + STEP - 1) / STEP), ctas = (uint64_t)sms * (p->rank <= 32 ? 3 : 1);
+    const uint64_t steps = (uint64_t)p->units * ((p->N + STEP - 1) / STEP), ctas = (uint64_t)sms * (p->rank <= 16 ? 4 : (p->rank <= 32 ? 3 : 1));
     p->outer_ctas = (uint32_t)(steps < ctas ? steps : ctas);
 }
 EE check(const bolt_b200_lora_call *a, LoraParams *p, DeviceCtx **c)
