@@ -34,13 +34,25 @@ struct AttentionParams {
     uint32_t sequences, heads, group, head_blocks, table_pages, window;
     float scale, out_scale;
     int i8, q_f16, out_kind;   // 0 binary32, 1 binary16, 2 u8
-    uint32_t team, part_count, share_bytes, out_pairs;
+    uint32_t team, part_count, share_bytes;
+    uint32_t step_pages, step_at, run_tiles;   // tokens of a tile in pages and what is left; tiles of a run
+    uint32_t page_magic;            // 2^32 / page_size
     uint32_t even_bytes, to_1152;   // 0x00FF00FF, 0x64806480   // warps that share a unit; parts of the row
     float *parts;   // workspace: two partial results for every part,
     struct Cut *cuts;   // and what is to be joined
     int *status;
 };
 
+// position / page_size and the remainder: the multiplication is one too low at most
+__device__ __forceinline__ void split_position(const AttentionParams &p, uint32_t position, uint32_t &page, uint32_t &at)
+{
+    page = __umulhi(position, p.page_magic);
+    at = position - page * p.cache.page_size;
+    if (at >= p.cache.page_size) {
+        at -= p.cache.page_size;
+        ++page;
+    }
+}
 __device__ __forceinline__ bool live_tokens(const AttentionParams &p, uint32_t sequence, uint32_t *begin, uint32_t *end)
 {
     return b200::live_tokens(p.length[sequence], p.table_pages, p.cache.page_size, p.window, begin, end);
@@ -61,20 +73,6 @@ __device__ __forceinline__ void store_out(const AttentionParams &p, uint64_t at,
         reinterpret_cast<uint8_t *>(p.out)[at] = (uint8_t)to_u8(x, p.out_scale);
     }
 }
-__device__ __forceinline__ void store_pair(const AttentionParams &p, uint64_t at, float x, float y)
-{
-    if (!p.out_pairs) {
-        store_out(p, at, x);
-        store_out(p, at + 1, y);
-    } else if (p.out_kind == 0) {
-        *reinterpret_cast<float2 *>(reinterpret_cast<float *>(p.out) + at) = make_float2(x, y);
-    } else if (p.out_kind == 1) {
-        *reinterpret_cast<uint32_t *>(reinterpret_cast<__half *>(p.out) + at) = half2_bits(x, y);
-    } else {
-        *reinterpret_cast<uint16_t *>(reinterpret_cast<uint8_t *>(p.out) + at) = (uint16_t)(to_u8(x, p.out_scale) | to_u8(y, p.out_scale) << 8);
-    }
-}
-
 // ---- how the work is divided -----------------------------------------------------------------------------------
 // A unit is one sequence, key head and block of query heads; it has tiles of team x STEP tokens on a grid that starts at
 // token 0.  All units' tiles stand in one row, in which every team of warps takes an equal, contiguous part.
@@ -97,7 +95,7 @@ __device__ __forceinline__ uint32_t count_tiles(const AttentionParams &p, uint32
 // By all warps of a CTA, for each its team's part: the row's length, and the sequence that holds the part's first tile with
 // that sequence's own first place.
 template <int WARPS>
-__device__ __forceinline__ uint32_t locate(const AttentionParams &p, uint32_t units, uint32_t tile_shift, uint32_t team, Counting *c, Found *mine)
+__device__ __forceinline__ Parts locate(const AttentionParams &p, uint32_t units, uint32_t tile_shift, uint32_t team, Counting *c, Found *mine)
 {
     const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, teams = WARPS / team;
     const bool shared = p.sequences > BY_WARP;
@@ -164,7 +162,7 @@ __device__ __forceinline__ uint32_t locate(const AttentionParams &p, uint32_t un
             *mine = c->found[warp / team];
         }
     }
-    return total;
+    return parts;
 }
 // By a warp: the first sequence behind `sequence` that has a token (there is one).
 __device__ __forceinline__ uint32_t next_sequence(const AttentionParams &p, uint32_t sequence)
@@ -275,7 +273,7 @@ struct Shape {
     static constexpr int WARPS = NUMBERS <= 32 && HB == 1 ? 16 : 8;
     static constexpr int Q_PITCH = DP * 2 + 16, Q_BYTES = 2 * HEADS * Q_PITCH;   // queries of a team
     static constexpr int TEAMS = 4 * Q_BYTES <= 20480 ? 4 : (2 * Q_BYTES <= 20480 ? 2 : 1);
-    static constexpr int GO = 16, MERGE = WARPS / 2 * GO * 32 * 4;               // numbers of a lane of half the warps
+    static constexpr int GO = 16, MERGE = WARPS * GO * 32 * 4;                   // numbers of a lane that the warps exchange at a time
     static constexpr int SMALL = 1024 + WARPS * 128;
     static constexpr int FIXED = TEAMS * Q_BYTES + MERGE + SMALL;
     static constexpr int FIT = (232448 - FIXED) / (WARPS * SLOT);
@@ -325,8 +323,7 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");    // nothing in front of this touches global memory
     Found found;
-    const uint32_t total = locate<WARPS>(p, units, tile_shift, team, counting, &found);
-    const Parts parts(total, p.part_count);
+    const Parts parts = locate<WARPS>(p, units, tile_shift, team, counting, &found);
     uint32_t place = part < parts.n ? parts.begin(part) : 0;
     const uint32_t stop = part < parts.n ? parts.begin(part + 1) : 0;
     if (lane == 0 && member == 0) {
@@ -346,27 +343,27 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
     uint32_t sequence = found.sequence, begin, end;
     live_tokens(p, sequence, &begin, &end);
     uint32_t tiles = max(tiles_of(begin, end, tile_shift), 1u);
-    uint32_t unit = min((place - found.first) / tiles, units - 1), tile = (place - found.first) % tiles;
+    const uint32_t units_before = (place - found.first) / tiles;
+    uint32_t unit = min(units_before, units - 1), tile = place - found.first - units_before * tiles;
 
     // ---- the copies ----
     const uint32_t page_size = p.cache.page_size;
     const bool one_page = page_size % S::STEP == 0;    // a step's tokens are neighbours in one page
-    const uint32_t lane_token = lane % S::STEP, step_pages = tile_tokens / page_size, step_at = tile_tokens % page_size;
-    // tiles whose steps lie in 32 pages: (n - 1) tile_tokens + STEP tokens, beginning anywhere in a page
-    const uint32_t run_tiles = 1 + (uint32_t)min((31ull * page_size - min(31ull * page_size, (unsigned long long)S::STEP + page_size - 2)) / tile_tokens, 1ull << 20);
+    const uint32_t lane_token = lane % S::STEP;
     Run run, ahead;
     // the cursor behind `ahead`
     uint32_t left = stop - place, a_sequence = sequence, a_unit = unit, a_tile = tile, a_tiles = tiles, a_begin = begin, a_end = end;
     auto look_ahead = [&]() {
-        ahead.left = min(min(run_tiles, a_tiles - a_tile), left);
+        ahead.left = min(min(p.run_tiles, a_tiles - a_tile), left);
         if (ahead.left == 0) {
             return;
         }
-        ahead.head = a_unit / p.head_blocks;
+        ahead.head = HB == 1 ? a_unit : a_unit / p.head_blocks;
         ahead.begin = a_begin;
         ahead.end = a_end;
         ahead.token = (((a_begin >> tile_shift) + a_tile) << tile_shift) + member * S::STEP;
-        ahead.first_page = ahead.token / page_size;
+        uint32_t within;
+        split_position(p, ahead.token, ahead.first_page, within);
         const uint64_t entry = (uint64_t)ahead.first_page + lane;
         ahead.pages = entry < p.table_pages && entry * page_size < a_end ? (uint32_t)__ldg(p.table + (uint64_t)a_sequence * p.table_pages + entry) : 0xFFFFFFFFu;
         left -= ahead.left;
@@ -384,9 +381,7 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
     uint32_t page_index = 0, at = 0;    // of the lane's token
     auto enter = [&]() {
         run = ahead;
-        const uint32_t t = run.token + (one_page ? 0 : lane_token);
-        page_index = t / page_size;
-        at = t - page_index * page_size;
+        split_position(p, run.token + (one_page ? 0 : lane_token), page_index, at);
         look_ahead();
     };
     look_ahead();
@@ -418,8 +413,8 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
             }
             coming[S::SLOTS / 2 - 1] = live;
             run.token += tile_tokens;
-            page_index += step_pages;
-            at += step_at;
+            page_index += p.step_pages;
+            at += p.step_at;
             if (at >= page_size) {
                 at -= page_size;
                 ++page_index;
@@ -493,10 +488,9 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
     for (;;) {
      if (!EVEN || n != 1 - S::SLOTS) {
       mask = coming[0];
-      if (turn(std::bool_constant<EVEN>())) {
-       if (done == count) {
+      if (n >= 0 && done == count) {
         // ---- a unit begins ----
-        const uint32_t head = unit / p.head_blocks, block = unit % p.head_blocks;
+        const uint32_t head = HB == 1 ? unit : unit / p.head_blocks, block = unit - head * (HB == 1 ? 1 : p.head_blocks);
         heads_here = min((uint32_t)S::HEADS, p.group - block * S::HEADS);
         head0 = head * p.group + block * S::HEADS;
         count = min(tiles - tile, stop - place);
@@ -553,7 +547,8 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
                 acc[n][e] = 0.f;
             }
         }
-       }
+      }
+      if (turn(std::bool_constant<EVEN>())) {
             // scores: [heads] x [tokens]
             float sc[NT][4];
             {
@@ -775,15 +770,25 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
         team_sync();
 #pragma unroll
         for (int b = 0; b < HB; ++b) {
+            // the four lanes of a head look at every fourth warp each
             const uint32_t h = g + 8 * b;
-            float top = -INFINITY, all = 0.f;
-            for (uint32_t w = 0; w < team; ++w) {
-                top = fmaxf(top, warp_m[(warp0 + w) * 16 + h]);
+            float wm[WARPS / 4], top = -INFINITY, all = 0.f;
+#pragma unroll
+            for (int k = 0; k < WARPS / 4; ++k) {
+                const uint32_t w = 4 * k + c4;
+                wm[k] = w < team ? warp_m[(warp0 + w) * 16 + h] : -INFINITY;
+                top = fmaxf(top, wm[k]);
             }
+            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
             const float base = top == -INFINITY ? 0.f : top;
-            for (uint32_t w = 0; w < team; ++w) {
-                all = fmaf(warp_l[(warp0 + w) * 16 + h], exp2_fast(warp_m[(warp0 + w) * 16 + h] - base), all);
+#pragma unroll
+            for (int k = 0; k < WARPS / 4; ++k) {
+                const uint32_t w = 4 * k + c4;
+                all += w < team ? warp_l[(warp0 + w) * 16 + h] * exp2_fast(wm[k] - base) : 0.f;
             }
+            all += __shfl_xor_sync(0xFFFFFFFFu, all, 1);
+            all += __shfl_xor_sync(0xFFFFFFFFu, all, 2);
             own[b] = exp2_fast(m[b] - base) * (I8 ? top_unit : 1.f);
             if (whole) {
                 own[b] *= all == 0.f ? 0.f : __frcp_rn(all);
@@ -800,65 +805,35 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
         if (!whole && tile == 0 && member == 0 && lane == 0) {
             p.cuts[part] = Cut{parts.of(place + tiles - 1) - part + 1, sequence, head0, heads_here};
         }
-        // Sums of the team's upper half are added to the lower half's, and so on; GO numbers of a lane at a time.
+        // GO numbers of every lane of every warp at a time; then each warp adds up some of them over its team.
         constexpr int NUMBERS = S::NUMBERS, GO = S::GO;
 #pragma unroll
-        for (int x = 0; x < NUMBERS; ++x) {
-            acc[x / (2 * HB)][x % (2 * HB)] *= own[x % (2 * HB) / 2];
-        }
-#pragma unroll
         for (int x0 = 0; x0 < NUMBERS; x0 += GO) {
+            if (x0 != 0) {
+                team_sync();
+            }
+#pragma unroll
+            for (int x = 0; x < GO; ++x) {
+                merge[(warp * GO + x) * 32 + lane] = acc[(x0 + x) / (2 * HB)][(x0 + x) % (2 * HB)] * own[(x0 + x) % (2 * HB) / 2];
+            }
+            team_sync();
 #pragma unroll 1
-            for (uint32_t half = team / 2; half != 0; half /= 2) {
-                float *const to = merge + (warp0 / 2 + member % half) * GO * 32 + lane;
-                if (member >= half && member < 2 * half) {
-#pragma unroll
-                    for (int x = 0; x < GO; ++x) {
-                        to[x * 32] = acc[(x0 + x) / (2 * HB)][(x0 + x) % (2 * HB)];
-                    }
+            for (uint32_t x = member; x < GO; x += team) {
+                float sum = 0.f;
+#pragma unroll 4
+                for (uint32_t w = 0; w < team; ++w) {
+                    sum += merge[((warp0 + w) * GO + x) * 32 + lane];
                 }
-                team_sync();
-                if (member < half) {
-#pragma unroll
-                    for (int x = 0; x < GO; ++x) {
-                        acc[(x0 + x) / (2 * HB)][(x0 + x) % (2 * HB)] += to[x * 32];
-                    }
+                const uint32_t t = (x0 + x) / (2 * HB), e = (x0 + x) % (2 * HB), h = g + e / 2 * 8;
+                const uint32_t d = I8 ? t / 2 * 16 + 4 * c4 + e % 2 * 2 + t % 2 : 8 * t + 2 * c4 + e % 2;
+                if (!whole) {
+                    share[h * DP + d] = sum;
+                } else if (h < heads_here && d < dim) {
+                    store_out(p, sequence * p.out_stride + (uint64_t)(head0 + h) * dim + d, sum);
                 }
-                team_sync();
             }
         }
-        if (member == 0) {
-            // neighbours of the row: pairs in two tiles, or (bytes) all four numbers of two tiles
-            auto pairs = [&](auto store) {
-#pragma unroll
-                for (int b = 0; b < HB; ++b) {
-#pragma unroll
-                    for (int n = 0; n < TILES_D; n += 2) {
-#pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            const uint32_t d = I8 ? 8 * n + 4 * c4 + 2 * k : 8 * (n + k) + 2 * c4;
-                            store(g + 8 * b, d, I8 ? acc[n][2 * b + k] : acc[n + k][2 * b], I8 ? acc[n + 1][2 * b + k] : acc[n + k][2 * b + 1]);
-                        }
-                    }
-                }
-            };
-            const uint64_t to = sequence * p.out_stride + (uint64_t)head0 * dim;
-            if (!whole) {
-                pairs([&](uint32_t h, uint32_t d, float x, float y) { *reinterpret_cast<float2 *>(share + h * DP + d) = make_float2(x, y); });
-            } else if (p.out_pairs && p.out_kind == 0) {
-                pairs([&](uint32_t h, uint32_t d, float x, float y) {
-                    if (h < heads_here && d < dim) {
-                        *reinterpret_cast<float2 *>(reinterpret_cast<float *>(p.out) + to + h * dim + d) = make_float2(x, y);
-                    }
-                });
-            } else {
-                pairs([&](uint32_t h, uint32_t d, float x, float y) {
-                    if (h < heads_here && d < dim) {
-                        store_pair(p, to + h * dim + d, x, y);
-                    }
-                });
-            }
-        }
+        team_sync();
         // ---- the next unit ----
         place += count;
         tile = 0;
@@ -995,6 +970,13 @@ EE plan(const DeviceCtx *c, AttentionParams *p, uint64_t units)
     }
     p->part_count = ctas * S::WARPS / p->team;
     p->share_bytes = p->part_count * 2 * S::PART * 4;
+    const uint32_t tile = p->team * S::STEP, page = p->cache.page_size;
+    p->step_pages = tile / page;
+    p->step_at = tile % page;
+    // tiles whose steps lie in 32 pages: (n - 1) tile + STEP tokens, beginning anywhere in a page
+    const uint64_t room = 31ull * page, taken = (uint64_t)S::STEP + page - 2, tiles = room > taken ? (room - taken) / tile : 0;
+    p->run_tiles = 1 + (uint32_t)(tiles < (1u << 20) ? tiles : (1u << 20));
+    p->page_magic = page == 1 ? 0xFFFFFFFFu : (uint32_t)((1ull << 32) / page);
     return SUCCESS;
 }
 template <int DP, bool I8, int HB>
@@ -1079,9 +1061,6 @@ EE check(const bolt_b200_kv_cache *cache, const bolt_b200_paged_attention_call *
     p->sequences = a->sequences;
     p->heads = a->heads;
     p->group = a->heads / cache->kv_heads;
-    // rows that can be written two elements at a time (dim is a multiple of 8)
-    const uint32_t out_size = a->out_dt == DT_F32 ? 4 : (a->out_dt == DT_F16 ? 2 : 1);
-    p->out_pairs = aligned(a->out, 2 * out_size) && a->out_stride % 2 == 0;
     p->head_blocks = p->group <= 8 ? 1 : (p->group + 15) / 16;
     p->table_pages = a->table_pages;
     p->window = a->window;
