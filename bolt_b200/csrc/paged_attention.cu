@@ -274,7 +274,7 @@ struct Shape {
     static constexpr int Q_PITCH = DP * 2 + 16, Q_BYTES = 2 * HEADS * Q_PITCH;   // queries of a team
     static constexpr int TEAMS = 4 * Q_BYTES <= 20480 ? 4 : (2 * Q_BYTES <= 20480 ? 2 : 1);
     static constexpr int GO = 16, MERGE = WARPS * GO * 32 * 4;                   // numbers of a lane that the warps exchange at a time
-    static constexpr int SMALL = 1024 + WARPS * 128;
+    static constexpr int SMALL = 1024 + WARPS * 320;
     static constexpr int FIXED = TEAMS * Q_BYTES + MERGE + SMALL;
     static constexpr int FIT = (232448 - FIXED) / (WARPS * SLOT);
     static constexpr int SLOTS = FIT > 6 ? 6 : FIT;                              // ring of a warp: K, V, K, V ...
@@ -289,7 +289,13 @@ struct Run {
     uint32_t left;                         // tiles
     uint32_t token;                        // first one of the warp's step
     uint32_t first_page;                   // of the table's row
-    uint32_t pages;
+};
+// The run behind it, and where the one after that begins: in shared memory, for registers are short.  (All lanes write the
+// same and read what they wrote.)
+struct Ahead {
+    Run run;
+    uint32_t sequence, unit, tile, tiles, begin, end, left;
+    uint32_t pages[32];
 };
 
 template <int DP, bool I8, int HB>
@@ -307,6 +313,8 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
     asm volatile("mov.u32 %0, %%laneid;" : "=r"(lane));     // (kept in a register, not asked for again and again)
     asm volatile("mov.u32 %0, %0;" : "+r"(warp));
     const uint32_t g = lane / 4, c4 = lane % 4;
+    static_assert(sizeof(Ahead) <= 192, "");
+    Ahead &ahead = *reinterpret_cast<Ahead *>(small + 1024 + WARPS * 128 + warp * 192);
     char *const ring = smem + S::FIXED + warp * S::SLOTS * S::SLOT;
     const uint32_t dim = p.cache.dim, pieces = dim * S::SIZE / 16, units = p.cache.kv_heads * p.head_blocks;
     const uint32_t team = p.team, member = warp % team, teams = WARPS / team;
@@ -350,37 +358,55 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
     const uint32_t page_size = p.cache.page_size;
     const bool one_page = page_size % S::STEP == 0;    // a step's tokens are neighbours in one page
     const uint32_t lane_token = lane % S::STEP;
-    Run run, ahead;
-    // the cursor behind `ahead`
-    uint32_t left = stop - place, a_sequence = sequence, a_unit = unit, a_tile = tile, a_tiles = tiles, a_begin = begin, a_end = end;
+    Run run;
+    uint32_t pages = 0;
+    ahead.left = stop - place;
+    ahead.sequence = sequence;
+    ahead.unit = unit;
+    ahead.tile = tile;
+    ahead.tiles = tiles;
+    ahead.begin = begin;
+    ahead.end = end;
     auto look_ahead = [&]() {
-        ahead.left = min(min(p.run_tiles, a_tiles - a_tile), left);
-        if (ahead.left == 0) {
+        Run next;
+        uint32_t t = ahead.tile, tiles = ahead.tiles, left = ahead.left;
+        next.left = min(min(p.run_tiles, tiles - t), left);
+        ahead.run.left = next.left;
+        if (next.left == 0) {
             return;
         }
-        ahead.head = HB == 1 ? a_unit : a_unit / p.head_blocks;
-        ahead.begin = a_begin;
-        ahead.end = a_end;
-        ahead.token = (((a_begin >> tile_shift) + a_tile) << tile_shift) + member * S::STEP;
+        next.head = HB == 1 ? ahead.unit : ahead.unit / p.head_blocks;
+        next.begin = ahead.begin;
+        next.end = ahead.end;
+        next.token = (((next.begin >> tile_shift) + t) << tile_shift) + member * S::STEP;
         uint32_t within;
-        split_position(p, ahead.token, ahead.first_page, within);
-        const uint64_t entry = (uint64_t)ahead.first_page + lane;
-        ahead.pages = entry < p.table_pages && entry * page_size < a_end ? (uint32_t)__ldg(p.table + (uint64_t)a_sequence * p.table_pages + entry) : 0xFFFFFFFFu;
-        left -= ahead.left;
-        a_tile += ahead.left;
-        if (a_tile == a_tiles && left != 0) {
-            a_tile = 0;
-            if (++a_unit == units) {
-                a_unit = 0;
-                a_sequence = next_sequence(p, a_sequence);
-                live_tokens(p, a_sequence, &a_begin, &a_end);
-                a_tiles = max(tiles_of(a_begin, a_end, tile_shift), 1u);
+        split_position(p, next.token, next.first_page, within);
+        ahead.run = next;
+        const uint64_t entry = (uint64_t)next.first_page + lane;
+        ahead.pages[lane] = entry < p.table_pages && entry * page_size < next.end ?
+            (uint32_t)__ldg(p.table + (uint64_t)ahead.sequence * p.table_pages + entry) : 0xFFFFFFFFu;
+        left -= next.left;
+        t += next.left;
+        if (t == tiles && left != 0) {
+            t = 0;
+            if (++ahead.unit == units) {
+                ahead.unit = 0;
+                const uint32_t s = next_sequence(p, ahead.sequence);
+                uint32_t b, e;
+                live_tokens(p, s, &b, &e);
+                ahead.sequence = s;
+                ahead.begin = b;
+                ahead.end = e;
+                ahead.tiles = max(tiles_of(b, e, tile_shift), 1u);
             }
         }
+        ahead.tile = t;
+        ahead.left = left;
     };
     uint32_t page_index = 0, at = 0;    // of the lane's token
     auto enter = [&]() {
-        run = ahead;
+        run = ahead.run;
+        pages = ahead.pages[lane];
         split_position(p, run.token + (one_page ? 0 : lane_token), page_index, at);
         look_ahead();
     };
@@ -397,7 +423,7 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
         constexpr bool values = decltype(kind)::value;
         if constexpr (!values) {
             // (a run that has come to its end has no tokens inside)
-            const uint32_t page = __shfl_sync(0xFFFFFFFFu, run.pages, page_index - run.first_page), t = run.token + lane_token;
+            const uint32_t page = __shfl_sync(0xFFFFFFFFu, pages, page_index - run.first_page), t = run.token + lane_token;
             const bool inside = t >= run.begin && t < run.end, good = page < p.cache.pages;
             live = __ballot_sync(0xFFFFFFFFu, inside && good) & S::ALL;
             if (live != S::ALL && inside && !good) {
@@ -451,7 +477,7 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
         if (!values && run.left == 0) {
-            if (ahead.left != 0) {
+            if (ahead.run.left != 0) {
                 enter();
             } else {
                 run.end = 0;
