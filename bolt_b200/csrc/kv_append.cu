@@ -93,174 +93,211 @@ struct AppendParams {
     int *status;
 };
 
-// one row of TIN by LANES lanes, VW neighbouring elements at a time, PER times
-template <typename TIN, int VW, int LANES, int PER>
+// ROWS neighbouring heads of a token, all queries, keys or values, by LANES lanes, VW neighbouring elements of a row at a
+// time, PER times.  They share the position, the page, the angles and all but the last step of every address: with one row
+// to a group of lanes 4005 tokens of 64 + 16 heads (277 MB) took 86 us, bound by the instructions.
+template <typename TIN, int VW, int LANES, int PER, int ROWS>
 __global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ AppendParams p)
 {
-    const uint32_t rows_per_token = p.heads + 2 * p.cache.kv_heads;
-    const uint64_t row = ((uint64_t)blockIdx.x * 256 + threadIdx.x) / LANES;
-    const uint32_t lane = threadIdx.x % LANES;
-    bool live = row < (uint64_t)p.tokens * rows_per_token;
-    const uint32_t token = live ? (uint32_t)row / rows_per_token : 0, h = live ? (uint32_t)row - token * rows_per_token : 0;
-    const int kind = h < p.heads ? 0 : (h < p.heads + p.cache.kv_heads ? 1 : 2);
-    const uint32_t head = kind == 0 ? h : (kind == 1 ? h - p.heads : h - p.heads - p.cache.kv_heads);
-    const uint32_t dim = p.cache.dim, rotary = kind == 2 ? 0 : p.rotary, half = rotary / 2;
-    const int32_t position = live ? p.position[token] : -1;
-    live = live && position >= 0;
-    uint32_t page = 0, at = 0;
-    if (live) {
-        const int64_t seq = p.sequence != nullptr ? p.sequence[token] : (int64_t)token;
-        const bool good = seq >= 0 && seq < (int64_t)p.sequences && (p.rotary == 0 || (uint32_t)position < p.rotary_positions) &&
-            page_of(p.table, (uint64_t)seq, p.table_pages, p.cache.pages, p.cache.page_size, (uint32_t)position, &page, &at);
-        if (!good) {
-            if (lane == 0) {
-                atomicExch(p.status, BAD_APPEND);
-            }
-            live = false;
-        }
-    }
-    const TIN *src = reinterpret_cast<const TIN *>(p.src[kind]) + token * p.stride[kind] + (uint64_t)head * dim;
-    const float *cos = p.cos + (uint64_t)(uint32_t)position * (p.rotary / 2), *sin = p.sin + (uint64_t)(uint32_t)position * (p.rotary / 2);
-    float x[PER][VW];
-    int top = 0;
+    const uint32_t q_groups = (p.heads + ROWS - 1) / ROWS, kv_groups = (p.cache.kv_heads + ROWS - 1) / ROWS, groups = q_groups + 2 * kv_groups;
+    const uint32_t group = (uint32_t)(((uint64_t)blockIdx.x * 256 + threadIdx.x) / LANES), lane = threadIdx.x % LANES;
+    const uint32_t token = group / groups, of_token = group - token * groups, dim = p.cache.dim;
+    const bool there = token < p.tokens;
+    const int kind = of_token < q_groups ? 0 : (of_token < q_groups + kv_groups ? 1 : 2);   // queries, keys, values
+    const uint32_t h0 = (of_token - (kind == 0 ? 0 : (kind == 1 ? q_groups : q_groups + kv_groups))) * ROWS;
+    const uint32_t rows = there ? min((uint32_t)ROWS, (kind == 0 ? p.heads : p.cache.kv_heads) - h0) : 0;
+    // Everything that does not hang on the position is asked for with it: the rows, and (y) the other halves of their pairs.
+    const int32_t position = there ? p.position[token] : -1;
+    const int64_t sequence = !there ? -1 : (p.sequence != nullptr ? p.sequence[token] : (int64_t)token);
+    const uint32_t rotary = kind == 2 ? 0 : p.rotary, half = rotary / 2;
+    const bool halves = VW == 4 && !p.interleaved;
+    const TIN *const src = reinterpret_cast<const TIN *>(p.src[kind]) + token * p.stride[kind] + (uint64_t)h0 * dim;
+    float x[ROWS][PER][VW], y[ROWS][PER][VW];
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
         const uint32_t i = (lane + j * LANES) * VW;
+        const TIN *from = src + i, *other = src + (i < half ? i + half : i - half);
 #pragma unroll
-        for (int e = 0; e < VW; ++e) {
-            x[j][e] = 0.f;
+        for (int r = 0; r < ROWS; ++r) {
+#pragma unroll
+            for (int e = 0; e < VW; ++e) {
+                x[r][j][e] = y[r][j][e] = 0.f;
+            }
+            if (r < rows && i < dim) {
+                if constexpr (VW == 4) {
+                    load4(from, x[r][j]);
+                    if (halves && i < rotary) {
+                        load4(other, y[r][j]);
+                    }
+                } else {
+                    x[r][j][0] = load1(from);
+                }
+            }
+            from += dim;
+            other += dim;
         }
-        if (!live || i >= dim) {
+    }
+    // the page, asked for with the angles
+    const bool turns = position >= 0 && (uint32_t)position < p.rotary_positions;
+    uint32_t page = 0, at = 0;
+    const bool live = position >= 0 && sequence >= 0 && sequence < (int64_t)p.sequences && (p.rotary == 0 || turns) &&
+        page_of(p.table, (uint64_t)sequence, p.table_pages, p.cache.pages, p.cache.page_size, (uint32_t)position, &page, &at);
+    const uint64_t angles = (uint64_t)(uint32_t)position * (p.rotary / 2);
+    const float *cos = p.cos + angles, *sin = p.sin + angles;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const uint32_t i = (lane + j * LANES) * VW;
+        if (!turns || i >= rotary) {
             continue;
         }
         if constexpr (VW == 4) {
-            load4(src + i, x[j]);
-            if (i < rotary) {
-                if (p.interleaved) {
+            if (p.interleaved) {
+                const float c[2] = {cos[i / 2], cos[i / 2 + 1]}, s[2] = {sin[i / 2], sin[i / 2 + 1]};
 #pragma unroll
-                    for (int e = 0; e < 4; e += 2) {
-                        const float c = cos[(i + e) / 2], s = sin[(i + e) / 2], a = x[j][e], b = x[j][e + 1];
-                        x[j][e] = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s));
-                        x[j][e + 1] = __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s));
+                for (int r = 0; r < ROWS; ++r) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float a = x[r][j][2 * e], b = x[r][j][2 * e + 1];
+                        x[r][j][2 * e] = __fsub_rn(__fmul_rn(a, c[e]), __fmul_rn(b, s[e]));
+                        x[r][j][2 * e + 1] = __fadd_rn(__fmul_rn(b, c[e]), __fmul_rn(a, s[e]));
                     }
-                } else {
-                    float y[4], c[4], s[4];
-                    const bool first = i < half;
-                    const uint32_t k = first ? i : i - half;
-                    load4(src + (first ? i + half : k), y);
-                    load4(cos + k, c);
-                    load4(sin + k, s);
+                }
+            } else {
+                float c[4], s[4];
+                load4(cos + (i < half ? i : i - half), c);
+                load4(sin + (i < half ? i : i - half), s);
+                // a' = a c + b (-s), b' = b c + a s: a sum with the negative is the difference, bit for bit
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[e] = i < half ? -s[e] : s[e];
+                }
+#pragma unroll
+                for (int r = 0; r < ROWS; ++r) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float own = __fmul_rn(x[j][e], c[e]), other = __fmul_rn(y[e], s[e]);
-                        x[j][e] = first ? __fsub_rn(own, other) : __fadd_rn(own, other);
+                        x[r][j][e] = __fadd_rn(__fmul_rn(x[r][j][e], c[e]), __fmul_rn(y[r][j][e], s[e]));
                     }
                 }
             }
         } else {
-            x[j][0] = load1(src + i);
-            if (i < rotary) {
-                const bool first = p.interleaved ? (i & 1) == 0 : i < half;
-                const uint32_t k = p.interleaved ? i / 2 : (first ? i : i - half);
-                const uint32_t o = p.interleaved ? i ^ 1 : (first ? i + half : k);
-                const float own = __fmul_rn(x[j][0], cos[k]), other = __fmul_rn(load1(src + o), sin[k]);
-                x[j][0] = first ? __fsub_rn(own, other) : __fadd_rn(own, other);
-            }
-        }
+            const bool first = p.interleaved ? (i & 1) == 0 : i < half;
+            const uint32_t k = p.interleaved ? i / 2 : (first ? i : i - half), o = p.interleaved ? i ^ 1 : (first ? i + half : k);
 #pragma unroll
-        for (int e = 0; e < VW; ++e) {
-            top = max(top, magnitude(x[j][e]));
-        }
-    }
-    __syncwarp();   // q_out may be q: every lane has read its row
-    if (kind == 0) {
-        if (!live) {
-            return;
-        }
-        const uint64_t o = token * p.q_out_stride + (uint64_t)head * dim;
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const uint32_t i = (lane + j * LANES) * VW;
-            if (i < dim) {
-                if constexpr (VW == 4) {
-                    if (p.q_out_f16) {
-                        *reinterpret_cast<uint2 *>(reinterpret_cast<__half *>(p.q_out) + o + i) =
-                            make_uint2(half2_bits(x[j][0], x[j][1]), half2_bits(x[j][2], x[j][3]));
-                    } else {
-                        *reinterpret_cast<float4 *>(reinterpret_cast<float *>(p.q_out) + o + i) = make_float4(x[j][0], x[j][1], x[j][2], x[j][3]);
-                    }
-                } else if (p.q_out_f16) {
-                    reinterpret_cast<__half *>(p.q_out)[o + i] = __float2half_rn(x[j][0]);
-                } else {
-                    reinterpret_cast<float *>(p.q_out)[o + i] = x[j][0];
+            for (int r = 0; r < ROWS; ++r) {
+                if (r < rows) {
+                    const float own = __fmul_rn(x[r][j][0], cos[k]), other = __fmul_rn(load1(src + r * dim + o), sin[k]);
+                    x[r][j][0] = first ? __fsub_rn(own, other) : __fadd_rn(own, other);
                 }
             }
         }
-        return;
     }
-    const uint64_t o = row_element(p.cache, page, at, head);
-    void *cache = kind == 1 ? p.k_cache : p.v_cache;
-    if (!p.i8) {
-        if (!live) {
-            return;
-        }
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const uint32_t i = (lane + j * LANES) * VW;
-            if (i < dim) {
-                __half *d = reinterpret_cast<__half *>(cache) + o + i;
-                if constexpr (VW == 4) {
-                    *reinterpret_cast<uint2 *>(d) = make_uint2(half2_bits(x[j][0], x[j][1]), half2_bits(x[j][2], x[j][3]));
-                } else {
-                    *d = __float2half_rn(x[j][0]);
-                }
-            }
-        }
-        return;
+    if (position >= 0 && !live && lane == 0) {
+        atomicExch(p.status, BAD_APPEND);
     }
-    const unsigned mask = LANES == 32 ? 0xFFFFFFFFu : 0xFFFFu << (threadIdx.x & 16);
-#pragma unroll
-    for (int s = LANES / 2; s > 0; s >>= 1) {
-        top = max(top, __shfl_xor_sync(mask, top, s, LANES));
-    }
+    __syncwarp();   // q_out may be q: every lane has read its rows
     if (!live) {
-        return;
+        return;     // (the same for all lanes of a group)
     }
-    const float scale = top == 0 ? 1.0f : __fdiv_rn(127.0f, __int_as_float(top));
-    auto byte = [scale](float v) { return (uint32_t)(min(127, max(-127, cvt_rne_x86(__fmul_rn(v, scale)))) & 0xFF); };
+    // the rows, `step` elements apart from `to` on
+    const uint64_t to = kind == 0 ? token * p.q_out_stride + (uint64_t)h0 * dim : row_element(p.cache, page, at, h0);
+    const uint64_t step = kind == 0 ? dim : p.cache.head_stride;
+    if (kind == 0 && !p.q_out_f16) {
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        const uint32_t i = (lane + j * LANES) * VW;
-        if (i < dim) {
-            uint8_t *d = reinterpret_cast<uint8_t *>(cache) + o + i;
-            if constexpr (VW == 4) {
-                *reinterpret_cast<uint32_t *>(d) = byte(x[j][0]) | byte(x[j][1]) << 8 | byte(x[j][2]) << 16 | byte(x[j][3]) << 24;
-            } else {
-                *d = (uint8_t)byte(x[j][0]);
+        for (int j = 0; j < PER; ++j) {
+            const uint32_t i = (lane + j * LANES) * VW;
+            float *d = reinterpret_cast<float *>(p.q_out) + to + i;
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r, d += step) {
+                if (r < rows && i < dim) {
+                    if constexpr (VW == 4) {
+                        *reinterpret_cast<float4 *>(d) = make_float4(x[r][j][0], x[r][j][1], x[r][j][2], x[r][j][3]);
+                    } else {
+                        *d = x[r][j][0];
+                    }
+                }
             }
         }
-    }
-    if (lane == 0) {
-        (kind == 1 ? p.k_scale : p.v_scale)[scale_element(p.cache, page, at, head)] = scale;
+    } else if (kind == 0 || !p.i8) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const uint32_t i = (lane + j * LANES) * VW;
+            __half *d = reinterpret_cast<__half *>(kind == 0 ? p.q_out : (kind == 1 ? p.k_cache : p.v_cache)) + to + i;
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r, d += step) {
+                if (r < rows && i < dim) {
+                    if constexpr (VW == 4) {
+                        *reinterpret_cast<uint2 *>(d) = make_uint2(half2_bits(x[r][j][0], x[r][j][1]), half2_bits(x[r][j][2], x[r][j][3]));
+                    } else {
+                        *d = __float2half_rn(x[r][j][0]);
+                    }
+                }
+            }
+        }
+    } else {
+        const unsigned mask = LANES == 32 ? 0xFFFFFFFFu : 0xFFFFu << (threadIdx.x & 16);
+        uint8_t *d = reinterpret_cast<uint8_t *>(kind == 1 ? p.k_cache : p.v_cache) + to;
+        float *scales = (kind == 1 ? p.k_scale : p.v_scale) + scale_element(p.cache, page, at, h0);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r, d += step, scales += p.cache.page_size) {
+            if (r >= rows) {
+                break;
+            }
+            int top = 0;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+#pragma unroll
+                for (int e = 0; e < VW; ++e) {
+                    top = max(top, magnitude(x[r][j][e]));
+                }
+            }
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o >>= 1) {
+                top = max(top, __shfl_xor_sync(mask, top, o, LANES));
+            }
+            const float scale = top == 0 ? 1.0f : __fdiv_rn(127.0f, __int_as_float(top));
+            // rne, then the limits, as F32 -> I8 has it (the limits are whole numbers: their order does not matter; NaN: -127)
+            auto byte = [scale](float v) { return (uint32_t)__float2int_rn(fminf(fmaxf(__fmul_rn(v, scale), -127.f), 127.f)) & 0xFFu; };
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const uint32_t i = (lane + j * LANES) * VW;
+                if (i < dim) {
+                    if constexpr (VW == 4) {
+                        *reinterpret_cast<uint32_t *>(d + i) =
+                            byte(x[r][j][0]) | byte(x[r][j][1]) << 8 | byte(x[r][j][2]) << 16 | byte(x[r][j][3]) << 24;
+                    } else {
+                        d[i] = (uint8_t)byte(x[r][j][0]);
+                    }
+                }
+            }
+            if (lane == 0) {
+                *scales = scale;
+            }
+        }
     }
 }
 
-template <typename TIN>
-EE launch(const AppendParams &p, bool vectors, cudaStream_t st)
+template <typename TIN, int VW, int LANES, int PER, int ROWS>
+EE launch_rows(const AppendParams &p, cudaStream_t st)
 {
-    const uint64_t rows = (uint64_t)p.tokens * (p.heads + 2 * p.cache.kv_heads);
-    const uint32_t lanes = vectors && p.cache.dim <= 64 ? 16 : 32;
-    const uint32_t grid = (uint32_t)((rows * lanes + 255) / 256);
+    const uint64_t groups = (uint64_t)p.tokens * ((p.heads + ROWS - 1) / ROWS + 2 * ((p.cache.kv_heads + ROWS - 1) / ROWS));
+    return launch_kernel(dim3((uint32_t)((groups * LANES + 255) / 256)), 256, 0, st, kv_append_kernel<TIN, VW, LANES, PER, ROWS>, p);
+}
+template <typename TIN>
+EE launch(const AppendParams &p, bool vectors, int sms, cudaStream_t st)
+{
     if (!vectors) {
-        return launch_kernel(grid, 256, 0, st, kv_append_kernel<TIN, 1, 32, 8>, p);
+        return launch_rows<TIN, 1, 32, 8, 1>(p, st);
     }
+    // One row to a group of lanes as long as all of them run at once (64 tokens of 64 + 16 heads: 2.9 us in a graph, 4.1 with
+    // four rows), four beyond.
+    const bool few = (uint64_t)p.tokens * (p.heads + 2 * p.cache.kv_heads) <= (uint64_t)sms * 64;
     if (p.cache.dim <= 64) {
-        return launch_kernel(grid, 256, 0, st, kv_append_kernel<TIN, 4, 16, 1>, p);
+        return few ? launch_rows<TIN, 4, 16, 1, 1>(p, st) : launch_rows<TIN, 4, 16, 1, 4>(p, st);
     }
     if (p.cache.dim <= 128) {
-        return launch_kernel(grid, 256, 0, st, kv_append_kernel<TIN, 4, 32, 1>, p);
+        return few ? launch_rows<TIN, 4, 32, 1, 1>(p, st) : launch_rows<TIN, 4, 32, 1, 4>(p, st);
     }
-    return launch_kernel(grid, 256, 0, st, kv_append_kernel<TIN, 4, 32, 2>, p);
+    return few ? launch_rows<TIN, 4, 32, 2, 1>(p, st) : launch_rows<TIN, 4, 32, 2, 2>(p, st);
 }
 
 }  // namespace
@@ -348,5 +385,5 @@ extern "C" EE bolt_b200_kv_append(const bolt_b200_kv_cache *cache, const bolt_b2
     const bool vectors = aligned(a->k, q4) && aligned(a->v, q4) && a->k_stride % 4 == 0 && a->v_stride % 4 == 0 &&
         (a->heads == 0 || (aligned(a->q, q4) && a->q_stride % 4 == 0 && aligned(a->q_out, q_size * 4) && a->q_out_stride % 4 == 0)) &&
         (a->rotary_dim == 0 || (a->interleaved ? a->rotary_dim % 4 == 0 : a->rotary_dim % 8 == 0 && aligned(a->cos, 16) && aligned(a->sin, 16)));
-    return a->dt == DT_F32 ? launch<float>(p, vectors, tls().stream) : launch<__half>(p, vectors, tls().stream);
+    return a->dt == DT_F32 ? launch<float>(p, vectors, c->sm_count, tls().stream) : launch<__half>(p, vectors, c->sm_count, tls().stream);
 }
