@@ -347,537 +347,550 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
         }
     };
 
-  if (place < stop) {
-    uint32_t sequence = found.sequence, begin, end;
-    live_tokens(p, sequence, &begin, &end);
-    uint32_t tiles = max(tiles_of(begin, end, tile_shift), 1u);
-    const uint32_t units_before = (place - found.first) / tiles;
-    uint32_t unit = min(units_before, units - 1), tile = place - found.first - units_before * tiles;
+    if (place < stop) {
+        uint32_t sequence = found.sequence, begin, end;
+        live_tokens(p, sequence, &begin, &end);
+        uint32_t tiles = max(tiles_of(begin, end, tile_shift), 1u);
+        const uint32_t units_before = (place - found.first) / tiles;
+        uint32_t unit = min(units_before, units - 1), tile = place - found.first - units_before * tiles;
 
-    // ---- the copies ----
-    const uint32_t page_size = p.cache.page_size;
-    const bool one_page = page_size % S::STEP == 0;    // a step's tokens are neighbours in one page
-    const uint32_t lane_token = lane % S::STEP;
-    Run run;
-    uint32_t pages = 0;
-    ahead.left = stop - place;
-    ahead.sequence = sequence;
-    ahead.unit = unit;
-    ahead.tile = tile;
-    ahead.tiles = tiles;
-    ahead.begin = begin;
-    ahead.end = end;
-    auto look_ahead = [&]() {
-        Run next;
-        uint32_t t = ahead.tile, tiles = ahead.tiles, left = ahead.left;
-        next.left = min(min(p.run_tiles, tiles - t), left);
-        ahead.run.left = next.left;
-        if (next.left == 0) {
-            return;
-        }
-        next.head = HB == 1 ? ahead.unit : ahead.unit / p.head_blocks;
-        next.begin = ahead.begin;
-        next.end = ahead.end;
-        next.token = (((next.begin >> tile_shift) + t) << tile_shift) + member * S::STEP;
-        uint32_t within;
-        split_position(p, next.token, next.first_page, within);
-        ahead.run = next;
-        const uint64_t entry = (uint64_t)next.first_page + lane;
-        ahead.pages[lane] = entry < p.table_pages && entry * page_size < next.end ?
-            (uint32_t)__ldg(p.table + (uint64_t)ahead.sequence * p.table_pages + entry) : 0xFFFFFFFFu;
-        left -= next.left;
-        t += next.left;
-        if (t == tiles && left != 0) {
-            t = 0;
-            if (++ahead.unit == units) {
-                ahead.unit = 0;
-                const uint32_t s = next_sequence(p, ahead.sequence);
-                uint32_t b, e;
-                live_tokens(p, s, &b, &e);
-                ahead.sequence = s;
-                ahead.begin = b;
-                ahead.end = e;
-                ahead.tiles = max(tiles_of(b, e, tile_shift), 1u);
+        // ---- the copies ----
+        const uint32_t page_size = p.cache.page_size;
+        const bool one_page = page_size % S::STEP == 0;    // a step's tokens are neighbours in one page
+        const uint32_t lane_token = lane % S::STEP;
+        Run run;
+        uint32_t pages = 0;
+        ahead.left = stop - place;
+        ahead.sequence = sequence;
+        ahead.unit = unit;
+        ahead.tile = tile;
+        ahead.tiles = tiles;
+        ahead.begin = begin;
+        ahead.end = end;
+        auto look_ahead = [&]() {
+            Run next;
+            uint32_t t = ahead.tile, tiles = ahead.tiles, left = ahead.left;
+            next.left = min(min(p.run_tiles, tiles - t), left);
+            ahead.run.left = next.left;
+            if (next.left == 0) {
+                return;
             }
-        }
-        ahead.tile = t;
-        ahead.left = left;
-    };
-    uint32_t page_index = 0, at = 0;    // of the lane's token
-    auto enter = [&]() {
-        run = ahead.run;
-        pages = ahead.pages[lane];
-        split_position(p, run.token + (one_page ? 0 : lane_token), page_index, at);
+            next.head = HB == 1 ? ahead.unit : ahead.unit / p.head_blocks;
+            next.begin = ahead.begin;
+            next.end = ahead.end;
+            next.token = (((next.begin >> tile_shift) + t) << tile_shift) + member * S::STEP;
+            uint32_t within;
+            split_position(p, next.token, next.first_page, within);
+            ahead.run = next;
+            const uint64_t entry = (uint64_t)next.first_page + lane;
+            ahead.pages[lane] = entry < p.table_pages && entry * page_size < next.end ?
+                (uint32_t)__ldg(p.table + (uint64_t)ahead.sequence * p.table_pages + entry) : 0xFFFFFFFFu;
+            left -= next.left;
+            t += next.left;
+            if (t == tiles && left != 0) {
+                t = 0;
+                if (++ahead.unit == units) {
+                    ahead.unit = 0;
+                    const uint32_t s = next_sequence(p, ahead.sequence);
+                    uint32_t b, e;
+                    live_tokens(p, s, &b, &e);
+                    ahead.sequence = s;
+                    ahead.begin = b;
+                    ahead.end = e;
+                    ahead.tiles = max(tiles_of(b, e, tile_shift), 1u);
+                }
+            }
+            ahead.tile = t;
+            ahead.left = left;
+        };
+        uint32_t page_index = 0, at = 0;    // of the lane's token
+        auto enter = [&]() {
+            run = ahead.run;
+            pages = ahead.pages[lane];
+            split_position(p, run.token + (one_page ? 0 : lane_token), page_index, at);
+            look_ahead();
+        };
         look_ahead();
-    };
-    look_ahead();
-    enter();
-    uint64_t row = 0, scale_row = 0;    // elements of the lane's row in the tile at hand
-    uint32_t live = 0;                  // its tokens that count
-    const uint32_t copy_row = lane / (S::ROW / 16), copy_piece = lane % (S::ROW / 16);   // of the first piece that the lane copies
-    const uint64_t token_bytes = p.cache.token_stride * S::SIZE;
-    const uint32_t ring_at = smem_at(ring), lane_at = copy_row * S::PITCH + copy_piece * 16;
-    const bool plain = one_page && dim == DP;
-    uint32_t coming[S::SLOTS / 2];      // `live` of the steps that have been asked for and not been used
-    auto issue = [&](auto kind, uint32_t slot) {    // asks for K (and V) of the next step
-        constexpr bool values = decltype(kind)::value;
-        if constexpr (!values) {
-            // (a run that has come to its end has no tokens inside)
-            const uint32_t page = __shfl_sync(0xFFFFFFFFu, pages, page_index - run.first_page), t = run.token + lane_token;
-            const bool inside = t >= run.begin && t < run.end, good = page < p.cache.pages;
-            live = __ballot_sync(0xFFFFFFFFu, inside && good) & S::ALL;
-            if (live != S::ALL && inside && !good) {
-                atomicExch(p.status, BAD_ATTENTION);
-            }
-            row = good ? row_element(p.cache, page, at, run.head) : 0;
-            if (I8) {
-                scale_row = good ? scale_element(p.cache, page, at, run.head) + (one_page ? lane_token : 0) : 0;
-            }
+        enter();
+        uint64_t row = 0, scale_row = 0;    // elements of the lane's row in the tile at hand
+        uint32_t live = 0;                  // its tokens that count
+        const uint32_t copy_row = lane / (S::ROW / 16), copy_piece = lane % (S::ROW / 16);   // of the first piece that the lane copies
+        const uint64_t token_bytes = p.cache.token_stride * S::SIZE;
+        const uint32_t ring_at = smem_at(ring), lane_at = copy_row * S::PITCH + copy_piece * 16;
+        uint32_t coming[S::SLOTS / 2];      // `live` of the steps that have been asked for and not been used
+        auto issue = [&](auto kind, uint32_t slot) {    // asks for K (and V) of the next step
+            constexpr bool values = decltype(kind)::value;
+            if constexpr (!values) {
+                // (a run that has come to its end has no tokens inside)
+                const uint32_t page = __shfl_sync(0xFFFFFFFFu, pages, page_index - run.first_page), t = run.token + lane_token;
+                const bool inside = t >= run.begin && t < run.end, good = page < p.cache.pages;
+                live = __ballot_sync(0xFFFFFFFFu, inside && good) & S::ALL;
+                if (live != S::ALL && inside && !good) {
+                    atomicExch(p.status, BAD_ATTENTION);
+                }
+                row = good ? row_element(p.cache, page, at, run.head) : 0;
+                if (I8) {
+                    scale_row = good ? scale_element(p.cache, page, at, run.head) + (one_page ? lane_token : 0) : 0;
+                }
 #pragma unroll
-            for (int k = 0; k + 1 < S::SLOTS / 2; ++k) {
-                coming[k] = coming[k + 1];
+                for (int k = 0; k + 1 < S::SLOTS / 2; ++k) {
+                    coming[k] = coming[k + 1];
+                }
+                coming[S::SLOTS / 2 - 1] = live;
+                run.token += tile_tokens;
+                page_index += p.step_pages;
+                at += p.step_at;
+                if (at >= page_size) {
+                    at -= page_size;
+                    ++page_index;
+                }
+                --run.left;
             }
-            coming[S::SLOTS / 2 - 1] = live;
-            run.token += tile_tokens;
-            page_index += p.step_pages;
-            at += p.step_at;
-            if (at >= page_size) {
-                at -= page_size;
-                ++page_index;
-            }
-            --run.left;
-        }
-        constexpr int ROWS = 32 / (S::ROW / 16);      // rows of one instruction
-        const char *base = reinterpret_cast<const char *>(values ? p.v : p.k);
-        const uint32_t dst = slot + lane_at;
-        if (plain && live == S::ALL) {
-            const char *src = base + row * S::SIZE + copy_row * token_bytes + copy_piece * 16;
+            constexpr int ROWS = 32 / (S::ROW / 16);      // rows of one instruction
+            const char *base = reinterpret_cast<const char *>(values ? p.v : p.k);
+            const uint32_t dst = slot + lane_at;
+            // (pages smaller than a step: every row's place comes from the lane that has looked it up)
+            if (live == S::ALL) {
+                if (one_page) {
+                    const char *src = base + row * S::SIZE + copy_row * token_bytes + copy_piece * 16;
+                    if (copy_piece < pieces) {
 #pragma unroll
-            for (int i = 0; i < S::STEP / ROWS; ++i) {
-                copy16(dst + i * ROWS * S::PITCH, src);
-                src += ROWS * token_bytes;
-            }
-        } else if (live != 0) {
+                        for (int i = 0; i < S::STEP / ROWS; ++i) {
+                            copy16(dst + i * ROWS * S::PITCH, src);
+                            src += ROWS * token_bytes;
+                        }
+                    }
+                } else {
+                    const uint64_t from = row * S::SIZE;
+#pragma unroll
+                    for (int i = 0; i < S::STEP / ROWS; ++i) {
+                        const char *src = base + __shfl_sync(0xFFFFFFFFu, from, copy_row + i * ROWS) + copy_piece * 16;
+                        if (copy_piece < pieces) {
+                            copy16(dst + i * ROWS * S::PITCH, src);
+                        }
+                    }
+                }
+            } else if (live != 0) {
 #pragma unroll 4
-            for (int i = 0; i < S::STEP / ROWS; ++i) {
-                const uint32_t r = copy_row + i * ROWS;
-                const uint64_t from = one_page ? row + r * p.cache.token_stride : __shfl_sync(0xFFFFFFFFu, row, r);
-                if (copy_piece < pieces) {
-                    const bool on = live >> r & 1;
-                    copy16(dst + i * ROWS * S::PITCH, on ? base + from * S::SIZE + copy_piece * 16 : base, on ? 16 : 0);
+                for (int i = 0; i < S::STEP / ROWS; ++i) {
+                    const uint32_t r = copy_row + i * ROWS;
+                    const uint64_t from = one_page ? row + r * p.cache.token_stride : __shfl_sync(0xFFFFFFFFu, row, r);
+                    if (copy_piece < pieces) {
+                        const bool on = live >> r & 1;
+                        copy16(dst + i * ROWS * S::PITCH, on ? base + from * S::SIZE + copy_piece * 16 : base, on ? 16 : 0);
+                    }
                 }
             }
-        }
-        if constexpr (I8) {
-            const bool on = live >> (lane % S::STEP) & 1;
-            if (S::STEP == 32 || lane < S::STEP) {
-                const float *scales = values ? p.v_scale : p.k_scale;
-                copy4(slot + S::STEP * S::PITCH + lane * 4, on ? scales + scale_row : scales, on ? 4 : 0);
+            if constexpr (I8) {
+                const bool on = live >> (lane % S::STEP) & 1;
+                if (S::STEP == 32 || lane < S::STEP) {
+                    const float *scales = values ? p.v_scale : p.k_scale;
+                    copy4(slot + S::STEP * S::PITCH + lane * 4, on ? scales + scale_row : scales, on ? 4 : 0);
+                }
             }
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        if (!values && run.left == 0) {
-            if (ahead.run.left != 0) {
-                enter();
-            } else {
-                run.end = 0;
-                run.left = 0xFFFFFFFFu;
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            if (!values && run.left == 0) {
+                if (ahead.run.left != 0) {
+                    enter();
+                } else {
+                    run.end = 0;
+                    run.left = 0xFFFFFFFFu;
+                }
             }
-        }
-    };
-    __syncwarp();
+        };
+        __syncwarp();
 
-    // ---- item by item (K, V, K, V ...) ----
-    // In turn n the warp uses item n and asks for item n + SLOTS - 1, into the slot of item n - 1.  The first turns only
-    // ask, so that the code, which a short call has to fetch before it can run, is there once.
-    constexpr int NT = S::STEP / 8, KS = DP / 16, TILES_D = DP / 8;
-    constexpr bool EVEN = S::SLOTS % 2 == 0;        // then a K turn asks for V, and a V turn for K
-    uint32_t item = ring_at + S::SLOT, count = 0, done = 0;    // tiles of the unit, and how many of them are through
-    uint32_t head0 = 0, heads_here = 0, mask = 0;
-    float fac[HB], m[HB], l[HB], keep[HB], w[HB][NT][2], acc[TILES_D][2 * HB], top_unit = 0.f;
-    const uint32_t q_at = smem_at(q_smem + (lane % 16) * S::Q_PITCH + lane / 16 * 16);
-    int n = 1 - S::SLOTS;
-    auto turn = [&](auto asks_for_values) {
-        if (n >= 0) {
-            // the item is there, and everybody is through with the one before it
-            asm volatile("cp.async.wait_group %0;" ::"n"(S::SLOTS - 2) : "memory");
-            __syncwarp();
-        }
-        issue(asks_for_values, item == ring_at ? ring_at + (S::SLOTS - 1) * S::SLOT : item - S::SLOT);
-        return n >= 0;
-    };
-    auto turned = [&]() {
-        ++n;
-        item = item == ring_at + (S::SLOTS - 1) * S::SLOT ? ring_at : item + S::SLOT;
-    };
+        // ---- item by item (K, V, K, V ...) ----
+        // In turn n the warp uses item n and asks for item n + SLOTS - 1, into the slot of item n - 1.  The first turns only
+        // ask, so that the code, which a short call has to fetch before it can run, is there once.
+        constexpr int NT = S::STEP / 8, KS = DP / 16, TILES_D = DP / 8;
+        constexpr bool EVEN = S::SLOTS % 2 == 0;        // then a K turn asks for V, and a V turn for K
+        uint32_t item = ring_at + S::SLOT, count = 0, done = 0;    // tiles of the unit, and how many of them are through
+        uint32_t head0 = 0, heads_here = 0, mask = 0;
+        float fac[HB], m[HB], l[HB], keep[HB], w[HB][NT][2], acc[TILES_D][2 * HB], top_unit = 0.f;
+        const uint32_t q_at = smem_at(q_smem + (lane % 16) * S::Q_PITCH + lane / 16 * 16);
+        int n = 1 - S::SLOTS;
+        auto turn = [&](auto asks_for_values) {
+            if (n >= 0) {
+                // the item is there, and everybody is through with the one before it
+                asm volatile("cp.async.wait_group %0;" ::"n"(S::SLOTS - 2) : "memory");
+                __syncwarp();
+            }
+            issue(asks_for_values, item == ring_at ? ring_at + (S::SLOTS - 1) * S::SLOT : item - S::SLOT);
+            return n >= 0;
+        };
+        auto turned = [&]() {
+            ++n;
+            item = item == ring_at + (S::SLOTS - 1) * S::SLOT ? ring_at : item + S::SLOT;
+        };
 #pragma unroll 1
-    for (;;) {
-     if (!EVEN || n != 1 - S::SLOTS) {
-      mask = coming[0];
-      if (n >= 0 && done == count) {
-        // ---- a unit begins ----
-        const uint32_t head = HB == 1 ? unit : unit / p.head_blocks, block = unit - head * (HB == 1 ? 1 : p.head_blocks);
-        heads_here = min((uint32_t)S::HEADS, p.group - block * S::HEADS);
-        head0 = head * p.group + block * S::HEADS;
-        count = min(tiles - tile, stop - place);
-        done = 0;
-        // Queries: brought to 2^13 .. 2^14 by a power of two (which the factor of the scores takes back), then two binary16
-        // numbers each, in the rows (hi of every head, lo of every head) of the matrix instruction's left operand.  Bytes come
-        // out of their words in the order 0, 2, 1, 3; the queries' elements stand in the same order.
-        const uint64_t q_row = sequence * p.q_stride + (uint64_t)head0 * dim;
+        for (;;) {
+            if (!EVEN || n != 1 - S::SLOTS) {
+                mask = coming[0];
+                if (n >= 0 && done == count) {
+                    // ---- a unit begins ----
+                    const uint32_t head = HB == 1 ? unit : unit / p.head_blocks, block = unit - head * (HB == 1 ? 1 : p.head_blocks);
+                    heads_here = min((uint32_t)S::HEADS, p.group - block * S::HEADS);
+                    head0 = head * p.group + block * S::HEADS;
+                    count = min(tiles - tile, stop - place);
+                    done = 0;
+                    // Queries: brought to 2^13 .. 2^14 by a power of two (which the factor of the scores takes back), then two binary16
+                    // numbers each, in the rows (hi of every head, lo of every head) of the matrix instruction's left operand.  Bytes come
+                    // out of their words in the order 0, 2, 1, 3; the queries' elements stand in the same order.
+                    const uint64_t q_row = sequence * p.q_stride + (uint64_t)head0 * dim;
 #pragma unroll 1
-        for (uint32_t h = member; h < S::HEADS; h += team) {
-            // (rows of heads that do not exist repeat the first: nobody reads their results)
-            const uint64_t from = q_row + (h < heads_here ? h : 0) * dim;
-            float x[DP / 32];
-            int top = 0;
+                    for (uint32_t h = member; h < S::HEADS; h += team) {
+                        // (rows of heads that do not exist repeat the first: nobody reads their results)
+                        const uint64_t from = q_row + (h < heads_here ? h : 0) * dim;
+                        float x[DP / 32];
+                        int top = 0;
 #pragma unroll
-            for (int i = 0; i < DP / 32; ++i) {
-                const uint32_t d = lane + 32 * i;
-                x[i] = 0.f;
-                if (d < dim) {
-                    x[i] = p.q_f16 ? load1(reinterpret_cast<const __half *>(p.q) + from + d) : load1(reinterpret_cast<const float *>(p.q) + from + d);
-                }
-                top = max(top, magnitude(x[i]));
-            }
-            const int e = max(__reduce_max_sync(0xFFFFFFFFu, top) >> 23, 20);
-            const float up = __int_as_float((127 + 13 + 127 - e) << 23);
-            if (lane == 0) {
-                factor[h] = __int_as_float((e - 13) << 23) * (p.scale * LOG2E);
-            }
-#pragma unroll
-            for (int i = 0; i < DP / 32; ++i) {
-                const uint32_t d = lane + 32 * i, r = d % 4;
-                const uint32_t k = I8 ? d / 16 * 16 + d % 16 / 4 * 2 + r / 2 + r % 2 * 8 : d;
-                const float v = x[i] * up;
-                const __half hi = __float2half_rn(v);
-                *reinterpret_cast<__half *>(q_smem + h * S::Q_PITCH + k * 2) = hi;
-                *reinterpret_cast<__half *>(q_smem + (S::HEADS + h) * S::Q_PITCH + k * 2) = __float2half_rn(v - __half2float(hi));
-            }
-        }
-        team_sync();
-#pragma unroll
-        for (int b = 0; b < HB; ++b) {
-            fac[b] = factor[g + 8 * b];
-        }
-        top_unit = 0.f;
-#pragma unroll
-        for (int b = 0; b < HB; ++b) {
-            m[b] = -INFINITY;
-            l[b] = 0.f;
-        }
-#pragma unroll
-        for (int n = 0; n < TILES_D; ++n) {
-#pragma unroll
-            for (int e = 0; e < 2 * HB; ++e) {
-                acc[n][e] = 0.f;
-            }
-        }
-      }
-      if (turn(std::bool_constant<EVEN>())) {
-            // scores: [heads] x [tokens]
-            float sc[NT][4];
-            {
-                uint32_t qa[4], q_lo[4];
-                auto multiply = [&](int s, int j, uint32_t b0, uint32_t b1) {
-                    if (s == 0) {
-                        mma_first(sc[j], qa, b0, b1);
-                    } else {
-                        mma(sc[j], qa, b0, b1);
-                    }
-                    if constexpr (HB == 2) {
-                        mma(sc[j], q_lo, b0, b1);
-                    }
-                };
-#pragma unroll
-                for (int s = 0; s < KS; ++s) {
-                    matrices(qa, q_at + s * 32);
-                    if constexpr (HB == 2) {
-                        matrices(q_lo, q_at + 16 * S::Q_PITCH + s * 32);
-                    }
-                    uint32_t r[4];
-                    if constexpr (!I8) {
-#pragma unroll
-                        for (int j = 0; j < NT; j += 2) {
-                            matrices(r, item + (lane % 8 + lane / 16 * 8) * S::PITCH + lane / 8 % 2 * 16 + 8 * j * S::PITCH + s * 32);
-                            multiply(s, j, r[0], r[1]);
-                            multiply(s, j + 1, r[2], r[3]);
+                        for (int i = 0; i < DP / 32; ++i) {
+                            const uint32_t d = lane + 32 * i;
+                            x[i] = 0.f;
+                            if (d < dim) {
+                                x[i] = p.q_f16 ? load1(reinterpret_cast<const __half *>(p.q) + from + d) : load1(reinterpret_cast<const float *>(p.q) + from + d);
+                            }
+                            top = max(top, magnitude(x[i]));
                         }
-                    } else if constexpr (S::STEP == 32) {
-                        matrices(r, item + lane * S::PITCH + s * 16);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            multiply(s, j, bytes_to_half2<0>(p, r[j]), bytes_to_half2<8>(p, r[j]));
+                        const int e = max(__reduce_max_sync(0xFFFFFFFFu, top) >> 23, 20);
+                        const float up = __int_as_float((127 + 13 + 127 - e) << 23);
+                        if (lane == 0) {
+                            factor[h] = __int_as_float((e - 13) << 23) * (p.scale * LOG2E);
                         }
-                    } else {
-                        matrices(r, item + lane % 16 * S::PITCH + s * 16);
-                        multiply(s, 0, bytes_to_half2<0>(p, r[0]), bytes_to_half2<8>(p, r[0]));
-                        multiply(s, 1, bytes_to_half2<0>(p, r[1]), bytes_to_half2<8>(p, r[1]));
+#pragma unroll
+                        for (int i = 0; i < DP / 32; ++i) {
+                            const uint32_t d = lane + 32 * i, r = d % 4;
+                            const uint32_t k = I8 ? d / 16 * 16 + d % 16 / 4 * 2 + r / 2 + r % 2 * 8 : d;
+                            const float v = x[i] * up;
+                            const __half hi = __float2half_rn(v);
+                            *reinterpret_cast<__half *>(q_smem + h * S::Q_PITCH + k * 2) = hi;
+                            *reinterpret_cast<__half *>(q_smem + (S::HEADS + h) * S::Q_PITCH + k * 2) = __float2half_rn(v - __half2float(hi));
+                        }
+                    }
+                    team_sync();
+#pragma unroll
+                    for (int b = 0; b < HB; ++b) {
+                        fac[b] = factor[g + 8 * b];
+                    }
+                    top_unit = 0.f;
+#pragma unroll
+                    for (int b = 0; b < HB; ++b) {
+                        m[b] = -INFINITY;
+                        l[b] = 0.f;
+                    }
+#pragma unroll
+                    for (int n = 0; n < TILES_D; ++n) {
+#pragma unroll
+                        for (int e = 0; e < 2 * HB; ++e) {
+                            acc[n][e] = 0.f;
+                        }
                     }
                 }
-            }
-            // weights: exp(s - m) times 2^14, which the division by their sum takes back
+                if (turn(std::bool_constant<EVEN>())) {
+                    // scores: [heads] x [tokens]
+                    float sc[NT][4];
+                    {
+                        uint32_t qa[4], q_lo[4];
+                        auto multiply = [&](int s, int j, uint32_t b0, uint32_t b1) {
+                            if (s == 0) {
+                                mma_first(sc[j], qa, b0, b1);
+                            } else {
+                                mma(sc[j], qa, b0, b1);
+                            }
+                            if constexpr (HB == 2) {
+                                mma(sc[j], q_lo, b0, b1);
+                            }
+                        };
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                float unit_k[2] = {1.f, 1.f};
-                if constexpr (I8) {
-                    const float2 u = shared_pair(item + S::STEP * S::PITCH + (8 * j + 2 * c4) * 4);
-                    unit_k[0] = reciprocal(u.x);
-                    unit_k[1] = reciprocal(u.y);
-                }
+                        for (int s = 0; s < KS; ++s) {
+                            matrices(qa, q_at + s * 32);
+                            if constexpr (HB == 2) {
+                                matrices(q_lo, q_at + 16 * S::Q_PITCH + s * 32);
+                            }
+                            uint32_t r[4];
+                            if constexpr (!I8) {
 #pragma unroll
-                for (int b = 0; b < HB; ++b) {
+                                for (int j = 0; j < NT; j += 2) {
+                                    matrices(r, item + (lane % 8 + lane / 16 * 8) * S::PITCH + lane / 8 % 2 * 16 + 8 * j * S::PITCH + s * 32);
+                                    multiply(s, j, r[0], r[1]);
+                                    multiply(s, j + 1, r[2], r[3]);
+                                }
+                            } else if constexpr (S::STEP == 32) {
+                                matrices(r, item + lane * S::PITCH + s * 16);
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        w[b][j][e] = (HB == 1 ? sc[j][e] + sc[j][e + 2] : sc[j][e + 2 * b]) * (fac[b] * unit_k[e]);
+                                for (int j = 0; j < 4; ++j) {
+                                    multiply(s, j, bytes_to_half2<0>(p, r[j]), bytes_to_half2<8>(p, r[j]));
+                                }
+                            } else {
+                                matrices(r, item + lane % 16 * S::PITCH + s * 16);
+                                multiply(s, 0, bytes_to_half2<0>(p, r[0]), bytes_to_half2<8>(p, r[0]));
+                                multiply(s, 1, bytes_to_half2<0>(p, r[1]), bytes_to_half2<8>(p, r[1]));
+                            }
+                        }
                     }
-                }
-            }
-            if (mask != S::ALL) {
+                    // weights: exp(s - m) times 2^14, which the division by their sum takes back
 #pragma unroll
-                for (int j = 0; j < NT; ++j) {
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const bool on = mask >> (8 * j + 2 * c4 + e) & 1;
+                    for (int j = 0; j < NT; ++j) {
+                        float unit_k[2] = {1.f, 1.f};
+                        if constexpr (I8) {
+                            const float2 u = shared_pair(item + S::STEP * S::PITCH + (8 * j + 2 * c4) * 4);
+                            unit_k[0] = reciprocal(u.x);
+                            unit_k[1] = reciprocal(u.y);
+                        }
 #pragma unroll
                         for (int b = 0; b < HB; ++b) {
-                            w[b][j][e] = on ? w[b][j][e] : -INFINITY;
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                w[b][j][e] = (HB == 1 ? sc[j][e] + sc[j][e + 2] : sc[j][e + 2 * b]) * (fac[b] * unit_k[e]);
+                            }
+                        }
+                    }
+                    if (mask != S::ALL) {
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) {
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const bool on = mask >> (8 * j + 2 * c4 + e) & 1;
+#pragma unroll
+                                for (int b = 0; b < HB; ++b) {
+                                    w[b][j][e] = on ? w[b][j][e] : -INFINITY;
+                                }
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int b = 0; b < HB; ++b) {
+                        float top = m[b];
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) {
+                            top = fmaxf(top, fmaxf(w[b][j][0], w[b][j][1]));
+                        }
+                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+                        const float base = top == -INFINITY ? 0.f : top;
+                        keep[b] = exp2_fast(m[b] - base);
+                        m[b] = top;
+                        l[b] *= keep[b];
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) {
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                w[b][j][e] = exp2_fast(w[b][j][e] - (base - 14.f));
+                                l[b] += w[b][j][e];
+                            }
                         }
                     }
                 }
+                turned();
             }
+            if (turn(std::bool_constant<!EVEN>())) {
+                if (mask != 0) {
+                    if constexpr (I8) {
+                        // Rows of bytes have units of their own.  They go into the weights, relative to the largest unit so far:
+                        // weights stay within binary16.
+                        float unit_v[NT][2], top = top_unit;
 #pragma unroll
-            for (int b = 0; b < HB; ++b) {
-                float top = m[b];
+                        for (int j = 0; j < NT; ++j) {
+                            const float2 u = shared_pair(item + S::STEP * S::PITCH + (8 * j + 2 * c4) * 4);
+                            unit_v[j][0] = reciprocal(u.x);
+                            unit_v[j][1] = reciprocal(u.y);
+                        }
+                        if (mask != S::ALL) {
 #pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    top = fmaxf(top, fmaxf(w[b][j][0], w[b][j][1]));
-                }
-                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-                const float base = top == -INFINITY ? 0.f : top;
-                keep[b] = exp2_fast(m[b] - base);
-                m[b] = top;
-                l[b] *= keep[b];
+                            for (int j = 0; j < NT; ++j) {
+                                unit_v[j][0] = mask >> (8 * j + 2 * c4) & 1 ? unit_v[j][0] : 0.f;
+                                unit_v[j][1] = mask >> (8 * j + 2 * c4 + 1) & 1 ? unit_v[j][1] : 0.f;
+                            }
+                        }
 #pragma unroll
-                for (int j = 0; j < NT; ++j) {
+                        for (int j = 0; j < NT; ++j) {
+                            top = fmaxf(top, fmaxf(unit_v[j][0], unit_v[j][1]));
+                        }
+                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+                        const float inv = top > 0.f ? reciprocal(top) : 0.f, change = top_unit * inv;
+                        top_unit = top;
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        w[b][j][e] = exp2_fast(w[b][j][e] - (base - 14.f));
-                        l[b] += w[b][j][e];
+                        for (int b = 0; b < HB; ++b) {
+                            keep[b] *= change;
+#pragma unroll
+                            for (int j = 0; j < NT; ++j) {
+                                w[b][j][0] *= unit_v[j][0] * inv;
+                                w[b][j][1] *= unit_v[j][1] * inv;
+                            }
+                        }
                     }
-                }
-            }
-      }
-      turned();
-     }
-     if (turn(std::bool_constant<!EVEN>())) {
-        if (mask != 0) {
-            if constexpr (I8) {
-                // Rows of bytes have units of their own.  They go into the weights, relative to the largest unit so far:
-                // weights stay within binary16.
-                float unit_v[NT][2], top = top_unit;
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    const float2 u = shared_pair(item + S::STEP * S::PITCH + (8 * j + 2 * c4) * 4);
-                    unit_v[j][0] = reciprocal(u.x);
-                    unit_v[j][1] = reciprocal(u.y);
-                }
-                if (mask != S::ALL) {
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        unit_v[j][0] = mask >> (8 * j + 2 * c4) & 1 ? unit_v[j][0] : 0.f;
-                        unit_v[j][1] = mask >> (8 * j + 2 * c4 + 1) & 1 ? unit_v[j][1] : 0.f;
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    top = fmaxf(top, fmaxf(unit_v[j][0], unit_v[j][1]));
-                }
-                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-                const float inv = top > 0.f ? reciprocal(top) : 0.f, change = top_unit * inv;
-                top_unit = top;
-#pragma unroll
-                for (int b = 0; b < HB; ++b) {
-                    keep[b] *= change;
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        w[b][j][0] *= unit_v[j][0] * inv;
-                        w[b][j][1] *= unit_v[j][1] * inv;
-                    }
-                }
-            }
-            uint32_t pa[HB][NT / 2][4];    // HB 1: rows hi, lo; HB 2: [0] hi, [1] lo
-#pragma unroll
-            for (int t = 0; t < NT / 2; ++t) {
-                if constexpr (HB == 1) {
-                    split_pair(w[0][2 * t][0], w[0][2 * t][1], pa[0][t][0], pa[0][t][1]);
-                    split_pair(w[0][2 * t + 1][0], w[0][2 * t + 1][1], pa[0][t][2], pa[0][t][3]);
-                } else {
-                    split_pair(w[0][2 * t][0], w[0][2 * t][1], pa[0][t][0], pa[HB - 1][t][0]);
-                    split_pair(w[HB - 1][2 * t][0], w[HB - 1][2 * t][1], pa[0][t][1], pa[HB - 1][t][1]);
-                    split_pair(w[0][2 * t + 1][0], w[0][2 * t + 1][1], pa[0][t][2], pa[HB - 1][t][2]);
-                    split_pair(w[HB - 1][2 * t + 1][0], w[HB - 1][2 * t + 1][1], pa[0][t][3], pa[HB - 1][t][3]);
-                }
-            }
-            // sums: the step's share is added to the running sum in binary32 (round to nearest: the matrix instruction's own
-            // accumulation truncates, which adds up over thousands of steps)
-            auto add = [&](int n, const float (&c)[4]) {
-                if constexpr (HB == 1) {
-                    acc[n][0] = fmaf(acc[n][0], keep[0], c[0] + c[2]);
-                    acc[n][1] = fmaf(acc[n][1], keep[0], c[1] + c[3]);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        acc[n][e % (2 * HB)] = fmaf(acc[n][e % (2 * HB)], keep[e / 2 % HB], c[e]);
-                    }
-                }
-            };
-            auto weigh = [&](float (&c)[4], int t, uint32_t b0, uint32_t b1) {
-                if (t == 0) {
-                    mma_first(c, pa[0][t], b0, b1);
-                } else {
-                    mma(c, pa[0][t], b0, b1);
-                }
-                if constexpr (HB == 2) {
-                    mma(c, pa[HB - 1][t], b0, b1);
-                }
-            };
-            if constexpr (!I8) {
-#pragma unroll
-                for (int n = 0; n < TILES_D; n += 2) {
-                    float c0[4], c1[4];
+                    uint32_t pa[HB][NT / 2][4];    // HB 1: rows hi, lo; HB 2: [0] hi, [1] lo
 #pragma unroll
                     for (int t = 0; t < NT / 2; ++t) {
-                        uint32_t r[4];
-                        matrices_t(r, item + lane % 16 * S::PITCH + lane / 16 * 16 + 16 * t * S::PITCH + n * 16);
-                        weigh(c0, t, r[0], r[1]);
-                        weigh(c1, t, r[2], r[3]);
+                        if constexpr (HB == 1) {
+                            split_pair(w[0][2 * t][0], w[0][2 * t][1], pa[0][t][0], pa[0][t][1]);
+                            split_pair(w[0][2 * t + 1][0], w[0][2 * t + 1][1], pa[0][t][2], pa[0][t][3]);
+                        } else {
+                            split_pair(w[0][2 * t][0], w[0][2 * t][1], pa[0][t][0], pa[HB - 1][t][0]);
+                            split_pair(w[HB - 1][2 * t][0], w[HB - 1][2 * t][1], pa[0][t][1], pa[HB - 1][t][1]);
+                            split_pair(w[0][2 * t + 1][0], w[0][2 * t + 1][1], pa[0][t][2], pa[HB - 1][t][2]);
+                            split_pair(w[HB - 1][2 * t + 1][0], w[HB - 1][2 * t + 1][1], pa[0][t][3], pa[HB - 1][t][3]);
+                        }
                     }
-                    add(n, c0);
-                    add(n + 1, c1);
-                }
-            } else {
+                    // sums: the step's share is added to the running sum in binary32 (round to nearest: the matrix instruction's own
+                    // accumulation truncates, which adds up over thousands of steps)
+                    auto add = [&](int n, const float (&c)[4]) {
+                        if constexpr (HB == 1) {
+                            acc[n][0] = fmaf(acc[n][0], keep[0], c[0] + c[2]);
+                            acc[n][1] = fmaf(acc[n][1], keep[0], c[1] + c[3]);
+                        } else {
 #pragma unroll
-                for (int n = 0; n < TILES_D; n += 4) {     // 32 bytes of a row: even and odd elements of two pieces
-                    float c[4][4];
+                            for (int e = 0; e < 4; ++e) {
+                                acc[n][e % (2 * HB)] = fmaf(acc[n][e % (2 * HB)], keep[e / 2 % HB], c[e]);
+                            }
+                        }
+                    };
+                    auto weigh = [&](float (&c)[4], int t, uint32_t b0, uint32_t b1) {
+                        if (t == 0) {
+                            mma_first(c, pa[0][t], b0, b1);
+                        } else {
+                            mma(c, pa[0][t], b0, b1);
+                        }
+                        if constexpr (HB == 2) {
+                            mma(c, pa[HB - 1][t], b0, b1);
+                        }
+                    };
+                    if constexpr (!I8) {
 #pragma unroll
-                    for (int t = 0; t < NT / 2; ++t) {
-                        uint32_t r[4];
-                        matrices_t(r, item + lane % 16 * S::PITCH + lane / 16 * 16 + 16 * t * S::PITCH + n * 8);
-                        weigh(c[0], t, bytes_to_half2<0>(p, r[0]), bytes_to_half2<0>(p, r[1]));
-                        weigh(c[1], t, bytes_to_half2<8>(p, r[0]), bytes_to_half2<8>(p, r[1]));
-                        weigh(c[2], t, bytes_to_half2<0>(p, r[2]), bytes_to_half2<0>(p, r[3]));
-                        weigh(c[3], t, bytes_to_half2<8>(p, r[2]), bytes_to_half2<8>(p, r[3]));
+                        for (int n = 0; n < TILES_D; n += 2) {
+                            float c0[4], c1[4];
+#pragma unroll
+                            for (int t = 0; t < NT / 2; ++t) {
+                                uint32_t r[4];
+                                matrices_t(r, item + lane % 16 * S::PITCH + lane / 16 * 16 + 16 * t * S::PITCH + n * 16);
+                                weigh(c0, t, r[0], r[1]);
+                                weigh(c1, t, r[2], r[3]);
+                            }
+                            add(n, c0);
+                            add(n + 1, c1);
+                        }
+                    } else {
+#pragma unroll
+                        for (int n = 0; n < TILES_D; n += 4) {     // 32 bytes of a row: even and odd elements of two pieces
+                            float c[4][4];
+#pragma unroll
+                            for (int t = 0; t < NT / 2; ++t) {
+                                uint32_t r[4];
+                                matrices_t(r, item + lane % 16 * S::PITCH + lane / 16 * 16 + 16 * t * S::PITCH + n * 8);
+                                weigh(c[0], t, bytes_to_half2<0>(p, r[0]), bytes_to_half2<0>(p, r[1]));
+                                weigh(c[1], t, bytes_to_half2<8>(p, r[0]), bytes_to_half2<8>(p, r[1]));
+                                weigh(c[2], t, bytes_to_half2<0>(p, r[2]), bytes_to_half2<0>(p, r[3]));
+                                weigh(c[3], t, bytes_to_half2<8>(p, r[2]), bytes_to_half2<8>(p, r[3]));
+                            }
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                add(n + k, c[k]);
+                            }
+                        }
                     }
+                }
+                if (++done == count) {
+                    // ---- the warps' shares, and out ----
+                    const bool whole = count == tiles;
+                    float *const share = p.parts + ((uint64_t)part * 2 + (tile != 0 ? 0 : 1)) * S::PART;
+                    float own[HB];
+                    const uint32_t warp0 = warp - member;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        add(n + k, c[k]);
+                    for (int b = 0; b < HB; ++b) {
+                        l[b] += __shfl_xor_sync(0xFFFFFFFFu, l[b], 1);
+                        l[b] += __shfl_xor_sync(0xFFFFFFFFu, l[b], 2);
+                        if (c4 == 0) {
+                            warp_m[warp * 16 + g + 8 * b] = m[b];
+                            warp_l[warp * 16 + g + 8 * b] = l[b];
+                        }
                     }
-                }
-            }
-        }
-        if (++done == count) {
-        // ---- the warps' shares, and out ----
-        const bool whole = count == tiles;
-        float *const share = p.parts + ((uint64_t)part * 2 + (tile != 0 ? 0 : 1)) * S::PART;
-        float own[HB];
-        const uint32_t warp0 = warp - member;
+                    team_sync();
 #pragma unroll
-        for (int b = 0; b < HB; ++b) {
-            l[b] += __shfl_xor_sync(0xFFFFFFFFu, l[b], 1);
-            l[b] += __shfl_xor_sync(0xFFFFFFFFu, l[b], 2);
-            if (c4 == 0) {
-                warp_m[warp * 16 + g + 8 * b] = m[b];
-                warp_l[warp * 16 + g + 8 * b] = l[b];
-            }
-        }
-        team_sync();
+                    for (int b = 0; b < HB; ++b) {
+                        // the four lanes of a head look at every fourth warp each
+                        const uint32_t h = g + 8 * b;
+                        float wm[WARPS / 4], top = -INFINITY, all = 0.f;
 #pragma unroll
-        for (int b = 0; b < HB; ++b) {
-            // the four lanes of a head look at every fourth warp each
-            const uint32_t h = g + 8 * b;
-            float wm[WARPS / 4], top = -INFINITY, all = 0.f;
+                        for (int k = 0; k < WARPS / 4; ++k) {
+                            const uint32_t w = 4 * k + c4;
+                            wm[k] = w < team ? warp_m[(warp0 + w) * 16 + h] : -INFINITY;
+                            top = fmaxf(top, wm[k]);
+                        }
+                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+                        const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
-            for (int k = 0; k < WARPS / 4; ++k) {
-                const uint32_t w = 4 * k + c4;
-                wm[k] = w < team ? warp_m[(warp0 + w) * 16 + h] : -INFINITY;
-                top = fmaxf(top, wm[k]);
-            }
-            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-            const float base = top == -INFINITY ? 0.f : top;
+                        for (int k = 0; k < WARPS / 4; ++k) {
+                            const uint32_t w = 4 * k + c4;
+                            all += w < team ? warp_l[(warp0 + w) * 16 + h] * exp2_fast(wm[k] - base) : 0.f;
+                        }
+                        all += __shfl_xor_sync(0xFFFFFFFFu, all, 1);
+                        all += __shfl_xor_sync(0xFFFFFFFFu, all, 2);
+                        own[b] = exp2_fast(m[b] - base) * (I8 ? top_unit : 1.f);
+                        if (whole) {
+                            own[b] *= all == 0.f ? 0.f : __frcp_rn(all);
+                        }
+                        if (member == 0 && c4 == 0) {
+                            if (!whole) {
+                                share[S::HEADS * DP + h] = top;
+                                share[S::HEADS * (DP + 1) + h] = all;
+                            } else if (p.lse != nullptr && h < heads_here) {
+                                p.lse[(uint64_t)sequence * p.heads + head0 + h] = (top + log2f(all) - 14.f) * LN2;
+                            }
+                        }
+                    }
+                    if (!whole && tile == 0 && member == 0 && lane == 0) {
+                        p.cuts[part] = Cut{min(parts.of(place + tiles - 1), parts.n - 1) - part + 1, sequence, head0, heads_here};
+                    }
+                    // GO numbers of every lane of every warp at a time; then each warp adds up some of them over its team.
+                    constexpr int NUMBERS = S::NUMBERS, GO = S::GO;
 #pragma unroll
-            for (int k = 0; k < WARPS / 4; ++k) {
-                const uint32_t w = 4 * k + c4;
-                all += w < team ? warp_l[(warp0 + w) * 16 + h] * exp2_fast(wm[k] - base) : 0.f;
-            }
-            all += __shfl_xor_sync(0xFFFFFFFFu, all, 1);
-            all += __shfl_xor_sync(0xFFFFFFFFu, all, 2);
-            own[b] = exp2_fast(m[b] - base) * (I8 ? top_unit : 1.f);
-            if (whole) {
-                own[b] *= all == 0.f ? 0.f : __frcp_rn(all);
-            }
-            if (member == 0 && c4 == 0) {
-                if (!whole) {
-                    share[S::HEADS * DP + h] = top;
-                    share[S::HEADS * (DP + 1) + h] = all;
-                } else if (p.lse != nullptr && h < heads_here) {
-                    p.lse[(uint64_t)sequence * p.heads + head0 + h] = (top + log2f(all) - 14.f) * LN2;
-                }
-            }
-        }
-        if (!whole && tile == 0 && member == 0 && lane == 0) {
-            p.cuts[part] = Cut{parts.of(place + tiles - 1) - part + 1, sequence, head0, heads_here};
-        }
-        // GO numbers of every lane of every warp at a time; then each warp adds up some of them over its team.
-        constexpr int NUMBERS = S::NUMBERS, GO = S::GO;
+                    for (int x0 = 0; x0 < NUMBERS; x0 += GO) {
+                        if (x0 != 0) {
+                            team_sync();
+                        }
 #pragma unroll
-        for (int x0 = 0; x0 < NUMBERS; x0 += GO) {
-            if (x0 != 0) {
-                team_sync();
-            }
-#pragma unroll
-            for (int x = 0; x < GO; ++x) {
-                merge[(warp * GO + x) * 32 + lane] = acc[(x0 + x) / (2 * HB)][(x0 + x) % (2 * HB)] * own[(x0 + x) % (2 * HB) / 2];
-            }
-            team_sync();
+                        for (int x = 0; x < GO; ++x) {
+                            merge[(warp * GO + x) * 32 + lane] = acc[(x0 + x) / (2 * HB)][(x0 + x) % (2 * HB)] * own[(x0 + x) % (2 * HB) / 2];
+                        }
+                        team_sync();
 #pragma unroll 1
-            for (uint32_t x = member; x < GO; x += team) {
-                float sum = 0.f;
+                        for (uint32_t x = member; x < GO; x += team) {
+                            float sum = 0.f;
 #pragma unroll 4
-                for (uint32_t w = 0; w < team; ++w) {
-                    sum += merge[((warp0 + w) * GO + x) * 32 + lane];
-                }
-                const uint32_t t = (x0 + x) / (2 * HB), e = (x0 + x) % (2 * HB), h = g + e / 2 * 8;
-                const uint32_t d = I8 ? t / 2 * 16 + 4 * c4 + e % 2 * 2 + t % 2 : 8 * t + 2 * c4 + e % 2;
-                if (!whole) {
-                    share[h * DP + d] = sum;
-                } else if (h < heads_here && d < dim) {
-                    store_out(p, sequence * p.out_stride + (uint64_t)(head0 + h) * dim + d, sum);
+                            for (uint32_t w = 0; w < team; ++w) {
+                                sum += merge[((warp0 + w) * GO + x) * 32 + lane];
+                            }
+                            const uint32_t t = (x0 + x) / (2 * HB), e = (x0 + x) % (2 * HB), h = g + e / 2 * 8;
+                            const uint32_t d = I8 ? t / 2 * 16 + 4 * c4 + e % 2 * 2 + t % 2 : 8 * t + 2 * c4 + e % 2;
+                            if (!whole) {
+                                share[h * DP + d] = sum;
+                            } else if (h < heads_here && d < dim) {
+                                store_out(p, sequence * p.out_stride + (uint64_t)(head0 + h) * dim + d, sum);
+                            }
+                        }
+                    }
+                    team_sync();
+                    // ---- the next unit ----
+                    place += count;
+                    tile = 0;
+                    if (place >= stop) {
+                        break;
+                    }
+                    if (++unit == units) {
+                        unit = 0;
+                        sequence = next_sequence(p, sequence);
+                        live_tokens(p, sequence, &begin, &end);
+                        tiles = max(tiles_of(begin, end, tile_shift), 1u);
+                    }
                 }
             }
+            turned();
         }
-        team_sync();
-        // ---- the next unit ----
-        place += count;
-        tile = 0;
-        if (place >= stop) {
-            break;
-        }
-        if (++unit == units) {
-            unit = 0;
-            sequence = next_sequence(p, sequence);
-            live_tokens(p, sequence, &begin, &end);
-            tiles = max(tiles_of(begin, end, tile_shift), 1u);
-        }
-        }
-      }
-     turned();
+        asm volatile("cp.async.wait_all;" ::: "memory");
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-  }
     // sequences without a token, a warp each, and lengths that are none
     for (uint32_t s = blockIdx.x * WARPS + warp; s < p.sequences; s += gridDim.x * WARPS) {
         uint32_t begin, end;

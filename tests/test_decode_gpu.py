@@ -524,3 +524,218 @@ def test_lora_gives_the_same_bits_again():
         a, b = (lora_case(*args, torch.uint8 if args[3] == 16 else torch.float32, seed=3, scale=False, unit="host") for _ in range(2))
         if args[3] == 32:                       # (bytes of x come from the generator's state)
             assert torch.equal(a[1], b[1])
+
+
+# ---- many sequences, streams, host memory, all of them together ------------------------------------------------------
+@pytest.mark.parametrize("i8", [0, 1])
+@pytest.mark.parametrize("sequences,longest", [(1024, 70), (1025, 70), (5000, 40), (65535, 3)])
+def test_attention_of_many_sequences(i8, sequences, longest):
+    """more than a warp counts for itself, up to the most that a call takes; every third has no tokens"""
+    page, kv, dim, heads = 8, 1, 32, 3
+    g = torch.Generator(device="cuda")
+    g.manual_seed(sequences)
+    length = torch.randint(0, longest + 1, (sequences,), device="cuda", generator=g, dtype=torch.int32)
+    length[::3] = 0
+    tp = -(-longest // page)
+    cache = Cache(1, 3000, page, kv, dim, i8)
+    table = torch.randint(0, 3000, (sequences, tp), device="cuda", generator=g, dtype=torch.int32)
+    table[torch.arange(tp, device="cuda")[None, :] * page >= length[:, None]] = -1
+    q = rand(5, sequences, heads, dim)
+    got, lse = attend(cache, q, table, length)
+    assert status() == 0
+    t = torch.arange(longest, device="cuda")
+    pages, at = table.clamp(min=0).long()[:, t // page], (t % page)[None, :].expand(sequences, -1)
+    k, v = (x[pages, 0, at].double() / (s[pages, 0, at].double()[..., None] if i8 else 1) for x, s in ((cache.k, cache.ks), (cache.v, cache.vs)))
+    live = t[None, :] < length[:, None]
+    s = torch.einsum("bhd,btd->bht", q.double(), k) * np.float32(dim ** -0.5).item()
+    off = ((dim + 16) * U * dim ** -0.5 * torch.einsum("bhd,btd->bht", q.double().abs(), k.abs()) * live[:, None, :]).amax(-1)
+    s = torch.where(live[:, None, :], s, -math.inf)
+    top = torch.logsumexp(s, -1)
+    p = torch.where(live[:, None, :], torch.exp(s - top[..., None]), 0.0)
+    want, tol = torch.einsum("bht,btd->bhd", p, v), 2 * (off[..., None] + (longest / 16 + 72) * U) * torch.einsum("bht,btd->bhd", p, v.abs()) + 1e-30
+    n_bad = int(((got.double() - want).abs() > tol).sum())
+    n_lse = int(((lse.double() - top).abs() > off + (longest / 16 + 72) * U + 2 * U * top.abs()).sum()) + int((lse.isinf() != (length == 0)[:, None]).sum())
+    assert (n_bad, n_lse) == (0, 0)
+
+
+def test_calls_on_two_streams_do_not_mix():
+    """eager calls of all three operators, each stream with tensors and workspaces of its own"""
+    def make(seed):
+        cache, q, table, length = batch(seed, [900, 33, 0, 2000], (16, 2, 128, seed % 2, "hnd", 0), 16)
+        qkv = rand(seed + 1, 4, (16 + 4) * 128)
+        pos = (length.clamp(min=1) - 1).int()
+        pos[2] = -1
+        cos, sin = rand(seed + 2, 2048, 64), rand(seed + 3, 2048, 64)
+        out, tmp = torch.empty_like(q), torch.empty(1 << 24, dtype=torch.uint8, device="cuda")
+        a, b, y = rand(seed + 4, 2, 16, 2048, dtype=torch.float16), rand(seed + 5, 2, 512, 16, dtype=torch.float16), torch.zeros(4, 512, device="cuda")
+        first, adapter = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, 1, 4], [1, 0]))
+        qo = torch.empty_like(q)
+        e = qkv.data_ptr()
+
+        def run():
+            B.kv_append(cache.desc(), B.KvAppend(4, 16, B.DT_F32, B.DT_F32, e, e + 4 * 2048, e + 4 * 2304, qo.data_ptr(), 2560, 2560, 2560, 2048, None,
+                                                 pos.data_ptr(), table.data_ptr(), 4, table.shape[1], 128, 0, 2048, cos.data_ptr(), sin.data_ptr()))
+            B.paged_attention(cache.desc(), B.PagedAttention(4, 16, B.DT_F32, B.DT_F32, qo.data_ptr(), out.data_ptr(), None, 2048, 2048, table.data_ptr(),
+                                                             length.data_ptr(), table.shape[1], 0, 0.09, 1.0), tmp.numel(), tmp.data_ptr())
+            B.lora(B.Lora(4, 512, 2048, 16, 2, 2, B.DT_F32, out.data_ptr(), y.data_ptr(), 2048, 512, a.data_ptr(), b.data_ptr(), 2048, None, first.data_ptr(),
+                          adapter.data_ptr(), 1.0, None, None), tmp.numel(), tmp.data_ptr())
+        return run, (out, y, cache, q, qkv, pos, cos, sin, tmp, a, b, first, adapter, qo, table, length)
+
+    works = [make(10), make(21)]
+    qo_rows = []
+    for run, keep in works:
+        keep[13].zero_()
+        run()
+        torch.cuda.synchronize()
+        qo_rows.append((keep[0].clone(), keep[1].clone()))
+    streams = [torch.cuda.Stream() for _ in works]
+    for _ in range(20):
+        for _, keep in works:
+            keep[1].zero_()
+        torch.cuda.synchronize()
+        for (run, _), st in zip(works, streams):
+            B.lib().bolt_b200_set_stream(C.c_void_p(st.cuda_stream))
+            run()
+            B.lib().bolt_b200_set_stream(None)
+        torch.cuda.synchronize()
+        same = [torch.equal(k[0], o) and torch.equal(k[1], y) for (_, k), (o, y) in zip(works, qo_rows)]
+        assert same == [True, True]
+    assert status() == 0
+
+
+def test_host_memory_is_refused():
+    cache, q, table, length = batch(3, [20], (16, 1, 64, 0, "hnd", 0), 2)
+    host = torch.zeros(1 << 16, dtype=torch.float32)
+    call = B.PagedAttention(1, 2, B.DT_F32, B.DT_F32, q.data_ptr(), host.data_ptr(), None, 128, 128, table.data_ptr(), length.data_ptr(), table.shape[1], 0, 0.1, 1.0)
+    tmp = torch.empty(1 << 23, dtype=torch.uint8, device="cuda")
+    lib = B.lib()
+    assert lib.bolt_b200_paged_attention(cache.desc(), call, tmp.numel(), tmp.data_ptr()) == B.NOT_MATCH
+    call.out = q.data_ptr()
+    assert lib.bolt_b200_paged_attention(cache.desc(), call, tmp.numel(), host.data_ptr()) == B.NOT_MATCH
+    d = cache.desc()
+    d.k = host.data_ptr()
+    assert lib.bolt_b200_paged_attention(d, call, tmp.numel(), tmp.data_ptr()) == B.NOT_MATCH
+    ap = B.KvAppend(1, 0, B.DT_F32, B.DT_F32, None, q.data_ptr(), q.data_ptr(), None, 0, 0, 0, 0, None, host.data_ptr(), table.data_ptr(), 1, 2, 0, 0, 0, None, None)
+    assert lib.bolt_b200_kv_append(cache.desc(), ap) == B.NOT_MATCH
+    lo = B.Lora(1, 64, 64, 8, 1, 1, B.DT_F32, q.data_ptr(), tmp.data_ptr(), 64, 64, host.data_ptr(), tmp.data_ptr(), 64, None, length.data_ptr(), length.data_ptr(),
+                1.0, None, None)
+    assert lib.bolt_b200_lora(lo, tmp.numel() // 2, tmp.data_ptr() + tmp.numel() // 2) == B.NOT_MATCH
+    assert status() == 0
+
+
+def packed(seed, k, n):
+    """a pre-packed u8 x s8 weight: (bytes [k, n], packed, offset of its offsets, scale per column)"""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    w = torch.randint(-127, 128, (k, n), dtype=torch.int8, device="cuda", generator=g)
+    desc = B.tensor2df(B.DT_I8, B.DF_NORMAL, k, n)
+    nbytes, rhs = B.matrix_matrix_multiply_transform_rhs_bytes(desc)
+    p = torch.zeros(nbytes, dtype=torch.uint8, device="cuda")
+    B.matrix_matrix_multiply_transform_rhs(desc, w.data_ptr(), p.data_ptr())
+    return w, p, rhs, 800.0 + 200 * torch.rand(n, device="cuda", generator=g)
+
+
+def project(x, row_scale, weight, y):
+    """y = x W of the quantized product, a scale for every row of x and column of W"""
+    w, p, rhs, col = weight
+    ep = B.GemmEpilogue()
+    ep.out_dt, ep.out_scale, ep.row_scale, ep.col_scale, ep.sA, ep.sB = B.DT_F32, 1.0, row_scale.data_ptr(), col.data_ptr(), 1.0, 1.0
+    m, k = x.shape
+    B.CHECK_STATUS(B.lib().bolt_b200_gemm_u8s8_ex(w.shape[1], m, k, x.data_ptr(), p.data_ptr(), p.data_ptr() + rhs, y.data_ptr(), C.byref(ep)), "gemm")
+
+
+@pytest.mark.parametrize("i8", [0, 1])
+@pytest.mark.parametrize("graph", [0, 1])
+def test_decoding_steps(i8, graph):
+    """Prompts, then one token at a time: quantized projection with adapters, append, attention in 8 bits, projection with
+    adapters.  Every stage against 64 bits from the stage before it; the steps also as one captured graph."""
+    seqs, heads, kv, dim, hidden, page, tp, rank = 3, 8, 2, 64, 256, 16, 8, 8
+    width = (heads + 2 * kv) * dim
+    w_in, w_out = packed(1, hidden, width), packed(2, heads * dim, hidden)
+    cache = Cache(3, seqs * tp, page, kv, dim, i8)
+    table = perm(4, seqs * tp).int().view(seqs, tp).contiguous()
+    ang = torch.arange(tp * page, device="cuda", dtype=torch.float64)[:, None] * 1000.0 ** (-torch.arange(dim // 2, device="cuda") / (dim // 2))[None, :]
+    cos, sin = ang.cos().float().contiguous(), ang.sin().float().contiguous()
+    adapters = [(rand(5, 2, rank, k, dtype=torch.float16, scale=k ** -0.5), rand(6, 2, n, rank, dtype=torch.float16, scale=rank ** -0.5))
+                for k, n in ((hidden, width), (heads * dim, hidden))]
+    out_scale = 60.0
+    prompt = [5, 40, 17]
+    x_all = torch.randint(0, 256, (seqs, 64, hidden), dtype=torch.uint8, device="cuda", generator=torch.Generator(device="cuda").manual_seed(9))
+    tmp = torch.empty(1 << 24, dtype=torch.uint8, device="cuda")
+
+    def layer(x, row_scale, first, adapter, seq, pos, length, bufs):
+        """x [m, hidden] of any number of sequences; attention (decoding) if length is given"""
+        m = x.shape[0]
+        qkv, q, ctx, ones, y = bufs
+        project(x, row_scale, w_in, qkv)
+        (a, b), n_seg = adapters[0], first.numel() - 1
+        B.lora(B.Lora(m, width, hidden, rank, 2, n_seg, B.DT_U8_Q, x.data_ptr(), qkv.data_ptr(), hidden, width, a.data_ptr(), b.data_ptr(), hidden, None,
+                      first.data_ptr(), adapter.data_ptr(), 1.0, None, row_scale.data_ptr()), tmp.numel(), tmp.data_ptr())
+        e = qkv.data_ptr()
+        B.kv_append(cache.desc(), B.KvAppend(m, heads, B.DT_F32, B.DT_F32, e, e + 4 * heads * dim, e + 4 * (heads + kv) * dim, q.data_ptr(), width, width, width,
+                                             heads * dim, ptr(seq), pos.data_ptr(), table.data_ptr(), seqs, tp, dim, 0, tp * page, cos.data_ptr(), sin.data_ptr()))
+        if length is None:
+            return
+        B.paged_attention(cache.desc(), B.PagedAttention(seqs, heads, B.DT_F32, B.DT_U8_Q, q.data_ptr(), ctx.data_ptr(), None, heads * dim, heads * dim,
+                                                         table.data_ptr(), length.data_ptr(), tp, 0, dim ** -0.5, out_scale), tmp.numel(), tmp.data_ptr())
+        project(ctx, ones, w_out, y)
+        a, b = adapters[1]
+        B.lora(B.Lora(m, hidden, heads * dim, rank, 2, n_seg, B.DT_U8_Q, ctx.data_ptr(), y.data_ptr(), heads * dim, hidden, a.data_ptr(), b.data_ptr(),
+                      heads * dim, None, first.data_ptr(), adapter.data_ptr(), out_scale, None, None), tmp.numel(), tmp.data_ptr())
+
+    def buffers(m):
+        return (torch.zeros(m, width, device="cuda"), torch.zeros(m, heads * dim, device="cuda"), torch.zeros(m, heads * dim, dtype=torch.uint8, device="cuda"),
+                torch.full((m,), out_scale, device="cuda"), torch.zeros(m, hidden, device="cuda"))
+
+    def exact_projection(x, row_scale, weight, ad, which):
+        xx = (x.double() - 128) / row_scale.double()[:, None]
+        y = xx @ (weight[0].double() / weight[3].double()[None, :])
+        for i, w in enumerate(which):
+            if w >= 0:
+                y[i] += (xx[i] @ ad[0][w].double().T) @ ad[1][w].double().T
+        return y
+
+    # the prompts, all at once
+    which = [1, -1, 0]
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    m = sum(prompt)
+    x = torch.cat([x_all[i, :n] for i, n in enumerate(prompt)]).contiguous()
+    rs = 40 + 10 * torch.rand(m, device="cuda")
+    first, adapter = i32(np.concatenate(([0], np.cumsum(prompt))).tolist()), i32(which)
+    seq, pos = i32([i for i, n in enumerate(prompt) for _ in range(n)]), i32([t for n in prompt for t in range(n)])
+    bufs = buffers(m)
+    layer(x, rs, first, adapter, seq, pos, None, bufs)
+    want = exact_projection(x, rs, w_in, adapters[0], [which[i] for i in seq.tolist()])
+    off = float((bufs[0].double() - want).abs().max() / want.abs().max())
+    assert off < 1e-5, off
+    # decoding
+    length, dpos = i32(prompt), i32([0] * seqs)
+    first1, rs1, x1, bufs1 = i32([0, 1, 2, 3]), torch.full((seqs,), 44.0, device="cuda"), torch.empty(seqs, hidden, dtype=torch.uint8, device="cuda"), buffers(seqs)
+    step = lambda: layer(x1, rs1, first1, adapter, None, dpos, length, bufs1)  # noqa: E731
+    if graph:
+        x1.fill_(128)
+        dpos.copy_(length)
+        step()          # (everything loaded and planned; the row is written again by the first step)
+        torch.cuda.synchronize()
+        g, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        with torch.cuda.graph(g, stream=stream):
+            B.lib().bolt_b200_set_stream(C.c_void_p(torch.cuda.current_stream().cuda_stream))
+            step()
+            B.lib().bolt_b200_set_stream(None)
+        step = g.replay
+    for t in range(12):
+        x1.copy_(x_all[:, 45 + t])
+        dpos.copy_(length)
+        length += 1
+        step()
+        torch.cuda.synchronize()
+        qkv, q, ctx, ones, y = bufs1
+        want = exact_projection(x1, rs1, w_in, adapters[0], which)
+        assert float((qkv.double() - want).abs().max() / want.abs().max()) < 1e-5
+        rotated = turned(qkv.cpu().numpy().reshape(seqs, heads + 2 * kv, dim), dpos.cpu().numpy(), cos.cpu().numpy(), sin.cpu().numpy(), dim, 0)
+        same = np.array_equal(q.cpu().numpy().reshape(seqs, heads, dim), rotated[:, :heads])
+        assert same
+        check_attention(cache, q.view(seqs, heads, dim), table, length, ctx.view(seqs, heads, dim), None, out_scale=out_scale)
+        want = exact_projection(ctx, ones, w_out, adapters[1], which)
+        assert float((y.double() - want).abs().max() / want.abs().max()) < 1e-5
+    assert status() == 0
