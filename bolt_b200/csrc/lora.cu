@@ -24,7 +24,7 @@ struct LoraParams {
     const int32_t *first_row, *adapter;
     float sA;
     const float *d_sA, *row_scale;
-    int u8, x_vectors, y_vectors;   // whether rows can be read 8 bytes / 4 numbers, written four numbers at a time
+    int u8, x_vectors, y_width;   // whether rows of x can be read 8 bytes / 4 numbers at a time; numbers of y: 4, 2 or 1
     uint32_t units, splits, outer_ctas;   // blocks of 16 rows at most, parts of K, CTAs of the second kernel
     float *t;   // [splits][rows][rank]
     int *status;
@@ -196,6 +196,13 @@ struct Eight<true> {
             const uint2 v = __ldg(reinterpret_cast<const uint2 *>(x));
             w[0] = v.x;
             w[1] = v.y;
+        } else if (on && k + 8 <= p.K) {
+            // the aligned words that hold a byte of the eight, shifted into place
+            const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(x) & 3);
+            const uint32_t *words = reinterpret_cast<const uint32_t *>(x - off);
+            const uint32_t a = __ldg(words), b = __ldg(words + 1), c = off != 0 ? __ldg(words + 2) : 0;
+            w[0] = __funnelshift_r(a, b, 8 * off);
+            w[1] = __funnelshift_r(b, c, 8 * off);
         } else if (on) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -396,7 +403,7 @@ __device__ __forceinline__ uint32_t place_of(uint32_t r, uint32_t rank)
 constexpr uint32_t STEP = 256;
 // KS: blocks of 16 of the rank, rounded up
 template <int KS>
-__global__ void __launch_bounds__(256, KS <= 1 ? 4 : (KS <= 2 ? 3 : 1)) lora_outer_kernel(const __grid_constant__ LoraParams p)
+__global__ void __launch_bounds__(256, KS <= 1 ? 4 : (KS <= 2 ? 3 : 2)) lora_outer_kernel(const __grid_constant__ LoraParams p)
 {
     constexpr int PITCH = KS * 16 + 8, TILES = 4;   // columns of a warp at a time: 4 x 8
     constexpr int AT_ONCE = KS <= 2 ? 8 : 4;        // parts of K whose inner sums are asked for at a time
@@ -441,7 +448,41 @@ __global__ void __launch_bounds__(256, KS <= 1 ? 4 : (KS <= 2 ? 3 : 1)) lora_out
         y1 += STEP;
         b += (uint64_t)STEP * p.rank;
     };
-    auto whole = [&]() { return p.y_vectors && n0 + 8 * TILES <= p.N; };    // nothing to look after
+    auto whole = [&]() { return n0 + 8 * TILES <= p.N; };    // no column to look after
+    // four neighbours of a row of y
+    auto load_y = [&](const float *y, float (&x)[4]) {
+        if (p.y_width == 4) {
+            const float4 a = __ldcs(reinterpret_cast<const float4 *>(y));
+            x[0] = a.x;
+            x[1] = a.y;
+            x[2] = a.z;
+            x[3] = a.w;
+        } else if (p.y_width == 2) {
+            const float2 a = __ldcs(reinterpret_cast<const float2 *>(y)), b = __ldcs(reinterpret_cast<const float2 *>(y) + 1);
+            x[0] = a.x;
+            x[1] = a.y;
+            x[2] = b.x;
+            x[3] = b.y;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[e] = __ldcs(y + e);
+            }
+        }
+    };
+    auto store_y = [&](float *y, const float (&x)[4]) {
+        if (p.y_width == 4) {
+            __stcs(reinterpret_cast<float4 *>(y), make_float4(x[0], x[1], x[2], x[3]));
+        } else if (p.y_width == 2) {
+            __stcs(reinterpret_cast<float2 *>(y), make_float2(x[0], x[1]));
+            __stcs(reinterpret_cast<float2 *>(y) + 1, make_float2(x[2], x[3]));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                __stcs(y + e, x[e]);
+            }
+        }
+    };
     auto fetch_row = [&](int t, const __half *row, bool on) {
         if (KS == 1 && on && p.rank == 16) {
             const uint2 x = __ldg(reinterpret_cast<const uint2 *>(row + 4 * c4));
@@ -492,14 +533,10 @@ __global__ void __launch_bounds__(256, KS <= 1 ? 4 : (KS <= 2 ? 3 : 1)) lora_out
             for (int r = 0; r < 2; ++r) {
 #pragma unroll
                 for (int t = 0; t < TILES / 2; ++t) {
-                    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                    v[r][t][0] = v[r][t][1] = v[r][t][2] = v[r][t][3] = 0.f;
                     if (r == 0 ? on0 : on1) {
-                        x = __ldcs(reinterpret_cast<const float4 *>(r == 0 ? y0 : y1) + 4 * t);
+                        load_y((r == 0 ? y0 : y1) + 16 * t, v[r][t]);
                     }
-                    v[r][t][0] = x.x;
-                    v[r][t][1] = x.y;
-                    v[r][t][2] = x.z;
-                    v[r][t][3] = x.w;
                 }
             }
         } else {
@@ -587,31 +624,45 @@ __global__ void __launch_bounds__(256, KS <= 1 ? 4 : (KS <= 2 ? 3 : 1)) lora_out
             }
         }
         __syncthreads();
-        uint32_t th[KS][4], tl[KS][4];
+        // t's fragments: in registers, or (larger ranks) read again for every step
+        constexpr bool KEPT = KS <= 2;
+        uint32_t th[KEPT ? KS : 1][4], tl[KEPT ? KS : 1][4];
+        auto fragments = [&](int s, uint32_t (&h)[4], uint32_t (&l)[4]) {
+            matrices(h, &hi[lane % 16][16 * s + lane / 16 * 8]);
+            matrices(l, &lo[lane % 16][16 * s + lane / 16 * 8]);
+        };
+        if constexpr (KEPT) {
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            matrices(th[s], &hi[lane % 16][16 * s + lane / 16 * 8]);
-            matrices(tl[s], &lo[lane % 16][16 * s + lane / 16 * 8]);
+            for (int s = 0; s < KS; ++s) {
+                fragments(s, th[s], tl[s]);
+            }
         }
         const float down0 = down[g], down1 = down[g + 8];
 #pragma unroll 1
         for (;;) {
+            float c[TILES][4];
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                if constexpr (!KEPT) {
+                    fragments(s, th[0], tl[0]);
+                }
+                const uint32_t(&h)[4] = th[KEPT ? s : 0], (&l)[4] = tl[KEPT ? s : 0];
+#pragma unroll
+                for (int t = 0; t < TILES; ++t) {
+                    if (s == 0) {
+                        mma_f16_first(c[t], l[0], l[1], l[2], l[3], w[t][s][0], w[t][s][1]);
+                    } else {
+                        mma_f16(c[t], l[0], l[1], l[2], l[3], w[t][s][0], w[t][s][1]);
+                    }
+                    mma_f16(c[t], h[0], h[1], h[2], h[3], w[t][s][0], w[t][s][1]);
+                }
+            }
 #pragma unroll
             for (int t = 0; t < TILES; ++t) {
-                float c[4];
-#pragma unroll
-                for (int s = 0; s < KS; ++s) {
-                    if (s == 0) {
-                        mma_f16_first(c, tl[s][0], tl[s][1], tl[s][2], tl[s][3], w[t][s][0], w[t][s][1]);
-                    } else {
-                        mma_f16(c, tl[s][0], tl[s][1], tl[s][2], tl[s][3], w[t][s][0], w[t][s][1]);
-                    }
-                    mma_f16(c, th[s][0], th[s][1], th[s][2], th[s][3], w[t][s][0], w[t][s][1]);
-                }
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    v[0][t / 2][t % 2 * 2 + e] = fmaf(c[e], down0, v[0][t / 2][t % 2 * 2 + e]);
-                    v[1][t / 2][t % 2 * 2 + e] = fmaf(c[2 + e], down1, v[1][t / 2][t % 2 * 2 + e]);
+                    v[0][t / 2][t % 2 * 2 + e] = fmaf(c[t][e], down0, v[0][t / 2][t % 2 * 2 + e]);
+                    v[1][t / 2][t % 2 * 2 + e] = fmaf(c[t][2 + e], down1, v[1][t / 2][t % 2 * 2 + e]);
                 }
             }
             const bool all = whole();
@@ -624,7 +675,7 @@ __global__ void __launch_bounds__(256, KS <= 1 ? 4 : (KS <= 2 ? 3 : 1)) lora_out
                     }
                     float *y = (r == 0 ? y0 : y1) + 16 * t;
                     if (all) {
-                        __stcs(reinterpret_cast<float4 *>(y), make_float4(v[r][t][0], v[r][t][1], v[r][t][2], v[r][t][3]));
+                        store_y(y, v[r][t]);
                     } else {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
@@ -659,7 +710,7 @@ void divide(LoraParams *p, const DeviceCtx *c)
     p->splits = want < 1 ? 1 : (want < at_most ? want : at_most);
     p->splits = p->splits < 16 ? p->splits : 16;
     // as many CTAs as run at a time, and no more than there are steps
-    const uint64_t steps = (uint64_t)p->units * ((p->N + STEP - 1) / STEP), ctas = (uint64_t)sms * (p->rank <= 16 ? 4 : (p->rank <= 32 ? 3 : 1));
+    const uint64_t steps = (uint64_t)p->units * ((p->N + STEP - 1) / STEP), ctas = (uint64_t)sms * (p->rank <= 16 ? 4 : (p->rank <= 32 ? 3 : 2));
     p->outer_ctas = (uint32_t)(steps < ctas ? steps : ctas);
 }
 EE check(const bolt_b200_lora_call *a, LoraParams *p, DeviceCtx **c)
@@ -708,7 +759,7 @@ EE check(const bolt_b200_lora_call *a, LoraParams *p, DeviceCtx **c)
     p->row_scale = a->row_scale;
     p->u8 = a->x_dt == DT_U8_Q;
     p->x_vectors = p->u8 ? aligned(a->x, 8) && a->x_stride % 8 == 0 : aligned(a->x, 16) && a->x_stride % 4 == 0;
-    p->y_vectors = aligned(a->y, 16) && a->y_stride % 4 == 0;
+    p->y_width = aligned(a->y, 16) && a->y_stride % 4 == 0 ? 4 : (aligned(a->y, 8) && a->y_stride % 2 == 0 ? 2 : 1);
     p->status = (*c)->d_status;
     divide(p, *c);
     if ((uint64_t)p->splits * p->rows * p->rank > 0x3FFFFFFFull || (uint64_t)p->units * ((p->N + STEP - 1) / STEP) > 0xFFFFFFFFull) {
