@@ -937,20 +937,14 @@ __global__ void __launch_bounds__(512) paged_attention_join_kernel(const __grid_
     const float *const shares = p.parts + (uint64_t)part * 2 * PART + PART;
     auto share = [&](uint32_t c) { return shares + (c == 0 ? 0 : c * 2 * PART - PART); };
     float top = -INFINITY, all = 0.f, sum[PER] = {};
-    for (uint32_t c = lane; c < cut.parts; c += 32) {
-        top = fmaxf(top, share(c)[HEADS * DP + h]);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-    }
-    const float base = top == -INFINITY ? 0.f : top;
+    // what stands relative to one maximum is brought to another
+    auto factor = [](float from, float to) { return exp2_fast(from - (to == -INFINITY ? 0.f : to)); };
     for (uint32_t c0 = half * AT_ONCE; c0 < cut.parts; c0 += 2 * AT_ONCE) {
-        float x[AT_ONCE][PER], w[AT_ONCE], l[AT_ONCE];
+        float x[AT_ONCE][PER], m[AT_ONCE], l[AT_ONCE], higher = top;
 #pragma unroll
         for (int i = 0; i < AT_ONCE; ++i) {
             const float *q = share(min(c0 + i, cut.parts - 1));
-            w[i] = load_now(q + HEADS * DP + h);
+            m[i] = load_now(q + HEADS * DP + h);
             l[i] = load_now(q + HEADS * (DP + 1) + h);
 #pragma unroll
             for (int k = 0; k < PER; k += 2) {
@@ -959,8 +953,19 @@ __global__ void __launch_bounds__(512) paged_attention_join_kernel(const __grid_
         }
 #pragma unroll
         for (int i = 0; i < AT_ONCE; ++i) {
+            higher = fmaxf(higher, m[i]);    // (the last share counts again: it does not change the maximum)
+        }
+        const float keep = factor(top, higher);
+        top = higher;
+        all *= keep;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            sum[k] *= keep;
+        }
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
             const bool on = c0 + i < cut.parts;
-            const float v = exp2_fast(w[i] - base);
+            const float v = factor(m[i], top);
             all = on ? fmaf(l[i], v, all) : all;
 #pragma unroll
             for (int k = 0; k < PER; ++k) {
@@ -975,20 +980,29 @@ __global__ void __launch_bounds__(512) paged_attention_join_kernel(const __grid_
         }
         if (lane == 0) {
             other[warp % 8][DP] = all;
+            other[warp % 8][DP + 1] = top;
         }
     }
     __syncthreads();
     if (half == 1 || h >= cut.heads) {
         return;
     }
-    all += other[warp][DP];
+    {
+        const float theirs = other[warp][DP + 1], higher = fmaxf(top, theirs), a = factor(top, higher), b = factor(theirs, higher);
+        top = higher;
+        all = fmaf(all, a, other[warp][DP] * b);
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            sum[k] = fmaf(sum[k], a, other[warp][lane * PER + k] * b);
+        }
+    }
     const uint32_t hq = cut.head0 + h;
     const float inv = all == 0.f ? 0.f : __frcp_rn(all);
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
         const uint32_t d = lane * PER + k;
         if (d < p.cache.dim) {
-            store_out(p, cut.sequence * p.out_stride + (uint64_t)hq * p.cache.dim + d, (sum[k] + other[warp][d]) * inv);
+            store_out(p, cut.sequence * p.out_stride + (uint64_t)hq * p.cache.dim + d, sum[k] * inv);
         }
     }
     if (p.lse != nullptr && lane == 0) {
