@@ -9,6 +9,9 @@
 // Bytes of x become binary16 exactly.  Binary32 x enters as two tf32 numbers (22 bits; tf32 has binary32's range), t as two
 // binary16 numbers of rows brought to a common power of two.  The accumulation of the matrix instructions truncates, so
 // sums over K go on in binary32 registers every few instructions.
+//
+// 2048 rows, 8192 -> 28672, rank 16, six requests: 75 to 86 us, 5.4 to 6.3 TB/s of the 470 MB (the result, read and written); rank 64: 123 us.  16
+// rows with an adapter each: 14 us, two kernels of dependent loads over 23 MB.
 #include "decode.cuh"
 
 namespace b200 {
@@ -259,7 +262,7 @@ struct Eight<false> {
 template <bool U8, int NT>
 __global__ void __launch_bounds__(256) lora_inner_kernel(const __grid_constant__ LoraParams p)
 {
-    constexpr int AT_ONCE = NT <= 2 ? 4 : (NT <= 4 ? 2 : 1);   // blocks of 32 of K whose loads a warp has in flight
+    constexpr int AT_ONCE = NT <= 2 ? 4 : (NT <= 4 ? 2 : 1);   // blocks of 32 of K whose loads a warp has in flight (divide() knows)
     __shared__ float merge[4][NT * 4 * 32];
     const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, c4 = lane % 4;
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -704,9 +707,12 @@ void divide(LoraParams *p, const DeviceCtx *c)
 {
     const uint32_t most = p->rows / 16 + p->segments, sms = (uint32_t)c->sm_count;
     p->units = most < p->rows ? most : p->rows;
-    // K in as many parts as give every SM four CTAs, each at least 256 long (a warp's 32), and sixteen at most, which the
-    // second kernel asks for in two goes
-    const uint32_t want = p->units == 0 ? 1 : 4 * sms / p->units, at_most = (p->K + 255) / 256;
+    // K in as many parts as give every SM four CTAs (2048 rows of 8192: 86.0 us, with two 86.6, with eight 87.5), each at least
+    // as long as what a CTA asks for at a time, and sixteen at most, which the second kernel asks for in two goes.
+    // 16 rows of 8192 with adapters of rank 16: 13.3 us in 8 parts of 1024, 14.3 in 16, 18.8 in 32, 13.5 in 4; one row of 28672: 8.1
+    // in 16 parts, 9.6 in 8; rank 128: 25.8 and 34.8.
+    const uint32_t at_a_time = p->rank <= 16 ? 1024 : (p->rank <= 32 ? 512 : 256);
+    const uint32_t want = p->units == 0 ? 1 : 4 * sms / p->units, at_most = (p->K - 1) / at_a_time + 1;
     p->splits = want < 1 ? 1 : (want < at_most ? want : at_most);
     p->splits = p->splits < 16 ? p->splits : 16;
     // as many CTAs as run at a time, and no more than there are steps

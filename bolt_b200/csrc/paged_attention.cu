@@ -4,12 +4,18 @@
 // m: when it rises, what has been summed so far is scaled down.  Shares of a sequence are joined the same way.
 //
 // HBM bound: keys and values are read once, whatever the number of query heads, and everything else is small beside them.
-// One CTA per SM takes an equal part of all tokens of the batch (which the host does not know), cut where it may be; a
-// second kernel joins the units that were cut.  Inside a CTA every warp streams tokens of its own through a private
+// Every team of warps takes an equal part of all tokens of the batch (whose lengths the host does not know), cut where it
+// may be; a second kernel joins the units that were cut.  Inside a team every warp streams tokens of its own through a private
 // ring of asynchronous copies and keeps its own maximum, total and sums, so that warps meet only at the end of a unit.
 // The products run on mma.m16n8k16: eight query heads that share a key head are half a tile's rows, and the other half
 // holds what binary16 has cut off of them, so that one instruction per operand tile multiplies 22-bit queries (and
-// probabilities) with the cache's binary16; bytes become binary16 in registers, two instructions for two of them.
+// probabilities) with the cache's binary16; bytes become binary16 in registers, five instructions for four of them.
+//
+// Whole calls: binary16, 64 sequences of 8192 tokens, 8 key heads of 128: 6.1 TB/s; bytes: 5.2 TB/s, bound by about 1050
+// instructions for a step of 32 tokens (of which 290 make binary16 of bytes).  One sequence of 131072 tokens: 102 us, 5.3 TB/s.
+// One of 4000: 12 us, of which 8 are the chain length -> page -> keys -> values -> shares with the code that has to be fetched
+// on the way, 4 the join.  Rows of 256 elements and groups of more than eight query heads keep 64 running sums a lane
+// and run with eight warps: 2.5 TB/s in bytes with 16 heads, 5.7 TB/s in binary16 with rows of 256.
 #include <type_traits>
 
 #include "decode.cuh"
@@ -34,12 +40,12 @@ struct AttentionParams {
     uint32_t sequences, heads, group, head_blocks, table_pages, window;
     float scale, out_scale;
     int i8, q_f16, out_kind;   // 0 binary32, 1 binary16, 2 u8
-    uint32_t team, part_count, share_bytes;
+    uint32_t team, part_count, share_bytes;    // warps that share a unit; parts of the row; bytes of partial results
     uint32_t step_pages, step_at, run_tiles;   // tokens of a tile in pages and what is left; tiles of a run
-    uint32_t page_magic;            // 2^32 / page_size
-    uint32_t even_bytes, to_1152;   // 0x00FF00FF, 0x64806480   // warps that share a unit; parts of the row
-    float *parts;   // workspace: two partial results for every part,
-    struct Cut *cuts;   // and what is to be joined
+    uint32_t page_magic;                       // 2^32 / page_size
+    uint32_t even_bytes, to_1152;              // 0x00FF00FF, 0x64806480
+    float *parts;                              // workspace: two partial results for every part,
+    Cut *cuts;                                 // and what is to be joined
     int *status;
 };
 
@@ -73,12 +79,15 @@ __device__ __forceinline__ void store_out(const AttentionParams &p, uint64_t at,
         reinterpret_cast<uint8_t *>(p.out)[at] = (uint8_t)to_u8(x, p.out_scale);
     }
 }
+
 // ---- how the work is divided -----------------------------------------------------------------------------------
 // A unit is one sequence, key head and block of query heads; it has tiles of team x STEP tokens on a grid that starts at
 // token 0.  All units' tiles stand in one row, in which every team of warps takes an equal, contiguous part.
 constexpr int MAX_WARPS = 16;
 constexpr uint32_t MAX_SEQUENCES = 65535;
-constexpr uint32_t BY_WARP = 1024;    // up to so many sequences every warp counts for itself; beyond, the CTA's share the counting
+// Up to so many sequences every warp counts for itself, beyond, the CTA's warps share the counting and wait for one another
+// (64 sequences of some 150 tokens, 12 heads of 64: 23.4 us and, shared, 24.0; 512: 112.4 and 110.4).
+constexpr uint32_t BY_WARP = 256;
 struct Found {
     uint32_t sequence, first;
 };
@@ -269,7 +278,8 @@ struct Shape {
     static constexpr int SLOT = STEP * PITCH + (I8 ? STEP * 4 : 0);
     static constexpr int HEADS = 8 * HB;
     static constexpr int NUMBERS = DP / 8 * 2 * HB;                              // running sums of a lane
-    // Steps are chains of dependent instructions: sixteen warps (128 registers a lane) hide them where the running sums fit.
+    // Steps are chains of dependent instructions: sixteen warps (128 registers a lane) hide them where the running sums fit (64
+    // sequences of up to 8192 tokens in bytes: 141 us, with eight warps 165; in binary16 202 and 226).
     static constexpr int WARPS = NUMBERS <= 32 && HB == 1 ? 16 : 8;
     static constexpr int Q_PITCH = DP * 2 + 16, Q_BYTES = 2 * HEADS * Q_PITCH;   // queries of a team
     static constexpr int TEAMS = 4 * Q_BYTES <= 20480 ? 4 : (2 * Q_BYTES <= 20480 ? 2 : 1);
@@ -340,8 +350,6 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
     auto team_sync = [&]() {
         if (team == WARPS) {
             __syncthreads();
-        } else if (team == 1) {
-            __syncwarp();
         } else {
             asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / team), "r"(32 * team) : "memory");
         }
@@ -1010,8 +1018,9 @@ __global__ void __launch_bounds__(512) paged_attention_join_kernel(const __grid_
     }
 }
 
-// The team: as many warps as leave a part for every unit, so that few units mean few shares to join, and with many units no
-// more warps than need be wait for others at a unit's end.
+// The team: as many warps as leave a part for every unit, so that few units mean few shares to join (one sequence of 4000
+// tokens: 11.7 us, with teams of four 16.0), and with many units no more warps than need be wait for others at a unit's end (64
+// sequences of up to 8192 tokens in bytes: 141 us, with teams of sixteen 183).
 template <int DP, bool I8, int HB>
 EE plan(const DeviceCtx *c, AttentionParams *p, uint64_t units)
 {
