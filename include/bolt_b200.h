@@ -491,7 +491,7 @@ EE matmul_cuda_b200(const TensorDesc *matrixADesc, int transposeA, const void *m
  *   DT_I8:  signed bytes; row (page, token, head) stands for byte / scale[(page * kv_heads + head) * page_size + token],
  *           scale = 127 / absmax of the row as everywhere in this library.
  * A row has at most 256 elements; its size in bytes, the strides in bytes and k and v are multiples of 16 (else
- * NOT_SUPPORTED).  Rows must not overlap. */
+ * NOT_SUPPORTED).  Rows must not overlap.  At most 2^31 - 1 pages of as many tokens, 65535 heads, strides up to 2^36. */
 typedef struct {
     DataType dt;
     U32 pages, page_size, kv_heads, dim;
@@ -513,7 +513,8 @@ typedef struct {
  *   a' = a * cos - b * sin, b' = b * cos + a * sin, every product, difference and sum one binary32 operation.
  * DT_F16 results are rounded once.  A DT_I8 row is quantized as by quantize_cuda_b200 (F32 -> I8) with a dynamic
  * scale of its own: scale = 127 / absmax (1 for a row of zeros), byte = clamp(rne(x * scale), -127, 127).
- * A token that is refused on the device (see above) leaves cache and q_out as they were. */
+ * A token that is refused on the device (see above) leaves cache and q_out as they were.
+ * At most 65535 query heads, strides up to 2^30, 2^30 heads of all kinds and tokens together. */
 typedef struct {
     U32 tokens, heads; /* heads: of the queries */
     DataType dt;       /* of q, k and v: DT_F32 or DT_F16 */
@@ -537,7 +538,8 @@ EE bolt_b200_kv_append(const bolt_b200_kv_cache *cache, const bolt_b200_kv_appen
  * out_dt: DT_F32, DT_F16, or, for a projection that follows, DT_U8_Q as by quantize_cuda_b200 with the scale out_scale:
  * clamp(rne(x * out_scale + 128), 1, 255).
  * Statistics and sums are binary32; queries and probabilities enter the products with 22 bits at least.
- * At most 65535 sequences, and sequences * kv_heads * table_pages * page_size * ceil(heads / kv_heads / 16) below 2^36.
+ * At most 65535 sequences and query heads, strides up to 2^30, and below 2^32 groups of 16 tokens that the tables have room
+ * for, counted for every key head and (with more than 8) every 16 of its query heads.  q and out must not overlap.
  * tmp: the bytes asked for by _tmp_bytes, 16-byte aligned. */
 typedef struct {
     U32 sequences, heads;
@@ -566,7 +568,8 @@ EE bolt_b200_paged_attention(
  * lower rank are filled up with zeros).  a, b: binary16, 16-byte aligned, a_stride (elements from row to row of a,
  * >= K) a multiple of 8.  x: DT_F32, or DT_U8_Q = the product's own input, which stands for
  * (byte - 128) / (row_scale[m], or *d_sA, or sA).  x and y rows may start anywhere.  Sums are binary32 (22 bits at least
- * of x and of the inner sums enter the products).  x must not overlap y.  tmp: as for attention. */
+ * of x and of the inner sums enter the products).  x must not overlap y.  At most 2^22 rows, 2^23
+ * columns, 65535 segments, strides up to 2^30.  tmp: as for attention. */
 typedef struct {
     U32 rows, N, K, rank, adapters, segments;
     DataType x_dt; /* DT_F32 or DT_U8_Q */
