@@ -5,8 +5,8 @@
 // operation, so that the rows are the same bits wherever they are computed.  HBM bound: every row is read once and written
 // once, and the angles of a position are shared by the heads of a token.  16 or 32 lanes hold a row in registers, four
 // neighbouring elements each: its largest magnitude (signed bytes) is a few shuffles away, and nobody reads a row twice
-// except for the other halves of pairs, which come from L1.  4005 tokens of 64 + 16 heads of 128, binary32 into bytes: 60 us,
-// 4.6 TB/s of the 277 MB; one token of 32 + 16 heads 2.3 us in a graph (start and three dependent loads).
+// except for the other halves of pairs, which come from L1.  4005 tokens of 64 + 16 heads of 128, binary32 into bytes: 47 us,
+// 5.9 TB/s of the 277 MB; one token of 32 + 16 heads 2.5 us in a graph (start and three dependent loads).
 #include "decode.cuh"
 
 namespace b200 {
@@ -96,209 +96,246 @@ struct AppendParams {
 
 // ROWS neighbouring heads of a token, all queries, keys or values, by LANES lanes, VW neighbouring elements of a row at a
 // time, PER times.  They share the position, the page, the angles and all but the last step of every address: with one row
-// to a group of lanes 4005 tokens of 64 + 16 heads (277 MB) took 86 us, bound by the instructions.
+// to a group of lanes 4005 tokens of 64 + 16 heads (277 MB) take 99 us, bound by the instructions.
+//
+// With more than a row to a group of lanes the CTAs are as many as run at a time, and each goes from task to task: the next
+// one's position is asked for with this one's rows, and its rows go into L2 meanwhile (a task to a group and no more: 58.7 us, with
+// binary16 rows 72.5; now 47 and 51).
+constexpr int RESIDENT = 4;
 template <typename TIN, int VW, int LANES, int PER, int ROWS>
-__global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ AppendParams p)
+__global__ void __launch_bounds__(256, ROWS > 1 ? RESIDENT : 1) kv_append_kernel(const __grid_constant__ AppendParams p)
 {
     const uint32_t q_groups = (p.heads + ROWS - 1) / ROWS, kv_groups = (p.cache.kv_heads + ROWS - 1) / ROWS, groups = q_groups + 2 * kv_groups;
-    const uint32_t group = (uint32_t)(((uint64_t)blockIdx.x * 256 + threadIdx.x) / LANES), lane = threadIdx.x % LANES;
-    const uint32_t token = group / groups, of_token = group - token * groups, dim = p.cache.dim;
-    const bool there = token < p.tokens;
-    const int kind = of_token < q_groups ? 0 : (of_token < q_groups + kv_groups ? 1 : 2);   // queries, keys, values
-    const uint32_t h0 = (of_token - (kind == 0 ? 0 : (kind == 1 ? q_groups : q_groups + kv_groups))) * ROWS;
-    const uint32_t rows = there ? min((uint32_t)ROWS, (kind == 0 ? p.heads : p.cache.kv_heads) - h0) : 0;
-    // Everything that does not hang on the position is asked for with it: the rows, and (y) the other halves of their pairs.
-    const int32_t position = there ? p.position[token] : -1;
-    const int64_t sequence = !there ? -1 : (p.sequence != nullptr ? p.sequence[token] : (int64_t)token);
-    const uint32_t rotary = kind == 2 ? 0 : p.rotary, half = rotary / 2;
-    const bool halves = VW == 4 && !p.interleaved;
-    const TIN *const src = reinterpret_cast<const TIN *>(p.src[kind]) + token * p.stride[kind] + (uint64_t)h0 * dim;
-    float x[ROWS][PER][VW], y[ROWS][PER][VW];
+    const uint32_t lane = threadIdx.x % LANES, dim = p.cache.dim;
+    constexpr bool ON = ROWS > 1;
+    const uint32_t stride = ON ? gridDim.x * (256 / LANES) : 0, further = stride / groups, further_of = stride - further * groups;
+    // What a group of lanes works on: queries, keys or values (kind), so many heads from h0 on, of a token.
+    struct Task {
+        uint32_t token, of_token, h0, rows;
+        int kind;
+    };
+    auto task = [&](uint32_t token, uint32_t of_token) {
+        Task t = {token, of_token, 0, 0, of_token < q_groups ? 0 : (of_token < q_groups + kv_groups ? 1 : 2)};
+        t.h0 = (of_token - (t.kind == 0 ? 0 : (t.kind == 1 ? q_groups : q_groups + kv_groups))) * ROWS;
+        t.rows = token < p.tokens ? min((uint32_t)ROWS, (t.kind == 0 ? p.heads : p.cache.kv_heads) - t.h0) : 0;
+        return t;
+    };
+    auto source = [&](const Task &t) { return reinterpret_cast<const TIN *>(p.src[t.kind]) + t.token * p.stride[t.kind] + (uint64_t)t.h0 * dim; };
+    const uint32_t first = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    Task now = task(first / groups, first % groups);
+    int32_t position = now.rows != 0 ? p.position[now.token] : -1;
+    int64_t sequence = now.rows == 0 ? -1 : (p.sequence != nullptr ? p.sequence[now.token] : (int64_t)now.token);
+    do {
+        // Everything that does not hang on the position is asked for with it: the rows, and (y) the other halves of their pairs.
+        const int kind = now.kind;
+        const uint32_t token = now.token, h0 = now.h0, rows = now.rows;
+        const uint32_t rotary = kind == 2 ? 0 : p.rotary, half = rotary / 2;
+        const bool halves = VW == 4 && !p.interleaved;
+        const TIN *const src = source(now);
+        float x[ROWS][PER][VW], y[ROWS][PER][VW];
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        const uint32_t i = (lane + j * LANES) * VW;
-        const TIN *from = src + i, *other = src + (i < half ? i + half : i - half);
+        for (int j = 0; j < PER; ++j) {
+            const uint32_t i = (lane + j * LANES) * VW;
+            const TIN *from = src + i, *other = src + (i < half ? i + half : i - half);
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) {
+            for (int r = 0; r < ROWS; ++r) {
 #pragma unroll
-            for (int e = 0; e < VW; ++e) {
-                x[r][j][e] = y[r][j][e] = 0.f;
-            }
-            if (r < rows && i < dim) {
-                if constexpr (VW == 4) {
-                    load4(from, x[r][j]);
-                    if (halves && i < rotary) {
-                        load4(other, y[r][j]);
+                for (int e = 0; e < VW; ++e) {
+                    x[r][j][e] = y[r][j][e] = 0.f;
+                }
+                if (r < rows && i < dim) {
+                    if constexpr (VW == 4) {
+                        load4(from, x[r][j]);
+                        if (halves && i < rotary) {
+                            load4(other, y[r][j]);
+                        }
+                    } else {
+                        x[r][j][0] = load1(from);
                     }
-                } else {
-                    x[r][j][0] = load1(from);
+                }
+                from += dim;
+                other += dim;
+            }
+        }
+        // the next task: its position, and its rows on their way into L2
+        int32_t next_position = -1;
+        int64_t next_sequence = -1;
+        if constexpr (ON) {
+            const uint32_t of_token = now.of_token + further_of, over = of_token >= groups;
+            now = task(token + further + over, over ? of_token - groups : of_token);
+            if (now.rows != 0) {
+                next_position = p.position[now.token];
+                next_sequence = p.sequence != nullptr ? p.sequence[now.token] : (int64_t)now.token;
+                if (lane * 128 < now.rows * dim * sizeof(TIN)) {
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const char *>(source(now)) + lane * 128));
                 }
             }
-            from += dim;
-            other += dim;
         }
-    }
-    // the page, asked for with the angles
-    const bool turns = position >= 0 && (uint32_t)position < p.rotary_positions;
-    uint32_t page = 0, at = 0;
-    const bool live = position >= 0 && sequence >= 0 && sequence < (int64_t)p.sequences && (p.rotary == 0 || turns) &&
-        page_of(p.table, (uint64_t)sequence, p.table_pages, p.cache.pages, p.cache.page_size, (uint32_t)position, &page, &at);
-    const uint64_t angles = (uint64_t)(uint32_t)position * (p.rotary / 2);
-    const float *cos = p.cos + angles, *sin = p.sin + angles;
+        // the page, asked for with the angles
+        const bool turns = position >= 0 && (uint32_t)position < p.rotary_positions;
+        uint32_t page = 0, at = 0;
+        const bool live = position >= 0 && sequence >= 0 && sequence < (int64_t)p.sequences && (p.rotary == 0 || turns) &&
+            page_of(p.table, (uint64_t)sequence, p.table_pages, p.cache.pages, p.cache.page_size, (uint32_t)position, &page, &at);
+        const uint64_t angles = (uint64_t)(uint32_t)position * (p.rotary / 2);
+        const float *cos = p.cos + angles, *sin = p.sin + angles;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        const uint32_t i = (lane + j * LANES) * VW;
-        if (!turns || i >= rotary) {
-            continue;
-        }
-        if constexpr (VW == 4) {
-            if (p.interleaved) {
-                const float c[2] = {cos[i / 2], cos[i / 2 + 1]}, s[2] = {sin[i / 2], sin[i / 2 + 1]};
+        for (int j = 0; j < PER; ++j) {
+            const uint32_t i = (lane + j * LANES) * VW;
+            if (!turns || i >= rotary) {
+                continue;
+            }
+            if constexpr (VW == 4) {
+                if (p.interleaved) {
+                    const float c[2] = {cos[i / 2], cos[i / 2 + 1]}, s[2] = {sin[i / 2], sin[i / 2 + 1]};
 #pragma unroll
-                for (int r = 0; r < ROWS; ++r) {
+                    for (int r = 0; r < ROWS; ++r) {
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float a = x[r][j][2 * e], b = x[r][j][2 * e + 1];
-                        x[r][j][2 * e] = __fsub_rn(__fmul_rn(a, c[e]), __fmul_rn(b, s[e]));
-                        x[r][j][2 * e + 1] = __fadd_rn(__fmul_rn(b, c[e]), __fmul_rn(a, s[e]));
+                        for (int e = 0; e < 2; ++e) {
+                            const float a = x[r][j][2 * e], b = x[r][j][2 * e + 1];
+                            x[r][j][2 * e] = __fsub_rn(__fmul_rn(a, c[e]), __fmul_rn(b, s[e]));
+                            x[r][j][2 * e + 1] = __fadd_rn(__fmul_rn(b, c[e]), __fmul_rn(a, s[e]));
+                        }
+                    }
+                } else {
+                    float c[4], s[4];
+                    load4(cos + (i < half ? i : i - half), c);
+                    load4(sin + (i < half ? i : i - half), s);
+                    // a' = a c + b (-s), b' = b c + a s: a sum with the negative is the difference, bit for bit
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        s[e] = i < half ? -s[e] : s[e];
+                    }
+#pragma unroll
+                    for (int r = 0; r < ROWS; ++r) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            x[r][j][e] = __fadd_rn(__fmul_rn(x[r][j][e], c[e]), __fmul_rn(y[r][j][e], s[e]));
+                        }
                     }
                 }
             } else {
-                float c[4], s[4];
-                load4(cos + (i < half ? i : i - half), c);
-                load4(sin + (i < half ? i : i - half), s);
-                // a' = a c + b (-s), b' = b c + a s: a sum with the negative is the difference, bit for bit
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    s[e] = i < half ? -s[e] : s[e];
-                }
+                const bool first = p.interleaved ? (i & 1) == 0 : i < half;
+                const uint32_t k = p.interleaved ? i / 2 : (first ? i : i - half), o = p.interleaved ? i ^ 1 : (first ? i + half : k);
 #pragma unroll
                 for (int r = 0; r < ROWS; ++r) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        x[r][j][e] = __fadd_rn(__fmul_rn(x[r][j][e], c[e]), __fmul_rn(y[r][j][e], s[e]));
-                    }
-                }
-            }
-        } else {
-            const bool first = p.interleaved ? (i & 1) == 0 : i < half;
-            const uint32_t k = p.interleaved ? i / 2 : (first ? i : i - half), o = p.interleaved ? i ^ 1 : (first ? i + half : k);
-#pragma unroll
-            for (int r = 0; r < ROWS; ++r) {
-                if (r < rows) {
-                    const float own = __fmul_rn(x[r][j][0], cos[k]), other = __fmul_rn(load1(src + r * dim + o), sin[k]);
-                    x[r][j][0] = first ? __fsub_rn(own, other) : __fadd_rn(own, other);
-                }
-            }
-        }
-    }
-    if (position >= 0 && !live && lane == 0) {
-        atomicExch(p.status, BAD_APPEND);
-    }
-    __syncwarp();   // q_out may be q: every lane has read its rows
-    if (!live) {
-        return;     // (the same for all lanes of a group)
-    }
-    // the rows, `step` elements apart from `to` on
-    const uint64_t to = kind == 0 ? token * p.q_out_stride + (uint64_t)h0 * dim : row_element(p.cache, page, at, h0);
-    const uint64_t step = kind == 0 ? dim : p.cache.head_stride;
-    if (kind == 0 && !p.q_out_f16) {
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const uint32_t i = (lane + j * LANES) * VW;
-            float *d = reinterpret_cast<float *>(p.q_out) + to + i;
-#pragma unroll
-            for (int r = 0; r < ROWS; ++r, d += step) {
-                if (r < rows && i < dim) {
-                    if constexpr (VW == 4) {
-                        *reinterpret_cast<float4 *>(d) = make_float4(x[r][j][0], x[r][j][1], x[r][j][2], x[r][j][3]);
-                    } else {
-                        *d = x[r][j][0];
+                    if (r < rows) {
+                        const float own = __fmul_rn(x[r][j][0], cos[k]), other = __fmul_rn(load1(src + r * dim + o), sin[k]);
+                        x[r][j][0] = first ? __fsub_rn(own, other) : __fadd_rn(own, other);
                     }
                 }
             }
         }
-    } else if (kind == 0 || !p.i8) {
+        if (position >= 0 && !live && lane == 0) {
+            atomicExch(p.status, BAD_APPEND);
+        }
+        __syncwarp();   // q_out may be q: every lane has read its rows
+        if (live) {     // (the same for all lanes of a group)
+            // the rows, `step` elements apart from `to` on
+            const uint64_t to = kind == 0 ? token * p.q_out_stride + (uint64_t)h0 * dim : row_element(p.cache, page, at, h0);
+            const uint64_t step = kind == 0 ? dim : p.cache.head_stride;
+            if (kind == 0 && !p.q_out_f16) {
 #pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const uint32_t i = (lane + j * LANES) * VW;
-            __half *d = reinterpret_cast<__half *>(kind == 0 ? p.q_out : (kind == 1 ? p.k_cache : p.v_cache)) + to + i;
+                for (int j = 0; j < PER; ++j) {
+                    const uint32_t i = (lane + j * LANES) * VW;
+                    float *d = reinterpret_cast<float *>(p.q_out) + to + i;
 #pragma unroll
-            for (int r = 0; r < ROWS; ++r, d += step) {
-                if (r < rows && i < dim) {
-                    if constexpr (VW == 4) {
-                        *reinterpret_cast<uint2 *>(d) = make_uint2(half2_bits(x[r][j][0], x[r][j][1]), half2_bits(x[r][j][2], x[r][j][3]));
-                    } else {
-                        *d = __float2half_rn(x[r][j][0]);
+                    for (int r = 0; r < ROWS; ++r, d += step) {
+                        if (r < rows && i < dim) {
+                            if constexpr (VW == 4) {
+                                *reinterpret_cast<float4 *>(d) = make_float4(x[r][j][0], x[r][j][1], x[r][j][2], x[r][j][3]);
+                            } else {
+                                *d = x[r][j][0];
+                            }
+                        }
+                    }
+                }
+            } else if (kind == 0 || !p.i8) {
+#pragma unroll
+                for (int j = 0; j < PER; ++j) {
+                    const uint32_t i = (lane + j * LANES) * VW;
+                    __half *d = reinterpret_cast<__half *>(kind == 0 ? p.q_out : (kind == 1 ? p.k_cache : p.v_cache)) + to + i;
+#pragma unroll
+                    for (int r = 0; r < ROWS; ++r, d += step) {
+                        if (r < rows && i < dim) {
+                            if constexpr (VW == 4) {
+                                *reinterpret_cast<uint2 *>(d) = make_uint2(half2_bits(x[r][j][0], x[r][j][1]), half2_bits(x[r][j][2], x[r][j][3]));
+                            } else {
+                                *d = __float2half_rn(x[r][j][0]);
+                            }
+                        }
+                    }
+                }
+            } else {
+                const unsigned mask = LANES == 32 ? 0xFFFFFFFFu : 0xFFFFu << (threadIdx.x & 16);
+                uint8_t *d = reinterpret_cast<uint8_t *>(kind == 1 ? p.k_cache : p.v_cache) + to;
+                float *scales = (kind == 1 ? p.k_scale : p.v_scale) + scale_element(p.cache, page, at, h0);
+#pragma unroll
+                for (int r = 0; r < ROWS; ++r, d += step, scales += p.cache.page_size) {
+                    if (r >= rows) {
+                        break;
+                    }
+                    int top = 0;
+#pragma unroll
+                    for (int j = 0; j < PER; ++j) {
+#pragma unroll
+                        for (int e = 0; e < VW; ++e) {
+                            top = max(top, magnitude(x[r][j][e]));
+                        }
+                    }
+#pragma unroll
+                    for (int o = LANES / 2; o > 0; o >>= 1) {
+                        top = max(top, __shfl_xor_sync(mask, top, o, LANES));
+                    }
+                    const float scale = top == 0 ? 1.0f : __fdiv_rn(127.0f, __int_as_float(top));
+                    // rne, then the limits, as F32 -> I8 has it (the limits are whole numbers: their order does not matter; NaN: -127)
+                    auto byte = [scale](float v) { return (uint32_t)__float2int_rn(fminf(fmaxf(__fmul_rn(v, scale), -127.f), 127.f)) & 0xFFu; };
+#pragma unroll
+                    for (int j = 0; j < PER; ++j) {
+                        const uint32_t i = (lane + j * LANES) * VW;
+                        if (i < dim) {
+                            if constexpr (VW == 4) {
+                                *reinterpret_cast<uint32_t *>(d + i) =
+                                    byte(x[r][j][0]) | byte(x[r][j][1]) << 8 | byte(x[r][j][2]) << 16 | byte(x[r][j][3]) << 24;
+                            } else {
+                                d[i] = (uint8_t)byte(x[r][j][0]);
+                            }
+                        }
+                    }
+                    if (lane == 0) {
+                        *scales = scale;
                     }
                 }
             }
         }
-    } else {
-        const unsigned mask = LANES == 32 ? 0xFFFFFFFFu : 0xFFFFu << (threadIdx.x & 16);
-        uint8_t *d = reinterpret_cast<uint8_t *>(kind == 1 ? p.k_cache : p.v_cache) + to;
-        float *scales = (kind == 1 ? p.k_scale : p.v_scale) + scale_element(p.cache, page, at, h0);
-#pragma unroll
-        for (int r = 0; r < ROWS; ++r, d += step, scales += p.cache.page_size) {
-            if (r >= rows) {
-                break;
-            }
-            int top = 0;
-#pragma unroll
-            for (int j = 0; j < PER; ++j) {
-#pragma unroll
-                for (int e = 0; e < VW; ++e) {
-                    top = max(top, magnitude(x[r][j][e]));
-                }
-            }
-#pragma unroll
-            for (int o = LANES / 2; o > 0; o >>= 1) {
-                top = max(top, __shfl_xor_sync(mask, top, o, LANES));
-            }
-            const float scale = top == 0 ? 1.0f : __fdiv_rn(127.0f, __int_as_float(top));
-            // rne, then the limits, as F32 -> I8 has it (the limits are whole numbers: their order does not matter; NaN: -127)
-            auto byte = [scale](float v) { return (uint32_t)__float2int_rn(fminf(fmaxf(__fmul_rn(v, scale), -127.f), 127.f)) & 0xFFu; };
-#pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                const uint32_t i = (lane + j * LANES) * VW;
-                if (i < dim) {
-                    if constexpr (VW == 4) {
-                        *reinterpret_cast<uint32_t *>(d + i) =
-                            byte(x[r][j][0]) | byte(x[r][j][1]) << 8 | byte(x[r][j][2]) << 16 | byte(x[r][j][3]) << 24;
-                    } else {
-                        d[i] = (uint8_t)byte(x[r][j][0]);
-                    }
-                }
-            }
-            if (lane == 0) {
-                *scales = scale;
-            }
-        }
-    }
+        position = next_position;
+        sequence = next_sequence;
+    } while (ON && __any_sync(0xFFFFFFFFu, now.rows != 0));
 }
 
 template <typename TIN, int VW, int LANES, int PER, int ROWS>
-EE launch_rows(const AppendParams &p, cudaStream_t st)
+EE launch_rows(const AppendParams &p, int sms, cudaStream_t st)
 {
     const uint64_t groups = (uint64_t)p.tokens * ((p.heads + ROWS - 1) / ROWS + 2 * ((p.cache.kv_heads + ROWS - 1) / ROWS));
-    return launch_kernel(dim3((uint32_t)((groups * LANES + 255) / 256)), 256, 0, st, kv_append_kernel<TIN, VW, LANES, PER, ROWS>, p);
+    const uint64_t ctas = (groups * LANES + 255) / 256, most = ROWS > 1 ? (uint64_t)sms * RESIDENT : ctas;
+    return launch_kernel(dim3((uint32_t)(ctas < most ? ctas : most)), 256, 0, st, kv_append_kernel<TIN, VW, LANES, PER, ROWS>, p);
 }
 template <typename TIN>
 EE launch(const AppendParams &p, bool vectors, int sms, cudaStream_t st)
 {
     if (!vectors) {
-        return launch_rows<TIN, 1, 32, 8, 1>(p, st);
+        return launch_rows<TIN, 1, 32, 8, 1>(p, sms, st);
     }
-    // One row to a group of lanes as long as all of them run at once (64 tokens of 64 + 16 heads: 2.9 us in a graph, 4.1 with
-    // four rows), four beyond.
-    const bool few = (uint64_t)p.tokens * (p.heads + 2 * p.cache.kv_heads) <= (uint64_t)sms * 64;
+    // One row to a group of lanes as long as every SM has at most 1280 of them, half of what it holds (64 tokens of 64 + 16 heads:
+    // 3.5 us in a graph, 3.8 with four rows; 96 tokens: 4.7 and 3.9), two or four beyond.
+    const uint64_t lanes = (uint64_t)p.tokens * (p.heads + 2 * p.cache.kv_heads) * (p.cache.dim <= 64 ? 16 : 32);
+    const bool few = lanes <= (uint64_t)sms * 1280;
     if (p.cache.dim <= 64) {
-        return few ? launch_rows<TIN, 4, 16, 1, 1>(p, st) : launch_rows<TIN, 4, 16, 1, 4>(p, st);
+        return few ? launch_rows<TIN, 4, 16, 1, 1>(p, sms, st) : launch_rows<TIN, 4, 16, 1, 4>(p, sms, st);
     }
     if (p.cache.dim <= 128) {
-        return few ? launch_rows<TIN, 4, 32, 1, 1>(p, st) : launch_rows<TIN, 4, 32, 1, 4>(p, st);
+        return few ? launch_rows<TIN, 4, 32, 1, 1>(p, sms, st) : launch_rows<TIN, 4, 32, 1, 4>(p, sms, st);
     }
-    return few ? launch_rows<TIN, 4, 32, 2, 1>(p, st) : launch_rows<TIN, 4, 32, 2, 2>(p, st);
+    return few ? launch_rows<TIN, 4, 32, 2, 1>(p, sms, st) : launch_rows<TIN, 4, 32, 2, 2>(p, sms, st);
 }
 
 }  // namespace
