@@ -11,8 +11,8 @@
 // holds what binary16 has cut off of them, so that one instruction per operand tile multiplies 22-bit queries (and
 // probabilities) with the cache's binary16; bytes become binary16 in registers, five instructions for four of them.
 //
-// Whole calls: binary16, 64 sequences of 8192 tokens, 8 key heads of 128: 6.1 TB/s; bytes: 5.2 TB/s, bound by about 1050
-// instructions for a step of 32 tokens (of which 290 make binary16 of bytes).  One sequence of 131072 tokens: 102 us, 5.3 TB/s.
+// Whole calls: binary16, 64 sequences of 8192 tokens, 8 key heads of 128: 6.1 TB/s; bytes: 5.3 TB/s, bound by about 1050
+// instructions for a step of 32 tokens (of which 290 make binary16 of bytes).  One sequence of 131072 tokens: 95 to 101 us, 5.5 TB/s.
 // One of 4000: 12 us, of which 8 are the chain length -> page -> keys -> values -> shares with the code that has to be fetched
 // on the way, 4 the join.  Rows of 256 elements and groups of more than eight query heads keep 64 running sums a lane
 // and run with eight warps: 2.5 TB/s in bytes with 16 heads, 5.7 TB/s in binary16 with rows of 256.
@@ -279,18 +279,23 @@ struct Shape {
     static constexpr int HEADS = 8 * HB;
     static constexpr int NUMBERS = DP / 8 * 2 * HB;                              // running sums of a lane
     // Steps are chains of dependent instructions: sixteen warps (128 registers a lane) hide them where the running sums fit (64
-    // sequences of up to 8192 tokens in bytes: 141 us, with eight warps 165; in binary16 202 and 226).
+    // sequences of up to 8192 tokens in bytes: 141 us, with eight warps and six slots 165; in binary16 202 and 226).
     static constexpr int WARPS = NUMBERS <= 32 && HB == 1 ? 16 : 8;
     static constexpr int Q_PITCH = DP * 2 + 16, Q_BYTES = 2 * HEADS * Q_PITCH;   // queries of a team
     static constexpr int TEAMS = 4 * Q_BYTES <= 20480 ? 4 : (2 * Q_BYTES <= 20480 ? 2 : 1);
-    static constexpr int GO = 16, MERGE = WARPS * GO * 32 * 4;                   // numbers of a lane that the warps exchange at a time
+    // Numbers of a lane that the warps exchange at a time, in the slot that each is through with: as many as there are, or as fit.
+    static constexpr int GO = NUMBERS * 128 <= SLOT ? NUMBERS : (SLOT >= 4096 ? 32 : 16);
     static constexpr int SMALL = 1024 + WARPS * 320;
-    static constexpr int FIXED = TEAMS * Q_BYTES + MERGE + SMALL;
+    static constexpr int FIXED = TEAMS * Q_BYTES + SMALL;
     static constexpr int FIT = (232448 - FIXED) / (WARPS * SLOT);
-    static constexpr int SLOTS = FIT > 6 ? 6 : FIT;                              // ring of a warp: K, V, K, V ...
+    // Ring of a warp: K, V, K, V ...  Two slots, three for two blocks of heads (eight warps with twice the products):
+    // what shared memory does not take is L1, and more requests at a time do not help (64 sequences of up to 8192 tokens in
+    // binary16: 201 us with two, 215 with three; 16 heads to a key head: 276, 250, and 257 with six).
+    static constexpr int SLOTS = HB == 1 ? 2 : (FIT < 3 ? FIT : 3);
     static constexpr int SMEM = FIXED + WARPS * SLOTS * SLOT;
     static constexpr int PART = HEADS * (DP + 2);                                // floats of a partial result: sums, then maxima, then totals
     static_assert(SLOTS >= 2, "a ring needs two slots");
+    static_assert(GO * 128 <= SLOT && NUMBERS % GO == 0, "the numbers have room in a slot");
 };
 
 // What a warp loads next: a run of tiles of one unit whose pages are at most 32 neighbours of the table, one in each lane.
@@ -314,8 +319,7 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
     using S = Shape<DP, I8, HB>;
     constexpr int WARPS = S::WARPS;
     extern __shared__ __align__(16) char smem[];
-    float *const merge = reinterpret_cast<float *>(smem + S::TEAMS * S::Q_BYTES);
-    char *const small = smem + S::TEAMS * S::Q_BYTES + S::MERGE;
+    char *const small = smem + S::TEAMS * S::Q_BYTES;
     Counting *const counting = reinterpret_cast<Counting *>(small);             // 192 bytes
     float *const factors = reinterpret_cast<float *>(small + 512);              // [TEAMS][16]
     float *const warp_m = reinterpret_cast<float *>(small + 1024), *const warp_l = warp_m + WARPS * 16;     // [WARPS][16]
@@ -512,6 +516,7 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
         // In turn n the warp uses item n and asks for item n + SLOTS - 1, into the slot of item n - 1.  The first turns only
         // ask, so that the code, which a short call has to fetch before it can run, is there once.
         constexpr int NT = S::STEP / 8, KS = DP / 16, TILES_D = DP / 8;
+        constexpr uint32_t RING = S::SLOTS * S::SLOT / 4;   // floats
         constexpr bool EVEN = S::SLOTS % 2 == 0;        // then a K turn asks for V, and a V turn for K
         uint32_t item = ring_at + S::SLOT, count = 0, done = 0;    // tiles of the unit, and how many of them are through
         uint32_t head0 = 0, heads_here = 0, mask = 0;
@@ -852,7 +857,9 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
                     if (!whole && tile == 0 && member == 0 && lane == 0) {
                         p.cuts[part] = Cut{min(parts.of(place + tiles - 1), parts.n - 1) - part + 1, sequence, head0, heads_here};
                     }
-                    // GO numbers of every lane of every warp at a time; then each warp adds up some of them over its team.
+                    // GO numbers of every lane of every warp at a time, in the values' slot (no copy goes there before the next turn); then
+                    // each warp adds up some of them over its team, whose slots are at the same place of their rings.
+                    float *const merge = reinterpret_cast<float *>(ring + (item - ring_at)) + lane, *const merge0 = merge - member * RING;
                     constexpr int NUMBERS = S::NUMBERS, GO = S::GO;
 #pragma unroll
                     for (int x0 = 0; x0 < NUMBERS; x0 += GO) {
@@ -861,7 +868,7 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
                         }
 #pragma unroll
                         for (int x = 0; x < GO; ++x) {
-                            merge[(warp * GO + x) * 32 + lane] = acc[(x0 + x) / (2 * HB)][(x0 + x) % (2 * HB)] * own[(x0 + x) % (2 * HB) / 2];
+                            merge[x * 32] = acc[(x0 + x) / (2 * HB)][(x0 + x) % (2 * HB)] * own[(x0 + x) % (2 * HB) / 2];
                         }
                         team_sync();
 #pragma unroll 1
@@ -869,7 +876,7 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
                             float sum = 0.f;
 #pragma unroll 4
                             for (uint32_t w = 0; w < team; ++w) {
-                                sum += merge[((warp0 + w) * GO + x) * 32 + lane];
+                                sum += merge0[w * RING + x * 32];
                             }
                             const uint32_t t = (x0 + x) / (2 * HB), e = (x0 + x) % (2 * HB), h = g + e / 2 * 8;
                             const uint32_t d = I8 ? t / 2 * 16 + 4 * c4 + e % 2 * 2 + t % 2 : 8 * t + 2 * c4 + e % 2;
@@ -881,6 +888,11 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
                         }
                     }
                     team_sync();
+                    if (dim < DP) {
+                        for (uint32_t i = lane; i < S::SLOT / 16; i += 32) {
+                            reinterpret_cast<uint4 *>(ring + (item - ring_at))[i] = make_uint4(0, 0, 0, 0);
+                        }
+                    }
                     // ---- the next unit ----
                     place += count;
                     tile = 0;
