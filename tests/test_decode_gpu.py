@@ -102,7 +102,7 @@ def quantized(rows):
     return np.clip(np.rint(rows * s[..., None]), -127, 127).astype(np.int8), s
 
 
-def append_case(tokens, heads, kv, dim, i8, page, order, dt, rotary, interleaved, gap=0, offset=0, in_place=False, with_seq=True, pad=True, q_out=None):
+def append_case(tokens, heads, kv, dim, i8, page, order, dt, rotary, interleaved, gap=0, offset=0, in_place=False, with_seq=True, pad=True, q_out=None, pad_every=0):
     seqs, tp = 3, 6
     cap = tp * page
     tokens = min(tokens, seqs * cap)
@@ -115,6 +115,8 @@ def append_case(tokens, heads, kv, dim, i8, page, order, dt, rotary, interleaved
     seq, pos = (place // cap).int(), (place % cap).int()
     if pad and tokens > 2:
         pos[1] = -1
+    if pad_every:
+        pos[::pad_every] = -1
     width = (heads + 2 * kv) * dim + offset
     qkv = rand(11, tokens, width, dtype=dt)[:, offset:]
     qkv[0, heads * dim: (heads + 1) * dim] = 0                      # a row of zeros has scale 1
@@ -182,6 +184,15 @@ def test_append_off_the_grid(i8, interleaved):
     append_case(9, 4, 2, 128, i8, 5, "hnd", torch.float32, 64, interleaved, q_out=torch.float16)
     append_case(9, 4, 2, 128, i8, 5, "hnd", torch.float16, 64, interleaved, q_out=torch.float32)
     append_case(3, 4, 2, 128, i8, 5, "hnd", torch.float16, 64, interleaved, with_seq=False, pad=False)
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(12, 2, 64), (8, 2, 128), (5, 1, 256), (7, 3, 80), (0, 9, 192), (33, 5, 48)])
+@pytest.mark.parametrize("i8", [0, 1])
+@pytest.mark.parametrize("dt", [torch.float32, torch.float16])
+def test_append_of_prompts(heads, kv, dim, i8, dt):
+    """more rows than run at a time: every group of lanes goes through several tokens, some of them padding"""
+    for tokens, rotary, interleaved, in_place in ((3601, dim, 0, False), (5000, dim // 2, 1, True), (4999, 0, 0, False)):
+        append_case(tokens, heads, kv, dim, i8, 300, "hnd" if in_place else "nhd", dt, rotary, interleaved, in_place=in_place, pad_every=7)
 
 
 def test_append_refuses_on_the_device_what_leads_outside():
