@@ -512,6 +512,15 @@ def test_lora_segments(x_dt):
 
 
 @pytest.mark.parametrize("x_dt", [torch.float32, torch.uint8])
+@pytest.mark.parametrize("rank", [8, 16, 32, 56, 128])
+def test_lora_of_more_steps_than_run_at_a_time(rank, x_dt):
+    """CTAs that go on from unit to unit, in the middle of rows of B too; few rows to a request, and many"""
+    lora_case(1003, 4101, 1030, rank, [3, 100, 101, 400, 990], 3, x_dt, which=[2, 0, -1, 1], y_gap=3)
+    lora_case(200, 3001, 520, rank, list(range(0, 201, 2)), 9, x_dt)
+    assert status() == 0
+
+
+@pytest.mark.parametrize("x_dt", [torch.float32, torch.uint8])
 def test_lora_strides_and_units(x_dt):
     for x_off in (0, 1, 2, 3, 4):
         lora_case(37, 65, 120, 16, [0, 20, 37], 2, x_dt, x_off=x_off, x_gap=3, y_off=x_off % 3, y_gap=x_off, a_gap=8)
@@ -539,7 +548,7 @@ def test_lora_gives_the_same_bits_again():
 
 # ---- many sequences, streams, host memory, all of them together ------------------------------------------------------
 @pytest.mark.parametrize("i8", [0, 1])
-@pytest.mark.parametrize("sequences,longest", [(1024, 70), (1025, 70), (5000, 40), (65535, 3)])
+@pytest.mark.parametrize("sequences,longest", [(256, 70), (257, 70), (1024, 70), (1025, 70), (5000, 40), (65535, 3)])
 def test_attention_of_many_sequences(i8, sequences, longest):
     """more than a warp counts for itself, up to the most that a call takes; every third has no tokens"""
     page, kv, dim, heads = 8, 1, 32, 3
