@@ -1,17 +1,18 @@
 // lora.cu -- low-rank adapters of many requests beside a shared projection: y += s (x A^T) B^T for every segment of rows.
 //
 // HBM bound: with a few rows the adapters' own bytes, with many the result's (read and written once).  Two kernels: the
-// inner sums t = x A^T (rows x rank) into the workspace, K split over CTAs and warps, then y += t B^T.  Both work on blocks
-// of 16 rows of one segment, which one instruction of the tensor pipe takes at once; with one row to a request 15 of
-// the 16 stand idle, but the weights are streamed all the same.  Operands go from global memory straight into the
-// fragments: the order of K inside an instruction is free, so a lane loads 16 neighbouring bytes of a row of A or B.
+// inner sums t = x A^T (rows x rank) into the workspace, K split over CTAs and warps, then y += t B^T; where K is short, the
+// second alone makes its inner sums, too.  Both work on blocks of 16 rows of one segment, which one instruction of the tensor
+// pipe takes at once; with one row to a request 15 of the 16 stand idle, but the weights are streamed all the same.  Operands
+// go from global memory straight into the fragments: the order of K inside an instruction is free, so a lane loads 16
+// neighbouring bytes of a row of A or B.
 //
 // Bytes of x become binary16 exactly.  Binary32 x enters as two tf32 numbers (22 bits; tf32 has binary32's range), t as two
 // binary16 numbers of rows brought to a common power of two.  The accumulation of the matrix instructions truncates, so
 // sums over K go on in binary32 registers every few instructions.
 //
-// 2048 rows, 8192 -> 28672, rank 16, six requests: 75 to 86 us, 5.4 to 6.3 TB/s of the 470 MB (the result, read and written); rank 64: 123 us.  16
-// rows with an adapter each: 14 us, two kernels of dependent loads over 23 MB.
+// 2048 rows, 8192 -> 28672, rank 16, six requests: 75 to 86 us, 5.4 to 6.3 TB/s of the 470 MB of the result, read and written;
+// rank 64: 127 us.  16 rows with an adapter each: 13.4 us, two kernels of dependent loads over 23 MB.
 #include "decode.cuh"
 
 namespace b200 {
@@ -28,6 +29,7 @@ struct LoraParams {
     float sA;
     const float *d_sA, *row_scale;
     int u8, x_vectors, y_width;   // whether rows of x can be read 8 bytes / 4 numbers at a time; numbers of y: 4, 2 or 1
+    bool alone;                           // one kernel does it all
     uint32_t units, splits, outer_ctas;   // blocks of 16 rows at most, parts of K, CTAs of the second kernel
     float *t;   // [splits][rows][rank]
     int *status;
@@ -258,24 +260,14 @@ struct Eight<false> {
     __device__ __forceinline__ void convert() {}
 };
 
-// NT: blocks of eight of the rank, rounded up
+// By the 256 threads of a CTA: the sums over blocks from .. to - 1 of 32 of K for the rows of a unit, times their scales, in warp 0: sum
+// [n][0, 1] for row g and columns 8 n + 2 c4 and the next, [2, 3] for row g + 8.  NT: blocks of eight of the rank, rounded up.
 template <bool U8, int NT>
-__global__ void __launch_bounds__(256) lora_inner_kernel(const __grid_constant__ LoraParams p)
+__device__ __forceinline__ void inner_sums(const LoraParams &p, const Unit &u, uint32_t from, uint32_t to, float (*merge)[NT * 4 * 32], float (&sum)[NT][4])
 {
     constexpr int AT_ONCE = NT <= 2 ? 4 : (NT <= 4 ? 2 : 1);   // blocks of 32 of K whose loads a warp has in flight (divide() knows)
-    __shared__ float merge[4][NT * 4 * 32];
     const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, c4 = lane % 4;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // (what was in front of this kernel is over)
-    const Units units(p, blockIdx.x == 0 && blockIdx.y == 0);
-    if (blockIdx.x >= units.count()) {
-        return;
-    }
-    const Unit u = units.get(blockIdx.x);
-    const uint32_t blocks = (p.K + 31) / 32;
-    const uint32_t from = (uint32_t)((uint64_t)blocks * blockIdx.y / p.splits), to = (uint32_t)((uint64_t)blocks * (blockIdx.y + 1) / p.splits);
     const __half *a = p.a + (uint64_t)u.adapter * p.rank * p.a_stride + g * p.a_stride + 8 * c4;
-    float sum[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         sum[n][0] = sum[n][1] = sum[n][2] = sum[n][3] = 0.f;
@@ -366,22 +358,50 @@ __global__ void __launch_bounds__(256) lora_inner_kernel(const __grid_constant__
         }
         __syncthreads();
     }
-    if (warp != 0) {
+    if (warp == 0) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            if (g + 8 * r < u.rows) {
+                const uint32_t row = u.row + g + 8 * r;
+                float factor = p.scale != nullptr ? p.scale[u.adapter] : 1.f;
+                if (U8) {
+                    factor = __fdiv_rn(factor, p.row_scale != nullptr ? p.row_scale[row] : (p.d_sA != nullptr ? *p.d_sA : p.sA));
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    sum[n][2 * r] *= factor;
+                    sum[n][2 * r + 1] *= factor;
+                }
+            }
+        }
+    }
+}
+template <bool U8, int NT>
+__global__ void __launch_bounds__(256) lora_inner_kernel(const __grid_constant__ LoraParams p)
+{
+    __shared__ float merge[4][NT * 4 * 32];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // (what was in front of this kernel is over)
+    const Units units(p, blockIdx.x == 0 && blockIdx.y == 0);
+    if (blockIdx.x >= units.count()) {
         return;
     }
+    const Unit u = units.get(blockIdx.x);
+    const uint32_t blocks = (p.K + 31) / 32;
+    float sum[NT][4];
+    inner_sums<U8, NT>(p, u, (uint32_t)((uint64_t)blocks * blockIdx.y / p.splits), (uint32_t)((uint64_t)blocks * (blockIdx.y + 1) / p.splits), merge, sum);
+    if (threadIdx.x >= 32) {
+        return;
+    }
+    const uint32_t g = threadIdx.x / 4, c4 = threadIdx.x % 4;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-        const uint32_t row = u.row + g + 8 * r;
         if (g + 8 * r < u.rows) {
-            float factor = p.scale != nullptr ? p.scale[u.adapter] : 1.f;
-            if (U8) {
-                factor = __fdiv_rn(factor, p.row_scale != nullptr ? p.row_scale[row] : (p.d_sA != nullptr ? *p.d_sA : p.sA));
-            }
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 if (n * 8 < p.rank) {
-                    *reinterpret_cast<float2 *>(p.t + ((uint64_t)blockIdx.y * p.rows + row) * p.rank + n * 8 + 2 * c4) =
-                        make_float2(sum[n][2 * r] * factor, sum[n][2 * r + 1] * factor);
+                    *reinterpret_cast<float2 *>(p.t + ((uint64_t)blockIdx.y * p.rows + u.row + g + 8 * r) * p.rank + n * 8 + 2 * c4) =
+                        make_float2(sum[n][2 * r], sum[n][2 * r + 1]);
                 }
             }
         }
@@ -404,21 +424,27 @@ __device__ __forceinline__ uint32_t place_of(uint32_t r, uint32_t rank)
 }
 // Columns go in steps of 256 (32 to a warp); the steps of all units stand in one row, of which every CTA takes an equal part.
 constexpr uint32_t STEP = 256;
-// KS: blocks of 16 of the rank, rounded up
-template <int KS>
-__global__ void __launch_bounds__(256, KS <= 1 ? 4 : (KS <= 2 ? 3 : 2)) lora_outer_kernel(const __grid_constant__ LoraParams p)
+// KS: blocks of 16 of the rank, rounded up.  ALONE: there is no lora_inner_kernel in front, every CTA makes the inner sums of its
+// rows by itself (divide() says when); binary32 x takes all registers of one CTA for that.
+enum Alone { NOT_ALONE, ALONE_F32, ALONE_U8 };
+template <int KS, Alone ALONE>
+__global__ void __launch_bounds__(256, ALONE ? (ALONE == ALONE_U8 ? 2 : 1) : (KS <= 1 ? 4 : (KS <= 2 ? 3 : 2))) lora_outer_kernel(const __grid_constant__ LoraParams p)
 {
     constexpr int PITCH = KS * 16 + 8, TILES = 4;   // columns of a warp at a time: 4 x 8
     constexpr int AT_ONCE = KS <= 2 ? 8 : 4;        // parts of K whose inner sums are asked for at a time
     __shared__ __align__(16) __half hi[16][PITCH], lo[16][PITCH];
     __shared__ float down[16];
+    __shared__ float merge[ALONE ? 4 : 1][ALONE ? KS * 2 * 4 * 32 : 1], inner[ALONE ? 16 : 1][ALONE ? KS * 16 + 2 : 1];
     const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, c4 = lane % 4;
     for (uint32_t i = threadIdx.x; i < 16 * PITCH; i += 256) {
         (&hi[0][0])[i] = (&lo[0][0])[i] = __float2half_rn(0.f);
     }
-    // (nothing that the kernel in front of this one writes is read here: it writes the inner sums only, and has seen the end
-    // of what was in front of it)
-    const Units units(p, false);
+    if (ALONE) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+    }
+    // (nothing that lora_inner_kernel, in front of this one, writes is read here: it writes the inner sums only, and has seen
+    // the end of what was in front of it)
+    const Units units(p, ALONE && blockIdx.x == 0);
     const uint32_t steps = (p.N + STEP - 1) / STEP;
     const Parts parts(units.count() * steps, gridDim.x);
     const bool some = blockIdx.x < parts.n;
@@ -566,9 +592,22 @@ __global__ void __launch_bounds__(256, KS <= 1 ? 4 : (KS <= 2 ? 3 : 2)) lora_out
         fetch();    // on its way while the inner sums are still being made
     }
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (!ALONE) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+    }
 #pragma unroll 1
     while (at < stop) {
+        if constexpr (ALONE) {
+            float sum[KS * 2][4];
+            inner_sums<ALONE == ALONE_U8, KS * 2>(p, u, 0, (p.K + 31) / 32, merge, sum);
+            if (warp == 0) {
+#pragma unroll
+                for (int n = 0; n < KS * 2; ++n) {
+                    *reinterpret_cast<float2 *>(&inner[g][n * 8 + 2 * c4]) = make_float2(sum[n][0], sum[n][1]);
+                    *reinterpret_cast<float2 *>(&inner[g + 8][n * 8 + 2 * c4]) = make_float2(sum[n][2], sum[n][3]);
+                }
+            }
+        }
         __syncthreads();    // everybody is through with the unit before (and the zeros are there)
         {
             // sixteen threads to a row
@@ -579,7 +618,12 @@ __global__ void __launch_bounds__(256, KS <= 1 ? 4 : (KS <= 2 ? 3 : 2)) lora_out
             for (int i = 0; i < KS; ++i) {
                 x[i] = 0.f;
             }
-            if (row < u.rows) {
+            if (ALONE) {
+#pragma unroll
+                for (int i = 0; i < KS; ++i) {
+                    x[i] = l + 16 * i < p.rank ? inner[row][l + 16 * i] : 0.f;
+                }
+            } else if (row < u.rows) {
                 const float *t = p.t + (uint64_t)(u.row + row) * p.rank;
                 const uint64_t split = (uint64_t)p.rows * p.rank;
 #pragma unroll 1
@@ -715,8 +759,13 @@ void divide(LoraParams *p, const DeviceCtx *c)
     const uint32_t want = p->units == 0 ? 1 : 4 * sms / p->units, at_most = (p->K - 1) / at_a_time + 1;
     p->splits = want < 1 ? 1 : (want < at_most ? want : at_most);
     p->splits = p->splits < 16 ? p->splits : 16;
+    const uint64_t steps = (uint64_t)p->units * ((p->N + STEP - 1) / STEP), by_itself = (uint64_t)sms * (p->u8 ? 2 : 1);
+    // One kernel, in which every CTA makes its rows' inner sums, where they take no more than one go and few CTAs meet a second
+    // unit: 16 rows of 768 -> 768 6.3 us in place of 7.4 (binary32), 5.7 in place of 6.4 (bytes).  With four goes 16 rows of
+    // 4096 -> 4096 take 12.7 in place of 8.0, and 1024 rows of 768 -> 2304 with eight adapters 13.1 in place of 12.5.
+    p->alone = p->rank <= 32 && p->K <= at_a_time && steps <= 2 * by_itself;
     // as many CTAs as run at a time, and no more than there are steps
-    const uint64_t steps = (uint64_t)p->units * ((p->N + STEP - 1) / STEP), ctas = (uint64_t)sms * (p->rank <= 16 ? 4 : (p->rank <= 32 ? 3 : 2));
+    const uint64_t ctas = p->alone ? by_itself : (uint64_t)sms * (p->rank <= 16 ? 4 : (p->rank <= 32 ? 3 : 2));
     p->outer_ctas = (uint32_t)(steps < ctas ? steps : ctas);
 }
 EE check(const bolt_b200_lora_call *a, LoraParams *p, DeviceCtx **c)
@@ -800,16 +849,19 @@ EE launch_inner(const LoraParams &p, cudaStream_t st)
     }
     return p.rank <= 64 ? launch(lora_inner_kernel<U8, 8>, grid, p, st) : launch(lora_inner_kernel<U8, 16>, grid, p, st);
 }
+template <Alone ALONE>
 EE launch_outer(const LoraParams &p, cudaStream_t st)
 {
     const dim3 grid(p.outer_ctas);
     if (p.rank <= 16) {
-        return launch(lora_outer_kernel<1>, grid, p, st);
+        return launch(lora_outer_kernel<1, ALONE>, grid, p, st);
     }
-    if (p.rank <= 32) {
-        return launch(lora_outer_kernel<2>, grid, p, st);
+    if (ALONE || p.rank <= 32) {
+        return launch(lora_outer_kernel<2, ALONE>, grid, p, st);
     }
-    return p.rank <= 64 ? launch(lora_outer_kernel<4>, grid, p, st) : launch(lora_outer_kernel<8>, grid, p, st);
+    if constexpr (ALONE == NOT_ALONE) {
+        return p.rank <= 64 ? launch(lora_outer_kernel<4, ALONE>, grid, p, st) : launch(lora_outer_kernel<8, ALONE>, grid, p, st);
+    }
 }
 
 }  // namespace
@@ -856,8 +908,11 @@ EE bolt_b200_lora(const bolt_b200_lora_call *call, U32 tmpBytes, void *tmp)
     }
     p.t = reinterpret_cast<float *>(tmp);
     const cudaStream_t st = tls().stream;
+    if (p.alone) {
+        return p.u8 ? launch_outer<ALONE_U8>(p, st) : launch_outer<ALONE_F32>(p, st);
+    }
     B200_EE(p.u8 ? launch_inner<true>(p, st) : launch_inner<false>(p, st));
-    return launch_outer(p, st);
+    return launch_outer<NOT_ALONE>(p, st);
 }
 
 }  // extern "C"
