@@ -9,13 +9,15 @@
 // ring of asynchronous copies and keeps its own maximum, total and sums, so that warps meet only at the end of a unit.
 // The products run on mma.m16n8k16: eight query heads that share a key head are half a tile's rows, and the other half
 // holds what binary16 has cut off of them, so that one instruction per operand tile multiplies 22-bit queries (and
-// probabilities) with the cache's binary16; bytes become binary16 in registers, five instructions for four of them.
+// probabilities) with the cache's binary16; bytes become binary16 in registers, five instructions for four of them, unless
+// mma.m16n8k32 takes them as they are (keys).
 //
-// Whole calls: binary16, 64 sequences of 8192 tokens, 8 key heads of 128: 6.1 TB/s; bytes: 5.3 TB/s, bound by about 1050
-// instructions for a step of 32 tokens (of which 290 make binary16 of bytes).  One sequence of 131072 tokens: 95 to 101 us, 5.5 TB/s.
-// One of 4000: 12 us, of which 8 are the chain length -> page -> keys -> values -> shares with the code that has to be fetched
-// on the way, 4 the join.  Rows of 256 elements and groups of more than eight query heads keep 64 running sums a lane
-// and run with eight warps: 2.5 TB/s in bytes with 16 heads, 5.7 TB/s in binary16 with rows of 256.
+// Whole calls: binary16, 64 sequences of 8192 tokens, 8 key heads of 128: 6.1 TB/s; bytes: 5.3 TB/s, bound by about 940
+// instructions for a step of 32 tokens (of which 145 make binary16 of bytes) and, call after call, by the power that they take
+// (4.4 TB/s).  One sequence of 131072 tokens: 95 to 101 us, 5.4 TB/s.  One of 4000: 11.5 us, of which 8 are the chain length
+// -> page -> keys -> values -> shares with the code that has to be fetched on the way, 4 the join.  Rows of 256 elements and
+// groups of more than eight query heads keep 64 running sums a lane and run with eight warps: 2.6 TB/s in bytes with 16
+// heads, 5.7 TB/s in binary16 with rows of 256.
 #include <type_traits>
 
 #include "decode.cuh"
@@ -229,11 +231,31 @@ __device__ __forceinline__ void mma_first(float (&c)[4], const uint32_t (&a)[4],
         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f), "f"(0.f), "f"(0.f), "f"(0.f));
 }
+__device__ __forceinline__ void mma_s8(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ float2 shared_pair(uint32_t at)
 {
     float2 v;
     asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
     return v;
+}
+// two binary32 operations in one instruction: (x, y) = (x, y) * k + (a, b), and the sum of two pairs
+__device__ __forceinline__ void fma_pair(float &x, float &y, float k, float a, float b)
+{
+    asm("{\n\t.reg .b64 u, v, w;\n\tmov.b64 u, {%0, %1};\n\tmov.b64 v, {%2, %2};\n\tmov.b64 w, {%3, %4};\n\tfma.rn.f32x2 u, u, v, w;\n\tmov.b64 {%0, %1}, u;\n\t}"
+        : "+f"(x), "+f"(y)
+        : "f"(k), "f"(a), "f"(b));
+}
+__device__ __forceinline__ void fma_pair(float &x, float &y, float k, float a, float b, float c, float d)   // (a, b) + (c, d)
+{
+    asm("{\n\t.reg .b64 u, v, w, z;\n\tmov.b64 u, {%0, %1};\n\tmov.b64 v, {%2, %2};\n\tmov.b64 w, {%3, %4};\n\tmov.b64 z, {%5, %6};\n\t"
+        "add.rn.f32x2 w, w, z;\n\tfma.rn.f32x2 u, u, v, w;\n\tmov.b64 {%0, %1}, u;\n\t}"
+        : "+f"(x), "+f"(y)
+        : "f"(k), "f"(a), "f"(b), "f"(c), "f"(d));
 }
 __device__ __forceinline__ float exp2_fast(float x)
 {
@@ -281,7 +303,11 @@ struct Shape {
     // Steps are chains of dependent instructions: sixteen warps (128 registers a lane) hide them where the running sums fit (64
     // sequences of up to 8192 tokens in bytes: 141 us, with eight warps and six slots 165; in binary16 202 and 226).
     static constexpr int WARPS = NUMBERS <= 32 && HB == 1 ? 16 : 8;
-    static constexpr int Q_PITCH = DP * 2 + 16, Q_BYTES = 2 * HEADS * Q_PITCH;   // queries of a team
+    // With one block of heads queries meet bytes as whole numbers, four digits of base 256 each, and keys need no conversion (64
+    // sequences of up to 8192 tokens, 300 calls in a row: 146 us, as binary16 149; rows of 256 elements 161 and 167; two blocks
+    // would have 64 running numbers more: 261 and 242).
+    static constexpr bool DIGITS = I8 && HB == 1;
+    static constexpr int Q_PITCH = DP * (DIGITS ? 1 : 2) + 16, Q_ROWS = HEADS * (DIGITS ? 4 : 2), Q_BYTES = Q_ROWS * Q_PITCH;   // queries of a team
     static constexpr int TEAMS = 4 * Q_BYTES <= 20480 ? 4 : (2 * Q_BYTES <= 20480 ? 2 : 1);
     // Numbers of a lane that the warps exchange at a time, in the slot that each is through with: as many as there are, or as fit.
     static constexpr int GO = NUMBERS * 128 <= SLOT ? NUMBERS : (SLOT >= 4096 ? 32 : 16);
@@ -549,7 +575,8 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
                     done = 0;
                     // Queries: brought to 2^13 .. 2^14 by a power of two (which the factor of the scores takes back), then two binary16
                     // numbers each, in the rows (hi of every head, lo of every head) of the matrix instruction's left operand.  Bytes come
-                    // out of their words in the order 0, 2, 1, 3; the queries' elements stand in the same order.
+                    // out of their words in the order 0, 2, 1, 3; the queries' elements stand in the same order.  As digits: brought to
+                    // 2^29 .. 2^30 and rounded, then -128 .. 127 each, the highest first.
                     const uint64_t q_row = sequence * p.q_stride + (uint64_t)head0 * dim;
 #pragma unroll 1
                     for (uint32_t h = member; h < S::HEADS; h += team) {
@@ -566,19 +593,30 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
                             }
                             top = max(top, magnitude(x[i]));
                         }
-                        const int e = max(__reduce_max_sync(0xFFFFFFFFu, top) >> 23, 20);
-                        const float up = __int_as_float((127 + 13 + 127 - e) << 23);
+                        constexpr int BITS = S::DIGITS ? 29 : 13, LEAST = S::DIGITS ? 30 : 20;    // (the factor stays a normal number)
+                        const int highest = __reduce_max_sync(0xFFFFFFFFu, top) >> 23, e = max(highest, LEAST);
+                        const float up = __int_as_float((127 + BITS + 127 - e) << 23);
                         if (lane == 0) {
-                            factor[h] = __int_as_float((e - 13) << 23) * (p.scale * LOG2E);
+                            // (whole numbers know no infinity: what is none goes on in the factor)
+                            factor[h] = S::DIGITS && highest == 255 ? NAN : __int_as_float((e - BITS) << 23) * (p.scale * LOG2E);
                         }
 #pragma unroll
                         for (int i = 0; i < DP / 32; ++i) {
-                            const uint32_t d = lane + 32 * i, r = d % 4;
-                            const uint32_t k = I8 ? d / 16 * 16 + d % 16 / 4 * 2 + r / 2 + r % 2 * 8 : d;
+                            const uint32_t d = lane + 32 * i;
                             const float v = x[i] * up;
-                            const __half hi = __float2half_rn(v);
-                            *reinterpret_cast<__half *>(q_smem + h * S::Q_PITCH + k * 2) = hi;
-                            *reinterpret_cast<__half *>(q_smem + (S::HEADS + h) * S::Q_PITCH + k * 2) = __float2half_rn(v - __half2float(hi));
+                            if constexpr (S::DIGITS) {
+                                int rest = __float2int_rn(v);
+#pragma unroll
+                                for (int digit = 3; digit >= 0; --digit) {
+                                    q_smem[(digit * S::HEADS + h) * S::Q_PITCH + d] = (char)rest;
+                                    rest = (rest - (signed char)rest) >> 8;
+                                }
+                            } else {
+                                const uint32_t r = d % 4, k = I8 ? d / 16 * 16 + d % 16 / 4 * 2 + r / 2 + r % 2 * 8 : d;
+                                const __half hi = __float2half_rn(v);
+                                *reinterpret_cast<__half *>(q_smem + h * S::Q_PITCH + k * 2) = hi;
+                                *reinterpret_cast<__half *>(q_smem + (S::HEADS + h) * S::Q_PITCH + k * 2) = __float2half_rn(v - __half2float(hi));
+                            }
                         }
                     }
                     team_sync();
@@ -602,8 +640,35 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
                 }
                 if (turn(std::bool_constant<EVEN>())) {
                     // scores: [heads] x [tokens]
-                    float sc[NT][4];
-                    {
+                    float score[HB][NT][2];
+                    if constexpr (S::DIGITS) {
+                        // The digits' products are whole numbers, two neighbouring digits' together below 2^31.  A tile has the rows of two
+                        // digits of eight heads.
+#pragma unroll
+                        for (int j = 0; j < NT; j += 2) {
+                            int c[2][2][4] = {};
+#pragma unroll
+                            for (int s = 0; s < DP / 32; ++s) {
+                                uint32_t r[4], qa[4];
+                                matrices(r, item + (lane % 8 + lane / 16 * 8) * S::PITCH + lane / 8 % 2 * 16 + 8 * j * S::PITCH + s * 32);
+#pragma unroll
+                                for (int k = 0; k < 2; ++k) {
+                                    matrices(qa, q_at + 16 * k * S::Q_PITCH + s * 32);
+                                    mma_s8(c[k][0], qa, r[0], r[1]);
+                                    mma_s8(c[k][1], qa, r[2], r[3]);
+                                }
+                            }
+#pragma unroll
+                            for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    const int high = c[0][t][e] * 256 + c[0][t][e + 2], low = c[1][t][e] * 256 + c[1][t][e + 2];
+                                    score[0][j + t][e] = fmaf((float)high, 65536.f, (float)low);
+                                }
+                            }
+                        }
+                    } else {
+                        float sc[NT][4];
                         uint32_t qa[4], q_lo[4];
                         auto multiply = [&](int s, int j, uint32_t b0, uint32_t b1) {
                             if (s == 0) {
@@ -641,6 +706,16 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
                                 multiply(s, 1, bytes_to_half2<0>(p, r[1]), bytes_to_half2<8>(p, r[1]));
                             }
                         }
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) {
+#pragma unroll
+                            for (int b = 0; b < HB; ++b) {
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    score[b][j][e] = HB == 1 ? sc[j][e] + sc[j][e + 2] : sc[j][e + 2 * b];
+                                }
+                            }
+                        }
                     }
                     // weights: exp(s - m) times 2^14, which the division by their sum takes back
 #pragma unroll
@@ -655,7 +730,7 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
                         for (int b = 0; b < HB; ++b) {
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
-                                w[b][j][e] = (HB == 1 ? sc[j][e] + sc[j][e + 2] : sc[j][e + 2 * b]) * (fac[b] * unit_k[e]);
+                                w[b][j][e] = score[b][j][e] * (fac[b] * unit_k[e]);
                             }
                         }
                     }
@@ -751,13 +826,10 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
                     // accumulation truncates, which adds up over thousands of steps)
                     auto add = [&](int n, const float (&c)[4]) {
                         if constexpr (HB == 1) {
-                            acc[n][0] = fmaf(acc[n][0], keep[0], c[0] + c[2]);
-                            acc[n][1] = fmaf(acc[n][1], keep[0], c[1] + c[3]);
+                            fma_pair(acc[n][0], acc[n][1], keep[0], c[0], c[1], c[2], c[3]);
                         } else {
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                acc[n][e % (2 * HB)] = fmaf(acc[n][e % (2 * HB)], keep[e / 2 % HB], c[e]);
-                            }
+                            fma_pair(acc[n][0], acc[n][1], keep[0], c[0], c[1]);
+                            fma_pair(acc[n][2 * HB - 2], acc[n][2 * HB - 1], keep[HB - 1], c[2], c[3]);
                         }
                     };
                     auto weigh = [&](float (&c)[4], int t, uint32_t b0, uint32_t b1) {

@@ -3,7 +3,8 @@
 Tolerances (u = 2^-23, twice the unit roundoff of binary32, which also covers sums that truncate):
   append     every step is one binary32 operation of defined order: equal bits.
   attention  a score of dim products is off by at most (dim + 16) u sum |q_i k_i| scale (products, sums, 22-bit operands, the
-             multiplication with the scale); its exponential by that much relative, plus 8 u; the sum over n tokens adds
+             multiplication with the scale; a cache of bytes may round queries at 2^-30 of a head's largest element instead,
+             which is less for the noise that is used here); its exponential by that much relative, plus 8 u; the sum over n tokens adds
              16 at a time: (n / 16 + 64) u sum p |v|.  Numerator and denominator together: twice that.  Exponentials below
              2^-126, the smallest normal number, may count as nothing: n 2^-126 max |v|.
   lora       inner sums: (K / 16 + 40) u sum |x a|; outer: (rank / 16 + 40) u sum |t b|; y itself: 2 u |y|.
@@ -363,6 +364,21 @@ def test_attention_rows_that_are_not_finite_stay_with_their_sequence(group):
         cache.v[int(table[3, 20]), 1, 7] = 0
         clean, clean_lse = attend(cache, q, table, length)
         got[1, :group], lse[1, :group], got[3, group:] = clean[1, :group], clean_lse[1, :group], clean[3, group:]
+        same = torch.equal(got, clean), torch.equal(lse, clean_lse)
+        assert same == (True, True)
+
+
+@pytest.mark.parametrize("i8", [0, 1])
+@pytest.mark.parametrize("group", [2, 12])
+def test_attention_queries_that_are_not_finite_stay_with_their_head(i8, group):
+    for bad in (math.nan, math.inf, -math.inf):
+        cache, q, table, length = batch(4, [700, 33], (16, 2, 64, i8, "hnd", 0), 2 * group)
+        clean, clean_lse = attend(cache, q, table, length)
+        q[0, 1, 5] = q[1, group, 63] = bad
+        got, lse = attend(cache, q, table, length)
+        for i, h in ((0, 1), (1, group)):
+            assert bool(got[i, h].isnan().all()) and bool(lse[i, h].isnan())
+            got[i, h], lse[i, h] = clean[i, h], clean_lse[i, h]
         same = torch.equal(got, clean), torch.equal(lse, clean_lse)
         assert same == (True, True)
 
