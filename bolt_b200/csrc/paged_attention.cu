@@ -331,8 +331,9 @@ struct Run {
     uint32_t token;                        // first one of the warp's step
     uint32_t first_page;                   // of the table's row
 };
-// The run behind it, and where the one after that begins: in shared memory, for registers are short.  (All lanes write the
-// same and read what they wrote.)
+// The run behind it, and where the one after that begins: in shared memory, for registers are short.  All lanes write the
+// same; a barrier stands between what they read and the first write, and behind the last one, since nothing else keeps them
+// together.
 struct Ahead {
     Run run;
     uint32_t sequence, unit, tile, tiles, begin, end, left;
@@ -405,31 +406,34 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
         ahead.tiles = tiles;
         ahead.begin = begin;
         ahead.end = end;
+        __syncwarp();
         auto look_ahead = [&]() {
             Run next;
-            uint32_t t = ahead.tile, tiles = ahead.tiles, left = ahead.left;
-            next.left = min(min(p.run_tiles, tiles - t), left);
-            ahead.run.left = next.left;
-            if (next.left == 0) {
-                return;
-            }
-            next.head = HB == 1 ? ahead.unit : ahead.unit / p.head_blocks;
+            uint32_t t = ahead.tile, tiles = ahead.tiles, left = ahead.left, unit_ahead = ahead.unit, sequence_ahead = ahead.sequence;
             next.begin = ahead.begin;
             next.end = ahead.end;
+            __syncwarp();       // everybody has read the record, and (enter) the run in it
+            next.left = min(min(p.run_tiles, tiles - t), left);
+            if (next.left == 0) {
+                ahead.run.left = 0;
+                __syncwarp();
+                return;
+            }
+            next.head = HB == 1 ? unit_ahead : unit_ahead / p.head_blocks;
             next.token = (((next.begin >> tile_shift) + t) << tile_shift) + member * S::STEP;
             uint32_t within;
             split_position(p, next.token, next.first_page, within);
             ahead.run = next;
             const uint64_t entry = (uint64_t)next.first_page + lane;
-            ahead.pages[lane] = entry < p.table_pages && entry * page_size < next.end ?
-                (uint32_t)__ldg(p.table + (uint64_t)ahead.sequence * p.table_pages + entry) : 0xFFFFFFFFu;
+            const uint32_t page = entry < p.table_pages && entry * page_size < next.end ?
+                (uint32_t)__ldg(p.table + (uint64_t)sequence_ahead * p.table_pages + entry) : 0xFFFFFFFFu;
             left -= next.left;
             t += next.left;
             if (t == tiles && left != 0) {
                 t = 0;
-                if (++ahead.unit == units) {
-                    ahead.unit = 0;
-                    const uint32_t s = next_sequence(p, ahead.sequence);
+                if (++unit_ahead == units) {
+                    unit_ahead = 0;
+                    const uint32_t s = next_sequence(p, sequence_ahead);
                     uint32_t b, e;
                     live_tokens(p, s, &b, &e);
                     ahead.sequence = s;
@@ -437,9 +441,12 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
                     ahead.end = e;
                     ahead.tiles = max(tiles_of(b, e, tile_shift), 1u);
                 }
+                ahead.unit = unit_ahead;
             }
             ahead.tile = t;
             ahead.left = left;
+            __syncwarp();
+            ahead.pages[lane] = page;       // (every lane's own: behind the barrier, which need not wait for the table)
         };
         uint32_t page_index = 0, at = 0;    // of the lane's token
         auto enter = [&]() {
@@ -527,6 +534,7 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
                 }
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
+            __syncwarp();       // (lanes that have copied nothing and those that have go on together)
             if (!values && run.left == 0) {
                 if (ahead.run.left != 0) {
                     enter();
