@@ -7,9 +7,12 @@
 // go from global memory straight into the fragments: the order of K inside an instruction is free, so a lane loads 16
 // neighbouring bytes of a row of A or B.
 //
-// Bytes of x become binary16 exactly.  Binary32 x enters as two tf32 numbers (22 bits; tf32 has binary32's range), t as two
-// binary16 numbers of rows brought to a common power of two.  The accumulation of the matrix instructions truncates, so
-// sums over K go on in binary32 registers every few instructions.
+// Bytes of x become binary16 exactly.  Binary32 x enters as two tf32 numbers (23 bits; tf32 has binary32's range), t as two
+// binary16 numbers of rows brought to a common power of two.  The accumulation of the matrix instructions truncates, which adds
+// up: sums over K go on in binary32 registers after two instructions, what the first number of a pair leaves is summed up
+// by itself, and sums over the rank go on in binary32 after 64 of it.  Sums of 8192 positive products of binary32 numbers come
+// out 2^-23 too small on the average where one chain of 32 instructions made them 2^-19 too small, those of any sign are as near
+// as binary32 throughout (1.1 to 1.7 2^-23 of the result, in root mean square).
 //
 // 2048 rows, 8192 -> 28672, rank 16, six requests: 75 to 86 us, 5.4 to 6.3 TB/s of the 470 MB of the result, read and written;
 // rank 64: 127 us.  16 rows with an adapter each: 13.4 us, two kernels of dependent loads over 23 MB.
@@ -165,6 +168,12 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], uint32_t a0, uint32_t a1
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_tf32_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)   // c = a b
+{
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f), "f"(0.f), "f"(0.f), "f"(0.f));
+}
 __device__ __forceinline__ void matrices(uint32_t (&r)[4], const void *at)
 {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -180,10 +189,21 @@ __device__ __forceinline__ uint32_t centred(uint32_t x)
     const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&y), *reinterpret_cast<const __half2 *>(&k));
     return *reinterpret_cast<const uint32_t *>(&h);
 }
-// what the tensor pipe sees of a number, and the rest (which it sees eleven bits of)
-__device__ __forceinline__ uint32_t tf32_of(float x)
+// A number as the sum of two that the tensor pipe sees whole (tf32: eleven bits), each the nearest: what is left out is 2^-23 of
+// it at most.  (What would round to infinity, infinities and NaN are cut off as they stand.)
+__device__ __forceinline__ void tf32_pair(float x, uint32_t &hi, uint32_t &lo)
 {
-    return __float_as_uint(x) & 0xFFFFE000u;
+    const uint32_t b = __float_as_uint(x), half = (b & 0x7FFFFFFFu) < 0x7F7FF000u ? 0x1000u : 0u;
+    hi = (b + half) & 0xFFFFE000u;
+    lo = (__float_as_uint(x - __uint_as_float(hi)) + half) & 0xFFFFE000u;
+}
+
+__device__ __forceinline__ void add(float (&sum)[4], const float (&c)[4])
+{
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        sum[e] += c[e];
+    }
 }
 
 // ---- inner sums ---------------------------------------------------------------------------------------------------
@@ -227,10 +247,19 @@ struct Eight<true> {
         h[2] = centred<0>(b);
         h[3] = centred<1>(b);
     }
+    // sum += rows (this one's and another eight's) x eight neighbours of a row of A
+    __device__ __forceinline__ void multiply(const Eight &other, const uint32_t (&a)[4], float (&sum)[4]) const
+    {
+        float c[4];
+        mma_f16_first(c, h[0], other.h[0], h[1], other.h[1], a[0], a[1]);
+        mma_f16(c, h[2], other.h[2], h[3], other.h[3], a[2], a[3]);
+        add(sum, c);
+    }
 };
 template <>
 struct Eight<false> {
     float f[8];
+    uint32_t hi[8], lo[8];
     __device__ __forceinline__ void load(const LoraParams &p, uint64_t row, uint32_t k, bool on)
     {
         const float *x = reinterpret_cast<const float *>(p.x) + row * p.x_stride + k;
@@ -257,7 +286,36 @@ struct Eight<false> {
             }
         }
     }
-    __device__ __forceinline__ void convert() {}
+    __device__ __forceinline__ void convert()
+    {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            tf32_pair(f[i], hi[i], lo[i]);
+        }
+    }
+    __device__ __forceinline__ void multiply(const Eight &other, const uint32_t (&a)[4], float (&sum)[4]) const
+    {
+        float c[4], rest[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&a[e]));
+            const uint32_t b0 = __float_as_uint(v.x), b1 = __float_as_uint(v.y);
+            if (e == 0) {
+                mma_tf32_first(rest, lo[0], other.lo[0], lo[1], other.lo[1], b0, b1);
+            } else {
+                mma_tf32(rest, lo[2 * e], other.lo[2 * e], lo[2 * e + 1], other.lo[2 * e + 1], b0, b1);
+            }
+            if (e % 2 == 0) {
+                mma_tf32_first(c, hi[2 * e], other.hi[2 * e], hi[2 * e + 1], other.hi[2 * e + 1], b0, b1);
+            } else {
+                mma_tf32(c, hi[2 * e], other.hi[2 * e], hi[2 * e + 1], other.hi[2 * e + 1], b0, b1);
+            }
+            if (e % 2 == 1) {
+                add(sum, c);
+            }
+        }
+        add(sum, rest);
+    }
 };
 
 // By the 256 threads of a CTA: the sums over blocks from .. to - 1 of 32 of K for the rows of a unit, times their scales, in warp 0: sum
@@ -289,11 +347,6 @@ __device__ __forceinline__ void inner_sums(const LoraParams &p, const Unit &u, u
             x[i][0].load(p, u.row + g, k, b < to && k < p.K && g < u.rows);
             x[i][1].load(p, u.row + g + 8, k, b < to && k < p.K && g + 8 < u.rows);
         }
-        float c[NT][4];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
-        }
 #pragma unroll
         for (int i = 0; i < AT_ONCE; ++i) {
             const uint32_t k = 32 * (kb + 8 * i) + 8 * c4;
@@ -310,27 +363,7 @@ __device__ __forceinline__ void inner_sums(const LoraParams &p, const Unit &u, u
                         }
                     }
                 }
-                if constexpr (U8) {
-                    mma_f16(c[n], x[i][0].h[0], x[i][1].h[0], x[i][0].h[1], x[i][1].h[1], h[0], h[1]);
-                    mma_f16(c[n], x[i][0].h[2], x[i][1].h[2], x[i][0].h[3], x[i][1].h[3], h[2], h[3]);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&h[e]));
-                        const float r0 = x[i][0].f[2 * e], r1 = x[i][1].f[2 * e], r2 = x[i][0].f[2 * e + 1], r3 = x[i][1].f[2 * e + 1];
-                        const uint32_t b0 = __float_as_uint(b.x), b1 = __float_as_uint(b.y);
-                        mma_tf32(c[n], tf32_of(r0), tf32_of(r1), tf32_of(r2), tf32_of(r3), b0, b1);
-                        mma_tf32(c[n], tf32_of(r0 - __uint_as_float(tf32_of(r0))), tf32_of(r1 - __uint_as_float(tf32_of(r1))),
-                            tf32_of(r2 - __uint_as_float(tf32_of(r2))), tf32_of(r3 - __uint_as_float(tf32_of(r3))), b0, b1);
-                    }
-                }
-            }
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                sum[n][e] += c[n][e];
+                x[i][0].multiply(x[i][1], h, sum[n]);
             }
         }
     }
@@ -376,8 +409,10 @@ __device__ __forceinline__ void inner_sums(const LoraParams &p, const Unit &u, u
         }
     }
 }
+// (Binary32 x with ranks of 17 to 64: a few registers above half of them all without the bound; 2048 rows of rank 32 106 us, 117
+// without.)
 template <bool U8, int NT>
-__global__ void __launch_bounds__(256) lora_inner_kernel(const __grid_constant__ LoraParams p)
+__global__ void __launch_bounds__(256, !U8 && (NT == 4 || NT == 8) ? 2 : 0) lora_inner_kernel(const __grid_constant__ LoraParams p)
 {
     __shared__ float merge[4][NT * 4 * 32];
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -674,42 +709,51 @@ __global__ void __launch_bounds__(256, ALONE ? (ALONE == ALONE_U8 ? 2 : 1) : (KS
         // t's fragments: in registers, or (larger ranks) read again for every step
         constexpr bool KEPT = KS <= 2;
         uint32_t th[KEPT ? KS : 1][4], tl[KEPT ? KS : 1][4];
-        auto fragments = [&](int s, uint32_t (&h)[4], uint32_t (&l)[4]) {
-            matrices(h, &hi[lane % 16][16 * s + lane / 16 * 8]);
-            matrices(l, &lo[lane % 16][16 * s + lane / 16 * 8]);
-        };
+        auto fragment = [&](uint32_t (&r)[4], const __half (&of)[16][PITCH], int s) { matrices(r, &of[lane % 16][16 * s + lane / 16 * 8]); };
         if constexpr (KEPT) {
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
-                fragments(s, th[s], tl[s]);
+                fragment(th[s], hi, s);
+                fragment(tl[s], lo, s);
             }
         }
         const float down0 = down[g], down1 = down[g + 8];
 #pragma unroll 1
         for (;;) {
-            float c[TILES][4];
+            // The instruction's own accumulation truncates: what binary16 has cut off of t goes first, while the sums are small, and
+            // every 16 * FOLD of the rank the sums go on in binary32.
+            constexpr int FOLD = KS < 4 ? KS : 4;
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                if constexpr (!KEPT) {
-                    fragments(s, th[0], tl[0]);
+            for (int s0 = 0; s0 < KS; s0 += FOLD) {
+                float c[TILES][4];
+#pragma unroll
+                for (int i = 0; i < 2 * FOLD; ++i) {
+                    const int s = s0 + i % FOLD;
+                    uint32_t a[4];
+                    if constexpr (KEPT) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            a[e] = i < FOLD ? tl[s][e] : th[s][e];
+                        }
+                    } else {
+                        fragment(a, i < FOLD ? lo : hi, s);
+                    }
+#pragma unroll
+                    for (int t = 0; t < TILES; ++t) {
+                        if (i == 0) {
+                            mma_f16_first(c[t], a[0], a[1], a[2], a[3], w[t][s][0], w[t][s][1]);
+                        } else {
+                            mma_f16(c[t], a[0], a[1], a[2], a[3], w[t][s][0], w[t][s][1]);
+                        }
+                    }
                 }
-                const uint32_t(&h)[4] = th[KEPT ? s : 0], (&l)[4] = tl[KEPT ? s : 0];
 #pragma unroll
                 for (int t = 0; t < TILES; ++t) {
-                    if (s == 0) {
-                        mma_f16_first(c[t], l[0], l[1], l[2], l[3], w[t][s][0], w[t][s][1]);
-                    } else {
-                        mma_f16(c[t], l[0], l[1], l[2], l[3], w[t][s][0], w[t][s][1]);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        v[0][t / 2][t % 2 * 2 + e] = fmaf(c[t][e], down0, v[0][t / 2][t % 2 * 2 + e]);
+                        v[1][t / 2][t % 2 * 2 + e] = fmaf(c[t][2 + e], down1, v[1][t / 2][t % 2 * 2 + e]);
                     }
-                    mma_f16(c[t], h[0], h[1], h[2], h[3], w[t][s][0], w[t][s][1]);
-                }
-            }
-#pragma unroll
-            for (int t = 0; t < TILES; ++t) {
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    v[0][t / 2][t % 2 * 2 + e] = fmaf(c[t][e], down0, v[0][t / 2][t % 2 * 2 + e]);
-                    v[1][t / 2][t % 2 * 2 + e] = fmaf(c[t][2 + e], down1, v[1][t / 2][t % 2 * 2 + e]);
                 }
             }
             const bool all = whole();
