@@ -243,6 +243,18 @@ __device__ __forceinline__ float2 shared_pair(uint32_t at)
     asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
     return v;
 }
+__device__ __forceinline__ float shared_number(uint32_t at)
+{
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t shared_bits(uint32_t at)     // whether any of 16 bytes is set
+{
+    uint32_t a, b, c, d;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(at) : "memory");
+    return a | b | c | d;
+}
 // two binary32 operations in one instruction: (x, y) = (x, y) * k + (a, b), and the sum of two pairs
 __device__ __forceinline__ void fma_pair(float &x, float &y, float k, float a, float b)
 {
@@ -291,6 +303,13 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t &hi, uint3
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
+// Weights of rows of bytes are sums of two binary16 numbers in units of a power of two that puts the largest, ref or a little below,
+// at 2^14 .. 2^15.  (From 2^-126 on, so that it and its reciprocal are normal numbers.)
+__device__ __forceinline__ uint32_t weight_unit_bits(float ref)
+{
+    return max(__float_as_uint(ref) & 0x7F800000u, 15u << 23) - (14u << 23);
+}
+
 // DP: elements of a row, rounded up; HB: blocks of eight query heads
 template <int DP, bool I8, int HB>
 struct Shape {
@@ -307,6 +326,7 @@ struct Shape {
     // sequences of up to 8192 tokens, 300 calls in a row: 146 us, as binary16 149; rows of 256 elements 161 and 167; two blocks
     // would have 64 running numbers more: 261 and 242).
     static constexpr bool DIGITS = I8 && HB == 1;
+    static constexpr float LIFT = I8 ? 0.f : 14.f;     // binary16: weights are exp(s - m) 2^14
     static constexpr int Q_PITCH = DP * (DIGITS ? 1 : 2) + 16, Q_ROWS = HEADS * (DIGITS ? 4 : 2), Q_BYTES = Q_ROWS * Q_PITCH;   // queries of a team
     static constexpr int TEAMS = 4 * Q_BYTES <= 20480 ? 4 : (2 * Q_BYTES <= 20480 ? 2 : 1);
     // Numbers of a lane that the warps exchange at a time, in the slot that each is through with: as many as there are, or as fit.
@@ -554,7 +574,7 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
         constexpr bool EVEN = S::SLOTS % 2 == 0;        // then a K turn asks for V, and a V turn for K
         uint32_t item = ring_at + S::SLOT, count = 0, done = 0;    // tiles of the unit, and how many of them are through
         uint32_t head0 = 0, heads_here = 0, mask = 0;
-        float fac[HB], m[HB], l[HB], keep[HB], w[HB][NT][2], acc[TILES_D][2 * HB], top_unit = 0.f;
+        float fac[HB], m[HB], l[HB], keep[HB], w[HB][NT][2], acc[TILES_D][2 * HB], ref[HB];
         const uint32_t q_at = smem_at(q_smem + (lane % 16) * S::Q_PITCH + lane / 16 * 16);
         int n = 1 - S::SLOTS;
         auto turn = [&](auto asks_for_values) {
@@ -632,11 +652,10 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
                     for (int b = 0; b < HB; ++b) {
                         fac[b] = factor[g + 8 * b];
                     }
-                    top_unit = 0.f;
 #pragma unroll
                     for (int b = 0; b < HB; ++b) {
                         m[b] = -INFINITY;
-                        l[b] = 0.f;
+                        l[b] = ref[b] = 0.f;
                     }
 #pragma unroll
                     for (int n = 0; n < TILES_D; ++n) {
@@ -725,7 +744,7 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
                             }
                         }
                     }
-                    // weights: exp(s - m) times 2^14, which the division by their sum takes back
+                    // weights: exp(s - m), in binary16 times 2^14, which the division by their sum takes back
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
                         float unit_k[2] = {1.f, 1.f};
@@ -772,7 +791,7 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
                         for (int j = 0; j < NT; ++j) {
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
-                                w[b][j][e] = exp2_fast(w[b][j][e] - (base - 14.f));
+                                w[b][j][e] = exp2_fast(w[b][j][e] - (base - S::LIFT));
                                 l[b] += w[b][j][e];
                             }
                         }
@@ -783,37 +802,55 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
             if (turn(std::bool_constant<!EVEN>())) {
                 if (mask != 0) {
                     if constexpr (I8) {
-                        // Rows of bytes have units of their own.  They go into the weights, relative to the largest unit so far:
-                        // weights stay within binary16.
-                        float unit_v[NT][2], top = top_unit;
+                        // Rows of bytes have units of their own, which go into the weights, and these are taken relative to the largest of
+                        // a head so far (`ref`, as the sums relative to the running maximum of the scores): a row with a large unit that
+                        // weighs little leaves the others their bits.  Rows of zeros, whose scale is 1 whatever the others' are, have no share.
+                        const float own_scale = shared_number(item + S::STEP * S::PITCH + lane_token * 4);
+                        uint32_t counts = mask;
+#pragma unroll 1
+                        for (uint32_t ones = __ballot_sync(0xFFFFFFFFu, own_scale == 1.f) & mask; ones != 0; ones &= ones - 1) {
+                            const uint32_t r = __ffs(ones) - 1;
+                            uint32_t bytes = 0;
+                            if (lane < pieces) {
+                                bytes = shared_bits(item + r * S::PITCH + lane * 16);
+                            }
+                            if (!__any_sync(0xFFFFFFFFu, bytes != 0)) {
+                                counts &= ~(1u << r);
+                            }
+                        }
+                        float unit_v[NT][2];
 #pragma unroll
                         for (int j = 0; j < NT; ++j) {
                             const float2 u = shared_pair(item + S::STEP * S::PITCH + (8 * j + 2 * c4) * 4);
                             unit_v[j][0] = reciprocal(u.x);
                             unit_v[j][1] = reciprocal(u.y);
                         }
-                        if (mask != S::ALL) {
+                        if (counts != S::ALL) {
 #pragma unroll
                             for (int j = 0; j < NT; ++j) {
-                                unit_v[j][0] = mask >> (8 * j + 2 * c4) & 1 ? unit_v[j][0] : 0.f;
-                                unit_v[j][1] = mask >> (8 * j + 2 * c4 + 1) & 1 ? unit_v[j][1] : 0.f;
+                                unit_v[j][0] = counts >> (8 * j + 2 * c4) & 1 ? unit_v[j][0] : 0.f;
+                                unit_v[j][1] = counts >> (8 * j + 2 * c4 + 1) & 1 ? unit_v[j][1] : 0.f;
                             }
                         }
 #pragma unroll
-                        for (int j = 0; j < NT; ++j) {
-                            top = fmaxf(top, fmaxf(unit_v[j][0], unit_v[j][1]));
-                        }
-                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-                        const float inv = top > 0.f ? reciprocal(top) : 0.f, change = top_unit * inv;
-                        top_unit = top;
-#pragma unroll
                         for (int b = 0; b < HB; ++b) {
-                            keep[b] *= change;
+                            float top = 0.f;
 #pragma unroll
                             for (int j = 0; j < NT; ++j) {
-                                w[b][j][0] *= unit_v[j][0] * inv;
-                                w[b][j][1] *= unit_v[j][1] * inv;
+                                w[b][j][0] *= unit_v[j][0];
+                                w[b][j][1] *= unit_v[j][1];
+                                top = fmaxf(top, fmaxf(w[b][j][0], w[b][j][1]));
+                            }
+                            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+                            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+                            const float before = __uint_as_float(weight_unit_bits(ref[b]));
+                            ref[b] = fmaxf(ref[b] * keep[b], top);
+                            const float inv = __uint_as_float((254u << 23) - weight_unit_bits(ref[b]));
+                            keep[b] = keep[b] * before * inv;
+#pragma unroll
+                            for (int j = 0; j < NT; ++j) {
+                                w[b][j][0] *= inv;
+                                w[b][j][1] *= inv;
                             }
                         }
                     }
@@ -921,7 +958,7 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
                         }
                         all += __shfl_xor_sync(0xFFFFFFFFu, all, 1);
                         all += __shfl_xor_sync(0xFFFFFFFFu, all, 2);
-                        own[b] = exp2_fast(m[b] - base) * (I8 ? top_unit : 1.f);
+                        own[b] = exp2_fast(m[b] - base) * (I8 ? __uint_as_float(weight_unit_bits(ref[b])) : 1.f);
                         if (whole) {
                             own[b] *= all == 0.f ? 0.f : __frcp_rn(all);
                         }
@@ -930,7 +967,7 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
                                 share[S::HEADS * DP + h] = top;
                                 share[S::HEADS * (DP + 1) + h] = all;
                             } else if (p.lse != nullptr && h < heads_here) {
-                                p.lse[(uint64_t)sequence * p.heads + head0 + h] = (top + log2f(all) - 14.f) * LN2;
+                                p.lse[(uint64_t)sequence * p.heads + head0 + h] = (top + log2f(all) - S::LIFT) * LN2;
                             }
                         }
                     }
@@ -1106,7 +1143,7 @@ __global__ void __launch_bounds__(512) paged_attention_join_kernel(const __grid_
         }
     }
     if (p.lse != nullptr && lane == 0) {
-        p.lse[(uint64_t)cut.sequence * p.heads + hq] = (top + log2f(all) - 14.f) * LN2;
+        p.lse[(uint64_t)cut.sequence * p.heads + hq] = (top + log2f(all) - (p.i8 ? 0.f : 14.f)) * LN2;     // (Shape::LIFT)
     }
 }
 

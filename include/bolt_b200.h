@@ -537,8 +537,10 @@ EE bolt_b200_kv_append(const bolt_b200_kv_cache *cache, const bolt_b200_kv_appen
  * whatever it is; rows of live tokens have to be finite (one that is not spoils its own sequence and key head only).
  * out_dt: DT_F32, DT_F16, or, for a projection that follows, DT_U8_Q as by quantize_cuda_b200 with the scale out_scale:
  * clamp(rne(x * out_scale + 128), 1, 255).
- * Statistics and sums are binary32; queries and probabilities enter the products with 22 bits at least (queries of DT_I8 and
- * up to 8 heads to a key head: rounded to 2^-30 of the head's largest element).
+ * Statistics and sums are binary32.  What enters the products is off by 2^-22 of itself, or by this much where that is more: an
+ * element of a query by 2^-38 of the head's largest (DT_I8 and up to 8 heads to a key head: always by 2^-30 of it), a probability by
+ * 2^-39 of the head's largest, in DT_I8 each times 1 / v_scale of its row.  (Rows of zeros are left out of that if their scale is 1,
+ * as bolt_b200_kv_append leaves it.)
  * At most 65535 sequences and query heads, strides up to 2^30, and below 2^32 groups of 16 tokens that the tables have room
  * for, counted for every key head and (with more than 8) every 16 of its query heads.  q and out must not overlap.
  * tmp: the bytes asked for by _tmp_bytes, 16-byte aligned. */

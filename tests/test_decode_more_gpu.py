@@ -3,12 +3,13 @@ Tolerances are those of test_decode_gpu.py where nothing else is said (u = 2^-23
 import os
 import sys
 
+import numpy as np
 import pytest
 import torch
 
 sys.path.insert(0, os.path.dirname(__file__))
 import bolt_b200 as B  # noqa: E402
-from test_decode_gpu import DT, U, attend, batch, check_attention, status  # noqa: E402
+from test_decode_gpu import DT, U, Cache, attend, batch, check_attention, perm, rand, status  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -61,3 +62,54 @@ def test_lora_sums_of_one_sign(x_dt, rows, n, k, rank):
     want = (exact @ a[0, :, :k].double().T) @ b[0].double().T
     mean = float(((y.double() - want) / want).mean()) / U
     assert abs(mean) <= 3, mean
+
+
+# ---- caches of bytes whose rows differ -------------------------------------------------------------------------------
+def filled(i8, k, v, page):
+    """a cache of one sequence made by kv_append; k, v: [tokens, heads, dim] in binary32"""
+    n, kv, dim = k.shape
+    cache = Cache(1, -(-n // page), page, kv, dim, i8)
+    table = perm(2, cache.pages).int()[None, :].contiguous()
+    rows = torch.cat((k.reshape(n, -1), v.reshape(n, -1)), 1).contiguous()
+    seq, pos = torch.zeros(n, dtype=torch.int32, device="cuda"), torch.arange(n, dtype=torch.int32, device="cuda")
+    p = rows.data_ptr()
+    B.kv_append(cache.desc(), B.KvAppend(n, 0, B.DT_F32, B.DT_F32, None, p, p + 4 * kv * dim, None, 0, 2 * kv * dim, 2 * kv * dim, 0, seq.data_ptr(),
+                                         pos.data_ptr(), table.data_ptr(), 1, table.shape[1], 0, 0, 0, None, None))
+    return cache, table
+
+
+@pytest.mark.parametrize("kv,group,dim", [(2, 4, 128), (1, 1, 64), (1, 8, 256), (1, 12, 128), (3, 2, 80)])
+@pytest.mark.parametrize("small", [1e-2, 1e-4, 1e-6, 1e-8, 1e-20])
+@pytest.mark.parametrize("heavy", ["zeros", "ones", "large"])
+def test_attention_values_beside_a_heavy_row(kv, group, dim, small, heavy):
+    """Rows of small values beside rows that weigh most, are zeros and therefore have scale 1, or weigh next to nothing and are
+    large: the small ones keep their bits.  (ones: rows whose scale is 1, too, and that are no zeros count.)"""
+    n, heads = 700, kv * group
+    q = rand(3, 1, heads, dim)
+    k, v = rand(4, n, kv, dim), small * rand(5, n, kv, dim)
+    one = q[0].view(kv, group, dim).sum(1)
+    one = 16 * group ** 0.5 * one / one.norm(dim=-1, keepdim=True)      # a key whose score is about 16 for all heads of the group
+    spots = [0, 17, 300, 650, 699]
+    for t in spots:
+        k[t] = -2 * one if heavy == "large" else one
+        v[t] = 0 if heavy == "zeros" else (127 * rand(6 + t, kv, dim).sign() if heavy == "ones" else rand(6 + t, kv, dim))
+    length = torch.tensor([n], dtype=torch.int32, device="cuda")
+    cache, table = filled(1, k, v, 16)
+    if heavy != "large":
+        assert bool((cache.vs[table[0, 1], :, 1] == 1).all())
+    got, lse = attend(cache, q, table, length)
+    assert status() == 0
+    check_attention(cache, q, table, length, got, lse)
+    if small < 1e-3:
+        return                                                          # (below binary16)
+    # A cache of binary16: a weight is two binary16 numbers in units in which a head's largest is 2^14, the second a multiple of
+    # 2^-24 at worst: off by 2^-25, which is 2^-39 of the largest weight.
+    cache, table = filled(0, k, v, 16)
+    got, lse = attend(cache, q, table, length)
+    kk, vv = (cache.rows(x, table[0], 0, n).repeat_interleave(group, 0) for x in "kv")
+    s, size = (torch.einsum("hd,htd->ht", a, b) * np.float32(dim ** -0.5).item() for a, b in ((q[0].double(), kk), (q[0].double().abs(), kk.abs())))
+    p = torch.softmax(s, -1)
+    tol = 2 * ((dim + 16) * U * size.amax(-1)[:, None] + (n / 16 + 72) * U) * torch.einsum("ht,htd->hd", p, vv.abs()) + n * 2.0 ** -126 * vv.abs().amax(1)
+    tol += 2.0 ** -39 * p.amax(-1)[:, None] * vv.abs().sum(1)
+    n_bad = int((~((got[0].double() - torch.einsum("ht,htd->hd", p, vv)).abs() <= tol)).sum())
+    assert n_bad == 0
