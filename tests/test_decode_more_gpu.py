@@ -1,5 +1,6 @@
 """Cache append, paged attention and adapters, continued: rows, orders and values that the first file of tests does not meet.
 Tolerances are those of test_decode_gpu.py where nothing else is said (u = 2^-23)."""
+import math
 import os
 import sys
 
@@ -106,10 +107,102 @@ def test_attention_values_beside_a_heavy_row(kv, group, dim, small, heavy):
     # 2^-24 at worst: off by 2^-25, which is 2^-39 of the largest weight.
     cache, table = filled(0, k, v, 16)
     got, lse = attend(cache, q, table, length)
+    check_one(cache, q, table, n, got, lse, weight=2.0 ** -39)
+
+
+def check_one(cache, q, table, n, got, lse, query=0.0, weight=0.0):
+    """check_attention of one sequence, and what a query is off by, of its head's largest element, and a weight, of the largest"""
+    dim, group = q.shape[2], q.shape[1] // cache.heads
     kk, vv = (cache.rows(x, table[0], 0, n).repeat_interleave(group, 0) for x in "kv")
-    s, size = (torch.einsum("hd,htd->ht", a, b) * np.float32(dim ** -0.5).item() for a, b in ((q[0].double(), kk), (q[0].double().abs(), kk.abs())))
-    p = torch.softmax(s, -1)
-    tol = 2 * ((dim + 16) * U * size.amax(-1)[:, None] + (n / 16 + 72) * U) * torch.einsum("ht,htd->hd", p, vv.abs()) + n * 2.0 ** -126 * vv.abs().amax(1)
-    tol += 2.0 ** -39 * p.amax(-1)[:, None] * vv.abs().sum(1)
+    scale = np.float32(dim ** -0.5).item()
+    qq = q[0].double()
+    s = torch.einsum("hd,htd->ht", qq, kk) * scale
+    off = ((dim + 16) * U * torch.einsum("hd,htd->ht", qq.abs(), kk.abs()) + query * qq.abs().amax(-1)[:, None] * kk.abs().sum(-1)).amax(-1) * scale
+    top = torch.logsumexp(s, -1)
+    p = torch.exp(s - top[:, None])
+    tol = 2 * (off[:, None] + (n / 16 + 72) * U) * torch.einsum("ht,htd->hd", p, vv.abs()) + n * 2.0 ** -126 * vv.abs().amax(1)
+    tol += weight * p.amax(-1)[:, None] * vv.abs().sum(1)
     n_bad = int((~((got[0].double() - torch.einsum("ht,htd->hd", p, vv)).abs() <= tol)).sum())
-    assert n_bad == 0
+    n_lse = int((~((lse[0].double() - top).abs() <= off + (n / 16 + 72) * U + 2 * U * top.abs())).sum())
+    assert (n_bad, n_lse) == (0, 0)
+
+
+@pytest.mark.parametrize("kv,group,dim", [(2, 4, 128), (1, 1, 64), (1, 12, 128), (1, 8, 256)])
+@pytest.mark.parametrize("i8", [0, 1])
+@pytest.mark.parametrize("ratio", [2.0 ** 8, 2.0 ** 15, 2.0 ** 20])
+def test_attention_queries_of_different_magnitude(kv, group, dim, i8, ratio):
+    """Heads in which some elements are by far the largest, where the keys are nothing (and the others decide) or alike.  Whole
+    numbers for bytes are rounded to half a unit, 2^-30 of an element that has 2^29 units or more; the second of two binary16 numbers to
+    2^-25 beside 2^13 or more, 2^-38."""
+    n = 600
+    for big in (0.0, 1.0 / ratio, 1.0):
+        q = rand(3, 1, kv * group, dim)
+        k, v = rand(4, n, kv, dim), rand(5, n, kv, dim)
+        q[..., 3::40] *= ratio
+        k[..., 3::40] *= big
+        if big == 1:
+            q *= 8 / ratio                                             # (scores of some 10)
+        cache, table = filled(i8, k, v, 16)
+        length = torch.tensor([n], dtype=torch.int32, device="cuda")
+        got, lse = attend(cache, q, table, length)
+        assert status() == 0
+        check_one(cache, q, table, n, got, lse, query=2.0 ** -30 if i8 and group <= 8 else 2.0 ** -38)
+
+
+# ---- what other tests would let through ------------------------------------------------------------------------------
+@pytest.mark.parametrize("i8", [0, 1])
+@pytest.mark.parametrize("sequences,longest", [(256, 70), (257, 70), (1025, 70), (5000, 40), (65535, 3)])
+def test_attention_of_many_sequences_leaves_no_nan(i8, sequences, longest):
+    """every number of every sequence, those without tokens among them, is one"""
+    page, heads, dim = 8, 3, 32
+    g = torch.Generator(device="cuda")
+    g.manual_seed(sequences)
+    length = torch.randint(0, longest + 1, (sequences,), device="cuda", generator=g, dtype=torch.int32)
+    length[1::3] = 0
+    tp = -(-longest // page)
+    cache = Cache(1, 3000, page, 1, dim, i8)
+    table = torch.randint(0, 3000, (sequences, tp), device="cuda", generator=g, dtype=torch.int32)
+    table[torch.arange(tp, device="cuda")[None, :] * page >= length[:, None]] = -1
+    q = rand(5, sequences, heads, dim)
+    got, lse = attend(cache, q, table, length)
+    assert status() == 0
+    empty = length == 0
+    assert bool((got[empty] == 0).all()) and bool((lse[empty] == -math.inf).all())
+    assert bool(got.isfinite().all()) and bool(lse[~empty].isfinite().all())
+    t = torch.arange(longest, device="cuda")
+    pages, at = table.clamp(min=0).long()[:, t // page], (t % page)[None, :].expand(sequences, -1)
+    k, v = (x[pages, 0, at].double() / (s[pages, 0, at].double()[..., None] if i8 else 1) for x, s in ((cache.k, cache.ks), (cache.v, cache.vs)))
+    live = t[None, None, :] < length[:, None, None]
+    scale = np.float32(dim ** -0.5).item()
+    off = ((dim + 16) * U * scale * torch.einsum("bhd,btd->bht", q.double().abs(), k.abs()) * live).amax(-1)
+    s = torch.where(live, torch.einsum("bhd,btd->bht", q.double(), k) * scale, -math.inf)
+    top = torch.logsumexp(s, -1)
+    p = torch.where(live, torch.exp(s - top[..., None]), 0.0)
+    tol = 2 * (off[..., None] + (longest / 16 + 72) * U) * torch.einsum("bht,btd->bhd", p, v.abs()) + longest * 2.0 ** -126 * v.abs().amax()
+    n_bad = int((~((got.double() - torch.einsum("bht,btd->bhd", p, v)).abs() <= tol)).sum())
+    n_lse = int((~((lse.double() - top).abs() <= off + (longest / 16 + 72) * U + 2 * U * top.abs()))[~empty].sum())
+    assert (n_bad, n_lse) == (0, 0)
+
+
+@pytest.mark.parametrize("rows,n,k,rank,segments", [(64, 1000, 2048, 16, 64), (600, 700, 4096, 32, 3), (5, 768, 768, 8, 2), (40, 512, 28672, 128, 1)])
+def test_lora_of_bytes_gives_the_same_bits_again(rows, n, k, rank, segments):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(rows)
+    x = torch.randint(0, 256, (rows, k), device="cuda", generator=g, dtype=torch.uint8)
+    a, b, y = rand(1, segments, rank, k, dtype=torch.float16), rand(2, segments, n, rank, dtype=torch.float16), rand(3, rows, n)
+    scale, row_scale = rand(4, segments), 20 + torch.rand(rows, device="cuda", generator=g)
+    first = torch.tensor([rows * i // segments for i in range(segments + 1)], dtype=torch.int32, device="cuda")
+    adapter = torch.arange(segments, dtype=torch.int32, device="cuda")
+    results = []
+    for fill in (0, 0xFF, 0x5A):
+        out = y.clone()
+        call = B.Lora(rows, n, k, rank, segments, segments, B.DT_U8_Q, x.data_ptr(), out.data_ptr(), k, n, a.data_ptr(), b.data_ptr(), k, scale.data_ptr(),
+                      first.data_ptr(), adapter.data_ptr(), 1.0, None, row_scale.data_ptr())
+        nb = B.lora_tmp_bytes(call)
+        tmp = torch.full((nb,), fill, dtype=torch.uint8, device="cuda")
+        B.lora(call, nb, tmp.data_ptr())
+        assert status() == 0
+        results.append(out)
+    assert not torch.equal(results[0], y)
+    same = [torch.equal(r, results[0]) for r in results]
+    assert same == [True] * 3
