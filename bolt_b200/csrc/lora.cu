@@ -218,14 +218,14 @@ struct Eight<true> {
         uint32_t w[2] = {0x80808080u, 0x80808080u};
         const uint8_t *x = reinterpret_cast<const uint8_t *>(p.x) + row * p.x_stride + k;
         if (on && p.x_vectors && k + 8 <= p.K) {
-            const uint2 v = __ldg(reinterpret_cast<const uint2 *>(x));
+            const uint2 v = *reinterpret_cast<const uint2 *>(x);
             w[0] = v.x;
             w[1] = v.y;
         } else if (on && k + 8 <= p.K) {
             // the aligned words that hold a byte of the eight, shifted into place
             const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(x) & 3);
             const uint32_t *words = reinterpret_cast<const uint32_t *>(x - off);
-            const uint32_t a = __ldg(words), b = __ldg(words + 1), c = off != 0 ? __ldg(words + 2) : 0;
+            const uint32_t a = words[0], b = words[1], c = off != 0 ? words[2] : 0;
             w[0] = __funnelshift_r(a, b, 8 * off);
             w[1] = __funnelshift_r(b, c, 8 * off);
         } else if (on) {
@@ -268,7 +268,7 @@ struct Eight<false> {
             f[i] = 0.f;
         }
         if (on && p.x_vectors && k + 8 <= p.K) {
-            const float4 u = __ldg(reinterpret_cast<const float4 *>(x)), v = __ldg(reinterpret_cast<const float4 *>(x) + 1);
+            const float4 u = *reinterpret_cast<const float4 *>(x), v = reinterpret_cast<const float4 *>(x)[1];
             f[0] = u.x;
             f[1] = u.y;
             f[2] = u.z;
@@ -281,7 +281,7 @@ struct Eight<false> {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 if (k + i < p.K) {
-                    f[i] = __ldg(x + i);
+                    f[i] = x[i];
                 }
             }
         }
@@ -341,7 +341,7 @@ __device__ __forceinline__ void inner_sums(const LoraParams &p, const Unit &u, u
             for (int n = 0; n < NT; ++n) {
                 w[i][n] = make_uint4(0, 0, 0, 0);
                 if (b < to && n * 8 < p.rank && k < p.K) {
-                    w[i][n] = __ldg(reinterpret_cast<const uint4 *>(a + n * 8 * p.a_stride + 32 * b));
+                    w[i][n] = *reinterpret_cast<const uint4 *>(a + n * 8 * p.a_stride + 32 * b);
                 }
             }
             x[i][0].load(p, u.row + g, k, b < to && k < p.K && g < u.rows);
@@ -547,9 +547,19 @@ __global__ void __launch_bounds__(256, ALONE ? (ALONE == ALONE_U8 ? 2 : 1) : (KS
             }
         }
     };
+    // (Where this kernel starts behind lora_inner_kernel nothing that may write B still runs.  Alone it starts beside the end of what is
+    // in front of it: memory is no read-only memory then.  As plain loads, which stay behind the stores of the step before,
+    // 2048 rows of rank 128 take 246 us, not 213.)
+    auto weights = [](const auto *at) {
+        if constexpr (ALONE) {
+            return *at;
+        } else {
+            return __ldg(at);
+        }
+    };
     auto fetch_row = [&](int t, const __half *row, bool on) {
         if (KS == 1 && on && p.rank == 16) {
-            const uint2 x = __ldg(reinterpret_cast<const uint2 *>(row + 4 * c4));
+            const uint2 x = weights(reinterpret_cast<const uint2 *>(row + 4 * c4));
             w[t][0][0] = x.x;
             w[t][0][1] = x.y;
             return;
@@ -560,7 +570,7 @@ __global__ void __launch_bounds__(256, ALONE ? (ALONE == ALONE_U8 ? 2 : 1) : (KS
             const uint32_t left = p.rank - 16 * s;
             if (on && 16 * s < p.rank) {
                 if (KS > 1 && left >= 32) {
-                    const uint4 x = __ldg(reinterpret_cast<const uint4 *>(row + 16 * s + 8 * c4));
+                    const uint4 x = weights(reinterpret_cast<const uint4 *>(row + 16 * s + 8 * c4));
                     q[0] = x.x;
                     q[1] = x.y;
                     q[2] = x.z;
@@ -568,13 +578,13 @@ __global__ void __launch_bounds__(256, ALONE ? (ALONE == ALONE_U8 ? 2 : 1) : (KS
                 } else {
                     uint32_t r = 16 * s;
                     if (left >= 16) {
-                        const uint2 x = __ldg(reinterpret_cast<const uint2 *>(row + r + 4 * c4));
+                        const uint2 x = weights(reinterpret_cast<const uint2 *>(row + r + 4 * c4));
                         q[0] = x.x;
                         q[1] = x.y;
                         r += 16;
                     }
                     if (left % 16 == 8) {
-                        const uint32_t x = __ldg(reinterpret_cast<const uint32_t *>(row + r + 2 * c4));
+                        const uint32_t x = weights(reinterpret_cast<const uint32_t *>(row + r + 2 * c4));
                         q[left >= 16 ? 2 : 0] = x;
                     }
                 }

@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
             ahead.run = next;
             const uint64_t entry = (uint64_t)next.first_page + lane;
             const uint32_t page = entry < p.table_pages && entry * page_size < next.end ?
-                (uint32_t)__ldg(p.table + (uint64_t)sequence_ahead * p.table_pages + entry) : 0xFFFFFFFFu;
+                (uint32_t)p.table[(uint64_t)sequence_ahead * p.table_pages + entry] : 0xFFFFFFFFu;
             left -= next.left;
             t += next.left;
             if (t == tiles && left != 0) {

@@ -206,3 +206,42 @@ def test_lora_of_bytes_gives_the_same_bits_again(rows, n, k, rank, segments):
     assert not torch.equal(results[0], y)
     same = [torch.equal(r, results[0]) for r in results]
     assert same == [True] * 3
+
+
+@pytest.mark.parametrize("heads,n", [(8, 96), (32, 96), (8, 30000)])
+@pytest.mark.parametrize("out", [torch.uint8, torch.float32])
+def test_results_that_the_next_call_reads(heads, n, out):
+    """Attention into x of the adapters, whose first kernel starts beside the end of attention's last, over and over into the same
+    arrays, and a page table that a copy in front has written: the bits of calls that wait for one another."""
+    seqs, kv, dim, rank = 6, 2, 64, 16
+    cache, _, table, length = batch(5, [900, 33, 1, 517, 0, 64], (16, kv, dim, 0, "hnd", 0), heads)
+    tables = [table.clone(), table.clone()]
+    tables[1][0, :40] = table[0, :40].flip(0)
+    qs = [rand(s, seqs, heads * dim) for s in range(6)]
+    a, b = rand(1, 2, rank, heads * dim, dtype=torch.float16, scale=0.1), rand(2, 2, n, rank, dtype=torch.float16)
+    first, adapter = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, 2, 6], [1, 0]))
+    q, x, y = torch.empty_like(qs[0]), torch.empty(seqs, heads * dim, dtype=out, device="cuda"), torch.zeros(seqs, n, device="cuda")
+    tmp = torch.empty(1 << 24, dtype=torch.uint8, device="cuda")
+    attention = B.PagedAttention(seqs, heads, B.DT_F32, DT[out], q.data_ptr(), x.data_ptr(), None, heads * dim, heads * dim, table.data_ptr(), length.data_ptr(),
+                                 table.shape[1], 0, 0.125, 60.0)
+    lora = B.Lora(seqs, n, heads * dim, rank, 2, 2, DT[out], x.data_ptr(), y.data_ptr(), heads * dim, n, a.data_ptr(), b.data_ptr(), heads * dim, None,
+                  first.data_ptr(), adapter.data_ptr(), 60.0, None, None)
+
+    def steps(wait):
+        kept = []
+        y.zero_()
+        for i in range(24):
+            q.copy_(qs[i % 6])
+            table.copy_(tables[i % 2])
+            for call in (lambda: B.paged_attention(cache.desc(), attention, tmp.numel(), tmp.data_ptr()), lambda: B.lora(lora, tmp.numel(), tmp.data_ptr())):
+                call()
+                if wait:
+                    torch.cuda.synchronize()
+            kept.append(y.clone())
+        assert status() == 0
+        return kept
+
+    want = steps(True)
+    for _ in range(3):
+        same = [torch.equal(u, v) for u, v in zip(steps(False), want)]
+        assert same == [True] * 24
