@@ -77,8 +77,9 @@ inline bool aligned(const void *p, size_t n)
 {
     return reinterpret_cast<uintptr_t>(p) % n == 0;
 }
-// Strides are described by the caller; with this limit no offset (32-bit index times stride) leaves 64 bits.
-constexpr uint64_t MAX_STRIDE = 1ull << 30;
+// Strides are described by the caller.  With the first limit 2^32 rows of a call's own stay within 64 bits; what has more than
+// that to an index (pages, adapters, tables) is held below the second.
+constexpr uint64_t MAX_STRIDE = 1ull << 30, MAX_BYTES = 1ull << 62;
 
 // memory of the GPU that the calling thread's calls run on
 bool on_this_device(const void *p);

@@ -59,8 +59,15 @@ EE check_cache(const bolt_b200_kv_cache *c)
             return NOT_SUPPORTED;
         }
     }
-    // 2^62 bytes and 2^31 rows of one number: more is no cache, and offsets stay within 64 bits
+    // 2^62 bytes: more is no cache, and offsets stay within 64 bits
     if (c->pages > 0x7FFFFFFFu || c->page_size > 0x7FFFFFFFu || c->kv_heads > 65535u) {
+        return NOT_SUPPORTED;
+    }
+    unsigned __int128 elements = c->dim;
+    for (int i = 0; i < 3; ++i) {
+        elements += (unsigned __int128)(counts[i] - 1) * strides[i];
+    }
+    if (elements * size > MAX_BYTES || (c->dt == DT_I8 && (unsigned __int128)c->pages * c->page_size * c->kv_heads * 4 > MAX_BYTES)) {
         return NOT_SUPPORTED;
     }
     if (c->dt == DT_I8) {
@@ -368,7 +375,7 @@ extern "C" EE bolt_b200_kv_append(const bolt_b200_kv_cache *cache, const bolt_b2
         return NOT_MATCH;
     }
     const uint64_t rows = (uint64_t)a->tokens * ((uint64_t)a->heads + 2ull * cache->kv_heads);
-    if (a->heads > 65535u || rows > 0xFFFFFFFFull / 32 * 8) {
+    if (a->heads > 65535u || rows > 0xFFFFFFFFull / 32 * 8 || (unsigned __int128)a->sequences * a->table_pages * 4 > MAX_BYTES) {
         return NOT_SUPPORTED;
     }
     const uint32_t size = a->dt == DT_F32 ? 4 : 2, q_size = a->q_out_dt == DT_F32 ? 4 : 2;

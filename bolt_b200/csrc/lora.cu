@@ -844,7 +844,7 @@ EE check(const bolt_b200_lora_call *a, LoraParams *p, DeviceCtx **c)
         return NOT_MATCH;
     }
     if (a->x_stride > MAX_STRIDE || a->y_stride > MAX_STRIDE || a->a_stride > MAX_STRIDE || a->rows > (1u << 22) || a->N > (1u << 23) ||
-        a->adapters > 0x7FFFFFFFu || a->segments > MAX_SEGMENTS) {
+        a->adapters > 0x7FFFFFFFu || a->segments > MAX_SEGMENTS || (unsigned __int128)a->adapters * a->rank * a->a_stride * 2 > MAX_BYTES) {
         return NOT_SUPPORTED;
     }
     p->rows = a->rows;

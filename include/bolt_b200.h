@@ -491,7 +491,8 @@ EE matmul_cuda_b200(const TensorDesc *matrixADesc, int transposeA, const void *m
  *   DT_I8:  signed bytes; row (page, token, head) stands for byte / scale[(page * kv_heads + head) * page_size + token],
  *           scale = 127 / absmax of the row as everywhere in this library.
  * A row has at most 256 elements; its size in bytes, the strides in bytes and k and v are multiples of 16 (else
- * NOT_SUPPORTED).  Rows must not overlap.  At most 2^31 - 1 pages of as many tokens, 65535 heads, strides up to 2^36. */
+ * NOT_SUPPORTED).  Rows must not overlap.  At most 2^31 - 1 pages of as many tokens, 65535 heads, strides up to 2^36, 2^62 bytes
+ * of each array. */
 typedef struct {
     DataType dt;
     U32 pages, page_size, kv_heads, dim;
@@ -514,7 +515,7 @@ typedef struct {
  * DT_F16 results are rounded once.  A DT_I8 row is quantized as by quantize_cuda_b200 (F32 -> I8) with a dynamic
  * scale of its own: scale = 127 / absmax (1 for a row of zeros), byte = clamp(rne(x * scale), -127, 127).
  * A token that is refused on the device (see above) leaves cache and q_out as they were.
- * At most 65535 query heads, strides up to 2^30, 2^30 heads of all kinds and tokens together. */
+ * At most 65535 query heads, strides up to 2^30, 2^30 heads of all kinds and tokens together, a table of 2^62 bytes. */
 typedef struct {
     U32 tokens, heads; /* heads: of the queries */
     DataType dt;       /* of q, k and v: DT_F32 or DT_F16 */
@@ -572,7 +573,7 @@ EE bolt_b200_paged_attention(
  * >= K) a multiple of 8.  x: DT_F32, or DT_U8_Q = the product's own input, which stands for
  * (byte - 128) / (row_scale[m], or *d_sA, or sA).  x and y rows may start anywhere.  Sums are binary32 (22 bits at least
  * of x and of the inner sums enter the products).  x must not overlap y.  At most 2^22 rows, 2^23
- * columns, 65535 segments, strides up to 2^30.  tmp: as for attention. */
+ * columns, 65535 segments, strides up to 2^30, 2^62 bytes of a.  tmp: as for attention. */
 typedef struct {
     U32 rows, N, K, rank, adapters, segments;
     DataType x_dt; /* DT_F32 or DT_U8_Q */
