@@ -9,9 +9,9 @@
 //
 // Bytes of x become binary16 exactly.  Binary32 x enters as two tf32 numbers (23 bits; tf32 has binary32's range), t as two
 // binary16 numbers of rows brought to a common power of two.  The accumulation of the matrix instructions truncates, which adds
-// up: sums over K go on in binary32 registers after two instructions, what the first number of a pair leaves is summed up
-// by itself, and sums over the rank go on in binary32 after 64 of it.  Sums of 8192 positive products of binary32 numbers come
-// out 2^-23 too small on the average where one chain of 32 instructions made them 2^-19 too small, those of any sign are as near
+// up: what the first number of a pair leaves goes first, while the sum is small, and sums go on in binary32 registers, over K after
+// two instructions for the first numbers, over the rank after 64 of it.  Sums of positive products of binary32 numbers come out
+// 0.7 to 1.5 2^-23 too small on the average (5 to 14 with all of K that is in flight in one chain), those of any sign are as near
 // as binary32 throughout (1.1 to 1.7 2^-23 of the result, in root mean square).
 //
 // 2048 rows, 8192 -> 28672, rank 16, six requests: 75 to 86 us, 5.4 to 6.3 TB/s of the 470 MB of the result, read and written;
@@ -247,19 +247,10 @@ struct Eight<true> {
         h[2] = centred<0>(b);
         h[3] = centred<1>(b);
     }
-    // sum += rows (this one's and another eight's) x eight neighbours of a row of A
-    __device__ __forceinline__ void multiply(const Eight &other, const uint32_t (&a)[4], float (&sum)[4]) const
-    {
-        float c[4];
-        mma_f16_first(c, h[0], other.h[0], h[1], other.h[1], a[0], a[1]);
-        mma_f16(c, h[2], other.h[2], h[3], other.h[3], a[2], a[3]);
-        add(sum, c);
-    }
 };
 template <>
 struct Eight<false> {
     float f[8];
-    uint32_t hi[8], lo[8];
     __device__ __forceinline__ void load(const LoraParams &p, uint64_t row, uint32_t k, bool on)
     {
         const float *x = reinterpret_cast<const float *>(p.x) + row * p.x_stride + k;
@@ -286,37 +277,61 @@ struct Eight<false> {
             }
         }
     }
-    __device__ __forceinline__ void convert()
-    {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            tf32_pair(f[i], hi[i], lo[i]);
-        }
-    }
-    __device__ __forceinline__ void multiply(const Eight &other, const uint32_t (&a)[4], float (&sum)[4]) const
-    {
-        float c[4], rest[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&a[e]));
-            const uint32_t b0 = __float_as_uint(v.x), b1 = __float_as_uint(v.y);
-            if (e == 0) {
-                mma_tf32_first(rest, lo[0], other.lo[0], lo[1], other.lo[1], b0, b1);
-            } else {
-                mma_tf32(rest, lo[2 * e], other.lo[2 * e], lo[2 * e + 1], other.lo[2 * e + 1], b0, b1);
-            }
-            if (e % 2 == 0) {
-                mma_tf32_first(c, hi[2 * e], other.hi[2 * e], hi[2 * e + 1], other.hi[2 * e + 1], b0, b1);
-            } else {
-                mma_tf32(c, hi[2 * e], other.hi[2 * e], hi[2 * e + 1], other.hi[2 * e + 1], b0, b1);
-            }
-            if (e % 2 == 1) {
-                add(sum, c);
-            }
-        }
-        add(sum, rest);
-    }
 };
+
+// sum += sixteen rows x eight neighbours of rows of A (each lane's)
+template <int NT>
+__device__ __forceinline__ void add_products(Eight<true> &x0, Eight<true> &x1, const uint4 (&a)[NT], float (&sum)[NT][4])
+{
+    x0.convert();
+    x1.convert();
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        float c[4];
+        mma_f16_first(c, x0.h[0], x1.h[0], x0.h[1], x1.h[1], a[n].x, a[n].y);
+        mma_f16(c, x0.h[2], x1.h[2], x0.h[3], x1.h[3], a[n].z, a[n].w);
+        add(sum[n], c);
+    }
+}
+template <int NT>
+__device__ __forceinline__ void add_products(const Eight<false> &x0, const Eight<false> &x1, const uint4 (&a)[NT], float (&sum)[NT][4])
+{
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) {     // two instructions' worth: first what the first parts leave, while the sum is small
+        uint32_t hi[2][4], lo[2][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            tf32_pair(x0.f[e + i], hi[i / 2][i % 2 * 2], lo[i / 2][i % 2 * 2]);
+            tf32_pair(x1.f[e + i], hi[i / 2][i % 2 * 2 + 1], lo[i / 2][i % 2 * 2 + 1]);
+        }
+        constexpr int GROUP = NT < 8 ? NT : 8;    // instructions that do not wait for one another
+#pragma unroll
+        for (int n0 = 0; n0 < NT; n0 += GROUP) {
+            float c[GROUP][4];
+            auto multiply = [&](const uint32_t (&x)[4], int n, int i, bool first) {
+                const uint4 &w = a[n0 + n];
+                const uint32_t h = e == 0 ? (i == 0 ? w.x : w.y) : (i == 0 ? w.z : w.w);
+                const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&h));
+                if (first) {
+                    mma_tf32_first(c[n], x[0], x[1], x[2], x[3], __float_as_uint(b.x), __float_as_uint(b.y));
+                } else {
+                    mma_tf32(c[n], x[0], x[1], x[2], x[3], __float_as_uint(b.x), __float_as_uint(b.y));
+                }
+            };
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                for (int n = 0; n < GROUP; ++n) {
+                    multiply(i < 2 ? lo[i] : hi[i - 2], n, i % 2, i == 0);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < GROUP; ++n) {
+                add(sum[n0 + n], c[n]);
+            }
+        }
+    }
+}
 
 // By the 256 threads of a CTA: the sums over blocks from .. to - 1 of 32 of K for the rows of a unit, times their scales, in warp 0: sum
 // [n][0, 1] for row g and columns 8 n + 2 c4 and the next, [2, 3] for row g + 8.  NT: blocks of eight of the rank, rounded up.
@@ -350,21 +365,20 @@ __device__ __forceinline__ void inner_sums(const LoraParams &p, const Unit &u, u
 #pragma unroll
         for (int i = 0; i < AT_ONCE; ++i) {
             const uint32_t k = 32 * (kb + 8 * i) + 8 * c4;
-            x[i][0].convert();
-            x[i][1].convert();
+            if (k + 8 > p.K) {   // what lies behind K in a row of A is nobody's
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                uint32_t h[4] = {w[i][n].x, w[i][n].y, w[i][n].z, w[i][n].w};
-                if (k + 8 > p.K) {   // what lies behind K in a row of A is nobody's
+                for (int n = 0; n < NT; ++n) {
+                    uint32_t h[4] = {w[i][n].x, w[i][n].y, w[i][n].z, w[i][n].w};
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         if (k + e >= p.K) {
                             h[e / 2] &= e % 2 ? 0x0000FFFFu : 0xFFFF0000u;
                         }
                     }
+                    w[i][n] = make_uint4(h[0], h[1], h[2], h[3]);
                 }
-                x[i][0].multiply(x[i][1], h, sum[n]);
             }
+            add_products(x[i][0], x[i][1], w[i], sum);
         }
     }
     // the warps' shares, the upper half's added to the lower half's, and so on
@@ -409,7 +423,7 @@ __device__ __forceinline__ void inner_sums(const LoraParams &p, const Unit &u, u
         }
     }
 }
-// (Binary32 x with ranks of 17 to 64: a few registers above half of them all without the bound; 2048 rows of rank 32 106 us, 117
+// (Binary32 x with ranks of 17 to 64: a few registers above half of them all without the bound; 2048 rows of rank 64 130 us, 149
 // without.)
 template <bool U8, int NT>
 __global__ void __launch_bounds__(256, !U8 && (NT == 4 || NT == 8) ? 2 : 0) lora_inner_kernel(const __grid_constant__ LoraParams p)
