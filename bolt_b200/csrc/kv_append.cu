@@ -107,7 +107,8 @@ struct AppendParams {
 //
 // With more than a row to a group of lanes the CTAs are as many as run at a time, and each goes from task to task: the next
 // one's position is asked for with this one's rows, and its rows go into L2 meanwhile (a task to a group and no more: 58.7 us, with
-// binary16 rows 72.5; now 47 and 51).
+// binary16 rows 72.5; now 47 and 51).  Binary16 takes as many instructions a row as binary32, four elements at a time, and is bound
+// by them: its bytes would take 22 us.
 constexpr int RESIDENT = 4;
 template <typename TIN, int VW, int LANES, int PER, int ROWS>
 __global__ void __launch_bounds__(256, ROWS > 1 ? RESIDENT : 1) kv_append_kernel(const __grid_constant__ AppendParams p)

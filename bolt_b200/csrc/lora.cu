@@ -14,8 +14,9 @@
 // 0.7 to 1.5 2^-23 too small on the average (5 to 14 with all of K that is in flight in one chain), those of any sign are as near
 // as binary32 throughout (1.1 to 1.7 2^-23 of the result, in root mean square).
 //
-// 2048 rows, 8192 -> 28672, rank 16, six requests: 75 to 86 us, 5.4 to 6.3 TB/s of the 470 MB of the result, read and written;
-// rank 64: 127 us.  16 rows with an adapter each: 13.4 us, two kernels of dependent loads over 23 MB.
+// 2048 rows, 8192 -> 28672, rank 16, six requests: 75 to 92 us, 5.1 to 6.3 TB/s of the 470 MB of the result, read and written.  Every 16
+// rows read all of A and B, from L2: rank 64 118 us, rank 128 202.  16 rows with an adapter each: 13.3 us, two kernels of dependent
+// loads over 23 MB.
 #include "decode.cuh"
 
 namespace b200 {
@@ -819,18 +820,18 @@ void divide(LoraParams *p, const DeviceCtx *c)
 {
     const uint32_t most = p->rows / 16 + p->segments, sms = (uint32_t)c->sm_count;
     p->units = most < p->rows ? most : p->rows;
-    // K in as many parts as give every SM four CTAs (2048 rows of 8192: 86.0 us, with two 86.6, with eight 87.5), each at least
+    // K in as many parts as give every SM four CTAs (2048 rows of 8192: 86.5 us, with two 87.0, with eight 88.3), each at least
     // as long as what a CTA asks for at a time, and sixteen at most, which the second kernel asks for in two goes.
-    // 16 rows of 8192 with adapters of rank 16: 13.3 us in 8 parts of 1024, 14.3 in 16, 18.8 in 32, 13.5 in 4; one row of 28672: 8.1
-    // in 16 parts, 9.6 in 8; rank 128: 25.8 and 34.8.
+    // 16 rows of 8192 with adapters of rank 16: 13.3 us in 8 parts of 1024, 14.5 in 16, 18.9 in 32, 13.6 in 4; one row of 28672: 8.1
+    // in 16 parts, 9.4 in 8; 16 rows with one adapter of rank 128: 23.5 and 30.5.
     const uint32_t at_a_time = p->rank <= 16 ? 1024 : (p->rank <= 32 ? 512 : 256);
     const uint32_t want = p->units == 0 ? 1 : 4 * sms / p->units, at_most = (p->K - 1) / at_a_time + 1;
     p->splits = want < 1 ? 1 : (want < at_most ? want : at_most);
     p->splits = p->splits < 16 ? p->splits : 16;
     const uint64_t steps = (uint64_t)p->units * ((p->N + STEP - 1) / STEP), by_itself = (uint64_t)sms * (p->u8 ? 2 : 1);
     // One kernel, in which every CTA makes its rows' inner sums, where they take no more than one go and few CTAs meet a second
-    // unit: 16 rows of 768 -> 768 6.3 us in place of 7.4 (binary32), 5.7 in place of 6.4 (bytes).  With four goes 16 rows of
-    // 4096 -> 4096 take 12.7 in place of 8.0, and 1024 rows of 768 -> 2304 with eight adapters 13.1 in place of 12.5.
+    // unit: 16 rows of 768 -> 768 6.3 us in place of 7.4 (binary32), 5.5 in place of 6.5 (bytes).  With four goes 16 rows of
+    // 4096 -> 4096 take 12.6 in place of 8.0, and 1024 rows of 768 -> 2304 with eight adapters 13.0 in place of 12.7.
     p->alone = p->rank <= 32 && p->K <= at_a_time && steps <= 2 * by_itself;
     // as many CTAs as run at a time, and no more than there are steps
     const uint64_t ctas = p->alone ? by_itself : (uint64_t)sms * (p->rank <= 16 ? 4 : (p->rank <= 32 ? 3 : 2));

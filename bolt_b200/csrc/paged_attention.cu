@@ -3,7 +3,8 @@
 // out = sum_t exp(s_t - m) v_t / sum_t exp(s_t - m), s_t = scale q . k_t, in one pass over the tokens with a running maximum
 // m: when it rises, what has been summed so far is scaled down.  Shares of a sequence are joined the same way.
 //
-// HBM bound: keys and values are read once, whatever the number of query heads, and everything else is small beside them.
+// HBM bound: keys and values are read once for up to sixteen query heads of a key head (and once more for every sixteen beyond), and
+// everything else is small beside them.
 // Every team of warps takes an equal part of all tokens of the batch (whose lengths the host does not know), cut where it
 // may be; a second kernel joins the units that were cut.  Inside a team every warp streams tokens of its own through a private
 // ring of asynchronous copies and keeps its own maximum, total and sums, so that warps meet only at the end of a unit.
@@ -12,12 +13,11 @@
 // probabilities) with the cache's binary16; bytes become binary16 in registers, five instructions for four of them, unless
 // mma.m16n8k32 takes them as they are (keys).
 //
-// Whole calls: binary16, 64 sequences of 8192 tokens, 8 key heads of 128: 6.1 TB/s; bytes: 5.3 TB/s, bound by about 940
-// instructions for a step of 32 tokens (of which 145 make binary16 of bytes) and, call after call, by the power that they take
-// (4.4 TB/s).  One sequence of 131072 tokens: 95 to 101 us, 5.4 TB/s.  One of 4000: 11.5 us, of which 8 are the chain length
-// -> page -> keys -> values -> shares with the code that has to be fetched on the way, 4 the join.  Rows of 256 elements and
-// groups of more than eight query heads keep 64 running sums a lane and run with eight warps: 2.6 TB/s in bytes with 16
-// heads, 5.7 TB/s in binary16 with rows of 256.
+// Whole calls, 64 sequences of up to 8192 tokens, 8 key heads of 128: binary16 5.9 TB/s; bytes 4.6 TB/s in short bursts, bound by
+// 924 instructions for a step of 32 tokens, and call after call, by the power that they take, 4.0 TB/s.  One sequence of
+// 131072 tokens: 94 to 101 us, 5.3 to 5.7 TB/s.  One of 4000: 11.7 us, of which 8 are the chain length -> page -> keys -> values
+// -> shares with the code that has to be fetched on the way, 4 the join.  Rows of 256 elements and groups of more than eight query
+// heads keep 64 running sums a lane and run with eight warps: 2.6 TB/s in bytes with 16 heads, 4.7 in binary16.
 #include <type_traits>
 
 #include "decode.cuh"
@@ -88,7 +88,7 @@ __device__ __forceinline__ void store_out(const AttentionParams &p, uint64_t at,
 constexpr int MAX_WARPS = 16;
 constexpr uint32_t MAX_SEQUENCES = 65535;
 // Up to so many sequences every warp counts for itself, beyond, the CTA's warps share the counting and wait for one another
-// (64 sequences of some 150 tokens, 12 heads of 64: 23.4 us and, shared, 24.0; 512: 112.4 and 110.4).
+// (64 sequences of some 150 tokens, 12 heads of 64: 23.3 us and, shared, 24.0; 512: 112.3 and 110.7).
 constexpr uint32_t BY_WARP = 256;
 struct Found {
     uint32_t sequence, first;
@@ -320,11 +320,11 @@ struct Shape {
     static constexpr int HEADS = 8 * HB;
     static constexpr int NUMBERS = DP / 8 * 2 * HB;                              // running sums of a lane
     // Steps are chains of dependent instructions: sixteen warps (128 registers a lane) hide them where the running sums fit (64
-    // sequences of up to 8192 tokens in bytes: 141 us, with eight warps and six slots 165; in binary16 202 and 226).
+    // sequences of up to 8192 tokens in bytes: 135 us, with eight warps and six slots 164; in binary16 202 and 227).
     static constexpr int WARPS = NUMBERS <= 32 && HB == 1 ? 16 : 8;
     // With one block of heads queries meet bytes as whole numbers, four digits of base 256 each, and keys need no conversion (64
-    // sequences of up to 8192 tokens, 300 calls in a row: 146 us, as binary16 149; rows of 256 elements 161 and 167; two blocks
-    // would have 64 running numbers more: 261 and 242).
+    // sequences of up to 8192 tokens: 135 us, as binary16 137; rows of 256 elements 155 and 162; two blocks would have 64
+    // running numbers more, which took 261 us in place of 242).
     static constexpr bool DIGITS = I8 && HB == 1;
     static constexpr float LIFT = I8 ? 0.f : 14.f;     // binary16: weights are exp(s - m) 2^14
     static constexpr int Q_PITCH = DP * (DIGITS ? 1 : 2) + 16, Q_ROWS = HEADS * (DIGITS ? 4 : 2), Q_BYTES = Q_ROWS * Q_PITCH;   // queries of a team
@@ -336,7 +336,7 @@ struct Shape {
     static constexpr int FIT = (232448 - FIXED) / (WARPS * SLOT);
     // Ring of a warp: K, V, K, V ...  Two slots, three for two blocks of heads (eight warps with twice the products):
     // what shared memory does not take is L1, and more requests at a time do not help (64 sequences of up to 8192 tokens in
-    // binary16: 201 us with two, 215 with three; 16 heads to a key head: 276, 250, and 257 with six).
+    // binary16: 202 us with two, 212 with three; 16 heads to a key head: 274, 253, and 257 with six).
     static constexpr int SLOTS = HB == 1 ? 2 : (FIT < 3 ? FIT : 3);
     static constexpr int SMEM = FIXED + WARPS * SLOTS * SLOT;
     static constexpr int PART = HEADS * (DP + 2);                                // floats of a partial result: sums, then maxima, then totals
@@ -1148,8 +1148,8 @@ __global__ void __launch_bounds__(512) paged_attention_join_kernel(const __grid_
 }
 
 // The team: as many warps as leave a part for every unit, so that few units mean few shares to join (one sequence of 4000
-// tokens: 11.7 us, with teams of four 16.0), and with many units no more warps than need be wait for others at a unit's end (64
-// sequences of up to 8192 tokens in bytes: 141 us, with teams of sixteen 183).
+// tokens: 11.7 us, with teams of four 15.8), and with many units no more warps than need be wait for others at a unit's end (64
+// sequences of up to 8192 tokens in bytes: 135 us, with teams of sixteen 175).
 template <int DP, bool I8, int HB>
 EE plan(const DeviceCtx *c, AttentionParams *p, uint64_t units)
 {

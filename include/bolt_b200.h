@@ -478,11 +478,11 @@ EE matmul_cuda_b200(const TensorDesc *matrixADesc, int transposeA, const void *m
  * Bolt serves a language model through its engine's graphs and has no operator of these kinds (no counterpart).
  * All pointers are device pointers of the GPU the call runs on (anything else: NOT_MATCH); the work is enqueued on
  * the thread's stream and the call returns without waiting.  Lengths, positions, page numbers and segments are
- * read on the device, so one captured graph serves every step.  What they say is checked there: a number that
- * would lead outside the arrays described by the call is not followed, and the device status word is set (51 by
- * bolt_b200_kv_append, 52 by bolt_b200_paged_attention, 53 by bolt_b200_lora), so that the next
- * bolt_b200_synchronize returns UNKNOWN.  Calls that run at the same time need a tmp each, two captured graphs
- * that may do so as well; tmp need not be initialised. */
+ * read on the device, so one captured graph serves every step; they are read several times in a call and must not change
+ * while it runs.  What they say is checked there: a number that would lead outside the arrays described by the call is
+ * not followed, and the device status word is set (51 by bolt_b200_kv_append, 52 by bolt_b200_paged_attention, 53 by
+ * bolt_b200_lora), so that the next bolt_b200_synchronize returns UNKNOWN.  Calls that run at the same time need a tmp
+ * each, two captured graphs that may do so as well; tmp need not be initialised. */
 
 /* A cache of pages, each `page_size` tokens of `kv_heads` heads.  The row of (page, token of the page, head) is `dim`
  * contiguous elements at element page * page_stride + token * token_stride + head * head_stride of k and of v
@@ -571,8 +571,8 @@ EE bolt_b200_paged_attention(
  * whose adapter does not exist, is left out (and reported, see above).  rank: a multiple of 8 up to 128 (adapters of
  * lower rank are filled up with zeros).  a, b: binary16, 16-byte aligned, a_stride (elements from row to row of a,
  * >= K) a multiple of 8.  x: DT_F32, or DT_U8_Q = the product's own input, which stands for
- * (byte - 128) / (row_scale[m], or *d_sA, or sA).  x and y rows may start anywhere.  Sums are binary32 (22 bits at least
- * of x and of the inner sums enter the products).  x must not overlap y.  At most 2^22 rows, 2^23
+ * (byte - 128) / (row_scale[m], or *d_sA, or sA).  x and y rows may start anywhere.  Sums are binary32; x enters its products to
+ * 2^-23 of itself, an inner sum to 2^-22 of itself or 2^-38 of its row's largest.  x must not overlap y.  At most 2^22 rows, 2^23
  * columns, 65535 segments, strides up to 2^30, 2^62 bytes of a.  tmp: as for attention. */
 typedef struct {
     U32 rows, N, K, rank, adapters, segments;
