@@ -14,7 +14,7 @@
 // mma.m16n8k32 takes them as they are (keys).
 //
 // Whole calls, 64 sequences of up to 8192 tokens, 8 key heads of 128: binary16 5.9 TB/s; bytes 4.6 TB/s in short bursts, bound by
-// 924 instructions for a step of 32 tokens, and call after call, by the power that they take, 4.0 TB/s.  One sequence of
+// 924 instructions for a step of 32 tokens, and call after call, by the power that they take, 3.9 to 4.3 TB/s.  One sequence of
 // 131072 tokens: 94 to 101 us, 5.3 to 5.7 TB/s.  One of 4000: 11.7 us, of which 8 are the chain length -> page -> keys -> values
 // -> shares with the code that has to be fetched on the way, 4 the join.  Rows of 256 elements and groups of more than eight query
 // heads keep 64 running sums a lane and run with eight warps: 2.6 TB/s in bytes with 16 heads, 4.7 in binary16.
@@ -399,6 +399,7 @@ __global__ void __launch_bounds__(32 * Shape<DP, I8, HB>::WARPS, 1) paged_attent
         p.cuts[part].parts = 0;
     }
     auto team_sync = [&]() {
+        __syncwarp();       // (the barrier takes a warp as a whole, and comes behind branches that some lanes have taken)
         if (team == WARPS) {
             __syncthreads();
         } else {
