@@ -363,6 +363,7 @@ __device__ __forceinline__ void inner_sums(const LoraParams &p, const Unit &u, u
             x[i][0].load(p, u.row + g, k, b < to && k < p.K && g < u.rows);
             x[i][1].load(p, u.row + g + 8, k, b < to && k < p.K && g + 8 < u.rows);
         }
+        __syncwarp();       // (matrix instructions take a warp as a whole, and come behind branches that some lanes have taken)
 #pragma unroll
         for (int i = 0; i < AT_ONCE; ++i) {
             const uint32_t k = 32 * (kb + 8 * i) + 8 * c4;
@@ -745,6 +746,7 @@ __global__ void __launch_bounds__(256, ALONE ? (ALONE == ALONE_U8 ? 2 : 1) : (KS
         const float down0 = down[g], down1 = down[g + 8];
 #pragma unroll 1
         for (;;) {
+            __syncwarp();
             // The instruction's own accumulation truncates: what binary16 has cut off of t goes first, while the sums are small, and
             // every 16 * FOLD of the rank the sums go on in binary32.
             constexpr int FOLD = KS < 4 ? KS : 4;
